@@ -41,7 +41,7 @@ typedef struct ihipStream_t* hipStream_t;
 #define LQ_DT_BF16 3
 
 /* ABI version; bumped whenever a struct layout, or what a call asks of its caller, changes.  The function gives the library's. */
-#define LQ_ABI_VERSION 21
+#define LQ_ABI_VERSION 22
 int lq_abi_version(void);
 /* sizeof() of the named args struct as compiled into the library (negative if unknown); lets a binding
  * check its own struct layout before the first call. */
@@ -796,6 +796,178 @@ typedef struct {
   int32_t batch, seqlen, ngroups, dstate, chunk_size; /* N a multiple of 8 */
 } lq_absmax_cb_args;
 int lq_absmax_cb(const lq_absmax_cb_args* args, hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Serving: a Mamba-2 block that carries its convolution inputs and its state from call to call, the INT8 projections around
+ * it and the residual stream between blocks.  16-bit activations are fp16 or bf16 (LQ_DT_F16 / LQ_DT_BF16).
+ *
+ * `slots` (NULL: sequence i uses slot i) holds, for each sequence of a call, its place in the state tensors.  A negative slot
+ * marks a padding entry: a single-token call writes zeros to its output row, a prompt call starts it from a zero state and
+ * keeps none.  A slot of num_slots or more fails loudly without touching memory out of range: that sequence's outputs are NaN
+ * and no state is written.  Two sequences of one call must not name the same slot.
+ *
+ * `seq_starts` (n + 1 int32 on the device, ascending, the first >= 0, the last <= tokens) packs prompts of any lengths, zero
+ * among them, into one row of tokens; tokens outside it are neither read nor written.  NULL: nseq prompts of seqlen tokens.
+ * ------------------------------------------------------------------------------------------ */
+
+/* no counterpart in the reference (its quantizer, linquant/w4a8_linear.py:36-98, has one scale for a tensor): one scale a row,
+ * scale[r] = max_c |x[r,c]| / 127, codes rint(x / scale).  A row of zeros has scale 0 and codes 0; a row with an infinity or a
+ * NaN has scale NaN and codes 0, so that what is computed from it is NaN. */
+typedef struct {
+  const void* x;             /* (rows, cols), unit column stride */
+  int64_t x_stride;
+  int32_t dtype;             /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  int8_t* codes;             /* (rows, cols), unit column stride */
+  int64_t codes_stride;
+  float* scale;              /* (rows,) */
+  int32_t rows, cols;        /* cols up to 16384 */
+} lq_quantize_rows_args;
+int lq_quantize_rows(const lq_quantize_rows_args* args, hipStream_t stream);
+
+/* no counterpart in the reference (its projections are W4A8, linquant/w4a8_linear.py): INT8 matrix product,
+ *   out[m,n] = (sum_k a[m,k] b[n,k]) * a_scale[m] * b_scale[n] + bias[n], the sum exact in 32 bits. */
+typedef struct {
+  const int8_t* a;           /* (rows, inner), unit inner stride, 16-byte aligned rows */
+  int64_t a_stride;
+  const int8_t* b;           /* (cols, inner), unit inner stride, 16-byte aligned rows */
+  int64_t b_stride;
+  const float* a_scale;      /* (rows,), or one when a_scale_rows is 0 */
+  const float* b_scale;      /* (cols,), or one when b_scale_cols is 0 */
+  int32_t a_scale_rows, b_scale_cols;
+  const void* bias;          /* (cols,) or NULL */
+  int32_t bias_dtype;        /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  void* out;                 /* (rows, cols), unit column stride */
+  int64_t out_stride;
+  int32_t out_dtype;         /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  int32_t rows, cols, inner; /* inner a multiple of 16, at most 131056 (a sum of 128 * 128 each fits 32 bits) */
+} lq_int8_matmul_args;
+int lq_int8_matmul(const lq_int8_matmul_args* args, hipStream_t stream);
+
+/* no counterpart in the reference: the residual stream between two blocks, in fp32 and one rounding at each output,
+ *   u = x, or x * rsqrt(mean(x^2) + eps) * post_weight;  r = residual + scale * gate * u;
+ *   y = r * rsqrt(mean(r^2) + eps) * weight  ->  `out`, or INT8 codes on a scale of each row or on a given one.
+ * residual_out may be `residual` and out may be `x`. */
+typedef struct {
+  const void* x;             /* (rows, dim), unit dim stride */
+  int64_t x_stride;
+  int32_t dtype;             /* of x, gate and out: LQ_DT_F16 / LQ_DT_BF16 */
+  const void* residual;      /* (rows, dim), NULL: zero */
+  int64_t residual_stride;
+  int32_t residual_dtype;    /* of residual and residual_out: `dtype` or LQ_DT_F32 */
+  const void* gate;          /* NULL: one.  Row r takes row r / gate_rows of it */
+  int64_t gate_stride;       /* 0: one row for all */
+  int32_t gate_rows;
+  const void* post_weight;   /* (dim,) or NULL: no norm after the block */
+  const void* weight;        /* (dim,) */
+  int32_t weight_dtype;      /* of both: LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  float scale, eps;
+  void* residual_out;        /* (rows, dim) or NULL */
+  int64_t residual_out_stride;
+  void* out;                 /* (rows, dim), or NULL: codes */
+  int64_t out_stride;
+  int8_t* codes;             /* (rows, dim), or NULL: out.  Exactly one of the two */
+  int64_t codes_stride;
+  const float* code_scale;   /* device scalar: codes clamp(rint(y / scale), -128, 127).  NULL: row_scale */
+  float* row_scale;          /* (rows,): max |y| / 127 of each row, as lq_quantize_rows */
+  int32_t rows, dim;         /* dim up to 16384 */
+} lq_residual_rmsnorm_args;
+int lq_residual_rmsnorm(const lq_residual_rmsnorm_args* args, hipStream_t stream);
+
+/* no counterpart in the reference (its convolution, linquant/quantized_mamba2.py:262-268, starts every prompt from zeros):
+ * y[t,c] = act(bias[c] + sum_j weight[c,j] x[t-(width-1)+j, c]) over each prompt; the width - 1 tokens in front of its first
+ * come from its slot of `state`, which afterwards holds the last width - 1 (oldest first). */
+typedef struct {
+  const void* x;             /* (tokens, dim) with seq_starts, else (nseq, seqlen, dim); unit dim stride */
+  int64_t x_stride_b, x_stride_l;
+  int32_t dtype;             /* of x, weight, bias, state and out: LQ_DT_F16 / LQ_DT_BF16 */
+  const void* weight;        /* (dim, width) */
+  const void* bias;          /* (dim,) or NULL */
+  void* out;                 /* the shape of x, dense */
+  void* state;               /* (num_slots, width - 1, dim), unit dim stride, or NULL: zeros in front, nothing kept */
+  int64_t state_stride_s, state_stride_w;
+  const int32_t* slots;      /* (nseq,) or NULL */
+  const int32_t* seq_starts; /* (nseq + 1,) or NULL */
+  int32_t num_slots, nseq, seqlen, tokens; /* seqlen without seq_starts, tokens with */
+  int32_t dim, width;        /* dim a multiple of 8, width 2 to 4 */
+  int32_t silu;
+} lq_conv1d_prompt_args;
+int lq_conv1d_prompt(const lq_conv1d_prompt_args* args, hipStream_t stream);
+
+/* no counterpart in the reference: the same for one token of each sequence; state is updated in place. */
+typedef struct {
+  const void* x;             /* (batch, dim), unit dim stride */
+  int64_t x_stride;
+  int32_t dtype;
+  const void* weight;        /* (dim, width) */
+  const void* bias;          /* (dim,) or NULL */
+  void* out;                 /* (batch, dim) dense */
+  void* state;               /* (num_slots, width - 1, dim) */
+  int64_t state_stride_s, state_stride_w;
+  const int32_t* slots;      /* (batch,) or NULL */
+  int32_t num_slots, batch, dim, width, silu;
+} lq_conv1d_step_args;
+int lq_conv1d_step(const lq_conv1d_step_args* args, hipStream_t stream);
+
+/* no counterpart in the reference (its scan, linquant/kernels/mamba2/ssd_combined.py:19-131, is INT8, starts from zero and keeps
+ * no state): the selective state space scan on 16-bit activations with an fp32 state,
+ *   d = clamp(softplus(dt + dt_bias), dt_min, dt_max), or without the softplus;  S = exp(d A[h]) S + d x B^T;  y = S C + D x,
+ * S (headdim, dstate) for each head, starting from and ending in its slot of `state`. */
+typedef struct {
+  const void* x;             /* (tokens,H,P) with seq_starts, else (nseq,seqlen,H,P); unit P stride */
+  int64_t x_stride_b, x_stride_l, x_stride_h;
+  int32_t dtype;             /* of x, B, C and out: LQ_DT_F16 / LQ_DT_BF16 */
+  const void* dt;            /* (tokens,H) or (nseq,seqlen,H) */
+  int64_t dt_stride_b, dt_stride_l, dt_stride_h;
+  int32_t dt_dtype;          /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  const float* A;            /* (H,), negative */
+  const void* B;             /* (tokens,G,N) or (nseq,seqlen,G,N), unit N stride */
+  int64_t B_stride_b, B_stride_l, B_stride_g;
+  const void* C;             /* like B */
+  int64_t C_stride_b, C_stride_l, C_stride_g;
+  const float* D;            /* (H,) or (H,P) contiguous, or NULL */
+  int32_t D_has_hdim;
+  const float* dt_bias;      /* (H,) or NULL */
+  int32_t dt_softplus;
+  float dt_min, dt_max;
+  void* out;                 /* the shape of x, dense */
+  float* state;              /* (num_slots,H,P,N), the last three dense, or NULL: from zero, nothing kept */
+  int64_t state_stride_s;
+  const int32_t* slots;      /* (nseq,) or NULL */
+  const int32_t* seq_starts; /* (nseq + 1,) or NULL */
+  int32_t num_slots, nseq, seqlen, tokens; /* seqlen without seq_starts, tokens with */
+  int32_t nheads, headdim, ngroups, dstate; /* headdim and dstate multiples of 8, dstate up to 256 */
+  void* workspace;           /* 256-byte aligned; contents undefined on entry and on return */
+  int64_t workspace_bytes;
+} lq_ssm_prompt_args;
+int lq_ssm_prompt(const lq_ssm_prompt_args* args, hipStream_t stream);
+/* workspace size for the dims in `args` (pointers are not read but for whether seq_starts is NULL), written to *bytes */
+int lq_ssm_prompt_workspace_bytes(const lq_ssm_prompt_args* args, int64_t* bytes);
+
+/* no counterpart in the reference: the same for one token of each sequence; state is updated in place. */
+typedef struct {
+  const void* x;             /* (batch,H,P), unit P stride */
+  int64_t x_stride_b, x_stride_h;
+  int32_t dtype;
+  const void* dt;            /* (batch,H) */
+  int64_t dt_stride_b, dt_stride_h;
+  int32_t dt_dtype;
+  const float* A;            /* (H,) */
+  const void* B;             /* (batch,G,N), unit N stride */
+  int64_t B_stride_b, B_stride_g;
+  const void* C;
+  int64_t C_stride_b, C_stride_g;
+  const float* D;            /* (H,) or (H,P) contiguous, or NULL */
+  int32_t D_has_hdim;
+  const float* dt_bias;      /* (H,) or NULL */
+  int32_t dt_softplus;
+  float dt_min, dt_max;
+  void* out;                 /* (batch,H,P) dense */
+  float* state;              /* (num_slots,H,P,N), the last three dense */
+  int64_t state_stride_s;
+  const int32_t* slots;      /* (batch,) or NULL */
+  int32_t num_slots, batch, nheads, headdim, ngroups, dstate;
+} lq_ssm_step_args;
+int lq_ssm_step(const lq_ssm_step_args* args, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement aid (no counterpart in the reference): a matrix-core-only launch whose rate is the MFMA issue peak of

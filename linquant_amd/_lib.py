@@ -17,7 +17,7 @@ BINDING_PATH = ROOT / "_binding.so"
 _NATIVE_ENTRIES = ("lq_zoo_simple_gla", "lq_zoo_simple_gla_workspace_bytes", "lq_zoo_chunk_forward",
                    "lq_zoo_chunk_forward_workspace_bytes", "lq_zoo_rotate_qkv", "lq_split_rotate_quant_xBC", "lq_ssd_combined",
                    "lq_ssd_combined_workspace_bytes", "lq_abi_version", "lq_args_size")
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 LQ_DT_F16, LQ_DT_F32, LQ_DT_I8, LQ_DT_BF16 = 0, 1, 2, 3
 
@@ -62,7 +62,8 @@ FUNCTIONS = tuple(_funcs)
 # entry points whose first argument is another function's args struct
 _SHARED_ARGS = {"lq_ssd_combined_static": "lq_ssd_combined_args", "lq_ssd_combined_workspace_bytes": "lq_ssd_combined_args",
                 "lq_zoo_simple_gla_workspace_bytes": "lq_zoo_simple_gla_args",
-                "lq_zoo_chunk_forward_workspace_bytes": "lq_zoo_chunk_forward_args"}
+                "lq_zoo_chunk_forward_workspace_bytes": "lq_zoo_chunk_forward_args",
+                "lq_ssm_prompt_workspace_bytes": "lq_ssm_prompt_args"}
 
 _lib = None
 
@@ -147,6 +148,23 @@ def aligned(t, nbytes=16):
     """``t`` itself when its first byte sits on an ``nbytes`` boundary (or it is None), else a fresh copy: kernels that
     fetch small parameter tables as whole 16-byte pieces need this, and a view into a larger tensor need not have it."""
     return t if t is None or t.data_ptr() % nbytes == 0 else t.clone()
+
+
+def rows16(t):
+    """``t`` itself when it has unit stride along its last axis and every other row of it starts on a 16-byte boundary, else a
+    fresh dense copy: kernels that fetch activations as 16-byte pieces take any strides of that kind."""
+    n = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % n == 0 for s in t.stride()[:-1]):
+        return t
+    t = t.contiguous()
+    return aligned(t)
+
+
+def same_device(first, *others):
+    """Every tensor (or None) on the device of the first: a kernel must not be handed another device's memory."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"expected every tensor on {first.device}, got one on {t.device}")
 
 
 def current_stream(device):

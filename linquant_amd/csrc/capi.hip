@@ -38,6 +38,13 @@ extern "C" int lq_args_size(const char* name) {
   LQ_SIZE_OF(lq_zoo_rotate_qkv_args);
   LQ_SIZE_OF(lq_zoo_rotate_quant_args);
   LQ_SIZE_OF(lq_ssd_combined_args);
+  LQ_SIZE_OF(lq_quantize_rows_args);
+  LQ_SIZE_OF(lq_int8_matmul_args);
+  LQ_SIZE_OF(lq_residual_rmsnorm_args);
+  LQ_SIZE_OF(lq_conv1d_prompt_args);
+  LQ_SIZE_OF(lq_conv1d_step_args);
+  LQ_SIZE_OF(lq_ssm_prompt_args);
+  LQ_SIZE_OF(lq_ssm_step_args);
   LQ_SIZE_OF(lq_probe_mfma_args);
   return LQ_ERR_SHAPE;
 }
