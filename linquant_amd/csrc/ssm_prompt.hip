@@ -1,9 +1,28 @@
 // lq_ssm_prompt: the selective state space scan over prompts of any lengths, from and into an fp32 state.
-//   S = exp(d A) S + d x B^T,  y = S C + D x,  d = softplus(dt + bias)
-// Token by token, eight lanes to a row of the state, as in the single-token kernel.
+//   S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T,   y_t = S_t C_t + D x_t
+// in chunks of 64 tokens.  With c_t = sum of d A up to t inside a chunk and S the state in front of it,
+//   y_t = exp(c_t) S C_t + sum_{s <= t} exp(c_t - c_s) d_s (C_t . B_s) x_s + D x_t
+//   S'  = exp(c_63) S + sum_s exp(c_63 - c_s) d_s x_s B_s^T
+// which are products of matrices.  Three kernels:
+//   operands   per chunk and group: C, B^T and C B^T in the order in which the matrix instruction takes them, shared by the group's
+//              heads; per chunk and head: d, c (in powers of two) and exp(c_63 - c_s) d_s
+//   states     per segment of a prompt: the state at its end if it starts from zero, and what it multiplies an earlier one by;
+//   join       walks the segments: the state in front of each.  (states and join: only where prompts are cut into segments, because
+//              prompts times heads are too few for 256 compute units)
+//   chunks     walks a segment chunk by chunk, the state in registers
+//
+// Precision.  Activations are exact in bf16 (bf16: one piece, fp16: two of 8 and 3 bits).  What is formed in fp32 on the way (weights of
+// C B^T, the state, weighted x) enters a product in two bf16 pieces, 16 bits, with fp32 sums: an output in 16 bits is its rounding, a
+// state is within about 1e-6 of one computed in fp32.  bf16 has the range of fp32, so no size of activations or weights overflows a piece.
+#include <algorithm>
+
 #include "serve_common.h"
 
 namespace {
+
+constexpr int Q = 64;             // tokens of a chunk
+constexpr int kCB = 6 * 2 * 1024;  // bytes of a chunk's C B^T: six operands (32 rows, 16 tokens) on and below the diagonal, fp32
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct PromptParams {
   const uint16_t* x;
@@ -27,70 +46,558 @@ struct PromptParams {
   const int32_t* slots;
   const int32_t* starts;
   int num_slots, nseq, seqlen, tokens, H, P, G, N;
+  // workspace
+  char* tables;     // [unit][group] operands
+  float* steps;     // [unit][head][d, c, w][64]
+  float* seg_state;  // [segment][H][P][N], or NULL: prompts are not cut
+  float* seg_decay;  // [segment][H]
+  int units, segs, seg_chunks, per_group, waves;
 };
 
-template <typename T, int KN>
-__global__ __launch_bounds__(256) void ssm_prompt_kernel(PromptParams p) {
-  const int h = blockIdx.x, seq = blockIdx.y;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 7;
-  const int row = blockIdx.z * 32 + 8 * wave + (lane >> 3);
-  int t0 = 0, L = p.seqlen;
-  int64_t ob = (int64_t)seq * p.seqlen;
-  const int64_t b = p.starts ? 0 : seq;
-  if (p.starts) {
-    t0 = p.starts[seq];
-    const int t1 = p.starts[seq + 1];
-    L = t0 < 0 || t1 > p.tokens || t1 < t0 ? 0 : t1 - t0;
-    ob = t0;
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void glb_void;
+
+LQ_DEV v16f mfma(lq_v4i a, lq_v4i b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sv_v8bf, a), __builtin_bit_cast(sv_v8bf, b), c, 0, 0, 0);
+}
+LQ_DEV uint32_t pack_bf16(float a, float b) {
+  const sv_v2bf v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+// eight fp32 values as two bf16 pieces each: v = hi + lo up to 2^-17 of it
+LQ_DEV void split(const float (&v)[8], lq_v4i& hi, lq_v4i& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t h = pack_bf16(v[2 * i], v[2 * i + 1]);
+    hi[i] = (int)h;
+    lo[i] = (int)pack_bf16(v[2 * i] - __uint_as_float(h << 16), v[2 * i + 1] - __uint_as_float(h & 0xffff0000u));
   }
-  if (row >= p.P || L == 0) return;
-  const int slot = p.state || p.slots ? sv_slot(p.slots, seq, p.num_slots) : kSlotPad;
-  const bool keeps = p.state && slot >= 0;
-  const int g = h / (p.H / p.G);
-  float* S = keeps ? p.state + slot * p.ss_s + ((int64_t)h * p.P + row) * p.N : nullptr;
-  lq_v4f s[KN];
+}
+LQ_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The order of a contraction of 64: step ks, half hh of the wave and slot i stand for entry 16 ks + 8 (i / 4) + 4 hh + i % 4, in which the
+// accumulators of v_mfma_f32_32x32x16 hold their rows.  The state's and C B^T's accumulators then are operands as they are.
+LQ_DEV int entry(int ks, int hh, int i) { return 16 * ks + 8 * (i >> 2) + 4 * hh + (i & 3); }
+
+// sizes of a (chunk, group)'s operands.  NT: tiles of 32 state columns, PC: pieces of an activation
+template <int NT, int PC>
+struct Table {
+  static constexpr int kC = NT * PC * 4 * 1024, kB = NT * PC * 4 * 1024, kBytes = kCB + kC + kB;
+};
+
+// which unit (chunk) of which sequence
+LQ_DEV Unit unit_of(const PromptParams& p, int u) {
+  if (p.starts) return sv_locate<Q>(p.starts, p.nseq, p.tokens, u);
+  const int per = (p.seqlen + Q - 1) / Q;
+  Unit r;
+  r.seq = u / per, r.index = u - r.seq * per, r.begin = 0, r.end = p.seqlen;
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- operands
+template <typename T, int NT>
+LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint16_t* smem) {
+  constexpr int PC = std::is_same<T, F16>::value ? 2 : 1;
+  constexpr int LD = 32 * NT + 8;  // halves of a row in LDS
+  uint16_t *Bs = smem, *Cs = smem + Q * LD;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const int64_t seq = p.starts ? 0 : u.seq, t0 = u.begin + (int64_t)u.index * Q;
+  const int rem = min(Q, u.end - u.begin - u.index * Q);
+  const uint16_t* Bg = p.B + seq * p.sB_b + t0 * p.sB_l + g * p.sB_g;
+  const uint16_t* Cg = p.C + seq * p.sC_b + t0 * p.sC_l + g * p.sC_g;
 #pragma unroll
-  for (int k = 0; k < KN; ++k) {
-    s[k] = lq_v4f{0.f, 0.f, 0.f, 0.f};
-    if (keeps) s[k] = *(const lq_v4f*)(S + min(32 * k + 4 * sub, p.N - 4));
+  for (int i = 0; i < NT; ++i) {
+    const int pc = tid + 256 * i, t = pc / (4 * NT), n = (pc % (4 * NT)) * 8;
+    const bool in = t < rem && n < p.N;
+    const int tc = min(t, rem - 1), nc = min(n, p.N - 8);
+    const lq_v4i zero = {0, 0, 0, 0};
+    const lq_v4i b = *(const lq_v4i*)(Bg + tc * p.sB_l + nc), c = *(const lq_v4i*)(Cg + tc * p.sC_l + nc);
+    *(lq_v4i*)(Bs + t * LD + n) = in ? b : zero;
+    *(lq_v4i*)(Cs + t * LD + n) = in ? c : zero;
   }
-  const float A = p.A[h], bias = p.dt_bias ? p.dt_bias[h] : 0.0f, D = p.D ? p.D[p.D_has_hdim ? h * p.P + row : h] : 0.0f;
-  for (int i = 0; i < L; ++i) {
-    const int64_t t = t0 + i;
-    const float d = sv_step_size(sv_load(p.dt, b * p.sdt_b + t * p.sdt_l + h * p.sdt_h, p.dt_dtype), bias, p.softplus, p.dt_min, p.dt_max);
-    const float decay = lq_expf(d * A);
-    const float xv = T::to(p.x[b * p.sx_b + t * p.sx_l + h * p.sx_h + row]), dx = d * xv;
-    const uint16_t* Bp = p.B + b * p.sB_b + t * p.sB_l + g * p.sB_g;
-    const uint16_t* Cp = p.C + b * p.sC_b + t * p.sC_l + g * p.sC_g;
-    float y = 0.0f;
+  __syncthreads();
+  char* out = p.tables + ((int64_t)unit * p.G + g) * Table<NT, PC>::kBytes;
+  if (wave < 3) {  // C B^T of rows t (columns of the product) and tokens s (its rows); fp32 sums of exact products
+    const int tt = wave > 0, st = wave > 1;
+    v16f acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < KN; ++k) {
-      const int n = 32 * k + 4 * sub, at = min(n, p.N - 4);
-      const sv_v4u rb = *(const sv_v4u*)(Bp + at), rc = *(const sv_v4u*)(Cp + at);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[k][e] = __builtin_fmaf(dx, T::to(rb[e]), decay * s[k][e]);
-        y += n < p.N ? s[k][e] * T::to(rc[e]) : 0.0f;
-      }
+    for (int k = 0; k < 2 * NT; ++k) {
+      const lq_v4i b = *(const lq_v4i*)(Bs + (32 * st + (lane & 31)) * LD + 16 * k + 8 * hh);
+      const lq_v4i c = *(const lq_v4i*)(Cs + (32 * tt + (lane & 31)) * LD + 16 * k + 8 * hh);
+      if constexpr (PC == 1) acc = mfma(b, c, acc);
+      else acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lq_v8h, b), __builtin_bit_cast(lq_v8h, c), acc, 0, 0, 0);
     }
 #pragma unroll
-    for (int off = 4; off >= 1; off >>= 1) y += __shfl_xor(y, off, 64);
-    y = __builtin_fmaf(D, xv, y);
-    if (slot == kSlotBad) y = __builtin_nanf("");
-    if (sub == 0) p.out[((ob + i) * p.H + h) * p.P + row] = T::from(y);
+    for (int r = 0; r < 4; ++r) {  // operand 2 wave + r / 2, its slots 4 (r % 2) ..
+      const lq_v4f v = {acc[4 * r], acc[4 * r + 1], acc[4 * r + 2], acc[4 * r + 3]};
+      *(lq_v4f*)(out + ((2 * wave + (r >> 1)) * 2 + (r & 1)) * 1024 + lane * 16) = v;
+    }
   }
-  if (keeps) {
+  // eight activations as an operand's pieces
+  auto put = [&](const uint16_t (&v)[8], int op, char* at, int pieces_apart) {
+    lq_v4i hi;
+    if constexpr (PC == 1) {
 #pragma unroll
-    for (int k = 0; k < KN; ++k)
-      if (32 * k + 4 * sub < p.N) *(lq_v4f*)(S + 32 * k + 4 * sub) = s[k];
+      for (int i = 0; i < 4; ++i) hi[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = T::to(v[i]);
+      lq_v4i lo;
+      split(f, hi, lo);
+      *(lq_v4i*)(at + (pieces_apart + op) * 1024 + lane * 16) = lo;
+    }
+    *(lq_v4i*)(at + op * 1024 + lane * 16) = hi;
+  };
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {  // C: operand (tt, nt, q): rows t, state columns 32 nt + entry(q, ..)
+    const int op = wave + 4 * i, tt = op / (2 * NT), k = op % (2 * NT);
+    uint16_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = Cs[(32 * tt + (lane & 31)) * LD + entry(k, hh, e)];
+    put(v, op, out + kCB, 4 * NT);
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {  // B^T: operand (nt, ks): rows n, tokens entry(ks, ..)
+    const int op = wave + 4 * i, nt = op >> 2, ks = op & 3;
+    uint16_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = Bs[entry(ks, hh, e) * LD + 32 * nt + (lane & 31)];
+    put(v, op, out + kCB + Table<NT, PC>::kC, 4 * NT);
+  }
+}
+
+constexpr int kHeads = 16;  // heads of a workgroup that forms step sizes
+
+LQ_DEV void step_sizes(const PromptParams& p, const Unit& u, int unit, int h0, float* tile) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t seq = p.starts ? 0 : u.seq, t0 = u.begin + (int64_t)u.index * Q;
+  const int rem = min(Q, u.end - u.begin - u.index * Q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = (tid + 256 * i) / kHeads, h = (tid + 256 * i) % kHeads;
+    tile[t * (kHeads + 1) + h] = sv_load(p.dt, seq * p.sdt_b + (t0 + min(t, rem - 1)) * p.sdt_l + min(h0 + h, p.H - 1) * p.sdt_h, p.dt_dtype);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kHeads / 4; ++i) {
+    const int h = h0 + wave * (kHeads / 4) + i;
+    if (h >= p.H) break;
+    float d = sv_step_size(tile[lane * (kHeads + 1) + h - h0], p.dt_bias ? p.dt_bias[h] : 0.0f, p.softplus, p.dt_min, p.dt_max);
+    if (lane >= rem) d = 0.0f;  // a token behind the prompt changes nothing
+    // one factor of 2^-160 is zero in 32 bits, and sums of larger ones would cost the tokens behind them their last bits
+    const float e = d * (p.A[h] * kLog2e), a = e < -160.0f ? -160.0f : e;
+    float c = a, r = __shfl_down(a, 1, 64);  // sums up to and with this token; behind it (summed from the end: near it they are small and exact)
+    if (lane == 63) r = 0.0f;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const float up = __shfl_up(c, off, 64), down = __shfl_down(r, off, 64);
+      if (lane >= off) c += up;
+      if (lane + off < 64) r += down;
+    }
+    float* o = p.steps + ((int64_t)unit * p.H + h) * (3 * Q) + lane;
+    o[0] = d, o[Q] = c, o[2 * Q] = exp2_fast(r) * d;
+  }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(256) void ssm_operands_kernel(PromptParams p) {
+  __shared__ __align__(16) uint16_t smem[2 * Q * (32 * NT + 8)];
+  const int unit = blockIdx.x;
+  const Unit u = unit_of(p, unit);
+  if (u.seq < 0) return;
+  if ((int)blockIdx.y < p.G) operands<T, NT>(p, u, unit, blockIdx.y, smem);
+  else step_sizes(p, u, unit, ((int)blockIdx.y - p.G) * kHeads, (float*)smem);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- segments
+struct Segment {
+  int seq, begin, len;      // tokens of the sequence
+  int chunk0, chunks, unit0;  // its first chunk in the sequence, how many, and the unit of the first
+  bool first, last;
+};
+LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
+  Segment r;
+  r.seq = -1;
+  if (!p.starts) {
+    const int nc = (p.seqlen + Q - 1) / Q, per = (nc + p.seg_chunks - 1) / p.seg_chunks;
+    r.seq = sg / per;
+    r.begin = 0, r.len = p.seqlen, r.chunk0 = (sg - r.seq * per) * p.seg_chunks, r.unit0 = r.seq * nc + r.chunk0;
+    r.chunks = min(p.seg_chunks, nc - r.chunk0);
+    r.first = r.chunk0 == 0, r.last = r.chunk0 + r.chunks == nc;
+    return r;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0, ubefore = 0;
+  for (int s0 = 0; s0 < p.nseq; s0 += 64) {
+    const int s = s0 + lane;
+    int b = 0, e = 0;
+    if (s < p.nseq) b = p.starts[s], e = p.starts[s + 1];
+    if (b < 0 || e > p.tokens || e < b) b = e = 0;
+    const int units = (int)(((uint32_t)(e - b) + (Q - 1)) / Q), n = (units + p.seg_chunks - 1) / p.seg_chunks;
+    int sum = n, usum = units;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(sum, off, 64), v = __shfl_up(usum, off, 64);
+      sum += lane >= off ? o : 0, usum += lane >= off ? v : 0;
+    }
+    const int total = __shfl(sum, 63, 64);
+    if (sg < before + total) {
+      const int l = __builtin_ctzll(__ballot(sg < before + sum));
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      const int nc = of(units);
+      r.seq = s0 + l, r.begin = of(b), r.len = of(e) - r.begin;
+      r.chunk0 = (sg - before - of(sum - n)) * p.seg_chunks;
+      r.unit0 = ubefore + of(usum - units) + r.chunk0;
+      r.chunks = min(p.seg_chunks, nc - r.chunk0);
+      r.first = r.chunk0 == 0, r.last = r.chunk0 + r.chunks == nc;
+      return r;
+    }
+    before += total, ubefore += __shfl(usum, 63, 64);
+  }
+  return r;
+}
+
+// Which segment and which part of a group's heads a workgroup of the flat grid has.  Workgroups go round the 8 XCDs in launch order; the
+// parts of one segment read the same operands, so they are dealt to one XCD.
+LQ_DEV void place(const PromptParams& p, int& sg, int& part) {
+  const int parts = p.G * p.per_group, x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  sg = (j / parts) * 8 + x, part = j % parts;
+}
+
+// A wave has 32 channels of one head: the state's N x 32 as accumulators (rows n, columns the channels).  STATES: only the segment's
+// state and decay.
+template <typename T, int NT, bool STATES, int NBUF>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void ssm_chunks_kernel(PromptParams p) {
+  constexpr int PC = std::is_same<T, F16>::value ? 2 : 1;
+  using Tab = Table<NT, PC>;
+  constexpr int kSkip = STATES ? kCB + Tab::kC : 0, kLoad = Tab::kBytes - kSkip;  // bytes of a chunk's operands that are needed
+  __shared__ __align__(16) char buf[NBUF][kLoad];
+  __shared__ __align__(16) float tok[8][4 * Q];  // each wave's d, c, w, exp2(c)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
+  int sg, part;
+  place(p, sg, part);
+  if (sg >= p.segs) return;
+  const Segment s = segment_of(p, sg);
+  if (s.seq < 0 || (STATES && s.last)) return;
+  const int g = part / p.per_group, pblocks = (p.P + 31) >> 5, hpg = p.H / p.G;
+  const int block = (part - g * p.per_group) * p.waves + wave;
+  const bool live = block < hpg * pblocks;  // a wave without channels only helps to fetch the operands
+  const int h = g * hpg + (live ? block / pblocks : 0), ch = (live ? block % pblocks : 0) * 32 + col;
+  const bool chan = live && ch < p.P;
+  const int chc = min(ch, p.P - 1);
+  const int slot = p.state || p.slots ? sv_slot(p.slots, s.seq, p.num_slots) : kSlotPad;
+  const bool keeps = p.state && slot >= 0;
+  const int64_t row0 = (p.starts ? s.begin : (int64_t)s.seq * p.seqlen);  // of the dense output
+  const uint16_t* xs = p.x + (p.starts ? s.begin * p.sx_l : s.seq * p.sx_b) + h * p.sx_h;
+  uint16_t* os = p.out + (row0 * p.H + h) * p.P;
+  const int64_t ostride = (int64_t)p.H * p.P;
+
+  v16f S[NT];
+  const int64_t sbase = ((int64_t)h * p.P + chc) * p.N;
+  {
+    const float* src = STATES ? nullptr : (p.seg_state && !(s.first && s.last)) ? p.seg_state + (int64_t)sg * p.H * p.P * p.N + sbase : keeps ? p.state + slot * p.ss_s + sbase : nullptr;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = 32 * nt + 8 * j + 4 * hh;
+        lq_v4f v = {0.f, 0.f, 0.f, 0.f};
+        if (src && n < p.N) v = *(const lq_v4f*)(src + n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[nt][4 * j + e] = v[e];
+      }
+  }
+  const float Dv = !STATES && p.D ? p.D[p.D_has_hdim ? h * p.P + chc : h] : 0.0f;
+  const float bad = slot == kSlotBad ? __builtin_nanf("") : 0.0f;
+
+  const char* tab = p.tables + ((int64_t)s.unit0 * p.G + g) * Tab::kBytes + kSkip;
+  auto fetch = [&](int c, int b) {
+    const char* src = tab + (int64_t)c * p.G * Tab::kBytes;
+    for (int k = wave; k < kLoad / 1024; k += p.waves)
+      __builtin_amdgcn_global_load_lds((glb_void*)(src + k * 1024 + lane * 16), (lds_void*)(buf[b] + k * 1024), 16, 0, 0);
+  };
+  // the chunk's tokens and step sizes of this wave's head: requested a chunk ahead, taken in before that chunk's stores are made, which
+  // then need not be waited for
+  uint16_t xr[4][8];
+  lq_v4i xp[4];
+  float dv, cv, wv;
+  auto take = [&] {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xp[ks][i] = (int)(xr[ks][2 * i] | (uint32_t)xr[ks][2 * i + 1] << 16);
+    asm volatile("s_waitcnt vmcnt(0)" : "+v"(xp[0]), "+v"(xp[1]), "+v"(xp[2]), "+v"(xp[3]), "+v"(dv), "+v"(cv), "+v"(wv)::"memory");
+  };
+  auto request = [&](int c) {
+    const int rem = s.len - (s.chunk0 + c) * Q;
+    const uint16_t* xc = xs + (int64_t)(s.chunk0 + c) * Q * p.sx_l;
+    if (rem >= Q) {
+      const uint32_t at = (uint32_t)(4 * hh) * (uint32_t)p.sx_l + (uint32_t)chc;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xr[ks][i] = (xc + entry(ks, 0, i) * p.sx_l)[at];
+    } else {  // tokens behind the prompt: the last one again, at weight zero
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xr[ks][i] = xc[(uint32_t)min(entry(ks, hh, i), rem - 1) * (uint32_t)p.sx_l + (uint32_t)chc];
+    }
+    const float* o = p.steps + ((int64_t)(s.unit0 + c) * p.H + h) * (3 * Q) + lane;
+    dv = o[0], cv = o[Q], wv = o[2 * Q];
+  };
+
+  if (NBUF == 2) fetch(0, 0);
+  if (live) request(0), take();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  float decay = 0.0f;
+  float* my = tok[wave];
+  for (int c = 0; c < s.chunks; ++c) {
+    const int b = NBUF == 2 ? c & 1 : 0;
+    if constexpr (NBUF == 1) {
+      fetch(c, 0);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    // every wave's share of this chunk's operands is there (waited for below, or above), and none reads the last chunk's any more
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool more = c + 1 < s.chunks;
+    if (NBUF == 2 && more) fetch(c + 1, b ^ 1);
+    if (live) {
+      my[lane] = dv, my[Q + lane] = cv, my[2 * Q + lane] = wv, my[3 * Q + lane] = exp2_fast(cv);
+      decay += __shfl(cv, 63, 64);
+      // x as pieces
+      float xf[4][8];
+      lq_v4i xh[4], xl[4];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xf[ks][i] = T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1))));
+        if constexpr (PC == 1) xh[ks] = xp[ks];
+        else split(xf[ks], xh[ks], xl[ks]);
+      }
+      if (more) request(c + 1);
+      const lq_v4i* op = (const lq_v4i*)buf[b] + lane;
+      const lq_v4i* opB = op + (STATES ? 0 : (kCB + Tab::kC) / 16);
+      v16f Y[2];
+      if constexpr (!STATES) {  // exp(c_t) S C_t
+        const lq_v4i* opC = op + kCB / 16;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) Y[tt][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2 * NT; ++k) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i];
+          lq_v4i sh, sl;
+          split(v, sh, sl);
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            const lq_v4i chi = opC[(tt * 2 * NT + k) * 64];
+            Y[tt] = mfma(chi, sh, Y[tt]);
+            Y[tt] = mfma(chi, sl, Y[tt]);
+            if constexpr (PC == 2) Y[tt] = mfma(opC[(4 * NT + tt * 2 * NT + k) * 64], sh, Y[tt]);
+          }
+        }
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const lq_v4f e = *(const lq_v4f*)(my + 3 * Q + 32 * tt + 8 * j + 4 * hh);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Y[tt][4 * j + i] *= e[i];
+          }
+      }
+      // the state behind the chunk
+      {
+        const float all = my[3 * Q + 63];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[nt][e] *= all;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const lq_v4f w = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = w[i] * xf[ks][4 * j + i];
+          }
+          lq_v4i wh, wl;
+          split(v, wh, wl);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const lq_v4i bh = opB[(4 * nt + ks) * 64];
+            S[nt] = mfma(bh, wh, S[nt]);
+            S[nt] = mfma(bh, wl, S[nt]);
+            if constexpr (PC == 2) S[nt] = mfma(opB[(4 * NT + 4 * nt + ks) * 64], wh, S[nt]);
+          }
+        }
+      }
+      if constexpr (!STATES) {
+        // An activation that is no number must not reach the tokens in front of it, which the product below multiplies by zero: the state,
+        // which all of the chunk's tokens reach, tells.  Then such tokens are left out and every output from them on is NaN.
+        int from = Q;
+        if (__ballot(S[0][0] != S[0][0])) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (!(__builtin_fabsf(xf[ks][i]) < __builtin_inff())) {
+                from = min(from, entry(ks, hh, i));
+                xf[ks][i] = 0.0f;
+              }
+          from = min(from, __shfl_xor(from, 32, 64));
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) split(xf[ks], xh[ks], xl[ks]);
+        }
+        const lq_v4f* cb = (const lq_v4f*)buf[b] + lane;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const float ct = my[Q + 32 * tt + col];
+          const int t = 32 * tt + col;
+#pragma unroll
+          for (int ks = 0; ks < 2 * tt + 2; ++ks) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const lq_v4f f = cb[((tt * 2 + ks) * 2 + j) * 64];
+              const lq_v4f cs = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh), ds = *(const lq_v4f*)(my + 16 * ks + 8 * j + 4 * hh);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float m = f[i] * exp2_fast(ct - cs[i]) * ds[i];
+                v[4 * j + i] = ks >= 2 * tt && entry(ks, hh, 4 * j + i) > t ? 0.0f : m;
+              }
+            }
+            lq_v4i mh, ml;
+            split(v, mh, ml);
+            Y[tt] = mfma(mh, xh[ks], Y[tt]);
+            Y[tt] = mfma(ml, xh[ks], Y[tt]);
+            if constexpr (PC == 2) Y[tt] = mfma(mh, xl[ks], Y[tt]);
+          }
+        }
+        const int rem = s.len - (s.chunk0 + c) * Q;
+        uint16_t* oc = os + (int64_t)(s.chunk0 + c) * Q * ostride;
+        uint16_t yo[2][16];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int ks = 2 * tt + (r >> 3), t = entry(ks, hh, r & 7);
+            float y = __builtin_fmaf(Dv, xf[ks][r & 7], Y[tt][r]) + bad;
+            if (t >= from) y = __builtin_nanf("");
+            yo[tt][r] = T::from(y);
+          }
+        if (more) take();
+        const uint32_t at = (uint32_t)(4 * hh) * (uint32_t)ostride + (uint32_t)ch;
+        if (rem >= Q && p.P % 32 == 0) {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) (oc + entry(2 * tt + (r >> 3), 0, r & 7) * ostride)[at] = yo[tt][r];
+        } else if (chan) {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (entry(2 * tt + (r >> 3), hh, r & 7) < rem) (oc + entry(2 * tt + (r >> 3), 0, r & 7) * ostride)[at] = yo[tt][r];
+        }
+      } else if (more) {
+        take();
+      }
+    }
+    if (!live) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // its share of the next chunk's operands
+    if (NBUF == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  float* dst = STATES ? p.seg_state + (int64_t)sg * p.H * p.P * p.N + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
+  if (dst && chan) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = 32 * nt + 8 * j + 4 * hh;
+        const lq_v4f v = {S[nt][4 * j], S[nt][4 * j + 1], S[nt][4 * j + 2], S[nt][4 * j + 3]};
+        if (n < p.N) *(lq_v4f*)(dst + n) = v;
+      }
+  }
+  if (STATES && live && lane == 0 && block % pblocks == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(decay);
+}
+
+// The state in front of each segment, in the place of what the segment adds to one (the last one's is not read).  A workgroup has 1024
+// entries of one head's state and finds the sequence's segments as the other kernels do.
+__global__ __launch_bounds__(256) void ssm_join_kernel(PromptParams p) {
+  const int64_t per = (int64_t)p.P * p.N;
+  const int h = blockIdx.y, at = (blockIdx.z * 256 + threadIdx.x) * 4;
+  const Segment s0 = segment_of(p, blockIdx.x);
+  if (s0.seq < 0 || !s0.first || s0.last) return;  // a sequence's first segment walks the others
+  if (at >= per) return;
+  const int slot = p.state || p.slots ? sv_slot(p.slots, s0.seq, p.num_slots) : kSlotPad;
+  lq_v4f v = {0.f, 0.f, 0.f, 0.f};
+  if (p.state && slot >= 0) v = *(const lq_v4f*)(p.state + slot * p.ss_s + h * per + at);
+  const int nc = (s0.len + Q - 1) / Q, n = (nc + p.seg_chunks - 1) / p.seg_chunks;
+  for (int i = 0; i < n; ++i) {
+    const int64_t sg = blockIdx.x + i;
+    lq_v4f* o = (lq_v4f*)(p.seg_state + (sg * p.H + h) * per + at);
+    const lq_v4f add = *o;
+    *o = v;
+    if (i + 1 < n) {
+      const float d = p.seg_decay[sg * p.H + h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d, v[e], add[e]);
+    }
   }
 }
 
 int check_dims(const lq_ssm_prompt_args* a) {
-  if (a->nseq <= 0 || a->nseq > 65535 || a->nheads <= 0 || a->ngroups <= 0 || a->nheads % a->ngroups != 0) return LQ_ERR_SHAPE;
+  if (a->nseq <= 0 || a->nheads <= 0 || a->ngroups <= 0 || a->nheads % a->ngroups != 0) return LQ_ERR_SHAPE;
   if (a->headdim <= 0 || a->headdim % 8 != 0 || a->dstate <= 0 || a->dstate % 8 != 0 || a->dstate > 256) return LQ_ERR_SHAPE;
-  if (a->seq_starts ? a->tokens <= 0 : a->seqlen <= 0) return LQ_ERR_SHAPE;
+  if ((a->seq_starts ? a->tokens <= 0 : a->seqlen <= 0) || !sv_act(a->dtype)) return LQ_ERR_SHAPE;
+  if ((int64_t)a->nheads * a->headdim > 1 << 23 || a->ngroups + a->nheads / kHeads > 65000) return LQ_ERR_SHAPE;
   return LQ_OK;
+}
+
+int table_bytes(const lq_ssm_prompt_args* a) {
+  const int nt = a->dstate <= 32 ? 1 : a->dstate <= 64 ? 2 : a->dstate <= 128 ? 4 : 8, pc = a->dtype == LQ_DT_F16 ? 2 : 1;
+  return kCB + nt * pc * 8 * 1024;
+}
+
+// How a call is cut: the units, the waves of a workgroup, the chunks of a segment.
+struct Plan {
+  int64_t units, segs, tables, steps, states, decays, bytes;
+  int waves, per_group, seg_chunks, cut;
+};
+bool plan(const lq_ssm_prompt_args* a, Plan& r) {
+  const int64_t nseq = a->nseq, most = ((int64_t)(a->seq_starts ? a->tokens : a->seqlen) + Q - 1) / Q;  // chunks of the longest prompt there can be
+  r.units = a->seq_starts ? (int64_t)a->tokens / Q + nseq : nseq * most;
+  const int64_t blocks = (int64_t)(a->nheads / a->ngroups) * ((a->headdim + 31) / 32);
+  r.waves = blocks > 4 ? 8 : 4;
+  r.per_group = (int)((blocks + r.waves - 1) / r.waves);
+  const int64_t parts = (int64_t)a->ngroups * r.per_group;
+  // Chunk steps in a row that the chip takes for segments of n chunks, one workgroup to a compute unit, 256 at a time; cut prompts
+  // need their states first (about half a step each) and the join.
+  const int64_t even = std::max<int64_t>(1, r.units / nseq);  // a packed call's prompts are taken to be of one length
+  int64_t best = -1;
+  r.seg_chunks = (int)most, r.cut = 0;
+  for (int64_t k = 1; k <= 64 && (k == 1 || even / k >= 2); ++k) {
+    const int64_t n = (even + k - 1) / k, wgs = nseq * ((even + n - 1) / n) * parts;
+    const int64_t steps = (wgs + 255) / 256 * n;
+    const int64_t cost = k == 1 ? steps * 2 : steps * 3 + 12;
+    if (best < 0 || cost < best) best = cost, r.seg_chunks = k == 1 ? (int)most : (int)n, r.cut = k > 1;
+  }
+  const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
+  r.segs = a->seq_starts ? std::min<int64_t>(r.units / r.seg_chunks + nseq, r.units) : nseq * per;
+  if (!r.cut) r.segs = nseq;
+  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  r.tables = 0;
+  r.steps = up(r.units * a->ngroups * table_bytes(a));
+  r.states = r.steps + up(r.units * a->nheads * (3 * Q * 4));
+  r.decays = r.states + (r.cut ? up(r.segs * a->nheads * a->headdim * a->dstate * 4) : 0);
+  r.bytes = r.decays + (r.cut ? up(r.segs * a->nheads * 4) : 0);
+  return r.units <= 0x7fffffff && (r.segs + 7) / 8 * 8 * parts <= 0x7fffffff;
 }
 
 }  // namespace
@@ -98,28 +605,48 @@ int check_dims(const lq_ssm_prompt_args* a) {
 extern "C" int lq_ssm_prompt_workspace_bytes(const lq_ssm_prompt_args* a, int64_t* bytes) {
   if (!a || !bytes) return LQ_ERR_NULL;
   const int rc = check_dims(a);
-  if (rc == LQ_OK) *bytes = 0;
-  return rc;
+  Plan pl;
+  if (rc != LQ_OK) return rc;
+  if (!plan(a, pl)) return LQ_ERR_SHAPE;
+  *bytes = pl.bytes;
+  return LQ_OK;
 }
 
 extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
-  if (!a || !a->x || !a->dt || !a->A || !a->B || !a->C || !a->out) return LQ_ERR_NULL;
+  if (!a || !a->x || !a->dt || !a->A || !a->B || !a->C || !a->out || !a->workspace) return LQ_ERR_NULL;
   const int rc = check_dims(a);
   if (rc != LQ_OK) return rc;
-  if (!sv_act(a->dtype) || !sv_float(a->dt_dtype) || (a->state && a->num_slots <= 0)) return LQ_ERR_SHAPE;
+  if (!sv_float(a->dt_dtype) || (a->state && a->num_slots <= 0)) return LQ_ERR_SHAPE;
   for (const int64_t s : {a->B_stride_b, a->B_stride_l, a->B_stride_g, a->C_stride_b, a->C_stride_l, a->C_stride_g})
     if (s % 8 != 0) return LQ_ERR_SHAPE;
-  if (a->x_stride_b % 8 != 0 || a->x_stride_l % 8 != 0 || a->x_stride_h % 8 != 0) return LQ_ERR_SHAPE;
-  if (!sv_al(a->x, 16) || !sv_al(a->B, 16) || !sv_al(a->C, 16) || !sv_al(a->out, 16) || !sv_al(a->state, 16) || a->state_stride_s % 4 != 0 ||
+  if (a->x_stride_l < 0 || a->x_stride_l >= 1 << 24) return LQ_ERR_SHAPE;  // a chunk's rows are reached by 32-bit offsets
+  if (!sv_al(a->x, 2) || !sv_al(a->B, 16) || !sv_al(a->C, 16) || !sv_al(a->out, 2) || !sv_al(a->state, 16) || a->state_stride_s % 4 != 0 ||
       !sv_al(a->dt, sv_size(a->dt_dtype)) || !sv_al(a->A, 4) || !sv_al(a->D, 4) || !sv_al(a->dt_bias, 4) || !sv_al(a->slots, 4) || !sv_al(a->seq_starts, 4))
     return LQ_ERR_SHAPE;
+  Plan pl;
+  if (!plan(a, pl) || a->workspace_bytes < pl.bytes || !sv_al(a->workspace, 256)) return LQ_ERR_SHAPE;
+  char* ws = (char*)a->workspace;
   PromptParams p = {(const uint16_t*)a->x, a->x_stride_b, a->x_stride_l, a->x_stride_h, a->dt, a->dt_stride_b, a->dt_stride_l, a->dt_stride_h, a->dt_dtype, a->A,
                     (const uint16_t*)a->B, a->B_stride_b, a->B_stride_l, a->B_stride_g, (const uint16_t*)a->C, a->C_stride_b, a->C_stride_l, a->C_stride_g,
                     a->D, a->D_has_hdim, a->dt_bias, a->dt_softplus, a->dt_min, a->dt_max, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots,
-                    a->seq_starts, a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->headdim, a->ngroups, a->dstate};
-  const dim3 grid((unsigned)a->nheads, (unsigned)a->nseq, (unsigned)((a->headdim + 31) / 32));
+                    a->seq_starts, a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->headdim, a->ngroups, a->dstate,
+                    ws + pl.tables, (float*)(ws + pl.steps), pl.cut ? (float*)(ws + pl.states) : nullptr, pl.cut ? (float*)(ws + pl.decays) : nullptr,
+                    (int)pl.units, (int)pl.segs, pl.seg_chunks, pl.per_group, pl.waves};
+  const dim3 pre((unsigned)pl.units, (unsigned)(a->ngroups + (a->nheads + kHeads - 1) / kHeads));
+  const dim3 grid((unsigned)((pl.segs + 7) / 8 * 8 * a->ngroups * pl.per_group)), threads(64 * pl.waves);
+  const int64_t per = (int64_t)a->headdim * a->dstate;
+  const dim3 join((unsigned)pl.segs, (unsigned)a->nheads, (unsigned)((per + 1023) / 1024));
+  if (join.y > 65535 || join.z > 65535) return LQ_ERR_SHAPE;
   auto go = [&](auto t, auto k) {
-    hipLaunchKernelGGL((ssm_prompt_kernel<decltype(t), decltype(k)::value>), grid, dim3(256), 0, stream, p);
+    using T = decltype(t);
+    constexpr int NT = decltype(k)::value, PC = std::is_same<T, F16>::value ? 2 : 1;
+    constexpr int NBUF = 2 * Table<NT, PC>::kBytes + 8 * 4 * Q * 4 <= 160 * 1024 ? 2 : 1;
+    hipLaunchKernelGGL((ssm_operands_kernel<T, NT>), pre, dim3(256), 0, stream, p);
+    if (pl.cut) {
+      hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, true, 2>), grid, threads, 0, stream, p);
+      hipLaunchKernelGGL(ssm_join_kernel, join, dim3(256), 0, stream, p);
+    }
+    hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, false, NBUF>), grid, threads, 0, stream, p);
     return lq_check_launch();
   };
   auto with = [&](auto t) {

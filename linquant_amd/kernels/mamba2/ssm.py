@@ -78,7 +78,9 @@ def ssm_prompt(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_lim
         _check_state(state, x, N)
         num_slots = state.shape[0]
     slots = check_slots(slots, n, num_slots, x) if state is not None or slots is not None else None
-    x, B, C = (_lib.rows16(t) for t in (x, B, C))
+    B, C = _lib.rows16(B), _lib.rows16(C)
+    if x.stride(-1) != 1 or x.stride(-3) >= 1 << 24:
+        x = x.contiguous()
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if n == 0 or L + T == 0 or H == 0 or P == 0:
         return out
@@ -105,7 +107,8 @@ def ssm_step(state, x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, d
     n, H, P = x.shape
     _check_state(state, x, B.shape[-1])
     slots = check_slots(slots, n, state.shape[0], x)
-    x, B, C = (_lib.rows16(t) for t in (x, B, C))
+    B, C = _lib.rows16(B), _lib.rows16(C)
+    x = x if x.stride(2) == 1 else x.contiguous()
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if n and H and P:
         _lib.call("lq_ssm_step", x.device, x=_lib.ptr(x), x_stride_b=x.stride(0), x_stride_h=x.stride(1), dt=_lib.ptr(dt), dt_stride_b=dt.stride(0),

@@ -114,7 +114,7 @@ def test_ssm_refusals():
      [dict(dim=12), dict(width=5), dict(x_stride=12), dict(batch=0), dict(num_slots=0), dict(state_stride_w=4)]),
     ("lq_ssm_prompt", dict(x=1, dt=1, A=1, B=1, C=1, out=1, nseq=1, seqlen=4, nheads=2, headdim=8, ngroups=1, dstate=16, workspace=1,
                            workspace_bytes=1 << 40),
-     [dict(headdim=12), dict(dstate=264), dict(dstate=12), dict(ngroups=4), dict(seqlen=0), dict(B_stride_l=4), dict(x_stride_l=4),
+     [dict(headdim=12), dict(dstate=264), dict(dstate=12), dict(ngroups=4), dict(seqlen=0), dict(B_stride_l=4), dict(x_stride_l=1 << 24), dict(workspace_bytes=0),
       dict(state=1, num_slots=0), dict(dtype=1), dict(dt_dtype=2)]),
     ("lq_ssm_step", dict(x=1, dt=1, A=1, B=1, C=1, out=1, state=1, num_slots=1, batch=1, nheads=2, headdim=8, ngroups=1, dstate=16),
      [dict(headdim=12), dict(dstate=264), dict(ngroups=4), dict(batch=0), dict(batch=65536), dict(state_stride_s=2), dict(num_slots=0)]),
