@@ -11,9 +11,10 @@
 //              prompts times heads are too few for 256 compute units)
 //   chunks     walks a segment chunk by chunk, the state in registers
 //
-// Precision.  Activations are exact in bf16 (bf16: one piece, fp16: two of 8 and 3 bits).  What is formed in fp32 on the way (weights of
-// C B^T, the state, weighted x) enters a product in two bf16 pieces, 16 bits, with fp32 sums: an output in 16 bits is its rounding, a
-// state is within about 1e-6 of one computed in fp32.  bf16 has the range of fp32, so no size of activations or weights overflows a piece.
+// Precision.  Activations enter the matrix products as they are.  What is formed in fp32 on the way (weights of C B^T, the state,
+// weighted x) enters as two pieces of the activations' type, with fp32 sums.  bf16: 16 bits, and the range of fp32.  fp16: 22 bits, after a
+// multiplication by a power of two that brings the largest of what is multiplied (a channel's state and weighted x; C B^T of the chunk)
+// below 2^14, so no size of activations overflows a piece, and what is 2^28 times smaller than that largest starts to lose bits.
 #include <algorithm>
 
 #include "serve_common.h"
@@ -48,7 +49,8 @@ struct PromptParams {
   int num_slots, nseq, seqlen, tokens, H, P, G, N;
   // workspace
   char* tables;     // [unit][group] operands
-  float* steps;     // [unit][head][d, c, w][64]
+  float* steps;     // [unit][head][d, c, w, most][64]
+  float* rows;      // [unit][group][64]: largest |C B^T| of each row
   float* seg_state;  // [segment][H][P][N], or NULL: prompts are not cut
   float* seg_decay;  // [segment][H]
   int units, segs, seg_chunks, per_group, waves;
@@ -58,21 +60,60 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void glb_void;
 
+template <typename T>
 LQ_DEV v16f mfma(lq_v4i a, lq_v4i b, v16f c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sv_v8bf, a), __builtin_bit_cast(sv_v8bf, b), c, 0, 0, 0);
+  if constexpr (std::is_same<T, F16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lq_v8h, a), __builtin_bit_cast(lq_v8h, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sv_v8bf, a), __builtin_bit_cast(sv_v8bf, b), c, 0, 0, 0);
 }
 LQ_DEV uint32_t pack_bf16(float a, float b) {
   const sv_v2bf v = {(__bf16)a, (__bf16)b};
   return __builtin_bit_cast(uint32_t, v);
 }
-// eight fp32 values as two bf16 pieces each: v = hi + lo up to 2^-17 of it
-LQ_DEV void split(const float (&v)[8], lq_v4i& hi, lq_v4i& lo) {
+// eight products a b as two pieces each: fp16, hi = RN(a b), lo = RN(a b - hi), one mixed-precision instruction a piece; bf16 likewise
+// from the rounded product
+template <typename T>
+LQ_DEV void split(const float (&a)[8], const float (&b)[8], lq_v4i& hi, lq_v4i& lo) {
+  if constexpr (std::is_same<T, F16>::value) {
+    lq_v8h h, l;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t h = pack_bf16(v[2 * i], v[2 * i + 1]);
-    hi[i] = (int)h;
-    lo[i] = (int)pack_bf16(v[2 * i] - __uint_as_float(h << 16), v[2 * i + 1] - __uint_as_float(h & 0xffff0000u));
+    for (int i = 0; i < 8; ++i) {
+      h[i] = (_Float16)__builtin_fmaf(a[i], b[i], 0.0f);
+      l[i] = (_Float16)__builtin_fmaf(a[i], b[i], -(float)h[i]);
+    }
+    hi = __builtin_bit_cast(lq_v4i, h), lo = __builtin_bit_cast(lq_v4i, l);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = a[2 * i] * b[2 * i], v = a[2 * i + 1] * b[2 * i + 1];
+      const uint32_t h = pack_bf16(u, v);
+      hi[i] = (int)h;
+      lo[i] = (int)pack_bf16(u - __uint_as_float(h << 16), v - __uint_as_float(h & 0xffff0000u));
+    }
   }
+}
+// The power of two that brings m below 2^14 (and not below 2^13), within 2^-100 and 2^24: the quotient of two is a number, and pieces of
+// a value times 2^24 are 2^-49 of the activations' unit apart, less than matters to a sum that becomes fp16.
+LQ_DEV float scale_for(float m) {
+  const int e = (int)((__float_as_uint(m) >> 23) & 255u) - 127;  // (0: -127)
+  return __uint_as_float((uint32_t)(127 + min(max(13 - e, -100), 24)) << 23);
+}
+// the largest of a wave's non-negative values, by lane permutations of the vector unit; the same for the whole wave
+LQ_DEV float wave_top(float v) {
+#define LQ_TOP(CTRL) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)))
+  LQ_TOP(0xB1);   // lanes 1 0 3 2
+  LQ_TOP(0x4E);   // lanes 2 3 0 1
+  LQ_TOP(0x141);  // mirrored halves of a row of 16
+  LQ_TOP(0x140);  // mirrored rows
+  LQ_TOP(0x142);  // the last lane of a row to the next row
+  LQ_TOP(0x143);  // the last lane of the first half of the wave to the second
+#undef LQ_TOP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+LQ_DEV float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+// |v|, or 0 for what is no number and must not set a scale
+LQ_DEV float finite_size(float v) {
+  const float a = __builtin_fabsf(v);
+  return a < __builtin_inff() ? a : 0.0f;
 }
 LQ_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -80,10 +121,10 @@ LQ_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // accumulators of v_mfma_f32_32x32x16 hold their rows.  The state's and C B^T's accumulators then are operands as they are.
 LQ_DEV int entry(int ks, int hh, int i) { return 16 * ks + 8 * (i >> 2) + 4 * hh + (i & 3); }
 
-// sizes of a (chunk, group)'s operands.  NT: tiles of 32 state columns, PC: pieces of an activation
-template <int NT, int PC>
+// sizes of a (chunk, group)'s operands.  NT: tiles of 32 state columns
+template <int NT>
 struct Table {
-  static constexpr int kC = NT * PC * 4 * 1024, kB = NT * PC * 4 * 1024, kBytes = kCB + kC + kB;
+  static constexpr int kC = NT * 4 * 1024, kB = NT * 4 * 1024, kBytes = kCB + kC + kB;
 };
 
 // which unit (chunk) of which sequence
@@ -97,8 +138,7 @@ LQ_DEV Unit unit_of(const PromptParams& p, int u) {
 
 // ---------------------------------------------------------------------------------------------------------------- operands
 template <typename T, int NT>
-LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint16_t* smem) {
-  constexpr int PC = std::is_same<T, F16>::value ? 2 : 1;
+LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint16_t* smem, float* top) {
   constexpr int LD = 32 * NT + 8;  // halves of a row in LDS
   uint16_t *Bs = smem, *Cs = smem + Q * LD;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
@@ -117,7 +157,7 @@ LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint
     *(lq_v4i*)(Cs + t * LD + n) = in ? c : zero;
   }
   __syncthreads();
-  char* out = p.tables + ((int64_t)unit * p.G + g) * Table<NT, PC>::kBytes;
+  char* out = p.tables + ((int64_t)unit * p.G + g) * Table<NT>::kBytes;
   if (wave < 3) {  // C B^T of rows t (columns of the product) and tokens s (its rows); fp32 sums of exact products
     const int tt = wave > 0, st = wave > 1;
     v16f acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -125,30 +165,29 @@ LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint
     for (int k = 0; k < 2 * NT; ++k) {
       const lq_v4i b = *(const lq_v4i*)(Bs + (32 * st + (lane & 31)) * LD + 16 * k + 8 * hh);
       const lq_v4i c = *(const lq_v4i*)(Cs + (32 * tt + (lane & 31)) * LD + 16 * k + 8 * hh);
-      if constexpr (PC == 1) acc = mfma(b, c, acc);
-      else acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lq_v8h, b), __builtin_bit_cast(lq_v8h, c), acc, 0, 0, 0);
+      acc = mfma<T>(b, c, acc);
     }
+    float m = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {  // nothing above the diagonal
+      if (tt == st && entry(r >> 3, hh, r & 7) > (lane & 31)) acc[r] = 0.0f;
+      m = fmaxf(m, finite_size(acc[r]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    if (lane < 32) top[32 * wave + lane] = m;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {  // operand 2 wave + r / 2, its slots 4 (r % 2) ..
       const lq_v4f v = {acc[4 * r], acc[4 * r + 1], acc[4 * r + 2], acc[4 * r + 3]};
       *(lq_v4f*)(out + ((2 * wave + (r >> 1)) * 2 + (r & 1)) * 1024 + lane * 16) = v;
     }
   }
-  // eight activations as an operand's pieces
-  auto put = [&](const uint16_t (&v)[8], int op, char* at, int pieces_apart) {
-    lq_v4i hi;
-    if constexpr (PC == 1) {
+  __syncthreads();
+  if (tid < Q) p.rows[((int64_t)unit * p.G + g) * Q + tid] = tid < 32 ? top[tid] : fmaxf(top[tid], top[tid + 32]);
+  auto put = [&](const uint16_t (&v)[8], char* at) {
+    lq_v4i o;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) hi[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
-    } else {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = T::to(v[i]);
-      lq_v4i lo;
-      split(f, hi, lo);
-      *(lq_v4i*)(at + (pieces_apart + op) * 1024 + lane * 16) = lo;
-    }
-    *(lq_v4i*)(at + op * 1024 + lane * 16) = hi;
+    for (int i = 0; i < 4; ++i) o[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
+    *(lq_v4i*)(at + lane * 16) = o;
   };
 #pragma unroll
   for (int i = 0; i < NT; ++i) {  // C: operand (tt, nt, q): rows t, state columns 32 nt + entry(q, ..)
@@ -156,7 +195,7 @@ LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint
     uint16_t v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = Cs[(32 * tt + (lane & 31)) * LD + entry(k, hh, e)];
-    put(v, op, out + kCB, 4 * NT);
+    put(v, out + kCB + op * 1024);
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {  // B^T: operand (nt, ks): rows n, tokens entry(ks, ..)
@@ -164,7 +203,7 @@ LQ_DEV void operands(const PromptParams& p, const Unit& u, int unit, int g, uint
     uint16_t v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = Bs[entry(ks, hh, e) * LD + 32 * nt + (lane & 31)];
-    put(v, op, out + kCB + Table<NT, PC>::kC, 4 * NT);
+    put(v, out + kCB + Table<NT>::kC + op * 1024);
   }
 }
 
@@ -196,18 +235,26 @@ LQ_DEV void step_sizes(const PromptParams& p, const Unit& u, int unit, int h0, f
       if (lane >= off) c += up;
       if (lane + off < 64) r += down;
     }
-    float* o = p.steps + ((int64_t)unit * p.H + h) * (3 * Q) + lane;
-    o[0] = d, o[Q] = c, o[2 * Q] = exp2_fast(r) * d;
+    // the largest weight exp(c_t - c_s) |d_s| of a row of C B^T: a running maximum of log2 |d_s| - c_s
+    float most = __builtin_amdgcn_logf(finite_size(d)) - c;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const float up = __shfl_up(most, off, 64);
+      if (lane >= off) most = fmaxf(most, up);
+    }
+    float* o = p.steps + ((int64_t)unit * p.H + h) * (4 * Q) + lane;
+    o[0] = d, o[Q] = c, o[2 * Q] = exp2_fast(r) * d, o[3 * Q] = exp2_fast(most + c);
   }
 }
 
 template <typename T, int NT>
 __global__ __launch_bounds__(256) void ssm_operands_kernel(PromptParams p) {
   __shared__ __align__(16) uint16_t smem[2 * Q * (32 * NT + 8)];
+  __shared__ float top[96];
   const int unit = blockIdx.x;
   const Unit u = unit_of(p, unit);
   if (u.seq < 0) return;
-  if ((int)blockIdx.y < p.G) operands<T, NT>(p, u, unit, blockIdx.y, smem);
+  if ((int)blockIdx.y < p.G) operands<T, NT>(p, u, unit, blockIdx.y, smem, top);
   else step_sizes(p, u, unit, ((int)blockIdx.y - p.G) * kHeads, (float*)smem);
 }
 
@@ -260,21 +307,24 @@ LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
 }
 
 // Which segment and which part of a group's heads a workgroup of the flat grid has.  Workgroups go round the 8 XCDs in launch order; the
-// parts of one segment read the same operands, so they are dealt to one XCD.
+// parts of one segment read the same operands, so each XCD gets adjacent ones.  (A whole number of segments to an XCD instead left four of
+// the eight with twice the others' work.)
 LQ_DEV void place(const PromptParams& p, int& sg, int& part) {
-  const int parts = p.G * p.per_group, x = blockIdx.x & 7, j = blockIdx.x >> 3;
-  sg = (j / parts) * 8 + x, part = j % parts;
+  const int parts = p.G * p.per_group, i = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  sg = i / parts, part = i - sg * parts;
 }
 
 // A wave has 32 channels of one head: the state's N x 32 as accumulators (rows n, columns the channels).  STATES: only the segment's
-// state and decay.
+// state and decay.  A workgroup's waves share the chunk's operands in LDS, fetched there a chunk ahead (NBUF = 2) as they lie in memory; each
+// wave's x comes the same way, 64 tokens x 32 channels, into one of two places, and its y leaves through the same place.
 template <typename T, int NT, bool STATES, int NBUF>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void ssm_chunks_kernel(PromptParams p) {
-  constexpr int PC = std::is_same<T, F16>::value ? 2 : 1;
-  using Tab = Table<NT, PC>;
+  constexpr bool kHalf = std::is_same<T, F16>::value;
+  using Tab = Table<NT>;
   constexpr int kSkip = STATES ? kCB + Tab::kC : 0, kLoad = Tab::kBytes - kSkip;  // bytes of a chunk's operands that are needed
   __shared__ __align__(16) char buf[NBUF][kLoad];
-  __shared__ __align__(16) float tok[8][4 * Q];  // each wave's d, c, w, exp2(c)
+  __shared__ __align__(16) uint16_t xbuf[2][8][Q * 32];
+  __shared__ __align__(16) float tok[8][4 * Q];  // each wave's d, c, w, exp2(c) (fp16: scaled)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   int sg, part;
   place(p, sg, part);
@@ -284,14 +334,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int g = part / p.per_group, pblocks = (p.P + 31) >> 5, hpg = p.H / p.G;
   const int block = (part - g * p.per_group) * p.waves + wave;
   const bool live = block < hpg * pblocks;  // a wave without channels only helps to fetch the operands
-  const int h = g * hpg + (live ? block / pblocks : 0), ch = (live ? block % pblocks : 0) * 32 + col;
-  const bool chan = live && ch < p.P;
+  const int h = g * hpg + (live ? block / pblocks : 0), ch0 = (live ? block % pblocks : 0) * 32, ch = ch0 + col;
   const int chc = min(ch, p.P - 1);
   const int slot = p.state || p.slots ? sv_slot(p.slots, s.seq, p.num_slots) : kSlotPad;
   const bool keeps = p.state && slot >= 0;
   const int64_t row0 = (p.starts ? s.begin : (int64_t)s.seq * p.seqlen);  // of the dense output
-  const uint16_t* xs = p.x + (p.starts ? s.begin * p.sx_l : s.seq * p.sx_b) + h * p.sx_h;
-  uint16_t* os = p.out + (row0 * p.H + h) * p.P;
+  const uint16_t* xs = p.x + (p.starts ? s.begin * p.sx_l : s.seq * p.sx_b) + h * p.sx_h + ch0;
+  uint16_t* os = p.out + (row0 * p.H + h) * p.P + ch0;
   const int64_t ostride = (int64_t)p.H * p.P;
 
   v16f S[NT];
@@ -309,74 +358,83 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int e = 0; e < 4; ++e) S[nt][4 * j + e] = v[e];
       }
   }
+  float unit_S = 1.0f;  // fp16: S holds the state times this power of two
   const float Dv = !STATES && p.D ? p.D[p.D_has_hdim ? h * p.P + chc : h] : 0.0f;
-  const float bad = slot == kSlotBad ? __builtin_nanf("") : 0.0f;
+  const bool bad = slot == kSlotBad;
 
+  // what a chunk needs, requested while the one in front of it is worked on.  x: four rows of 16 bytes a lane, 8 channels each; tokens
+  // behind the prompt read its last one again (at weight zero), channels behind the head its last eight.
   const char* tab = p.tables + ((int64_t)s.unit0 * p.G + g) * Tab::kBytes + kSkip;
+  const uint32_t xcol = (uint32_t)min(8 * (lane & 3), p.P - 8 - ch0);
+  float dv = 0.f, cv = 0.f, wv = 0.f, mv = 0.f, rv = 0.f;
   auto fetch = [&](int c, int b) {
     const char* src = tab + (int64_t)c * p.G * Tab::kBytes;
     for (int k = wave; k < kLoad / 1024; k += p.waves)
       __builtin_amdgcn_global_load_lds((glb_void*)(src + k * 1024 + lane * 16), (lds_void*)(buf[b] + k * 1024), 16, 0, 0);
   };
-  // the chunk's tokens and step sizes of this wave's head: requested a chunk ahead, taken in before that chunk's stores are made, which
-  // then need not be waited for
-  uint16_t xr[4][8];
-  lq_v4i xp[4];
-  float dv, cv, wv;
-  auto take = [&] {
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xp[ks][i] = (int)(xr[ks][2 * i] | (uint32_t)xr[ks][2 * i + 1] << 16);
-    asm volatile("s_waitcnt vmcnt(0)" : "+v"(xp[0]), "+v"(xp[1]), "+v"(xp[2]), "+v"(xp[3]), "+v"(dv), "+v"(cv), "+v"(wv)::"memory");
-  };
   auto request = [&](int c) {
     const int rem = s.len - (s.chunk0 + c) * Q;
     const uint16_t* xc = xs + (int64_t)(s.chunk0 + c) * Q * p.sx_l;
-    if (rem >= Q) {
-      const uint32_t at = (uint32_t)(4 * hh) * (uint32_t)p.sx_l + (uint32_t)chc;
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) xr[ks][i] = (xc + entry(ks, 0, i) * p.sx_l)[at];
-    } else {  // tokens behind the prompt: the last one again, at weight zero
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) xr[ks][i] = xc[(uint32_t)min(entry(ks, hh, i), rem - 1) * (uint32_t)p.sx_l + (uint32_t)chc];
-    }
-    const float* o = p.steps + ((int64_t)(s.unit0 + c) * p.H + h) * (3 * Q) + lane;
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_global_load_lds((glb_void*)(xc + (uint32_t)min(16 * i + (lane >> 2), rem - 1) * (uint32_t)p.sx_l + xcol),
+                                       (lds_void*)(&xbuf[c & 1][wave][16 * 32 * i]), 16, 0, 0);
+    const float* o = p.steps + ((int64_t)(s.unit0 + c) * p.H + h) * (4 * Q) + lane;
     dv = o[0], cv = o[Q], wv = o[2 * Q];
+    if (kHalf && !STATES) mv = o[3 * Q], rv = p.rows[((int64_t)(s.unit0 + c) * p.G + g) * Q + lane];
   };
+  auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" : "+v"(dv), "+v"(cv), "+v"(wv), "+v"(mv), "+v"(rv)::"memory"); };
 
   if (NBUF == 2) fetch(0, 0);
-  if (live) request(0), take();
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (live) request(0);
+  arrived();
   float decay = 0.0f;
   float* my = tok[wave];
   for (int c = 0; c < s.chunks; ++c) {
     const int b = NBUF == 2 ? c & 1 : 0;
     if constexpr (NBUF == 1) {
       fetch(c, 0);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      arrived();
     }
     // every wave's share of this chunk's operands is there (waited for below, or above), and none reads the last chunk's any more
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const bool more = c + 1 < s.chunks;
     if (NBUF == 2 && more) fetch(c + 1, b ^ 1);
     if (live) {
-      my[lane] = dv, my[Q + lane] = cv, my[2 * Q + lane] = wv, my[3 * Q + lane] = exp2_fast(cv);
-      decay += __shfl(cv, 63, 64);
-      // x as pieces
-      float xf[4][8];
-      lq_v4i xh[4], xl[4];
+      uint16_t* xw = xbuf[c & 1][wave];
+      lq_v4i xp[4];  // this lane's channel, tokens in the order of an operand
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
+      for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xf[ks][i] = T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1))));
-        if constexpr (PC == 1) xh[ks] = xp[ks];
-        else split(xf[ks], xh[ks], xl[ks]);
+        for (int i = 0; i < 4; ++i)
+          xp[ks][i] = (int)(xw[entry(ks, hh, 2 * i) * 32 + col] | (uint32_t)xw[entry(ks, hh, 2 * i + 1) * 32 + col] << 16);
+      auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
+      const float last = lane63(cv), all = exp2_fast(last);
+      decay += last;
+      float rescale = 1.0f, row = 1.0f;
+      if constexpr (kHalf) {
+        // the wave's new unit: its state and what the chunk adds, each below 2^14 of it
+        float m = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(S[nt][e]));
+        uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            typedef uint16_t v2u __attribute__((ext_vector_type(2)));
+            top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
+          }
+        const float mx = T::to((uint16_t)max(top & 0xffffu, top >> 16));
+        const float u = scale_for(wave_top(fmaxf(finite_size(m) * (1.0f / unit_S), finite_size(mx) * wave_top(finite_size(wv)))));
+        rescale = u / unit_S;
+        unit_S = u;
+        if (!STATES) row = scale_for(rv * mv);  // brings the token's row of weighted C B^T below 2^14
       }
+      const float ui = kHalf ? 1.0f / unit_S : 1.0f;
+      my[lane] = dv, my[Q + lane] = cv, my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
       if (more) request(c + 1);
       const lq_v4i* op = (const lq_v4i*)buf[b] + lane;
       const lq_v4i* opB = op + (STATES ? 0 : (kCB + Tab::kC) / 16);
@@ -389,17 +447,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int e = 0; e < 16; ++e) Y[tt][e] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 2 * NT; ++k) {
-          float v[8];
+          float v[8], r[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i];
+          for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i], r[i] = rescale;
           lq_v4i sh, sl;
-          split(v, sh, sl);
+          split<T>(v, r, sh, sl);
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
-            const lq_v4i chi = opC[(tt * 2 * NT + k) * 64];
-            Y[tt] = mfma(chi, sh, Y[tt]);
-            Y[tt] = mfma(chi, sl, Y[tt]);
-            if constexpr (PC == 2) Y[tt] = mfma(opC[(4 * NT + tt * 2 * NT + k) * 64], sh, Y[tt]);
+            const lq_v4i cc = opC[(tt * 2 * NT + k) * 64];
+            Y[tt] = mfma<T>(cc, sh, Y[tt]);
+            Y[tt] = mfma<T>(cc, sl, Y[tt]);
           }
         }
 #pragma unroll
@@ -413,118 +470,125 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       // the state behind the chunk
       {
-        const float all = my[3 * Q + 63];
+        const float f = kHalf ? all * rescale : all;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[nt][e] *= all;
+          for (int e = 0; e < 16; ++e) S[nt][e] *= f;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          float v[8];
+          float w[8], xv[8];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const lq_v4f w = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
+            const lq_v4f v = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * j + i] = w[i] * xf[ks][4 * j + i];
+            for (int i = 0; i < 4; ++i) w[4 * j + i] = v[i], xv[4 * j + i] = x(ks, 4 * j + i);
           }
           lq_v4i wh, wl;
-          split(v, wh, wl);
+          split<T>(w, xv, wh, wl);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const lq_v4i bh = opB[(4 * nt + ks) * 64];
-            S[nt] = mfma(bh, wh, S[nt]);
-            S[nt] = mfma(bh, wl, S[nt]);
-            if constexpr (PC == 2) S[nt] = mfma(opB[(4 * NT + 4 * nt + ks) * 64], wh, S[nt]);
+            const lq_v4i bb = opB[(4 * nt + ks) * 64];
+            S[nt] = mfma<T>(bb, wh, S[nt]);
+            S[nt] = mfma<T>(bb, wl, S[nt]);
           }
         }
       }
       if constexpr (!STATES) {
         // An activation that is no number must not reach the tokens in front of it, which the product below multiplies by zero: the state,
         // which all of the chunk's tokens reach, tells.  Then such tokens are left out and every output from them on is NaN.
-        int from = Q;
-        if (__ballot(S[0][0] != S[0][0])) {
+        const bool odd = bad || __ballot(S[0][0] != S[0][0]) != 0;
+        int from = bad ? 0 : Q;
+        if (odd) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (!(__builtin_fabsf(xf[ks][i]) < __builtin_inff())) {
+              if (!(__builtin_fabsf(x(ks, i)) < __builtin_inff())) {
                 from = min(from, entry(ks, hh, i));
-                xf[ks][i] = 0.0f;
+                xp[ks][i >> 1] &= i & 1 ? 0xffff : 0xffff0000;
               }
           from = min(from, __shfl_xor(from, 32, 64));
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) split(xf[ks], xh[ks], xl[ks]);
         }
         const lq_v4f* cb = (const lq_v4f*)buf[b] + lane;
+        if (kHalf) my[2 * Q + lane] = 1.0f / row;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
-          const float ct = my[Q + 32 * tt + col];
-          const int t = 32 * tt + col;
+          float ct = my[Q + 32 * tt + col];
+          if (kHalf) ct += (float)(127 - (int)(__float_as_uint(my[2 * Q + 32 * tt + col]) >> 23));  // (a power of two times the row)
 #pragma unroll
           for (int ks = 0; ks < 2 * tt + 2; ++ks) {
-            float v[8];
+            float f[8], a[8];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const lq_v4f f = cb[((tt * 2 + ks) * 2 + j) * 64];
+              const lq_v4f v = cb[((tt * 2 + ks) * 2 + j) * 64];
               const lq_v4f cs = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh), ds = *(const lq_v4f*)(my + 16 * ks + 8 * j + 4 * hh);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float m = f[i] * exp2_fast(ct - cs[i]) * ds[i];
-                v[4 * j + i] = ks >= 2 * tt && entry(ks, hh, 4 * j + i) > t ? 0.0f : m;
+              for (int i = 0; i < 4; ++i) {  // (above the diagonal C B^T is stored as zero)
+                const float m = exp2_fast(ct - cs[i]) * ds[i];
+                f[4 * j + i] = v[i], a[4 * j + i] = ks >= 2 * tt && entry(ks - 2 * tt, hh, 4 * j + i) > col ? 0.0f : m;
               }
             }
             lq_v4i mh, ml;
-            split(v, mh, ml);
-            Y[tt] = mfma(mh, xh[ks], Y[tt]);
-            Y[tt] = mfma(ml, xh[ks], Y[tt]);
-            if constexpr (PC == 2) Y[tt] = mfma(mh, xl[ks], Y[tt]);
+            split<T>(f, a, mh, ml);
+            Y[tt] = mfma<T>(mh, xp[ks], Y[tt]);
+            Y[tt] = mfma<T>(ml, xp[ks], Y[tt]);
           }
         }
+        if (odd) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (entry(ks, hh, i) >= from) Y[ks >> 1][8 * (ks & 1) + i] = __builtin_nanf("");
+        }
+        // out through the place of x (the wave's own, read above): [token][channel], then 16 bytes a lane
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            lq_v4f ri;
+            if (kHalf) ri = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = Y[ks >> 1][8 * (ks & 1) + 4 * j + i], xi = x(ks, 4 * j + i);
+              xw[entry(ks, hh, 4 * j + i) * 32 + col] = T::from(kHalf ? __builtin_fmaf(v, ri[i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
+            }
+          }
+        lq_v4i yo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) yo[i] = *(const lq_v4i*)(xw + 16 * 32 * i + lane * 8);
         const int rem = s.len - (s.chunk0 + c) * Q;
         uint16_t* oc = os + (int64_t)(s.chunk0 + c) * Q * ostride;
-        uint16_t yo[2][16];
+        arrived();  // what is on its way for the next chunk: the stores below are not waited for
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int ks = 2 * tt + (r >> 3), t = entry(ks, hh, r & 7);
-            float y = __builtin_fmaf(Dv, xf[ks][r & 7], Y[tt][r]) + bad;
-            if (t >= from) y = __builtin_nanf("");
-            yo[tt][r] = T::from(y);
-          }
-        if (more) take();
-        const uint32_t at = (uint32_t)(4 * hh) * (uint32_t)ostride + (uint32_t)ch;
-        if (rem >= Q && p.P % 32 == 0) {
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) (oc + entry(2 * tt + (r >> 3), 0, r & 7) * ostride)[at] = yo[tt][r];
-        } else if (chan) {
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (entry(2 * tt + (r >> 3), hh, r & 7) < rem) (oc + entry(2 * tt + (r >> 3), 0, r & 7) * ostride)[at] = yo[tt][r];
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * i + (lane >> 2);
+          if (t < rem && ch0 + 8 * (lane & 3) < p.P) *(lq_v4i*)(oc + (uint32_t)t * (uint32_t)ostride + 8 * (lane & 3)) = yo[i];
         }
-      } else if (more) {
-        take();
+      } else {
+        arrived();
       }
+    } else {
+      arrived();  // its share of the next chunk's operands
     }
-    if (!live) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // its share of the next chunk's operands
     if (NBUF == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
   float* dst = STATES ? p.seg_state + (int64_t)sg * p.H * p.P * p.N + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
-  if (dst && chan) {
+  if (dst && live && ch < p.P) {
+    const float ui = kHalf ? 1.0f / unit_S : 1.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int n = 32 * nt + 8 * j + 4 * hh;
-        const lq_v4f v = {S[nt][4 * j], S[nt][4 * j + 1], S[nt][4 * j + 2], S[nt][4 * j + 3]};
+        lq_v4f v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = kHalf ? S[nt][4 * j + e] * ui : S[nt][4 * j + e];
         if (n < p.N) *(lq_v4f*)(dst + n) = v;
       }
   }
-  if (STATES && live && lane == 0 && block % pblocks == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(decay);
+  if (STATES && live && lane == 0 && ch0 == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(decay);
 }
 
 // The state in front of each segment, in the place of what the segment adds to one (the last one's is not read).  A workgroup has 1024
@@ -561,13 +625,12 @@ int check_dims(const lq_ssm_prompt_args* a) {
 }
 
 int table_bytes(const lq_ssm_prompt_args* a) {
-  const int nt = a->dstate <= 32 ? 1 : a->dstate <= 64 ? 2 : a->dstate <= 128 ? 4 : 8, pc = a->dtype == LQ_DT_F16 ? 2 : 1;
-  return kCB + nt * pc * 8 * 1024;
+  return kCB + (a->dstate <= 32 ? 1 : a->dstate <= 64 ? 2 : a->dstate <= 128 ? 4 : 8) * 8 * 1024;
 }
 
 // How a call is cut: the units, the waves of a workgroup, the chunks of a segment.
 struct Plan {
-  int64_t units, segs, tables, steps, states, decays, bytes;
+  int64_t units, segs, tables, steps, rows, states, decays, bytes;
   int waves, per_group, seg_chunks, cut;
 };
 bool plan(const lq_ssm_prompt_args* a, Plan& r) {
@@ -580,12 +643,13 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   // Chunk steps in a row that the chip takes for segments of n chunks, one workgroup to a compute unit, 256 at a time; cut prompts
   // need their states first (about half a step each) and the join.
   const int64_t even = std::max<int64_t>(1, r.units / nseq);  // a packed call's prompts are taken to be of one length
+  // in tenths of a microsecond: a step 35, one of the states' 15, and the segments' states written, joined and read at 3 TB/s
   int64_t best = -1;
   r.seg_chunks = (int)most, r.cut = 0;
   for (int64_t k = 1; k <= 64 && (k == 1 || even / k >= 2); ++k) {
-    const int64_t n = (even + k - 1) / k, wgs = nseq * ((even + n - 1) / n) * parts;
-    const int64_t steps = (wgs + 255) / 256 * n;
-    const int64_t cost = k == 1 ? steps * 2 : steps * 3 + 12;
+    const int64_t n = (even + k - 1) / k, segs = nseq * ((even + n - 1) / n);
+    const int64_t rounds = (segs * parts + 255) / 256, move = segs * a->nheads * a->headdim * a->dstate * 16 / 300000 + 100;
+    const int64_t cost = k == 1 ? rounds * n * 35 : rounds * n * 35 + ((segs - nseq) * parts + 255) / 256 * n * 15 + move;
     if (best < 0 || cost < best) best = cost, r.seg_chunks = k == 1 ? (int)most : (int)n, r.cut = k > 1;
   }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
@@ -594,10 +658,11 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   r.tables = 0;
   r.steps = up(r.units * a->ngroups * table_bytes(a));
-  r.states = r.steps + up(r.units * a->nheads * (3 * Q * 4));
+  r.rows = r.steps + up(r.units * a->nheads * (4 * Q * 4));
+  r.states = r.rows + up(r.units * a->ngroups * (Q * 4));
   r.decays = r.states + (r.cut ? up(r.segs * a->nheads * a->headdim * a->dstate * 4) : 0);
   r.bytes = r.decays + (r.cut ? up(r.segs * a->nheads * 4) : 0);
-  return r.units <= 0x7fffffff && (r.segs + 7) / 8 * 8 * parts <= 0x7fffffff;
+  return r.units <= 0x7fffffff && r.segs * parts <= 0x7ffffff0;
 }
 
 }  // namespace
@@ -620,7 +685,8 @@ extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
   for (const int64_t s : {a->B_stride_b, a->B_stride_l, a->B_stride_g, a->C_stride_b, a->C_stride_l, a->C_stride_g})
     if (s % 8 != 0) return LQ_ERR_SHAPE;
   if (a->x_stride_l < 0 || a->x_stride_l >= 1 << 24) return LQ_ERR_SHAPE;  // a chunk's rows are reached by 32-bit offsets
-  if (!sv_al(a->x, 2) || !sv_al(a->B, 16) || !sv_al(a->C, 16) || !sv_al(a->out, 2) || !sv_al(a->state, 16) || a->state_stride_s % 4 != 0 ||
+  if (a->x_stride_b % 8 != 0 || a->x_stride_l % 8 != 0 || a->x_stride_h % 8 != 0) return LQ_ERR_SHAPE;
+  if (!sv_al(a->x, 16) || !sv_al(a->B, 16) || !sv_al(a->C, 16) || !sv_al(a->out, 16) || !sv_al(a->state, 16) || a->state_stride_s % 4 != 0 ||
       !sv_al(a->dt, sv_size(a->dt_dtype)) || !sv_al(a->A, 4) || !sv_al(a->D, 4) || !sv_al(a->dt_bias, 4) || !sv_al(a->slots, 4) || !sv_al(a->seq_starts, 4))
     return LQ_ERR_SHAPE;
   Plan pl;
@@ -630,17 +696,18 @@ extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
                     (const uint16_t*)a->B, a->B_stride_b, a->B_stride_l, a->B_stride_g, (const uint16_t*)a->C, a->C_stride_b, a->C_stride_l, a->C_stride_g,
                     a->D, a->D_has_hdim, a->dt_bias, a->dt_softplus, a->dt_min, a->dt_max, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots,
                     a->seq_starts, a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->headdim, a->ngroups, a->dstate,
-                    ws + pl.tables, (float*)(ws + pl.steps), pl.cut ? (float*)(ws + pl.states) : nullptr, pl.cut ? (float*)(ws + pl.decays) : nullptr,
+                    ws + pl.tables, (float*)(ws + pl.steps), (float*)(ws + pl.rows), pl.cut ? (float*)(ws + pl.states) : nullptr, pl.cut ? (float*)(ws + pl.decays) : nullptr,
                     (int)pl.units, (int)pl.segs, pl.seg_chunks, pl.per_group, pl.waves};
   const dim3 pre((unsigned)pl.units, (unsigned)(a->ngroups + (a->nheads + kHeads - 1) / kHeads));
-  const dim3 grid((unsigned)((pl.segs + 7) / 8 * 8 * a->ngroups * pl.per_group)), threads(64 * pl.waves);
+  const dim3 grid((unsigned)((pl.segs * a->ngroups * pl.per_group + 7) / 8 * 8)), threads(64 * pl.waves);
   const int64_t per = (int64_t)a->headdim * a->dstate;
   const dim3 join((unsigned)pl.segs, (unsigned)a->nheads, (unsigned)((per + 1023) / 1024));
   if (join.y > 65535 || join.z > 65535) return LQ_ERR_SHAPE;
   auto go = [&](auto t, auto k) {
     using T = decltype(t);
-    constexpr int NT = decltype(k)::value, PC = std::is_same<T, F16>::value ? 2 : 1;
-    constexpr int NBUF = 2 * Table<NT, PC>::kBytes + 8 * 4 * Q * 4 <= 160 * 1024 ? 2 : 1;
+    constexpr int NT = decltype(k)::value;
+    constexpr int kOwn = 2 * 8 * Q * 32 * 2 + 8 * 4 * Q * 4;  // bytes of x and of the step sizes of eight waves
+    constexpr int NBUF = 2 * Table<NT>::kBytes + kOwn <= 160 * 1024 ? 2 : 1;
     hipLaunchKernelGGL((ssm_operands_kernel<T, NT>), pre, dim3(256), 0, stream, p);
     if (pl.cut) {
       hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, true, 2>), grid, threads, 0, stream, p);

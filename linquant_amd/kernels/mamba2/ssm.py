@@ -78,8 +78,8 @@ def ssm_prompt(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_lim
         _check_state(state, x, N)
         num_slots = state.shape[0]
     slots = check_slots(slots, n, num_slots, x) if state is not None or slots is not None else None
-    B, C = _lib.rows16(B), _lib.rows16(C)
-    if x.stride(-1) != 1 or x.stride(-3) >= 1 << 24:
+    x, B, C = (_lib.rows16(t) for t in (x, B, C))
+    if x.stride(-3) >= 1 << 24:
         x = x.contiguous()
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if n == 0 or L + T == 0 or H == 0 or P == 0:
