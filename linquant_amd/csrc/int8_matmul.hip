@@ -1,7 +1,14 @@
 // lq_int8_matmul: out[m,n] = (sum_k a[m,k] b[n,k]) * a_scale[m] * b_scale[n] + bias[n], INT8 in, the sum exact in 32 bits.
 //
-// The matrix instruction is v_mfma_i32_32x32x32_i8, which reaches 4.9 POPS here where the 16x16x64 form reaches 3.0.  Operands: lane l has
-// row l & 31 and the 16 contraction bytes of half l >> 5; the result: column l & 31, rows 8 (r >> 2) + 4 (l >> 5) + (r & 3).
+// Two kernels.  `tiles`: both operands go through LDS in stages of 64 contraction bytes, a ring of them, fetched straight from memory; each
+// wave has whole 32 x 32 tiles of the result.  `rows`: few rows of a (tokens that answer): a workgroup has 16 columns and its waves parts of
+// the contraction, every operand straight to registers, so that the weights stream from memory once.
+//
+// The matrix instruction of `tiles` is v_mfma_i32_32x32x32_i8, which reaches 4.9 POPS here where the 16x16x64 form reaches 3.0.  Operands:
+// lane l has row l & 31 and the 16 contraction bytes of half l >> 5; the result: column l & 31, rows 8 (r >> 2) + 4 (l >> 5) + (r & 3).  b is
+// the operand of the rows, so that a lane holds four adjacent columns of one row of `out`.
+#include <algorithm>
+
 #include "serve_common.h"
 
 namespace {
@@ -19,9 +26,10 @@ struct MatmulParams {
   void* out;
   int64_t out_stride;
   int rows, cols, inner;
+  int vec;  // out's rows can be written 16 bytes at a time
 };
 
-struct O32 {
+struct F32 {
   using type = float;
   static LQ_DEV float from(float f) { return f; }
 };
@@ -30,75 +38,233 @@ struct OutOf {
   using type = uint16_t;
 };
 template <>
-struct OutOf<O32> {
+struct OutOf<F32> {
   using type = float;
 };
 
-constexpr int kTile = 128, kStep = 128;  // rows of either operand in a tile, contraction bytes of a step
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void glb_void;
 
-template <typename O>
-__global__ __launch_bounds__(256) void int8_matmul_kernel(MatmulParams p) {
-  __shared__ __align__(16) int8_t As[kTile * kStep], Bs[kTile * kStep];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  lq_v16i acc[2][2];
+constexpr int kK = 64;  // contraction bytes of a stage
+
+__device__ const lq_v4i zero16[1] = {{0, 0, 0, 0}};  // what a contraction past its end reads
+
+// TM x TN of the result to a workgroup of four waves, 2 x 2; NS stages in the ring.
+// A stage's row has four pieces of 16 bytes, piece c at place c ^ (row / 4) & 3: the 16 lanes that a read serves at once then touch each bank once.
+template <int TM, int TN, int NS, typename O>
+__global__ __launch_bounds__(256) void int8_tiles_kernel(MatmulParams p) {
+  constexpr int MI = TM / 64, NI = TN / 64;      // 32-row tiles of a wave
+  constexpr int PA = TM / 64, PB = TN / 64;      // fetches of a wave and stage: 16 rows each
+  constexpr int kStage = (TM + TN) * kK;
+  constexpr int kOutRow = TN / 2 * (int)sizeof(typename OutOf<O>::type) + 16;  // bytes of a row of a wave's result on its way out
+  constexpr int kLds = std::max(NS * kStage, 4 * 32 * kOutRow + 2 * TN * 4);
+  __shared__ __align__(16) char lds[kLds];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  // Workgroups go round the 8 XCDs in launch order; each XCD takes adjacent tiles of an order in which 32 of them are 8 x 4, so that what its
+  // compute units read at one time is mostly the same and comes from its L2.
+  const int nm = (p.rows + TM - 1) / TM, nn = (p.cols + TN - 1) / TN;
+  int m0, n0;
+  {
+    const int i = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+    if (i >= nm * nn) return;
+    const int band = i / (8 * nn), first = band * 8, high = min(8, nm - first), j = i - band * 8 * nn;
+    m0 = (first + j % high) * TM, n0 = (j / high) * TN;
+  }
+  // fetch: 64 lanes are 16 rows of four pieces
+  const int fr = lane >> 2, fc = (lane & 3) ^ ((lane >> 4) & 3);
+  uint32_t offa[PA], offb[PB];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < PA; ++i) offa[i] = (uint32_t)min(16 * (wave * PA + i) + fr, p.rows - 1 - m0) * (uint32_t)p.a_stride + 16u * fc;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < PB; ++i) offb[i] = (uint32_t)min(16 * (wave * PB + i) + fr, p.cols - 1 - n0) * (uint32_t)p.b_stride + 16u * fc;
+  const int8_t* at = p.a + m0 * p.a_stride;
+  const int8_t* bt = p.b + n0 * p.b_stride;
+  const int ns = (p.inner + kK - 1) / kK;
+  auto fetch = [&](int s) {
+    char* st = lds + (s % NS) * kStage;
+    const int8_t *as = at + s * kK, *bs = bt + s * kK;
+    if ((s + 1) * kK <= p.inner) {
+#pragma unroll
+      for (int i = 0; i < PA; ++i) __builtin_amdgcn_global_load_lds((glb_void*)(as + offa[i]), (lds_void*)(st + (wave * PA + i) * 1024), 16, 0, 0);
+#pragma unroll
+      for (int i = 0; i < PB; ++i) __builtin_amdgcn_global_load_lds((glb_void*)(bs + offb[i]), (lds_void*)(st + TM * kK + (wave * PB + i) * 1024), 16, 0, 0);
+    } else {  // the last stage, cut short: zeros of either operand
+      const bool in = s * kK + 16 * fc < p.inner;
+#pragma unroll
+      for (int i = 0; i < PA; ++i)
+        __builtin_amdgcn_global_load_lds((glb_void*)(in ? (const void*)(as + offa[i]) : (const void*)zero16), (lds_void*)(st + (wave * PA + i) * 1024), 16, 0, 0);
+#pragma unroll
+      for (int i = 0; i < PB; ++i)
+        __builtin_amdgcn_global_load_lds((glb_void*)(in ? (const void*)(bs + offb[i]) : (const void*)zero16), (lds_void*)(st + TM * kK + (wave * PB + i) * 1024), 16, 0, 0);
+    }
+  };
+  const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
+  const int r0 = (lane & 31) * kK, x = (lane >> 2) & 3;
+  auto read = [&](int s, int k, lq_v4i (&fa)[MI], lq_v4i (&fb)[NI]) {
+    const char* st = lds + (s % NS) * kStage + r0 + (((2 * k + hh) ^ x) * 16);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa[i] = *(const lq_v4i*)(st + (wm + 32 * i) * kK);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) fb[j] = *(const lq_v4i*)(st + (TM + wn + 32 * j) * kK);
+  };
+  lq_v16i acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-  for (int k0 = 0; k0 < p.inner; k0 += kStep) {
-    lq_v4i ra[4], rb[4];
+  auto multiply = [&](const lq_v4i (&fa)[MI], const lq_v4i (&fb)[NI]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pc = tid + 256 * i, r = pc >> 3, k = k0 + (pc & 7) * 16;
-      const int kc = min(k, p.inner - 16);
-      ra[i] = *(const lq_v4i*)(p.a + min(m0 + r, p.rows - 1) * p.a_stride + kc);
-      rb[i] = *(const lq_v4i*)(p.b + min(n0 + r, p.cols - 1) * p.b_stride + kc);
-      if (k >= p.inner) ra[i] = lq_v4i{0, 0, 0, 0};  // (a zero of one operand is enough)
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
+  };
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < ns) fetch(s);
+  lq_v4i fa[2][MI], fb[2][NI];
+  // stage s: its first half's operands are in registers; the second half's are read while that is multiplied, and the next stage's first
+  // while the second is.  Between the two every wave has read all of stage s and its share of stage s + 1 has landed.
+  auto ready = [&](int s) {  // stage s has landed: NS - 2 later ones may be on their way
+    if (s + NS - 2 < ns) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * (PA + PB)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  ready(0);
+  read(0, 0, fa[0], fb[0]);
+  for (int s = 0; s < ns; ++s) {
+    read(s, 1, fa[1], fb[1]);
+    if (s + NS - 1 < ns) fetch(s + NS - 1);  // into the place of stage s - 1
+    multiply(fa[0], fb[0]);
+    if (s + 1 < ns) {
+      ready(s + 1);
+      read(s + 1, 0, fa[0], fb[0]);
     }
-    __syncthreads();
+    multiply(fa[1], fb[1]);
+  }
+  // out: scales and bias of the tile's columns in LDS, then 32 rows of a wave's result at a time through LDS
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  float* sb = (float*)(lds + 4 * 32 * kOutRow);
+  for (int i = tid; i < TN; i += 256) {
+    const int n = min(n0 + i, p.cols - 1);
+    sb[i] = p.b_scale[p.b_scale_cols ? n : 0];
+    sb[TN + i] = p.bias ? sv_load(p.bias, n, p.bias_dtype) : 0.0f;
+  }
+  __syncthreads();
+  using OT = typename OutOf<O>::type;
+  char* my = lds + wave * 32 * kOutRow;
+  OT* out = (OT*)p.out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pc = tid + 256 * i, r = pc >> 3, at = r * kStep + ((pc ^ r) & 7) * 16;
-      *(lq_v4i*)(As + at) = ra[i];
-      *(lq_v4i*)(Bs + at) = rb[i];
-    }
-    __syncthreads();
+  for (int i = 0; i < MI; ++i) {
+    const int m = m0 + wm + 32 * i;
+    const float sa = p.a_scale[p.a_scale_rows ? min(m + (lane & 31), p.rows - 1) : 0];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      lq_v4i fa[2], fb[2];
+    for (int j = 0; j < NI; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = 32 * i + (lane & 31), c = 2 * s + (lane >> 5);
-        fa[i] = *(const lq_v4i*)(As + (wm + r) * kStep + ((c ^ r) & 7) * 16);
-        fb[i] = *(const lq_v4i*)(Bs + (wn + r) * kStep + ((c ^ r) & 7) * 16);
+      for (int q = 0; q < 4; ++q) {
+        const int n = 32 * j + 8 * q + 4 * hh;
+        const lq_v4f s4 = *(const lq_v4f*)(sb + wn + n), b4 = *(const lq_v4f*)(sb + TN + wn + n);
+        typedef OT V4 __attribute__((ext_vector_type(4)));
+        V4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = O::from(__builtin_fmaf((float)acc[i][j][4 * q + e], sa * s4[e], b4[e]));
+        *(V4*)(my + (lane & 31) * kOutRow + n * sizeof(OT)) = o;
       }
+    // (a wave's LDS operations are in order)
+    constexpr int kPieces = TN / 2 * (int)sizeof(OT) / 16, kRows = 64 / kPieces;  // 16-byte pieces of a row, rows written at a time
+    constexpr int kPer = 16 / (int)sizeof(OT);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int r = 0; r < 32; r += kRows) {
+      const int row = r + lane / kPieces, pc = lane % kPieces, n = n0 + wn + pc * kPer;
+      const lq_v4i v = *(const lq_v4i*)(my + row * kOutRow + pc * 16);
+      if (m + row < p.rows) {
+        OT* o = out + (m + row) * p.out_stride + n;
+        if (p.vec && n + kPer <= p.cols) {
+          *(lq_v4i*)o = v;
+        } else {
+          typedef OT VP __attribute__((ext_vector_type(kPer)));
+          const VP e = __builtin_bit_cast(VP, v);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+          for (int k = 0; k < kPer; ++k)
+            if (n + k < p.cols) o[k] = e[k];
+        }
+      }
     }
   }
-  typename OutOf<O>::type* out = (typename OutOf<O>::type*)p.out;
+}
+
+// Few rows of a: 16 MT of them and 16 columns to a workgroup of eight waves, which share the contraction in steps of 64 bytes.
+// v_mfma_i32_16x16x64_i8: lane l has row l & 15 and the 16 bytes of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
+template <int MT, typename O>
+__global__ __launch_bounds__(512) void int8_rows_kernel(MatmulParams p) {
+  __shared__ __align__(16) int sums[8][MT][64][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const int8_t* b = p.b + min(n0 + (lane & 15), p.cols - 1) * p.b_stride;
+  const int8_t* a[MT];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = n0 + wn + 32 * j + (lane & 31);
-    if (n >= p.cols) continue;
-    const float sb = p.b_scale[p.b_scale_cols ? n : 0];
-    const float bias = p.bias ? sv_load(p.bias, n, p.bias_dtype) : 0.0f;
+  for (int i = 0; i < MT; ++i) a[i] = p.a + min(m0 + 16 * i + (lane & 15), p.rows - 1) * p.a_stride;
+  lq_v4i acc[MT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < MT; ++i) acc[i] = lq_v4i{0, 0, 0, 0};
+  const int steps = (p.inner + 63) / 64;
+  constexpr int U = 4;  // steps requested at a time
+  for (int s0 = wave; s0 < steps; s0 += 8 * U) {
+    lq_v4i fb[U], fa[U][MT];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int m = m0 + wm + 32 * i + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-        if (m >= p.rows) continue;
-        const float sa = p.a_scale[p.a_scale_rows ? m : 0];
-        out[m * p.out_stride + n] = O::from(__builtin_fmaf((float)acc[i][j][e], sa * sb, bias));
-      }
+    for (int u = 0; u < U; ++u) {
+      const int k = (s0 + 8 * u) * 64 + (lane >> 4) * 16, kc = min(k, p.inner - 16);
+      fb[u] = *(const lq_v4i*)(b + kc);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fa[u][i] = *(const lq_v4i*)(a[i] + kc);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (s0 + 8 * u) * 64 + (lane >> 4) * 16;
+      if (k >= p.inner) fb[u] = lq_v4i{0, 0, 0, 0};  // (a zero of one operand is enough)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = lq_mfma_i8(fb[u], fa[u][i], acc[i]);
+    }
   }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) *(lq_v4i*)sums[wave][i][lane] = acc[i];
+  __syncthreads();
+  using OT = typename OutOf<O>::type;
+  OT* out = (OT*)p.out;
+  for (int t = threadIdx.x; t < MT * 256; t += 512) {  // adjacent threads: adjacent columns
+    const int i = t >> 8, m = (t >> 4) & 15, n = t & 15;
+    int v = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += sums[w][i][(n >> 2) * 16 + m][n & 3];
+    const int row = m0 + 16 * i + m, col = n0 + n;
+    if (row < p.rows && col < p.cols) {
+      const float s = p.a_scale[p.a_scale_rows ? row : 0] * p.b_scale[p.b_scale_cols ? col : 0];
+      out[row * p.out_stride + col] = O::from(__builtin_fmaf((float)v, s, p.bias ? sv_load(p.bias, col, p.bias_dtype) : 0.0f));
+    }
+  }
+}
+
+template <typename O>
+int launch(const MatmulParams& p, hipStream_t stream) {
+  if (p.rows <= 64) {
+    const int mt = (p.rows + 15) / 16;
+    const dim3 grid((unsigned)((p.cols + 15) / 16), 1);
+    if (mt == 1) hipLaunchKernelGGL((int8_rows_kernel<1, O>), grid, dim3(512), 0, stream, p);
+    else if (mt == 2) hipLaunchKernelGGL((int8_rows_kernel<2, O>), grid, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((int8_rows_kernel<4, O>), grid, dim3(512), 0, stream, p);
+    return lq_check_launch();
+  }
+  auto tiles = [&](auto tm, auto tn, auto ns) {
+    constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, NS = decltype(ns)::value;
+    const int64_t n = (int64_t)((p.rows + TM - 1) / TM) * ((p.cols + TN - 1) / TN);
+    if (n > 0x7ffffff0) return LQ_ERR_SHAPE;
+    hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, NS, O>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256), 0, stream, p);
+    return lq_check_launch();
+  };
+  using std::integral_constant;
+  const int64_t large = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
+  if (large >= 256) return tiles(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{});
 }
 
 }  // namespace
@@ -108,16 +274,12 @@ extern "C" int lq_int8_matmul(const lq_int8_matmul_args* a, hipStream_t stream) 
   if (a->rows <= 0 || a->cols <= 0 || a->inner <= 0 || a->inner % 16 != 0 || a->inner > 131056) return LQ_ERR_SHAPE;
   if (!sv_float(a->out_dtype) || (a->bias && !sv_float(a->bias_dtype))) return LQ_ERR_SHAPE;
   if (a->a_stride % 16 != 0 || a->b_stride % 16 != 0 || !sv_al(a->a, 16) || !sv_al(a->b, 16)) return LQ_ERR_SHAPE;
+  if (a->a_stride < 0 || a->a_stride >= 1 << 23 || a->b_stride < 0 || a->b_stride >= 1 << 23) return LQ_ERR_SHAPE;  // a tile's rows are reached by 32-bit offsets
   if (!sv_al(a->out, sv_size(a->out_dtype)) || (a->bias && !sv_al(a->bias, sv_size(a->bias_dtype))) || !sv_al(a->a_scale, 4) || !sv_al(a->b_scale, 4))
     return LQ_ERR_SHAPE;
+  const int per = 16 / sv_size(a->out_dtype);
   MatmulParams p = {a->a, a->a_stride, a->b, a->b_stride, a->a_scale, a->b_scale, a->a_scale_rows, a->b_scale_cols, a->bias, a->bias_dtype,
-                    a->out, a->out_stride, a->rows, a->cols, a->inner};
-  const dim3 grid((unsigned)((a->cols + kTile - 1) / kTile), (unsigned)((a->rows + kTile - 1) / kTile));
-  if (grid.y > 65535) return LQ_ERR_SHAPE;
-  auto go = [&](auto o) {
-    hipLaunchKernelGGL((int8_matmul_kernel<decltype(o)>), grid, dim3(256), 0, stream, p);
-    return lq_check_launch();
-  };
-  if (a->out_dtype == LQ_DT_F32) return go(O32{});
-  return a->out_dtype == LQ_DT_F16 ? go(F16{}) : go(BF16{});
+                    a->out, a->out_stride, a->rows, a->cols, a->inner, sv_al(a->out, 16) && a->out_stride % per == 0};
+  if (a->out_dtype == LQ_DT_F32) return launch<F32>(p, stream);
+  return a->out_dtype == LQ_DT_F16 ? launch<F16>(p, stream) : launch<BF16>(p, stream);
 }

@@ -51,6 +51,7 @@ def _scale(s, n, device, what):
 def _matmul(a, b, a_scale, b_scale, bias, out):
     """a (M, K), b (N, K) in rows of whole 16-byte pieces; out (M, N) with unit column stride."""
     (M, K), N = a.shape, b.shape[0]
+    a, b = (t if t.stride(0) < 1 << 23 else t.contiguous() for t in (a, b))
     a_scale, per_row = _scale(a_scale, M, a.device, "a_scale")
     b_scale, per_col = _scale(b_scale, N, a.device, "b_scale")
     bias = None if bias is None else bias.contiguous()
