@@ -1,12 +1,18 @@
 // lq_int8_matmul: out[m,n] = (sum_k a[m,k] b[n,k]) * a_scale[m] * b_scale[n] + bias[n], INT8 in, the sum exact in 32 bits.
 //
-// Two kernels.  `tiles`: both operands go through LDS in stages of 64 contraction bytes, a ring of them, fetched straight from memory; each
-// wave has whole 32 x 32 tiles of the result.  `rows`: few rows of a (tokens that answer): a workgroup has 16 columns and its waves parts of
-// the contraction, every operand straight to registers, so that the weights stream from memory once.
+// Two kernels.  `tiles`: both operands go through LDS in stages of 128 contraction bytes, fetched straight from memory, and each wave has
+// whole 32 x 32 tiles of the result.  `rows`: few rows of a (tokens that answer): a workgroup has 16 columns and its waves parts of the
+// contraction, every operand straight to registers, so that the weights stream from memory once.
 //
 // The matrix instruction of `tiles` is v_mfma_i32_32x32x32_i8, which reaches 4.9 POPS here where the 16x16x64 form reaches 3.0.  Operands:
 // lane l has row l & 31 and the 16 contraction bytes of half l >> 5; the result: column l & 31, rows 8 (r >> 2) + 4 (l >> 5) + (r & 3).  b is
 // the operand of the rows, so that a lane holds four adjacent columns of one row of `out`.
+//
+// What bounds `tiles`: the fetches and the way out.  A compute unit takes in 97 to 115 bytes/ns from its L2 in rows of 128 bytes (in rows of
+// 64 half of that), a wave that waits to issue one issues no product either, and the result, twice the inputs at K = 2560, leaves at the
+// memory's rate.  So a stage has one place in LDS and several workgroups share a compute unit: while one fetches or writes its result out,
+// another multiplies.  32768 x 2560 x 10576: 913 us (1.94 POPS).  Rings of two to four stages with one workgroup of 256 x 256 to a compute
+// unit, the next stages on their way during the products: 1120 to 1380 us; two workgroups of 128 x 256 with three stages of 64: 1080.
 #include <algorithm>
 
 #include "serve_common.h"
@@ -45,21 +51,24 @@ struct OutOf<F32> {
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void glb_void;
 
-constexpr int kK = 64;  // contraction bytes of a stage
-
 __device__ const lq_v4i zero16[1] = {{0, 0, 0, 0}};  // what a contraction past its end reads
 
-// TM x TN of the result to a workgroup of four waves, 2 x 2; NS stages in the ring.
-// A stage's row has four pieces of 16 bytes, piece c at place c ^ (row / 4) & 3: the 16 lanes that a read serves at once then touch each bank once.
-template <int TM, int TN, int NS, typename O>
-__global__ __launch_bounds__(256) void int8_tiles_kernel(MatmulParams p) {
-  constexpr int MI = TM / 64, NI = TN / 64;      // 32-row tiles of a wave
-  constexpr int PA = TM / 64, PB = TN / 64;      // fetches of a wave and stage: 16 rows each
-  constexpr int kStage = (TM + TN) * kK;
+constexpr int KB = 128, PC = KB / 16, FR = 64 / PC;  // contraction bytes of a stage, 16-byte pieces of its rows, rows of a fetch
+// Piece c of a stage's row lies at place c ^ order(row): the 16 lanes that a read serves at once then touch each bank once.
+LQ_DEV int order(int row) { return (row >> 1) & 7; }
+
+// TM x TN of the result to KG groups of four waves, 2 x 2 of a tile; the groups have every KG-th stage each and are summed at the end.
+template <int TM, int TN, int KG, typename O>
+__global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) void int8_tiles_kernel(MatmulParams p) {
+  constexpr int MI = TM / 64, NI = TN / 64;          // 32-row tiles of a wave
+  constexpr int PA = TM / FR / 4, PB = TN / FR / 4;  // fetches of a wave and stage
+  constexpr int kStage = (TM + TN) * KB, SUB = KB / 32;
   constexpr int kOutRow = TN / 2 * (int)sizeof(typename OutOf<O>::type) + 16;  // bytes of a row of a wave's result on its way out
-  constexpr int kLds = std::max(NS * kStage, 4 * 32 * kOutRow + 2 * TN * 4);
+  constexpr int kLds = std::max(std::max(KG * kStage, 4 * 32 * kOutRow), KG / 2 * TM * TN * 4);
   __shared__ __align__(16) char lds[kLds];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  __shared__ __align__(16) float sb[2 * TN];  // the columns' scales and bias
+  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+  const int group = __builtin_amdgcn_readfirstlane(tid >> 8), wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
   // Workgroups go round the 8 XCDs in launch order; each XCD takes adjacent tiles of an order in which 32 of them are 8 x 4, so that what its
   // compute units read at one time is mostly the same and comes from its L2.
   const int nm = (p.rows + TM - 1) / TM, nn = (p.cols + TN - 1) / TN;
@@ -70,43 +79,58 @@ __global__ __launch_bounds__(256) void int8_tiles_kernel(MatmulParams p) {
     const int band = i / (8 * nn), first = band * 8, high = min(8, nm - first), j = i - band * 8 * nn;
     m0 = (first + j % high) * TM, n0 = (j / high) * TN;
   }
-  // fetch: 64 lanes are 16 rows of four pieces
-  const int fr = lane >> 2, fc = (lane & 3) ^ ((lane >> 4) & 3);
+  const int fr = lane / PC;
   uint32_t offa[PA], offb[PB];
+  auto piece = [&](int row) { return 16 * ((lane & (PC - 1)) ^ order(row)); };
 #pragma unroll
-  for (int i = 0; i < PA; ++i) offa[i] = (uint32_t)min(16 * (wave * PA + i) + fr, p.rows - 1 - m0) * (uint32_t)p.a_stride + 16u * fc;
+  for (int i = 0; i < PA; ++i) {
+    const int row = FR * (wave * PA + i) + fr;
+    offa[i] = (uint32_t)min(row, p.rows - 1 - m0) * (uint32_t)p.a_stride + (uint32_t)piece(row);
+  }
 #pragma unroll
-  for (int i = 0; i < PB; ++i) offb[i] = (uint32_t)min(16 * (wave * PB + i) + fr, p.cols - 1 - n0) * (uint32_t)p.b_stride + 16u * fc;
+  for (int i = 0; i < PB; ++i) {
+    const int row = FR * (wave * PB + i) + fr;
+    offb[i] = (uint32_t)min(row, p.cols - 1 - n0) * (uint32_t)p.b_stride + (uint32_t)piece(row);
+  }
   const int8_t* at = p.a + m0 * p.a_stride;
   const int8_t* bt = p.b + n0 * p.b_stride;
-  const int ns = (p.inner + kK - 1) / kK;
+  const int ns = (p.inner + KB - 1) / KB;
+  char* stage = lds + group * kStage;
   auto fetch = [&](int s) {
-    char* st = lds + (s % NS) * kStage;
-    const int8_t *as = at + s * kK, *bs = bt + s * kK;
-    if ((s + 1) * kK <= p.inner) {
+    const int8_t *as = at + s * KB, *bs = bt + s * KB;
+    if ((s + 1) * KB <= p.inner) {
 #pragma unroll
-      for (int i = 0; i < PA; ++i) __builtin_amdgcn_global_load_lds((glb_void*)(as + offa[i]), (lds_void*)(st + (wave * PA + i) * 1024), 16, 0, 0);
+      for (int i = 0; i < PA; ++i) __builtin_amdgcn_global_load_lds((glb_void*)(as + offa[i]), (lds_void*)(stage + (wave * PA + i) * 1024), 16, 0, 0);
 #pragma unroll
-      for (int i = 0; i < PB; ++i) __builtin_amdgcn_global_load_lds((glb_void*)(bs + offb[i]), (lds_void*)(st + TM * kK + (wave * PB + i) * 1024), 16, 0, 0);
-    } else {  // the last stage, cut short: zeros of either operand
-      const bool in = s * kK + 16 * fc < p.inner;
+      for (int i = 0; i < PB; ++i) __builtin_amdgcn_global_load_lds((glb_void*)(bs + offb[i]), (lds_void*)(stage + TM * KB + (wave * PB + i) * 1024), 16, 0, 0);
+    } else {  // the last stage, cut short: zeros of either operand behind the contraction
+      auto from = [&](const int8_t* q, uint32_t off, int row) { return s * KB + piece(row) < p.inner ? (const void*)(q + off) : (const void*)zero16; };
 #pragma unroll
       for (int i = 0; i < PA; ++i)
-        __builtin_amdgcn_global_load_lds((glb_void*)(in ? (const void*)(as + offa[i]) : (const void*)zero16), (lds_void*)(st + (wave * PA + i) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_void*)from(as, offa[i], FR * (wave * PA + i) + fr), (lds_void*)(stage + (wave * PA + i) * 1024), 16, 0, 0);
 #pragma unroll
       for (int i = 0; i < PB; ++i)
-        __builtin_amdgcn_global_load_lds((glb_void*)(in ? (const void*)(bs + offb[i]) : (const void*)zero16), (lds_void*)(st + TM * kK + (wave * PB + i) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_void*)from(bs, offb[i], FR * (wave * PB + i) + fr), (lds_void*)(stage + TM * KB + (wave * PB + i) * 1024), 16, 0, 0);
     }
   };
   const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
-  const int r0 = (lane & 31) * kK, x = (lane >> 2) & 3;
-  auto read = [&](int s, int k, lq_v4i (&fa)[MI], lq_v4i (&fb)[NI]) {
-    const char* st = lds + (s % NS) * kStage + r0 + (((2 * k + hh) ^ x) * 16);
+  const int r0 = (lane & 31) * KB, x = order(lane & 31);
+  auto read = [&](int k, lq_v4i (&fa)[MI], lq_v4i (&fb)[NI]) {
+    const char* st = stage + r0 + (((2 * k + hh) ^ x) * 16);
 #pragma unroll
-    for (int i = 0; i < MI; ++i) fa[i] = *(const lq_v4i*)(st + (wm + 32 * i) * kK);
+    for (int i = 0; i < MI; ++i) fa[i] = *(const lq_v4i*)(st + (wm + 32 * i) * KB);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) fb[j] = *(const lq_v4i*)(st + (TM + wn + 32 * j) * kK);
+    for (int j = 0; j < NI; ++j) fb[j] = *(const lq_v4i*)(st + (TM + wn + 32 * j) * KB);
   };
+  if (group < ns) fetch(group);
+  float sa[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) sa[i] = p.a_scale[p.a_scale_rows ? min(m0 + wm + 32 * i + (lane & 31), p.rows - 1) : 0];
+  for (int i = tid; i < TN; i += 256 * KG) {
+    const int n = min(n0 + i, p.cols - 1);
+    sb[i] = p.b_scale[p.b_scale_cols ? n : 0];
+    sb[TN + i] = p.bias ? sv_load(p.bias, n, p.bias_dtype) : 0.0f;
+  }
   lq_v16i acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -120,44 +144,62 @@ __global__ __launch_bounds__(256) void int8_tiles_kernel(MatmulParams p) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
   };
-#pragma unroll
-  for (int s = 0; s < NS - 1; ++s)
-    if (s < ns) fetch(s);
   lq_v4i fa[2][MI], fb[2][NI];
-  // stage s: its first half's operands are in registers; the second half's are read while that is multiplied, and the next stage's first
-  // while the second is.  Between the two every wave has read all of stage s and its share of stage s + 1 has landed.
-  auto ready = [&](int s) {  // stage s has landed: NS - 2 later ones may be on their way
-    if (s + NS - 2 < ns) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * (PA + PB)) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  };
-  ready(0);
-  read(0, 0, fa[0], fb[0]);
-  for (int s = 0; s < ns; ++s) {
-    read(s, 1, fa[1], fb[1]);
-    if (s + NS - 1 < ns) fetch(s + NS - 1);  // into the place of stage s - 1
-    multiply(fa[0], fb[0]);
-    if (s + 1 < ns) {
-      ready(s + 1);
-      read(s + 1, 0, fa[0], fb[0]);
+  for (int s0 = 0; s0 < ns; s0 += KG) {
+    const int s = s0 + group;
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's share of the stage has landed
+    if (s < ns) {
+      read(0, fa[0], fb[0]);
+#pragma unroll
+      for (int k = 0; k + 1 < SUB; ++k) {
+        read(k + 1, fa[(k + 1) & 1], fb[(k + 1) & 1]);
+        multiply(fa[k & 1], fb[k & 1]);
+      }
     }
-    multiply(fa[1], fb[1]);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave has read all of it
+    if (s + KG < ns) fetch(s + KG);
+    if (s < ns) multiply(fa[(SUB - 1) & 1], fb[(SUB - 1) & 1]);
   }
-  // out: scales and bias of the tile's columns in LDS, then 32 rows of a wave's result at a time through LDS
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  float* sb = (float*)(lds + 4 * 32 * kOutRow);
-  for (int i = tid; i < TN; i += 256) {
-    const int n = min(n0 + i, p.cols - 1);
-    sb[i] = p.b_scale[p.b_scale_cols ? n : 0];
-    sb[TN + i] = p.bias ? sv_load(p.bias, n, p.bias_dtype) : 0.0f;
+  // the groups' sums: each step halves how many there are, the upper ones' through LDS
+  if constexpr (KG > 1) {
+#pragma unroll
+    for (int n = KG / 2; n >= 1; n /= 2) {
+      int* at = (int*)lds + (group % n) * TM * TN + ((wave * 64 + lane) * 4);
+      if (group >= n && group < 2 * n) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const lq_v4i v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+              *(lq_v4i*)(at + ((i * NI + j) * 4 + q) * 1024) = v;
+            }
+      }
+      __syncthreads();
+      if (group < n) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const lq_v4i v = *(const lq_v4i*)(at + ((i * NI + j) * 4 + q) * 1024);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+            }
+      }
+      __syncthreads();
+    }
+    if (group > 0) return;
   }
-  __syncthreads();
+  // out: 32 rows of a wave's result at a time through LDS (nothing of it is read any more: the barrier behind the last stage's reads)
   using OT = typename OutOf<O>::type;
   char* my = lds + wave * 32 * kOutRow;
   OT* out = (OT*)p.out;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int m = m0 + wm + 32 * i;
-    const float sa = p.a_scale[p.a_scale_rows ? min(m + (lane & 31), p.rows - 1) : 0];
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -167,7 +209,7 @@ __global__ __launch_bounds__(256) void int8_tiles_kernel(MatmulParams p) {
         typedef OT V4 __attribute__((ext_vector_type(4)));
         V4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = O::from(__builtin_fmaf((float)acc[i][j][4 * q + e], sa * s4[e], b4[e]));
+        for (int e = 0; e < 4; ++e) o[e] = O::from(__builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]));
         *(V4*)(my + (lane & 31) * kOutRow + n * sizeof(OT)) = o;
       }
     // (a wave's LDS operations are in order)
@@ -254,17 +296,24 @@ int launch(const MatmulParams& p, hipStream_t stream) {
     else hipLaunchKernelGGL((int8_rows_kernel<4, O>), grid, dim3(512), 0, stream, p);
     return lq_check_launch();
   }
-  auto tiles = [&](auto tm, auto tn, auto ns) {
-    constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, NS = decltype(ns)::value;
+  auto tiles = [&](auto tm, auto tn, auto kg) {
+    constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, KG = decltype(kg)::value;
     const int64_t n = (int64_t)((p.rows + TM - 1) / TM) * ((p.cols + TN - 1) / TN);
     if (n > 0x7ffffff0) return LQ_ERR_SHAPE;
-    hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, NS, O>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, KG, O>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256 * KG), 0, stream, p);
     return lq_check_launch();
   };
   using std::integral_constant;
-  const int64_t large = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
-  if (large >= 256) return tiles(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{});
+  auto count = [&](int tm, int tn) { return (int64_t)((p.rows + tm - 1) / tm) * ((p.cols + tn - 1) / tn); };
+  // The larger a tile, the less is fetched; the more tiles, the more compute units fetch, and two or three workgroups must share each.  Where
+  // even small tiles are few, groups share their contraction.  us, rows x K x columns, for tiles of 128 x 256 / 128 x 128 / 64 x 128 in two
+  // groups / 64 x 64 in four: 8192 x 2560 x 10576 248 / 249 / 329 / 428, 3001 x 2560 x 10576 92 / 99 / 122 / 162, 1000 x 2560 x 10576 42 / 40 /
+  // 47 / 57, 2000 x 5120 x 2560 62 / 44 / 52 / 51, 1000 x 5120 x 2560 60 / 41 / 28 / 34, 300 x 2560 x 10576 34 / 24 / 19 / 23, 500 x 5120 x 2560
+  // 60 / 41 / 26 / 20, 100 x 5120 x 2560 46 / 30 / 19 / 17.
+  if (count(128, 256) >= 768) return tiles(integral_constant<int, 128>{}, integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  if (count(128, 128) >= 300) return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 1>{});
+  if (count(64, 64) > 512) return tiles(integral_constant<int, 64>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{});
+  return tiles(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 4>{});
 }
 
 }  // namespace
