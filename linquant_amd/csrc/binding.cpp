@@ -1,5 +1,5 @@
 // The Python wrappers' ordinary calls without their host work: argument checks, allocations and args structs of lq_zoo_simple_gla,
-// lq_zoo_chunk_forward, lq_zoo_rotate_qkv, lq_split_rotate_quant_xBC and lq_ssd_combined in native code.  Each function serves the
+// lq_zoo_chunk_forward, lq_zoo_rotate_qkv, lq_split_rotate_quant_xBC, lq_ssd_combined and the serving entry points in native code.  Each function serves the
 // ordinary form of its call (plain tensors on the current GPU, fp32 scales, shapes that need no padding) and returns None for any other,
 // and for what is to be refused: the caller then takes the wrapper's general path, which converts, pads, copies or raises.  Nothing is
 // kept from one call for the next.
@@ -37,6 +37,14 @@ decltype(&lq_zoo_rotate_qkv) rotate_entry;
 decltype(&lq_split_rotate_quant_xBC) split_rotate_entry;
 decltype(&lq_ssd_combined) ssd_entry;
 decltype(&lq_ssd_combined_workspace_bytes) ssd_bytes;
+decltype(&lq_quantize_rows) quantize_entry;
+decltype(&lq_int8_matmul) matmul_entry;
+decltype(&lq_residual_rmsnorm) norm_entry;
+decltype(&lq_conv1d_prompt) conv_prompt_entry;
+decltype(&lq_conv1d_step) conv_step_entry;
+decltype(&lq_ssm_prompt) ssm_prompt_entry;
+decltype(&lq_ssm_prompt_workspace_bytes) ssm_prompt_bytes;
+decltype(&lq_ssm_step) ssm_step_entry;
 PyObject* raise_failed;
 
 using at::ScalarType;
@@ -430,6 +438,291 @@ PyObject* ssd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- serving: ordinary calls of linquant_amd.w8a8_linear, norm.residual_rmsnorm, kernels.mamba2.conv1d_state and .ssm
+bool act16(const Tensor& t) { return t.scalar_type() == ScalarType::Half || t.scalar_type() == ScalarType::BFloat16; }
+int code(ScalarType st) { return st == ScalarType::Half ? LQ_DT_F16 : (st == ScalarType::BFloat16 ? LQ_DT_BF16 : LQ_DT_F32); }
+bool floats(const Tensor& t) { return act16(t) || t.scalar_type() == ScalarType::Float; }
+// unit last stride and every row on a 16-byte boundary (2-byte entries)
+bool rows16(const Tensor& t) {
+  if (t.dim() < 1 || t.stride(-1) != 1 || !aligned(t) || !fits(t.sizes())) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.stride(i) % 8 != 0) return false;
+  return true;
+}
+bool list32(const Tensor& t, int64_t n) { return t.scalar_type() == ScalarType::Int && t.dim() == 1 && t.size(0) == n && t.is_contiguous(); }
+const int32_t* i32(const Tensor& t) { return t.defined() ? (const int32_t*)t.const_data_ptr() : nullptr; }
+const void* at(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// quantize_rows(x, pad): (codes in rows of `pad` bytes or multiples, scale) for a dense matrix
+PyObject* quantize(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, codes, scale;
+  int64_t pad;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !integer(arg[1], pad) || pad < 1) Py_RETURN_NONE;
+  if (x.dim() != 2 || !floats(x) || !fits(x.sizes()) || x.stride(1) != 1 || x.size(1) > 16384) Py_RETURN_NONE;
+  const int64_t M = x.size(0), K = x.size(1);
+  lq_quantize_rows_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    codes = empty({M, (K + pad - 1) / pad * pad}, ScalarType::Char, dev), scale = empty({M}, ScalarType::Float, dev);
+    a.x = x.const_data_ptr(), a.x_stride = x.stride(0), a.dtype = code(x.scalar_type());
+    a.codes = (int8_t*)codes.data_ptr(), a.codes_stride = codes.stride(0), a.scale = (float*)scale.data_ptr(), a.rows = (int)M, a.cols = (int)K;
+    rc = quantize_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_quantize_rows", rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(codes), THPVariable_Wrap(scale));
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_matmul(a, b, a_scale, b_scale, bias, out_dtype): matrices of whole 16-byte rows, fp32 scales on the GPU, a new output
+PyObject* int8_matmul(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, w, xs, ws, bias, out;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !plain(arg[1], dev, w) || !plain(arg[2], dev, xs) || !plain(arg[3], dev, ws) || !optional(arg[4], dev, bias)) Py_RETURN_NONE;
+  if (!THPDtype_Check(arg[5])) Py_RETURN_NONE;
+  const ScalarType ot = ((THPDtype*)arg[5])->scalar_type;
+  if (ot != ScalarType::Half && ot != ScalarType::BFloat16 && ot != ScalarType::Float) Py_RETURN_NONE;
+  for (const Tensor* t : {&x, &w})
+    if (t->dim() != 2 || t->scalar_type() != ScalarType::Char || !fits(t->sizes()) || t->stride(1) != 1 || t->stride(0) % 16 != 0 || t->stride(0) >= 1 << 23 || !aligned(*t)) Py_RETURN_NONE;
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  if (w.size(1) != K || K % 16 != 0 || K > 131056) Py_RETURN_NONE;
+  if (xs.scalar_type() != ScalarType::Float || !xs.is_contiguous() || (xs.numel() != 1 && xs.numel() != M)) Py_RETURN_NONE;
+  if (ws.scalar_type() != ScalarType::Float || !ws.is_contiguous() || (ws.numel() != 1 && ws.numel() != N)) Py_RETURN_NONE;
+  if (bias.defined() && (!floats(bias) || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous())) Py_RETURN_NONE;
+  lq_int8_matmul_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty({M, N}, ot, dev);
+    a.a = (const int8_t*)x.const_data_ptr(), a.a_stride = x.stride(0), a.b = (const int8_t*)w.const_data_ptr(), a.b_stride = w.stride(0);
+    a.a_scale = f32(xs), a.b_scale = f32(ws), a.a_scale_rows = xs.numel() != 1, a.b_scale_cols = ws.numel() != 1;
+    a.bias = at(bias), a.bias_dtype = bias.defined() ? code(bias.scalar_type()) : 0;
+    a.out = out.data_ptr(), a.out_stride = N, a.out_dtype = code(ot), a.rows = (int)M, a.cols = (int)N, a.inner = (int)K;
+    rc = matmul_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_int8_matmul", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// residual_rmsnorm(x, weight, residual, eps, gate, scale, post_weight, rows): rows that are dense, a gate for each channel or of x's shape,
+// weights of one type; y in 16 bits, or with `rows` codes on a scale of each row
+PyObject* residual_rmsnorm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, w, res, gate, post, y, r, codes, rs;
+  double eps, scale;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !plain(arg[1], dev, w) || !plain(arg[2], dev, res) || !number(arg[3], eps) || !optional(arg[4], dev, gate) ||
+      !number(arg[5], scale) || !optional(arg[6], dev, post))
+    Py_RETURN_NONE;
+  const int quant = PyObject_IsTrue(arg[7]);
+  if (quant < 0) return nullptr;
+  if (!act16(x) || x.dim() < 1 || !fits(x.sizes()) || !x.is_contiguous() || x.size(-1) > 16384) Py_RETURN_NONE;
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  if (rows > INT_MAX || res.sizes() != x.sizes() || !res.is_contiguous() || (res.scalar_type() != x.scalar_type() && res.scalar_type() != ScalarType::Float)) Py_RETURN_NONE;
+  if (!floats(w) || w.dim() != 1 || w.size(0) != D || !w.is_contiguous()) Py_RETURN_NONE;
+  if (post.defined() && (post.scalar_type() != w.scalar_type() || post.dim() != 1 || post.size(0) != D || !post.is_contiguous())) Py_RETURN_NONE;
+  const bool channel = gate.defined() && gate.dim() == 1 && gate.size(0) == D;
+  if (gate.defined() && (gate.scalar_type() != x.scalar_type() || !gate.is_contiguous() || !(channel || gate.sizes() == x.sizes()))) Py_RETURN_NONE;
+  lq_residual_rmsnorm_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    r = empty(x.sizes(), res.scalar_type(), dev);
+    if (quant) codes = empty(x.sizes(), ScalarType::Char, dev), rs = empty(x.sizes().slice(0, x.dim() - 1), ScalarType::Float, dev);
+    else y = empty(x.sizes(), x.scalar_type(), dev);
+    a.x = x.const_data_ptr(), a.x_stride = D, a.dtype = code(x.scalar_type()), a.residual = res.const_data_ptr(), a.residual_stride = D;
+    a.residual_dtype = code(res.scalar_type()), a.gate = at(gate), a.gate_stride = channel ? 0 : D, a.gate_rows = 1, a.post_weight = at(post);
+    a.weight = w.const_data_ptr(), a.weight_dtype = code(w.scalar_type()), a.scale = (float)scale, a.eps = (float)eps;
+    a.residual_out = r.data_ptr(), a.residual_out_stride = D, a.out = quant ? nullptr : y.data_ptr(), a.out_stride = D;
+    a.codes = quant ? (int8_t*)codes.data_ptr() : nullptr, a.codes_stride = D, a.row_scale = quant ? (float*)rs.data_ptr() : nullptr;
+    a.rows = (int)rows, a.dim = (int)D;
+    rc = norm_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_residual_rmsnorm", rc);
+  if (quant) return Py_BuildValue("(NNN)", THPVariable_Wrap(codes), THPVariable_Wrap(rs), THPVariable_Wrap(r));
+  return Py_BuildValue("(NN)", THPVariable_Wrap(y), THPVariable_Wrap(r));
+  END_HANDLE_TH_ERRORS
+}
+
+bool activation(PyObject* o, int& silu) {
+  silu = o != Py_None;
+  return !silu || (PyUnicode_Check(o) && (PyUnicode_CompareWithASCIIString(o, "silu") == 0 || PyUnicode_CompareWithASCIIString(o, "swish") == 0));
+}
+// taps, bias and state of x's type that need no copy
+bool conv_operands(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& state) {
+  if (!act16(x) || !rows16(x) || w.dim() != 2 || w.scalar_type() != x.scalar_type() || !w.is_contiguous() || !aligned(w)) return false;
+  const int64_t D = w.size(0), W = w.size(1);
+  if (x.size(-1) != D || D % 8 != 0 || W < 2 || W > 4) return false;
+  if (bias.defined() && (bias.scalar_type() != x.scalar_type() || bias.dim() != 1 || bias.size(0) != D || !bias.is_contiguous() || !aligned(bias))) return false;
+  return !state.defined() || (state.dim() == 3 && state.size(1) == W - 1 && state.size(2) == D && state.scalar_type() == x.scalar_type() && rows16(state));
+}
+// n sequences, their slots (or none) in a state
+bool slots_of(const Tensor& slots, int64_t n, const Tensor& state) { return slots.defined() ? list32(slots, n) : n <= state.size(0); }
+
+// conv1d_step(x, state, weight, bias, activation, slots)
+PyObject* conv1d_step(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, state, w, bias, slots, out;
+  int silu;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !plain(arg[1], dev, state) || !plain(arg[2], dev, w) || !optional(arg[3], dev, bias) || !activation(arg[4], silu) ||
+      !optional(arg[5], dev, slots))
+    Py_RETURN_NONE;
+  if (x.dim() != 2 || !conv_operands(x, w, bias, state) || !slots_of(slots, x.size(0), state)) Py_RETURN_NONE;
+  lq_conv1d_step_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(x.sizes(), x.scalar_type(), dev);
+    a.x = x.const_data_ptr(), a.x_stride = x.stride(0), a.dtype = code(x.scalar_type()), a.weight = w.const_data_ptr(), a.bias = at(bias), a.out = out.data_ptr();
+    a.state = state.data_ptr(), a.state_stride_s = state.stride(0), a.state_stride_w = state.stride(1), a.slots = i32(slots), a.num_slots = (int)state.size(0);
+    a.batch = (int)x.size(0), a.dim = (int)w.size(0), a.width = (int)w.size(1), a.silu = silu;
+    rc = conv_step_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_conv1d_step", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// conv1d_prompt(x, weight, bias, activation, state, slots, seq_starts), with a state
+PyObject* conv1d_prompt(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, w, bias, state, slots, starts, out;
+  int silu;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !plain(arg[1], dev, w) || !optional(arg[2], dev, bias) || !activation(arg[3], silu) || !plain(arg[4], dev, state) ||
+      !optional(arg[5], dev, slots) || !optional(arg[6], dev, starts))
+    Py_RETURN_NONE;
+  const bool packed = starts.defined();
+  if (x.dim() != (packed ? 2 : 3) || !conv_operands(x, w, bias, state)) Py_RETURN_NONE;
+  if (packed && (starts.dim() != 1 || starts.size(0) < 2 || !list32(starts, starts.size(0)))) Py_RETURN_NONE;
+  const int64_t seqs = packed ? starts.size(0) - 1 : x.size(0);
+  if (seqs > INT_MAX || !slots_of(slots, seqs, state)) Py_RETURN_NONE;
+  lq_conv1d_prompt_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(x.sizes(), x.scalar_type(), dev);
+    a.x = x.const_data_ptr(), a.x_stride_b = packed ? 0 : x.stride(0), a.x_stride_l = x.stride(-2), a.dtype = code(x.scalar_type());
+    a.weight = w.const_data_ptr(), a.bias = at(bias), a.out = out.data_ptr();
+    a.state = state.data_ptr(), a.state_stride_s = state.stride(0), a.state_stride_w = state.stride(1), a.slots = i32(slots), a.seq_starts = i32(starts);
+    a.num_slots = (int)state.size(0), a.nseq = (int)seqs, a.seqlen = packed ? 0 : (int)x.size(1), a.tokens = packed ? (int)x.size(0) : 0;
+    a.dim = (int)w.size(0), a.width = (int)w.size(1), a.silu = silu;
+    rc = conv_prompt_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_conv1d_prompt", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// what both forms of the scan take: arg = x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots
+struct Scan {
+  Tensor x, dt, A, B, C, D, bias, state, slots;
+  int softplus = 0;
+  double lo = 0.0, hi = 0.0;
+  int64_t H = 0, P = 0, G = 0, N = 0;
+};
+bool scan_operands(PyObject* const* arg, const c10::Device& dev, int lead, Scan& s) {
+  if (!plain(arg[0], dev, s.x) || !plain(arg[1], dev, s.dt) || !plain(arg[2], dev, s.A) || !plain(arg[3], dev, s.B) || !plain(arg[4], dev, s.C) || !optional(arg[5], dev, s.D) ||
+      !optional(arg[6], dev, s.bias) || !plain(arg[9], dev, s.state) || !optional(arg[10], dev, s.slots))
+    return false;
+  if (!PyBool_Check(arg[7]) || !PyTuple_CheckExact(arg[8]) || PyTuple_GET_SIZE(arg[8]) != 2 || !number(PyTuple_GET_ITEM(arg[8], 0), s.lo) || !number(PyTuple_GET_ITEM(arg[8], 1), s.hi))
+    return false;
+  s.softplus = arg[7] == Py_True;
+  const Tensor &x = s.x, &B = s.B, &C = s.C, &dt = s.dt;
+  if (x.dim() != lead + 2 || B.dim() != lead + 2 || dt.dim() != lead + 1 || !act16(x) || B.scalar_type() != x.scalar_type() || C.scalar_type() != x.scalar_type() || !floats(dt)) return false;
+  if (!rows16(x) || !rows16(B) || !rows16(C) || B.sizes() != C.sizes() || !fits(dt.sizes())) return false;
+  s.H = x.size(lead), s.P = x.size(lead + 1), s.G = B.size(lead), s.N = B.size(lead + 1);
+  for (int i = 0; i < lead; ++i)
+    if (B.size(i) != x.size(i) || dt.size(i) != x.size(i)) return false;
+  if (dt.size(lead) != s.H || s.H % s.G != 0 || s.P % 8 != 0 || s.N % 8 != 0 || s.N > 256 || x.stride(lead - 1) >= 1 << 24) return false;
+  if (s.A.dim() != 1 || !table(s.A, s.H) || (s.bias.defined() && (s.bias.dim() != 1 || !table(s.bias, s.H)))) return false;
+  if (s.D.defined() && !(s.D.dim() == 1 ? table(s.D, s.H) : s.D.dim() == 2 && s.D.size(0) == s.H && table(s.D, s.H * s.P))) return false;
+  const Tensor& st = s.state;
+  return st.dim() == 4 && st.scalar_type() == ScalarType::Float && fits(st.sizes()) && st.size(1) == s.H && st.size(2) == s.P && st.size(3) == s.N && st.stride(3) == 1 &&
+         st.stride(2) == s.N && st.stride(1) == s.P * s.N && aligned(st);
+}
+template <typename Args>
+void scan_args(const Scan& s, Args& a) {
+  a.x = s.x.const_data_ptr(), a.dtype = code(s.x.scalar_type()), a.dt = s.dt.const_data_ptr(), a.dt_dtype = code(s.dt.scalar_type()), a.A = f32(s.A);
+  a.B = s.B.const_data_ptr(), a.C = s.C.const_data_ptr(), a.D = f32(s.D), a.D_has_hdim = s.D.defined() && s.D.dim() == 2, a.dt_bias = f32(s.bias);
+  a.dt_softplus = s.softplus, a.dt_min = (float)s.lo, a.dt_max = (float)s.hi;
+  a.state = (float*)s.state.data_ptr(), a.state_stride_s = s.state.stride(0), a.slots = i32(s.slots), a.num_slots = (int)s.state.size(0);
+  a.nheads = (int)s.H, a.headdim = (int)s.P, a.ngroups = (int)s.G, a.dstate = (int)s.N;
+}
+
+// ssm_step(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots)
+PyObject* ssm_step(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Scan s;
+  Tensor out;
+  if (!device_of(arg[0], dev) || !scan_operands(arg, dev, 1, s)) Py_RETURN_NONE;
+  const int64_t B = s.x.size(0);
+  if (B > 65535 || !slots_of(s.slots, B, s.state)) Py_RETURN_NONE;
+  lq_ssm_step_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(s.x.sizes(), s.x.scalar_type(), dev);
+    scan_args(s, a);
+    a.x_stride_b = s.x.stride(0), a.x_stride_h = s.x.stride(1), a.dt_stride_b = s.dt.stride(0), a.dt_stride_h = s.dt.stride(1);
+    a.B_stride_b = s.B.stride(0), a.B_stride_g = s.B.stride(1), a.C_stride_b = s.C.stride(0), a.C_stride_g = s.C.stride(1);
+    a.out = out.data_ptr(), a.batch = (int)B;
+    rc = ssm_step_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_ssm_step", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// ssm_prompt(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots, seq_starts), with a state
+PyObject* ssm_prompt(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Scan s;
+  Tensor starts, out;
+  if (!device_of(arg[0], dev) || !optional(arg[11], dev, starts)) Py_RETURN_NONE;
+  const bool packed = starts.defined();
+  if (!scan_operands(arg, dev, packed ? 1 : 2, s)) Py_RETURN_NONE;
+  if (packed && (starts.dim() != 1 || starts.size(0) < 2 || !list32(starts, starts.size(0)))) Py_RETURN_NONE;
+  const int64_t seqs = packed ? starts.size(0) - 1 : s.x.size(0);
+  if (seqs > INT_MAX || !slots_of(s.slots, seqs, s.state)) Py_RETURN_NONE;
+  lq_ssm_prompt_args a = {};
+  scan_args(s, a);
+  const int l = packed ? 0 : 1;
+  auto batch = [&](const Tensor& t) { return packed ? 0 : t.stride(0); };
+  a.x_stride_b = batch(s.x), a.x_stride_l = s.x.stride(l), a.x_stride_h = s.x.stride(l + 1);
+  a.dt_stride_b = batch(s.dt), a.dt_stride_l = s.dt.stride(l), a.dt_stride_h = s.dt.stride(l + 1);
+  a.B_stride_b = batch(s.B), a.B_stride_l = s.B.stride(l), a.B_stride_g = s.B.stride(l + 1);
+  a.C_stride_b = batch(s.C), a.C_stride_l = s.C.stride(l), a.C_stride_g = s.C.stride(l + 1);
+  a.seq_starts = i32(starts), a.nseq = (int)seqs, a.seqlen = packed ? 0 : (int)s.x.size(1), a.tokens = packed ? (int)s.x.size(0) : 0;
+  int64_t bytes = 0;
+  if (ssm_prompt_bytes(&a, &bytes) != 0) Py_RETURN_NONE;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(s.x.sizes(), s.x.scalar_type(), dev);
+    Tensor ws = empty({bytes}, ScalarType::Byte, dev);
+    a.out = out.data_ptr(), a.workspace = ws.data_ptr(), a.workspace_bytes = bytes;
+    rc = ssm_prompt_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_ssm_prompt", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // whether the library was built from the header that this file was: its ABI version and the structs that are filled here
 bool same_abi(decltype(&lq_abi_version) version, decltype(&lq_args_size) size) {
   const int v = version();
@@ -442,6 +735,13 @@ bool same_abi(decltype(&lq_abi_version) version, decltype(&lq_args_size) size) {
   LQ_SAME_SIZE(lq_zoo_rotate_qkv_args);
   LQ_SAME_SIZE(lq_split_rotate_quant_xBC_args);
   LQ_SAME_SIZE(lq_ssd_combined_args);
+  LQ_SAME_SIZE(lq_quantize_rows_args);
+  LQ_SAME_SIZE(lq_int8_matmul_args);
+  LQ_SAME_SIZE(lq_residual_rmsnorm_args);
+  LQ_SAME_SIZE(lq_conv1d_prompt_args);
+  LQ_SAME_SIZE(lq_conv1d_step_args);
+  LQ_SAME_SIZE(lq_ssm_prompt_args);
+  LQ_SAME_SIZE(lq_ssm_step_args);
 #undef LQ_SAME_SIZE
   return true;
 }
@@ -468,7 +768,16 @@ PyObject* init(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   chunk_forward_entry = (decltype(chunk_forward_entry))entry("lq_zoo_chunk_forward");
   chunk_forward_bytes = (decltype(chunk_forward_bytes))entry("lq_zoo_chunk_forward_workspace_bytes");
   rotate_entry = (decltype(rotate_entry))entry("lq_zoo_rotate_qkv");
-  if (!simple_gla_entry || !simple_gla_bytes || !chunk_forward_entry || !chunk_forward_bytes || !rotate_entry || !split_rotate_entry || !ssd_entry || !ssd_bytes) {
+  quantize_entry = (decltype(quantize_entry))entry("lq_quantize_rows");
+  matmul_entry = (decltype(matmul_entry))entry("lq_int8_matmul");
+  norm_entry = (decltype(norm_entry))entry("lq_residual_rmsnorm");
+  conv_prompt_entry = (decltype(conv_prompt_entry))entry("lq_conv1d_prompt");
+  conv_step_entry = (decltype(conv_step_entry))entry("lq_conv1d_step");
+  ssm_prompt_entry = (decltype(ssm_prompt_entry))entry("lq_ssm_prompt");
+  ssm_prompt_bytes = (decltype(ssm_prompt_bytes))entry("lq_ssm_prompt_workspace_bytes");
+  ssm_step_entry = (decltype(ssm_step_entry))entry("lq_ssm_step");
+  if (!quantize_entry || !matmul_entry || !norm_entry || !conv_prompt_entry || !conv_step_entry || !ssm_prompt_entry || !ssm_prompt_bytes || !ssm_step_entry ||
+      !simple_gla_entry || !simple_gla_bytes || !chunk_forward_entry || !chunk_forward_bytes || !rotate_entry || !split_rotate_entry || !ssd_entry || !ssd_bytes) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "an entry point is missing");
     return nullptr;
   }
@@ -483,6 +792,13 @@ PyMethodDef methods[] = {{"init", (PyCFunction)(void*)init, METH_FASTCALL, nullp
                          {"rotate_qkv", (PyCFunction)(void*)rotate_qkv, METH_FASTCALL, nullptr},
                          {"split_rotate", (PyCFunction)(void*)split_rotate, METH_FASTCALL, nullptr},
                          {"ssd", (PyCFunction)(void*)ssd, METH_FASTCALL, nullptr},
+                         {"quantize_rows", (PyCFunction)(void*)quantize, METH_FASTCALL, nullptr},
+                         {"int8_matmul", (PyCFunction)(void*)int8_matmul, METH_FASTCALL, nullptr},
+                         {"residual_rmsnorm", (PyCFunction)(void*)residual_rmsnorm, METH_FASTCALL, nullptr},
+                         {"conv1d_step", (PyCFunction)(void*)conv1d_step, METH_FASTCALL, nullptr},
+                         {"conv1d_prompt", (PyCFunction)(void*)conv1d_prompt, METH_FASTCALL, nullptr},
+                         {"ssm_step", (PyCFunction)(void*)ssm_step, METH_FASTCALL, nullptr},
+                         {"ssm_prompt", (PyCFunction)(void*)ssm_prompt, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods};
 

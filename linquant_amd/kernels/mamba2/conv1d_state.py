@@ -51,6 +51,10 @@ def conv1d_prompt(x, weight, bias=None, activation=None, *, state=None, slots=No
     read and then replaced by its last W-1 (a prompt of no tokens leaves them); None: zeros in front, nothing kept.  ``slots``
     (n,) int32: each prompt's place in the state, all different; negative: zeros in front, nothing kept; beyond the state: NaN
     outputs.  Returns y, dense, in the shape of x."""
+    if state is not None:
+        out = _lib.native().conv1d_prompt(x, weight, bias, activation, state, slots, seq_starts)
+        if out is not None:
+            return out
     weight, bias = _taps(x, weight, bias, activation)
     D, W = weight.shape
     if seq_starts is None:
@@ -81,6 +85,9 @@ def conv1d_prompt(x, weight, bias=None, activation=None, *, state=None, slots=No
 def conv1d_step(x, state, weight, bias=None, activation=None, *, slots=None):
     """The same for one token of each sequence: ``x`` (B, D) -> (B, D), ``state`` moved on by it.  ``slots`` (B,) int32, all different;
     negative marks a padding entry (zeros out, no state touched), beyond the state: NaN outputs."""
+    out = _lib.native().conv1d_step(x, state, weight, bias, activation, slots)
+    if out is not None:
+        return out
     weight, bias = _taps(x, weight, bias, activation)
     D, W = weight.shape
     assert x.dim() == 2, "x: (B, D)"

@@ -62,6 +62,10 @@ def ssm_prompt(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_lim
     ``state`` (slots, H, P, N) fp32: what each prompt starts from, replaced by what it ends in (a prompt of no tokens leaves it);
     None: zero, nothing kept.  ``slots`` (n,) int32: each prompt's place in the state, all different; negative: from zero, nothing
     kept; beyond the state: NaN outputs.  Returns y, dense, in the shape and type of x."""
+    if state is not None:
+        out = _lib.native().ssm_prompt(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots, seq_starts)
+        if out is not None:
+            return out
     packed = seq_starts is not None
     assert x.dim() == (3 if packed else 4), "x: (B, L, H, P), or (T, H, P) with seq_starts"
     lead = x.shape[:-2]
@@ -102,6 +106,9 @@ def ssm_step(state, x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, d
     """The same for one token of each sequence: ``x`` (B, H, P), ``dt`` (B, H), ``B``, ``C`` (B, G, N) -> y (B, H, P), ``state``
     (slots, H, P, N) fp32 moved on by it.  ``slots`` (B,) int32, all different; negative marks a padding entry (zeros out, no
     state touched), beyond the state: NaN outputs."""
+    out = _lib.native().ssm_step(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots)
+    if out is not None:
+        return out
     assert x.dim() == 3, "x: (B, H, P)"
     fields, keep = _params(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, x.shape[:1])
     n, H, P = x.shape

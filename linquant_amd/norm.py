@@ -84,6 +84,10 @@ def residual_rmsnorm(x, weight, residual=None, eps=1e-5, *, gate=None, scale=1.0
     16384.  Returns (y, r), or (codes, scale, r) with ``quantize``: "rows" for INT8 codes on a scale of each row (fp32, the
     shape of x without dim; a row of zeros has 0, one with an infinity or a NaN has NaN), a 0-dim fp32 tensor for codes
     clamp(rint(y / quantize), -128, 127)."""
+    if residual_dtype is None and not isinstance(quantize, torch.Tensor) and quantize in (None, "rows"):
+        out = _lib.native().residual_rmsnorm(x, weight, residual, eps, gate, scale, post_weight, quantize is not None)
+        if out is not None:
+            return out
     assert x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1
     dim = x.shape[-1]
     assert 1 <= dim <= 16384 and weight.shape == (dim,) and weight.dtype in _CODES

@@ -20,6 +20,9 @@ def _padded(n):
 
 def _quantize(x):
     """Codes in rows of whole 16-byte pieces, (rows, padded), the surplus undefined; scales (rows,)."""
+    out = _lib.native().quantize_rows(x, _K)
+    if out is not None:
+        return out
     assert x.dtype in _CODES and x.dim() >= 1 and 1 <= x.shape[-1] <= 16384
     K = x.shape[-1]
     x2 = x.reshape(-1, K)
@@ -38,7 +41,9 @@ def quantize_rows(x):
     """``x`` (..., K) fp16, bf16 or fp32, K up to 16384 -> (codes int8 (..., K), scale fp32 (...)): scale = max |x| / 127 of each row,
     codes = rint(x / scale).  A row of zeros has scale 0 and codes 0; one with an infinity or a NaN has scale NaN and codes 0."""
     codes, scale = _quantize(x)
-    return codes[:, :x.shape[-1]].unflatten(0, x.shape[:-1]) if x.dim() != 2 else codes[:, :x.shape[-1]], scale.view(x.shape[:-1])
+    K = x.shape[-1]
+    codes = codes if codes.shape[1] == K else codes[:, :K]
+    return (codes, scale) if x.dim() == 2 else (codes.unflatten(0, x.shape[:-1]), scale.view(x.shape[:-1]))
 
 
 def _scale(s, n, device, what):
@@ -69,6 +74,10 @@ def int8_matmul(a, b, a_scale, b_scale, bias=None, out_dtype=torch.float16, out=
     131056, the sum exact; ``a_scale`` a number, one entry or one for each row of a, ``b_scale`` a number, one entry or (N,);
     ``bias`` (N,) or None and ``out_dtype`` fp16, bf16 or fp32.  ``out``: a (M, N) view of that type with unit column stride to
     write into, for ``a`` of two dimensions.  Rows of K bytes that are not whole 16-byte pieces are copied first."""
+    if out is None:
+        res = _lib.native().int8_matmul(a, b, a_scale, b_scale, bias, out_dtype)
+        if res is not None:
+            return res
     assert a.dtype == torch.int8 and b.dtype == torch.int8 and b.dim() == 2 and a.dim() >= 1
     K, N = a.shape[-1], b.shape[0]
     assert b.shape[1] == K and 1 <= K <= 131056, f"contraction lengths {K} and {b.shape[1]}"
