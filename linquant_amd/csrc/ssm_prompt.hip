@@ -53,7 +53,7 @@ struct PromptParams {
   float* rows;      // [unit][group][64]: largest |C B^T| of each row
   float* seg_state;  // [segment][H][P][N], or NULL: prompts are not cut
   float* seg_decay;  // [segment][H]
-  int units, segs, seg_chunks, per_group, waves;
+  int units, segs, seg_chunks, per_group;
 };
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -314,17 +314,20 @@ LQ_DEV void place(const PromptParams& p, int& sg, int& part) {
   sg = i / parts, part = i - sg * parts;
 }
 
+constexpr int W = 4;  // waves of a workgroup
+
 // A wave has 32 channels of one head: the state's N x 32 as accumulators (rows n, columns the channels).  STATES: only the segment's
-// state and decay.  A workgroup's waves share the chunk's operands in LDS, fetched there a chunk ahead (NBUF = 2) as they lie in memory; each
-// wave's x comes the same way, 64 tokens x 32 channels, into one of two places, and its y leaves through the same place.
-template <typename T, int NT, bool STATES, int NBUF>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void ssm_chunks_kernel(PromptParams p) {
+// state and decay.  A workgroup's waves share the chunk's operands in LDS, fetched there as they lie in memory; each wave's x comes the same
+// way, 64 tokens x 32 channels, a chunk ahead into one of two places, and its y leaves through the same place.  Two workgroups share a
+// compute unit, so that one computes while the other's operands are on their way.
+template <typename T, int NT, bool STATES>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void ssm_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
   using Tab = Table<NT>;
   constexpr int kSkip = STATES ? kCB + Tab::kC : 0, kLoad = Tab::kBytes - kSkip;  // bytes of a chunk's operands that are needed
-  __shared__ __align__(16) char buf[NBUF][kLoad];
-  __shared__ __align__(16) uint16_t xbuf[2][8][Q * 32];
-  __shared__ __align__(16) float tok[8][4 * Q];  // each wave's d, c, w, exp2(c) (fp16: scaled)
+  __shared__ __align__(16) char buf[kLoad];
+  __shared__ __align__(16) uint16_t xbuf[2][W][Q * 32];
+  __shared__ __align__(16) float tok[W][4 * Q];  // each wave's d, c, w, exp2(c) (fp16: scaled)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   int sg, part;
   place(p, sg, part);
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const Segment s = segment_of(p, sg);
   if (s.seq < 0 || (STATES && s.last)) return;
   const int g = part / p.per_group, pblocks = (p.P + 31) >> 5, hpg = p.H / p.G;
-  const int block = (part - g * p.per_group) * p.waves + wave;
+  const int block = (part - g * p.per_group) * W + wave;
   const bool live = block < hpg * pblocks;  // a wave without channels only helps to fetch the operands
   const int h = g * hpg + (live ? block / pblocks : 0), ch0 = (live ? block % pblocks : 0) * 32, ch = ch0 + col;
   const int chc = min(ch, p.P - 1);
@@ -367,11 +370,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const char* tab = p.tables + ((int64_t)s.unit0 * p.G + g) * Tab::kBytes + kSkip;
   const uint32_t xcol = (uint32_t)min(8 * (lane & 3), p.P - 8 - ch0);
   float dv = 0.f, cv = 0.f, wv = 0.f, mv = 0.f, rv = 0.f;
-  auto fetch = [&](int c, int b) {
+  auto fetch = [&](int c) {
     const char* src = tab + (int64_t)c * p.G * Tab::kBytes;
-    for (int k = wave; k < kLoad / 1024; k += p.waves)
-      __builtin_amdgcn_global_load_lds((glb_void*)(src + k * 1024 + lane * 16), (lds_void*)(buf[b] + k * 1024), 16, 0, 0);
+#pragma unroll
+    for (int k = 0; k < kLoad / 1024 / W; ++k)
+      __builtin_amdgcn_global_load_lds((glb_void*)(src + (k * W + wave) * 1024 + lane * 16), (lds_void*)(buf + (k * W + wave) * 1024), 16, 0, 0);
   };
+  static_assert(kLoad % (1024 * W) == 0);
   auto request = [&](int c) {
     const int rem = s.len - (s.chunk0 + c) * Q;
     const uint16_t* xc = xs + (int64_t)(s.chunk0 + c) * Q * p.sx_l;
@@ -383,23 +388,22 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     dv = o[0], cv = o[Q], wv = o[2 * Q];
     if (kHalf && !STATES) mv = o[3 * Q], rv = p.rows[((int64_t)(s.unit0 + c) * p.G + g) * Q + lane];
   };
+  // What was requested is there; or it is but for the four stores behind it (memory operations end in order), which are not waited for.
   auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" : "+v"(dv), "+v"(cv), "+v"(wv), "+v"(mv), "+v"(rv)::"memory"); };
-
-  if (NBUF == 2) fetch(0, 0);
+  auto arrived_before_stores = [&] { asm volatile("s_waitcnt vmcnt(4)" : "+v"(dv), "+v"(cv), "+v"(wv), "+v"(mv), "+v"(rv)::"memory"); };
+  // every wave has read all of a chunk's operands: the next chunk's take their place
+  auto taken = [&](int c) {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (c + 1 < s.chunks) fetch(c + 1);
+  };
+  fetch(0);
   if (live) request(0);
   arrived();
   float decay = 0.0f;
   float* my = tok[wave];
   for (int c = 0; c < s.chunks; ++c) {
-    const int b = NBUF == 2 ? c & 1 : 0;
-    if constexpr (NBUF == 1) {
-      fetch(c, 0);
-      arrived();
-    }
-    // every wave's share of this chunk's operands is there (waited for below, or above), and none reads the last chunk's any more
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const bool more = c + 1 < s.chunks;
-    if (NBUF == 2 && more) fetch(c + 1, b ^ 1);
+    asm volatile("s_barrier" ::: "memory");  // every wave's share of this chunk's operands is there
     if (live) {
       uint16_t* xw = xbuf[c & 1][wave];
       lq_v4i xp[4];  // this lane's channel, tokens in the order of an operand
@@ -436,7 +440,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const float ui = kHalf ? 1.0f / unit_S : 1.0f;
       my[lane] = dv, my[Q + lane] = cv, my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
       if (more) request(c + 1);
-      const lq_v4i* op = (const lq_v4i*)buf[b] + lane;
+      const lq_v4i* op = (const lq_v4i*)buf + lane;
       const lq_v4i* opB = op + (STATES ? 0 : (kCB + Tab::kC) / 16);
       v16f Y[2];
       if constexpr (!STATES) {  // exp(c_t) S C_t
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
               }
           from = min(from, __shfl_xor(from, 32, 64));
         }
-        const lq_v4f* cb = (const lq_v4f*)buf[b] + lane;
+        const lq_v4f* cb = (const lq_v4f*)buf + lane;
         if (kHalf) my[2 * Q + lane] = 1.0f / row;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
@@ -535,6 +539,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             Y[tt] = mfma<T>(ml, xp[ks], Y[tt]);
           }
         }
+        taken(c);
         if (odd) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
@@ -560,19 +565,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 4; ++i) yo[i] = *(const lq_v4i*)(xw + 16 * 32 * i + lane * 8);
         const int rem = s.len - (s.chunk0 + c) * Q;
         uint16_t* oc = os + (int64_t)(s.chunk0 + c) * Q * ostride;
-        arrived();  // what is on its way for the next chunk: the stores below are not waited for
+        const uint32_t o0 = (uint32_t)(lane >> 2) * (uint32_t)ostride + 8 * (lane & 3);
+        if (rem >= Q && ch0 + 32 <= p.P) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 16 * i + (lane >> 2);
-          if (t < rem && ch0 + 8 * (lane & 3) < p.P) *(lq_v4i*)(oc + (uint32_t)t * (uint32_t)ostride + 8 * (lane & 3)) = yo[i];
+          for (int i = 0; i < 4; ++i) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
+          arrived_before_stores();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * i + (lane >> 2) < rem && ch0 + 8 * (lane & 3) < p.P) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
+          arrived();
         }
       } else {
+        taken(c);
         arrived();
       }
     } else {
-      arrived();  // its share of the next chunk's operands
+      taken(c);
+      arrived();
     }
-    if (NBUF == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
   float* dst = STATES ? p.seg_state + (int64_t)sg * p.H * p.P * p.N + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
   if (dst && live && ch < p.P) {
@@ -628,28 +639,27 @@ int table_bytes(const lq_ssm_prompt_args* a) {
   return kCB + (a->dstate <= 32 ? 1 : a->dstate <= 64 ? 2 : a->dstate <= 128 ? 4 : 8) * 8 * 1024;
 }
 
-// How a call is cut: the units, the waves of a workgroup, the chunks of a segment.
+// How a call is cut: the units, the chunks of a segment.
 struct Plan {
   int64_t units, segs, tables, steps, rows, states, decays, bytes;
-  int waves, per_group, seg_chunks, cut;
+  int per_group, seg_chunks, cut;
 };
 bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   const int64_t nseq = a->nseq, most = ((int64_t)(a->seq_starts ? a->tokens : a->seqlen) + Q - 1) / Q;  // chunks of the longest prompt there can be
   r.units = a->seq_starts ? (int64_t)a->tokens / Q + nseq : nseq * most;
   const int64_t blocks = (int64_t)(a->nheads / a->ngroups) * ((a->headdim + 31) / 32);
-  r.waves = blocks > 4 ? 8 : 4;
-  r.per_group = (int)((blocks + r.waves - 1) / r.waves);
+  r.per_group = (int)((blocks + W - 1) / W);
   const int64_t parts = (int64_t)a->ngroups * r.per_group;
-  // Chunk steps in a row that the chip takes for segments of n chunks, one workgroup to a compute unit, 256 at a time; cut prompts
-  // need their states first (about half a step each) and the join.
+  // Chunk steps in a row that the chip takes for segments of n chunks, two workgroups to a compute unit, 512 at a time; cut prompts
+  // need their states first and the join.
   const int64_t even = std::max<int64_t>(1, r.units / nseq);  // a packed call's prompts are taken to be of one length
   // in tenths of a microsecond: a step 35, one of the states' 15, and the segments' states written, joined and read at 3 TB/s
   int64_t best = -1;
   r.seg_chunks = (int)most, r.cut = 0;
   for (int64_t k = 1; k <= 64 && (k == 1 || even / k >= 2); ++k) {
     const int64_t n = (even + k - 1) / k, segs = nseq * ((even + n - 1) / n);
-    const int64_t rounds = (segs * parts + 255) / 256, move = segs * a->nheads * a->headdim * a->dstate * 16 / 300000 + 100;
-    const int64_t cost = k == 1 ? rounds * n * 35 : rounds * n * 35 + ((segs - nseq) * parts + 255) / 256 * n * 15 + move;
+    const int64_t rounds = (segs * parts + 511) / 512, move = segs * a->nheads * a->headdim * a->dstate * 16 / 300000 + 100;
+    const int64_t cost = k == 1 ? rounds * n * 35 : rounds * n * 35 + ((segs - nseq) * parts + 511) / 512 * n * 15 + move;
     if (best < 0 || cost < best) best = cost, r.seg_chunks = k == 1 ? (int)most : (int)n, r.cut = k > 1;
   }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
@@ -697,23 +707,21 @@ extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
                     a->D, a->D_has_hdim, a->dt_bias, a->dt_softplus, a->dt_min, a->dt_max, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots,
                     a->seq_starts, a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->headdim, a->ngroups, a->dstate,
                     ws + pl.tables, (float*)(ws + pl.steps), (float*)(ws + pl.rows), pl.cut ? (float*)(ws + pl.states) : nullptr, pl.cut ? (float*)(ws + pl.decays) : nullptr,
-                    (int)pl.units, (int)pl.segs, pl.seg_chunks, pl.per_group, pl.waves};
+                    (int)pl.units, (int)pl.segs, pl.seg_chunks, pl.per_group};
   const dim3 pre((unsigned)pl.units, (unsigned)(a->ngroups + (a->nheads + kHeads - 1) / kHeads));
-  const dim3 grid((unsigned)((pl.segs * a->ngroups * pl.per_group + 7) / 8 * 8)), threads(64 * pl.waves);
+  const dim3 grid((unsigned)((pl.segs * a->ngroups * pl.per_group + 7) / 8 * 8)), threads(64 * W);
   const int64_t per = (int64_t)a->headdim * a->dstate;
   const dim3 join((unsigned)pl.segs, (unsigned)a->nheads, (unsigned)((per + 1023) / 1024));
   if (join.y > 65535 || join.z > 65535) return LQ_ERR_SHAPE;
   auto go = [&](auto t, auto k) {
     using T = decltype(t);
     constexpr int NT = decltype(k)::value;
-    constexpr int kOwn = 2 * 8 * Q * 32 * 2 + 8 * 4 * Q * 4;  // bytes of x and of the step sizes of eight waves
-    constexpr int NBUF = 2 * Table<NT>::kBytes + kOwn <= 160 * 1024 ? 2 : 1;
     hipLaunchKernelGGL((ssm_operands_kernel<T, NT>), pre, dim3(256), 0, stream, p);
     if (pl.cut) {
-      hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, true, 2>), grid, threads, 0, stream, p);
+      hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, true>), grid, threads, 0, stream, p);
       hipLaunchKernelGGL(ssm_join_kernel, join, dim3(256), 0, stream, p);
     }
-    hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, false, NBUF>), grid, threads, 0, stream, p);
+    hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, false>), grid, threads, 0, stream, p);
     return lq_check_launch();
   };
   auto with = [&](auto t) {
