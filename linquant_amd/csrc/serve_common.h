@@ -101,21 +101,29 @@ LQ_DEV Unit sv_locate(const int32_t* __restrict__ starts, int nseq, int tokens, 
       const int o = __shfl_up(sum, off, 64);
       sum += lane >= off ? o : 0;
     }
-    const int total = __shfl(sum, 63, 64);
+    const int total = __builtin_amdgcn_readlane(sum, 63);
     if (u < before + total) {  // (u is the same for the whole wave)
       const uint64_t m = __ballot(u < before + sum);
       const int l = __builtin_ctzll(m);
       Unit r;
       r.seq = s0 + l;
-      r.index = u - (before + __shfl(sum - units, l, 64));
-      r.begin = __shfl(b, l, 64), r.end = __shfl(e, l, 64);
-      r.seq = __builtin_amdgcn_readfirstlane(r.seq), r.index = __builtin_amdgcn_readfirstlane(r.index);
-      r.begin = __builtin_amdgcn_readfirstlane(r.begin), r.end = __builtin_amdgcn_readfirstlane(r.end);
+      r.index = u - (before + __builtin_amdgcn_readlane(sum - units, l));
+      r.begin = __builtin_amdgcn_readlane(b, l), r.end = __builtin_amdgcn_readlane(e, l);
       return r;
     }
     before += total;
   }
   return Unit{-1, 0, 0, 0};
+}
+
+// 16 bytes a lane from base + offset straight into LDS, at `at` and on, lane after lane (base and at are the same for the wave).  As an
+// instruction: where the compiler knows of such a write it waits for all memory operations in front of every LDS access that might be meant,
+// the caller's stores among them; so the caller waits for vmcnt itself before it reads.
+// (m0 cannot be named as overwritten; nothing else in a kernel that calls this may need it: no __builtin_amdgcn_global_load_lds.)
+LQ_DEV void sv_fetch16(const void* base, uint32_t offset, const void* at) {
+  typedef const __attribute__((address_space(3))) char lds_char;
+  const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)at);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 static inline bool sv_al(const void* q, int n) { return ((uintptr_t)q % n) == 0; }

@@ -57,9 +57,6 @@ struct PromptParams {
 };
 
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void glb_void;
-
 template <typename T>
 LQ_DEV v16f mfma(lq_v4i a, lq_v4i b, v16f c) {
   if constexpr (std::is_same<T, F16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lq_v8h, a), __builtin_bit_cast(lq_v8h, b), c, 0, 0, 0);
@@ -109,7 +106,12 @@ LQ_DEV float wave_top(float v) {
 #undef LQ_TOP
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
+LQ_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 LQ_DEV float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+// a power of two's reciprocal
+LQ_DEV float pow2_inverse(float v) { return __uint_as_float(0x7f000000u - __float_as_uint(v)); }
+// LDS reads stay where they are written (everything else may move): as the compiler orders them, most stand right in front of their use
+LQ_DEV void reads_stay() { __builtin_amdgcn_sched_barrier(0xf); }
 // |v|, or 0 for what is no number and must not set a scale
 LQ_DEV float finite_size(float v) {
   const float a = __builtin_fabsf(v);
@@ -289,19 +291,19 @@ LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
       const int o = __shfl_up(sum, off, 64), v = __shfl_up(usum, off, 64);
       sum += lane >= off ? o : 0, usum += lane >= off ? v : 0;
     }
-    const int total = __shfl(sum, 63, 64);
+    const int total = __builtin_amdgcn_readlane(sum, 63);
     if (sg < before + total) {
       const int l = __builtin_ctzll(__ballot(sg < before + sum));
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       const int nc = of(units);
-      r.seq = s0 + l, r.begin = of(b), r.len = of(e) - r.begin;
+      r.seq = s0 + l, r.begin = of(b), r.len = of(e) - r.begin;  // (scalar already)
       r.chunk0 = (sg - before - of(sum - n)) * p.seg_chunks;
       r.unit0 = ubefore + of(usum - units) + r.chunk0;
       r.chunks = min(p.seg_chunks, nc - r.chunk0);
       r.first = r.chunk0 == 0, r.last = r.chunk0 + r.chunks == nc;
       return r;
     }
-    before += total, ubefore += __shfl(usum, 63, 64);
+    before += total, ubefore += __builtin_amdgcn_readlane(usum, 63);
   }
   return r;
 }
@@ -331,15 +333,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   int sg, part;
   place(p, sg, part);
+  // (what is the same for the whole wave goes to scalar registers: a division leaves it in vector ones, and every address made of it too)
+  sg = uniform(sg), part = uniform(part);
   if (sg >= p.segs) return;
-  const Segment s = segment_of(p, sg);
+  Segment s = segment_of(p, sg);
   if (s.seq < 0 || (STATES && s.last)) return;
-  const int g = part / p.per_group, pblocks = (p.P + 31) >> 5, hpg = p.H / p.G;
+  s.seq = uniform(s.seq), s.begin = uniform(s.begin), s.len = uniform(s.len), s.chunk0 = uniform(s.chunk0), s.chunks = uniform(s.chunks), s.unit0 = uniform(s.unit0);
+  const int g = uniform(part / p.per_group), pblocks = (p.P + 31) >> 5, hpg = uniform(p.H / p.G);
   const int block = (part - g * p.per_group) * W + wave;
   const bool live = block < hpg * pblocks;  // a wave without channels only helps to fetch the operands
-  const int h = g * hpg + (live ? block / pblocks : 0), ch0 = (live ? block % pblocks : 0) * 32, ch = ch0 + col;
+  const int h = uniform(g * hpg + (live ? block / pblocks : 0)), ch0 = uniform((live ? block % pblocks : 0) * 32), ch = ch0 + col;
   const int chc = min(ch, p.P - 1);
-  const int slot = p.state || p.slots ? sv_slot(p.slots, s.seq, p.num_slots) : kSlotPad;
+  const int slot = p.state || p.slots ? uniform(sv_slot(p.slots, s.seq, p.num_slots)) : kSlotPad;
   const bool keeps = p.state && slot >= 0;
   const int64_t row0 = (p.starts ? s.begin : (int64_t)s.seq * p.seqlen);  // of the dense output
   const uint16_t* xs = p.x + (p.starts ? s.begin * p.sx_l : s.seq * p.sx_b) + h * p.sx_h + ch0;
@@ -374,7 +379,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     const char* src = tab + (int64_t)c * p.G * Tab::kBytes;
 #pragma unroll
     for (int k = 0; k < kLoad / 1024 / W; ++k)
-      __builtin_amdgcn_global_load_lds((glb_void*)(src + (k * W + wave) * 1024 + lane * 16), (lds_void*)(buf + (k * W + wave) * 1024), 16, 0, 0);
+      sv_fetch16(src + (k * W + wave) * 1024, (uint32_t)lane * 16u, buf + (k * W + wave) * 1024);
   };
   static_assert(kLoad % (1024 * W) == 0);
   auto request = [&](int c) {
@@ -382,11 +387,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     const uint16_t* xc = xs + (int64_t)(s.chunk0 + c) * Q * p.sx_l;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_global_load_lds((glb_void*)(xc + (uint32_t)min(16 * i + (lane >> 2), rem - 1) * (uint32_t)p.sx_l + xcol),
-                                       (lds_void*)(&xbuf[c & 1][wave][16 * 32 * i]), 16, 0, 0);
-    const float* o = p.steps + ((int64_t)(s.unit0 + c) * p.H + h) * (4 * Q) + lane;
-    dv = o[0], cv = o[Q], wv = o[2 * Q];
-    if (kHalf && !STATES) mv = o[3 * Q], rv = p.rows[((int64_t)(s.unit0 + c) * p.G + g) * Q + lane];
+      sv_fetch16(xc, ((uint32_t)min(16 * i + (lane >> 2), rem - 1) * (uint32_t)p.sx_l + xcol) * 2u, &xbuf[c & 1][wave][16 * 32 * i]);
+    const float* o = p.steps + ((int64_t)(s.unit0 + c) * p.H + h) * (4 * Q);
+    uint32_t l = (uint32_t)lane;
+    asm volatile("" : "+v"(l));  // (a scalar base and this offset: sums of both kept over the loop are registers that it lacks)
+    dv = o[l], cv = o[l + Q], wv = o[l + 2 * Q];
+    if (kHalf && !STATES) mv = o[l + 3 * Q], rv = (p.rows + ((int64_t)(s.unit0 + c) * p.G + g) * Q)[l];
   };
   // What was requested is there; or it is but for the four stores behind it (memory operations end in order), which are not waited for.
   auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" : "+v"(dv), "+v"(cv), "+v"(wv), "+v"(mv), "+v"(rv)::"memory"); };
@@ -406,16 +412,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     asm volatile("s_barrier" ::: "memory");  // every wave's share of this chunk's operands is there
     if (live) {
       uint16_t* xw = xbuf[c & 1][wave];
+      uint16_t* xl = xw + 4 * hh * 32 + col;  // (entry(ks, hh, i) = entry(ks, 0, i) + 4 hh)
       lq_v4i xp[4];  // this lane's channel, tokens in the order of an operand
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          xp[ks][i] = (int)(xw[entry(ks, hh, 2 * i) * 32 + col] | (uint32_t)xw[entry(ks, hh, 2 * i + 1) * 32 + col] << 16);
+          xp[ks][i] = (int)(xl[entry(ks, 0, 2 * i) * 32] | (uint32_t)xl[entry(ks, 0, 2 * i + 1) * 32] << 16);
       auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
+      const float sum64 = cv, step = dv;  // (the next chunk's are requested below)
       const float last = lane63(cv), all = exp2_fast(last);
       decay += last;
-      float rescale = 1.0f, row = 1.0f;
+      float rescale = 1.0f, row = 1.0f, lrow = 0.0f, ui = 1.0f;
       if constexpr (kHalf) {
         // the wave's new unit: its state and what the chunk adds, each below 2^14 of it
         float m = 0.0f;
@@ -432,48 +440,77 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
             top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
           }
         const float mx = T::to((uint16_t)max(top & 0xffffu, top >> 16));
-        const float u = scale_for(wave_top(fmaxf(finite_size(m) * (1.0f / unit_S), finite_size(mx) * wave_top(finite_size(wv)))));
-        rescale = u / unit_S;
-        unit_S = u;
-        if (!STATES) row = scale_for(rv * mv);  // brings the token's row of weighted C B^T below 2^14
+        const float u = scale_for(wave_top(fmaxf(finite_size(m) * pow2_inverse(unit_S), finite_size(mx) * wave_top(finite_size(wv)))));
+        rescale = u * pow2_inverse(unit_S);
+        unit_S = u, ui = pow2_inverse(u);
+        if (!STATES) {
+          row = scale_for(rv * mv);  // brings the token's row of weighted C B^T below 2^14
+          lrow = (float)((int)(__float_as_uint(row) >> 23) - 127);
+        }
       }
-      const float ui = kHalf ? 1.0f / unit_S : 1.0f;
-      my[lane] = dv, my[Q + lane] = cv, my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
+      // The weight exp(c_t - c_s) d_s of an entry of C B^T.  Where no eight tokens decay by 2^60, it is r q: r = exp(c_t - c) for each row and
+      // block of eight tokens, c that in front of the block, and q = exp(c - c_s) d_s, at most 2^60 d_s: twelve exponentials a lane instead of
+      // 48, and what r rounds to zero is below 2^-66.
+      const float before = __shfl(cv, (lane & 56) - 1, 64), ahead = (lane < 8 ? 0.0f : before) - cv;
+      const bool apart = !STATES && __ballot(!(ahead < 60.0f)) == 0;
+      my[lane] = apart ? exp2_fast(ahead) * dv : dv, my[Q + lane] = cv;
+      my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
       if (more) request(c + 1);
       const lq_v4i* op = (const lq_v4i*)buf + lane;
       const lq_v4i* opB = op + (STATES ? 0 : (kCB + Tab::kC) / 16);
       v16f Y[2];
       if constexpr (!STATES) {  // exp(c_t) S C_t
         const lq_v4i* opC = op + kCB / 16;
+        lq_v4i cc[3][2];
+        auto ask = [&](int k) {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) cc[k % 3][tt] = opC[(tt * 2 * NT + k) * 64];
+        };
+        ask(0);
+        ask(1);
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) Y[tt][e] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 2 * NT; ++k) {
+          if (k + 2 < 2 * NT) ask(k + 2);
+          reads_stay();
           float v[8], r[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i], r[i] = rescale;
           lq_v4i sh, sl;
           split<T>(v, r, sh, sl);
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt) {
-            const lq_v4i cc = opC[(tt * 2 * NT + k) * 64];
-            Y[tt] = mfma<T>(cc, sh, Y[tt]);
-            Y[tt] = mfma<T>(cc, sl, Y[tt]);
-          }
+          for (int tt = 0; tt < 2; ++tt) Y[tt] = mfma<T>(cc[k % 3][tt], sh, Y[tt]);
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) Y[tt] = mfma<T>(cc[k % 3][tt], sl, Y[tt]);
         }
+      }
+      if constexpr (!STATES) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int tt = 0; tt < 2; ++tt) {
+          lq_v4f e4[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const lq_v4f e = *(const lq_v4f*)(my + 3 * Q + 32 * tt + 8 * j + 4 * hh);
+          for (int j = 0; j < 4; ++j) e4[j] = *(const lq_v4f*)(my + 3 * Q + 32 * tt + 8 * j + 4 * hh);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Y[tt][4 * j + i] *= e[i];
-          }
+          for (int e = 0; e < 16; ++e) Y[tt][e] *= e4[e >> 2][e & 3];
+        }
       }
       // the state behind the chunk
       {
+        lq_v4i bb[4];
+        lq_v4f w4[4][2];
+        auto ask = [&](int i) {  // operand i = NT ks + nt
+          bb[i & 3] = opB[(4 * (i % NT) + i / NT) * 64];
+          if (i % NT == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w4[i / NT][j] = *(const lq_v4f*)(my + 2 * Q + 16 * (i / NT) + 8 * j + 4 * hh);
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ask(i);
+        reads_stay();
         const float f = kHalf ? all * rescale : all;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -482,19 +519,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           float w[8], xv[8];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const lq_v4f v = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[4 * j + i] = v[i], xv[4 * j + i] = x(ks, 4 * j + i);
-          }
           lq_v4i wh, wl;
-          split<T>(w, xv, wh, wl);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const lq_v4i bb = opB[(4 * nt + ks) * 64];
-            S[nt] = mfma<T>(bb, wh, S[nt]);
-            S[nt] = mfma<T>(bb, wl, S[nt]);
+            const int i = NT * ks + nt;
+            if (i + 3 < 4 * NT) ask(i + 3);
+            reads_stay();
+            if (nt == 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = w4[ks][e >> 2][e & 3], xv[e] = x(ks, e);
+              split<T>(w, xv, wh, wl);
+            }
+            S[nt] = mfma<T>(bb[i & 3], wh, S[nt]);
+            S[nt] = mfma<T>(bb[i & 3], wl, S[nt]);
           }
         }
       }
@@ -502,41 +539,75 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         // An activation that is no number must not reach the tokens in front of it, which the product below multiplies by zero: the state,
         // which all of the chunk's tokens reach, tells.  Then such tokens are left out and every output from them on is NaN.
         const bool odd = bad || __ballot(S[0][0] != S[0][0]) != 0;
-        int from = bad ? 0 : Q;
+        int from = bad ? -4 : Q;  // counted from token 4 hh, as this lane's entries are
         if (odd) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               if (!(__builtin_fabsf(x(ks, i)) < __builtin_inff())) {
-                from = min(from, entry(ks, hh, i));
+                from = min(from, entry(ks, 0, i));
                 xp[ks][i >> 1] &= i & 1 ? 0xffff : 0xffff0000;
               }
-          from = min(from, __shfl_xor(from, 32, 64));
+          from = min(from, __shfl_xor(from, 32, 64) + (hh ? -4 : 4));
         }
         const lq_v4f* cb = (const lq_v4f*)buf + lane;
-        if (kHalf) my[2 * Q + lane] = 1.0f / row;
+        if (kHalf) my[2 * Q + lane] = pow2_inverse(row);
+        float ct[2];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          float ct = my[Q + 32 * tt + col];
-          if (kHalf) ct += (float)(127 - (int)(__float_as_uint(my[2 * Q + 32 * tt + col]) >> 23));  // (a power of two times the row)
+        for (int tt = 0; tt < 2; ++tt) ct[tt] = __shfl(sum64 + lrow, 32 * tt + col, 64);
+        // six steps: rows tt, tokens ks (above the diagonal C B^T is stored as zero)
+        constexpr int kT[6] = {0, 1, 0, 1, 1, 1}, kS[6] = {0, 0, 1, 1, 2, 3};
+        auto add = [&](int n, const float (&f)[8], const float (&a)[8]) {
+          lq_v4i mh, ml;
+          split<T>(f, a, mh, ml);
+          Y[kT[n]] = mfma<T>(mh, xp[kS[n]], Y[kT[n]]);
+          Y[kT[n]] = mfma<T>(ml, xp[kS[n]], Y[kT[n]]);
+        };
+        if (apart && !odd) {
+          lq_v4f f4[2][2], q4[2][2];  // (the q of a ks serve two steps)
+          auto ask = [&](int n) {
 #pragma unroll
-          for (int ks = 0; ks < 2 * tt + 2; ++ks) {
+            for (int j = 0; j < 2; ++j) {
+              f4[n & 1][j] = cb[((kT[n] * 2 + kS[n]) * 2 + j) * 64];
+              if (n == 0 || kS[n] != kS[n - 1]) q4[kS[n] & 1][j] = *(const lq_v4f*)(my + 16 * kS[n] + 8 * j + 4 * hh);
+            }
+          };
+          ask(0);
+#pragma unroll
+          for (int n = 0; n < 6; ++n) {
+            if (n < 5) ask(n + 1);
+            reads_stay();
             float f[8], a[8];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const lq_v4f v = cb[((tt * 2 + ks) * 2 + j) * 64];
-              const lq_v4f cs = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh), ds = *(const lq_v4f*)(my + 16 * ks + 8 * j + 4 * hh);
+              const int kb = 2 * kS[n] + j;
+              // (rows in front of the block, whose entries are zero, must not overflow)
+              const float r = exp2_fast(fminf(ct[kT[n]] - (kb ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum64), 8 * kb - 1)) : 0.0f), 30.0f));
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {  // (above the diagonal C B^T is stored as zero)
-                const float m = exp2_fast(ct - cs[i]) * ds[i];
-                f[4 * j + i] = v[i], a[4 * j + i] = ks >= 2 * tt && entry(ks - 2 * tt, hh, 4 * j + i) > col ? 0.0f : m;
+              for (int i = 0; i < 4; ++i) f[4 * j + i] = f4[n & 1][j][i], a[4 * j + i] = r * q4[kS[n] & 1][j][i];
+            }
+            add(n, f, a);
+          }
+        } else {
+          my[lane] = step;
+#pragma unroll
+          for (int n = 0; n < 6; ++n) {
+            __builtin_amdgcn_sched_barrier(0);  // (a seldom way: nothing of it is worth a register elsewhere)
+            int t = col;
+            asm volatile("" : "+v"(t));
+            float f[8], a[8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const lq_v4f f4 = cb[((kT[n] * 2 + kS[n]) * 2 + j) * 64];
+              const lq_v4f c4 = *(const lq_v4f*)(my + Q + 16 * kS[n] + 8 * j + 4 * hh), d4 = *(const lq_v4f*)(my + 16 * kS[n] + 8 * j + 4 * hh);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float m = exp2_fast(ct[kT[n]] - c4[i]) * d4[i];
+                f[4 * j + i] = f4[i], a[4 * j + i] = kS[n] >= 2 * kT[n] && entry(kS[n] - 2 * kT[n], hh, 4 * j + i) > t ? 0.0f : m;
               }
             }
-            lq_v4i mh, ml;
-            split<T>(f, a, mh, ml);
-            Y[tt] = mfma<T>(mh, xp[ks], Y[tt]);
-            Y[tt] = mfma<T>(ml, xp[ks], Y[tt]);
+            add(n, f, a);
           }
         }
         taken(c);
@@ -545,19 +616,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (entry(ks, hh, i) >= from) Y[ks >> 1][8 * (ks & 1) + i] = __builtin_nanf("");
+              if (entry(ks, 0, i) >= from) Y[ks >> 1][8 * (ks & 1) + i] = __builtin_nanf("");
         }
         // out through the place of x (the wave's own, read above): [token][channel], then 16 bytes a lane
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            reads_stay();
             lq_v4f ri;
             if (kHalf) ri = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float v = Y[ks >> 1][8 * (ks & 1) + 4 * j + i], xi = x(ks, 4 * j + i);
-              xw[entry(ks, hh, 4 * j + i) * 32 + col] = T::from(kHalf ? __builtin_fmaf(v, ri[i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
+              xl[entry(ks, 0, 4 * j + i) * 32] = T::from(kHalf ? __builtin_fmaf(v, ri[i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
             }
           }
         lq_v4i yo[4];
