@@ -122,7 +122,7 @@ LQ_DEV Unit sv_locate(const int32_t* __restrict__ starts, int nseq, int tokens, 
 // (m0 cannot be named as overwritten; nothing else in a kernel that calls this may need it: no __builtin_amdgcn_global_load_lds.)
 LQ_DEV void sv_fetch16(const void* base, uint32_t offset, const void* at) {
   typedef const __attribute__((address_space(3))) char lds_char;
-  const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)at);
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)at;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 

@@ -110,6 +110,13 @@ LQ_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 LQ_DEV float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
 // a power of two's reciprocal
 LQ_DEV float pow2_inverse(float v) { return __uint_as_float(0x7f000000u - __float_as_uint(v)); }
+// Four rows of 16 entries of 16 bits, given by the 16 lanes of a quarter of the wave as four pieces a row, come back by columns: lane i has
+// entry i of the rows
+LQ_DEV lq_v2i read_columns(const void* at) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  return __builtin_bit_cast(lq_v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at));
+}
 // LDS reads stay where they are written (everything else may move): as the compiler orders them, most stand right in front of their use
 LQ_DEV void reads_stay() { __builtin_amdgcn_sched_barrier(0xf); }
 // |v|, or 0 for what is no number and must not set a scale
@@ -323,12 +330,12 @@ constexpr int W = 4;  // waves of a workgroup
 // way, 64 tokens x 32 channels, a chunk ahead into one of two places, and its y leaves through the same place.  Two workgroups share a
 // compute unit, so that one computes while the other's operands are on their way.
 template <typename T, int NT, bool STATES>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void ssm_chunks_kernel(PromptParams p) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : STATES ? 3 : 2, NT == 8 ? 1 : STATES ? 3 : 2))) void ssm_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
   using Tab = Table<NT>;
   constexpr int kSkip = STATES ? kCB + Tab::kC : 0, kLoad = Tab::kBytes - kSkip;  // bytes of a chunk's operands that are needed
   __shared__ __align__(16) char buf[kLoad];
-  __shared__ __align__(16) uint16_t xbuf[2][W][Q * 32];
+  __shared__ __align__(256) uint16_t xbuf[2][W][Q * 32];
   __shared__ __align__(16) float tok[W][4 * Q];  // each wave's d, c, w, exp2(c) (fp16: scaled)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   int sg, part;
@@ -347,7 +354,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   const int slot = p.state || p.slots ? uniform(sv_slot(p.slots, s.seq, p.num_slots)) : kSlotPad;
   const bool keeps = p.state && slot >= 0;
   const int64_t row0 = (p.starts ? s.begin : (int64_t)s.seq * p.seqlen);  // of the dense output
-  const uint16_t* xs = p.x + (p.starts ? s.begin * p.sx_l : s.seq * p.sx_b) + h * p.sx_h + ch0;
   uint16_t* os = p.out + (row0 * p.H + h) * p.P + ch0;
   const int64_t ostride = (int64_t)p.H * p.P;
 
@@ -373,88 +379,104 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   // what a chunk needs, requested while the one in front of it is worked on.  x: four rows of 16 bytes a lane, 8 channels each; tokens
   // behind the prompt read its last one again (at weight zero), channels behind the head its last eight.
   const char* tab = p.tables + ((int64_t)s.unit0 * p.G + g) * Tab::kBytes + kSkip;
+  const uint16_t* xs = p.x + (p.starts ? s.begin * p.sx_l : s.seq * p.sx_b) + h * p.sx_h + ch0 + (int64_t)s.chunk0 * Q * p.sx_l;
+  const float* steps = p.steps + ((int64_t)s.unit0 * p.H + h) * (4 * Q);
+  const float* rows = p.rows + ((int64_t)s.unit0 * p.G + g) * Q;
+  int left = s.len - s.chunk0 * Q;  // tokens that are not requested yet
   const uint32_t xcol = (uint32_t)min(8 * (lane & 3), p.P - 8 - ch0);
-  float dv = 0.f, cv = 0.f, wv = 0.f, mv = 0.f, rv = 0.f;
-  auto fetch = [&](int c) {
-    const char* src = tab + (int64_t)c * p.G * Tab::kBytes;
+  uint32_t xoff[4];
 #pragma unroll
-    for (int k = 0; k < kLoad / 1024 / W; ++k)
-      sv_fetch16(src + (k * W + wave) * 1024, (uint32_t)lane * 16u, buf + (k * W + wave) * 1024);
+  for (int i = 0; i < 4; ++i) xoff[i] = ((uint32_t)(16 * i + (lane >> 2)) * (uint32_t)p.sx_l + xcol) * 2u;
+  float dv = 0.f, cv = 0.f, wv = 0.f, mv = 0.f, rv = 0.f;
+  auto fetch = [&] {  // the next chunk's operands
+#pragma unroll
+    for (int k = 0; k < kLoad / (1024 * W); ++k) sv_fetch16(tab + (k * W + wave) * 1024, (uint32_t)lane * 16u, buf + (k * W + wave) * 1024);
+    tab += (int64_t)p.G * Tab::kBytes;
   };
   static_assert(kLoad % (1024 * W) == 0);
-  auto request = [&](int c) {
-    const int rem = s.len - (s.chunk0 + c) * Q;
-    const uint16_t* xc = xs + (int64_t)(s.chunk0 + c) * Q * p.sx_l;
+  auto request = [&](int c) {  // the next chunk's x and step sizes
+    uint16_t* to = xbuf[c & 1][wave];
+    if (left >= Q) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      sv_fetch16(xc, ((uint32_t)min(16 * i + (lane >> 2), rem - 1) * (uint32_t)p.sx_l + xcol) * 2u, &xbuf[c & 1][wave][16 * 32 * i]);
-    const float* o = p.steps + ((int64_t)(s.unit0 + c) * p.H + h) * (4 * Q);
+      for (int i = 0; i < 4; ++i) sv_fetch16(xs, xoff[i], to + 16 * 32 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sv_fetch16(xs, ((uint32_t)min(16 * i + (lane >> 2), left - 1) * (uint32_t)p.sx_l + xcol) * 2u, to + 16 * 32 * i);
+    }
     uint32_t l = (uint32_t)lane;
     asm volatile("" : "+v"(l));  // (a scalar base and this offset: sums of both kept over the loop are registers that it lacks)
-    dv = o[l], cv = o[l + Q], wv = o[l + 2 * Q];
-    if (kHalf && !STATES) mv = o[l + 3 * Q], rv = (p.rows + ((int64_t)(s.unit0 + c) * p.G + g) * Q)[l];
+    dv = steps[l], cv = steps[l + Q], wv = steps[l + 2 * Q];
+    if (kHalf && !STATES) mv = steps[l + 3 * Q], rv = rows[l];
+    xs += Q * p.sx_l, steps += (int64_t)p.H * (4 * Q), rows += (int64_t)p.G * Q, left -= Q;
   };
-  // What was requested is there; or it is but for the four stores behind it (memory operations end in order), which are not waited for.
+  // Everything is there; or all but the last four stores (memory operations end in order), which are not waited for.
   auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" : "+v"(dv), "+v"(cv), "+v"(wv), "+v"(mv), "+v"(rv)::"memory"); };
-  auto arrived_before_stores = [&] { asm volatile("s_waitcnt vmcnt(4)" : "+v"(dv), "+v"(cv), "+v"(wv), "+v"(mv), "+v"(rv)::"memory"); };
+  auto all_but_stores = [&] { asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); };
   // every wave has read all of a chunk's operands: the next chunk's take their place
   auto taken = [&](int c) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (c + 1 < s.chunks) fetch(c + 1);
+    if (c + 1 < s.chunks) fetch();
   };
-  fetch(0);
+  fetch();
   if (live) request(0);
   arrived();
+  // What a chunk's products need of the wave's own: x in registers, step sizes in LDS, the state's unit.  Done at the end of the chunk in
+  // front, whose operands' successors are then on their way.
   float decay = 0.0f;
   float* my = tok[wave];
+  lq_v4i xp[4];  // this lane's channel, tokens in the order of an operand
+  auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
+  float sum64 = 0.0f, step = 0.0f, all = 0.0f, rescale = 1.0f, row = 1.0f, lrow = 0.0f;
+  bool apart = false;
+  auto begin = [&](int c) {
+    const uint16_t* xl = xbuf[c & 1][wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const lq_v2i lo = read_columns(xl + 16 * ks * 32), hi = read_columns(xl + (16 * ks + 8) * 32);
+      xp[ks] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
+    }
+    sum64 = cv, step = dv;  // (the next chunk's are requested soon)
+    const float last = lane63(cv);
+    all = exp2_fast(last);
+    decay += last;
+    float ui = 1.0f;
+    if constexpr (kHalf) {
+      // the wave's new unit: its state and what the chunk adds, each below 2^14 of it
+      float m = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(S[nt][e]));
+      uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          typedef uint16_t v2u __attribute__((ext_vector_type(2)));
+          top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
+        }
+      const float mx = T::to((uint16_t)max(top & 0xffffu, top >> 16));
+      const float u = scale_for(wave_top(fmaxf(finite_size(m) * pow2_inverse(unit_S), finite_size(mx) * wave_top(finite_size(wv)))));
+      rescale = u * pow2_inverse(unit_S);
+      unit_S = u, ui = pow2_inverse(u);
+      if (!STATES) {
+        row = scale_for(rv * mv);  // brings the token's row of weighted C B^T below 2^14
+        lrow = (float)((int)(__float_as_uint(row) >> 23) - 127);
+      }
+    }
+    // The weight exp(c_t - c_s) d_s of an entry of C B^T.  Where no eight tokens decay by 2^60, it is r q: r = exp(c_t - c) for each row and
+    // block of eight tokens, c that in front of the block, and q = exp(c - c_s) d_s, at most 2^60 d_s: twelve exponentials a lane instead of
+    // 48, and what r rounds to zero is below 2^-66.
+    const float before = __shfl(cv, (lane & 56) - 1, 64), ahead = (lane < 8 ? 0.0f : before) - cv;
+    apart = !STATES && __ballot(!(ahead < 60.0f)) == 0;
+    my[lane] = apart ? exp2_fast(ahead) * dv : dv, my[Q + lane] = cv;
+    my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
+  };
+  if (live) begin(0);
   for (int c = 0; c < s.chunks; ++c) {
     const bool more = c + 1 < s.chunks;
     asm volatile("s_barrier" ::: "memory");  // every wave's share of this chunk's operands is there
     if (live) {
-      uint16_t* xw = xbuf[c & 1][wave];
-      uint16_t* xl = xw + 4 * hh * 32 + col;  // (entry(ks, hh, i) = entry(ks, 0, i) + 4 hh)
-      lq_v4i xp[4];  // this lane's channel, tokens in the order of an operand
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          xp[ks][i] = (int)(xl[entry(ks, 0, 2 * i) * 32] | (uint32_t)xl[entry(ks, 0, 2 * i + 1) * 32] << 16);
-      auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
-      const float sum64 = cv, step = dv;  // (the next chunk's are requested below)
-      const float last = lane63(cv), all = exp2_fast(last);
-      decay += last;
-      float rescale = 1.0f, row = 1.0f, lrow = 0.0f, ui = 1.0f;
-      if constexpr (kHalf) {
-        // the wave's new unit: its state and what the chunk adds, each below 2^14 of it
-        float m = 0.0f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(S[nt][e]));
-        uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            typedef uint16_t v2u __attribute__((ext_vector_type(2)));
-            top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
-          }
-        const float mx = T::to((uint16_t)max(top & 0xffffu, top >> 16));
-        const float u = scale_for(wave_top(fmaxf(finite_size(m) * pow2_inverse(unit_S), finite_size(mx) * wave_top(finite_size(wv)))));
-        rescale = u * pow2_inverse(unit_S);
-        unit_S = u, ui = pow2_inverse(u);
-        if (!STATES) {
-          row = scale_for(rv * mv);  // brings the token's row of weighted C B^T below 2^14
-          lrow = (float)((int)(__float_as_uint(row) >> 23) - 127);
-        }
-      }
-      // The weight exp(c_t - c_s) d_s of an entry of C B^T.  Where no eight tokens decay by 2^60, it is r q: r = exp(c_t - c) for each row and
-      // block of eight tokens, c that in front of the block, and q = exp(c - c_s) d_s, at most 2^60 d_s: twelve exponentials a lane instead of
-      // 48, and what r rounds to zero is below 2^-66.
-      const float before = __shfl(cv, (lane & 56) - 1, 64), ahead = (lane < 8 ? 0.0f : before) - cv;
-      const bool apart = !STATES && __ballot(!(ahead < 60.0f)) == 0;
-      my[lane] = apart ? exp2_fast(ahead) * dv : dv, my[Q + lane] = cv;
-      my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
       if (more) request(c + 1);
       const lq_v4i* op = (const lq_v4i*)buf + lane;
       const lq_v4i* opB = op + (STATES ? 0 : (kCB + Tab::kC) / 16);
@@ -610,6 +632,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
             add(n, f, a);
           }
         }
+        arrived();  // (requested at the chunk's beginning)
         taken(c);
         if (odd) {
 #pragma unroll
@@ -618,7 +641,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
             for (int i = 0; i < 8; ++i)
               if (entry(ks, 0, i) >= from) Y[ks >> 1][8 * (ks & 1) + i] = __builtin_nanf("");
         }
-        // out through the place of x (the wave's own, read above): [token][channel], then 16 bytes a lane
+        // Out through the place of x (the wave's own, and in registers since the chunk's beginning): [channel][block of four tokens], block b
+        // at place b ^ channel % 16, and back by columns, 16 tokens of eight channels a lane.
+        char* yw = (char*)xbuf[c & 1][wave];
+        const uint32_t y0 = (uint32_t)(col * 128 + ((hh ^ (col & 15)) * 8));
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -626,30 +652,43 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
             reads_stay();
             lq_v4f ri;
             if (kHalf) ri = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
+            sv_v4u y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float v = Y[ks >> 1][8 * (ks & 1) + 4 * j + i], xi = x(ks, 4 * j + i);
-              xl[entry(ks, 0, 4 * j + i) * 32] = T::from(kHalf ? __builtin_fmaf(v, ri[i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
+              y[i] = T::from(kHalf ? __builtin_fmaf(v, ri[i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
             }
+            *(sv_v4u*)(yw + (y0 ^ (32 * ks + 16 * j))) = y;
           }
         lq_v4i yo[4];
+        {
+          const int q8 = 8 * (lane >> 4) + ((lane & 15) >> 2);  // channels q8 and q8 + 4 of this lane's pieces
+          const uint32_t a0 = (uint32_t)(q8 * 128 + (((lane & 3) ^ (q8 & 15)) * 8)), a1 = (uint32_t)((q8 + 4) * 128 + (((lane & 3) ^ ((q8 + 4) & 15)) * 8));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) yo[i] = *(const lq_v4i*)(xw + 16 * 32 * i + lane * 8);
+          for (int i = 0; i < 4; ++i) {
+            const lq_v2i lo = read_columns(yw + (a0 ^ (32 * i))), hi = read_columns(yw + (a1 ^ (32 * i)));
+            yo[i] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
+          }
+        }
         const int rem = s.len - (s.chunk0 + c) * Q;
         uint16_t* oc = os + (int64_t)(s.chunk0 + c) * Q * ostride;
-        const uint32_t o0 = (uint32_t)(lane >> 2) * (uint32_t)ostride + 8 * (lane & 3);
+        const uint32_t o0 = (uint32_t)(lane & 15) * (uint32_t)ostride + 8 * (lane >> 4);
         if (rem >= Q && ch0 + 32 <= p.P) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
-          arrived_before_stores();
+          if (more) begin(c + 1);
+          all_but_stores();
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (16 * i + (lane >> 2) < rem && ch0 + 8 * (lane & 3) < p.P) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
+            if (16 * i + (lane & 15) < rem && ch0 + 8 * (lane >> 4) < p.P) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
+          if (more) begin(c + 1);
           arrived();
         }
       } else {
+        arrived();
         taken(c);
+        if (more) begin(c + 1);
         arrived();
       }
     } else {
