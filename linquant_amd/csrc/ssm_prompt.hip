@@ -336,7 +336,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   constexpr int kSkip = STATES ? kCB + Tab::kC : 0, kLoad = Tab::kBytes - kSkip;  // bytes of a chunk's operands that are needed
   __shared__ __align__(16) char buf[kLoad];
   __shared__ __align__(256) uint16_t xbuf[2][W][Q * 32];
-  __shared__ __align__(16) float tok[W][4 * Q];  // each wave's d, c, w, exp2(c) (fp16: scaled)
+  __shared__ __align__(16) float tok[W][3 * Q];  // each wave's q (or d), w, exp2(c) (fp16: scaled)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   int sg, part;
   place(p, sg, part);
@@ -469,8 +469,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     // 48, and what r rounds to zero is below 2^-66.
     const float before = __shfl(cv, (lane & 56) - 1, 64), ahead = (lane < 8 ? 0.0f : before) - cv;
     apart = !STATES && __ballot(!(ahead < 60.0f)) == 0;
-    my[lane] = apart ? exp2_fast(ahead) * dv : dv, my[Q + lane] = cv;
-    my[2 * Q + lane] = kHalf ? wv * unit_S : wv, my[3 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
+    my[lane] = apart ? exp2_fast(ahead) * dv : dv;
+    my[Q + lane] = kHalf ? wv * unit_S : wv, my[2 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
   };
   if (live) begin(0);
   for (int c = 0; c < s.chunks; ++c) {
@@ -514,7 +514,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         for (int tt = 0; tt < 2; ++tt) {
           lq_v4f e4[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) e4[j] = *(const lq_v4f*)(my + 3 * Q + 32 * tt + 8 * j + 4 * hh);
+          for (int j = 0; j < 4; ++j) e4[j] = *(const lq_v4f*)(my + 2 * Q + 32 * tt + 8 * j + 4 * hh);
 #pragma unroll
           for (int e = 0; e < 16; ++e) Y[tt][e] *= e4[e >> 2][e & 3];
         }
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           bb[i & 3] = opB[(4 * (i % NT) + i / NT) * 64];
           if (i % NT == 0) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) w4[i / NT][j] = *(const lq_v4f*)(my + 2 * Q + 16 * (i / NT) + 8 * j + 4 * hh);
+            for (int j = 0; j < 2; ++j) w4[i / NT][j] = *(const lq_v4f*)(my + Q + 16 * (i / NT) + 8 * j + 4 * hh);
           }
         };
 #pragma unroll
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           from = min(from, __shfl_xor(from, 32, 64) + (hh ? -4 : 4));
         }
         const lq_v4f* cb = (const lq_v4f*)buf + lane;
-        if (kHalf) my[2 * Q + lane] = pow2_inverse(row);
+        if (kHalf) my[Q + lane] = pow2_inverse(row);
         float ct[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) ct[tt] = __shfl(sum64 + lrow, 32 * tt + col, 64);
@@ -612,7 +612,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
             add(n, f, a);
           }
         } else {
-          my[lane] = step;
+          my[lane] = step, my[2 * Q + lane] = sum64;
 #pragma unroll
           for (int n = 0; n < 6; ++n) {
             __builtin_amdgcn_sched_barrier(0);  // (a seldom way: nothing of it is worth a register elsewhere)
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const lq_v4f f4 = cb[((kT[n] * 2 + kS[n]) * 2 + j) * 64];
-              const lq_v4f c4 = *(const lq_v4f*)(my + Q + 16 * kS[n] + 8 * j + 4 * hh), d4 = *(const lq_v4f*)(my + 16 * kS[n] + 8 * j + 4 * hh);
+              const lq_v4f c4 = *(const lq_v4f*)(my + 2 * Q + 16 * kS[n] + 8 * j + 4 * hh), d4 = *(const lq_v4f*)(my + 16 * kS[n] + 8 * j + 4 * hh);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float m = exp2_fast(ct[kT[n]] - c4[i]) * d4[i];
@@ -645,18 +645,23 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         // at place b ^ channel % 16, and back by columns, 16 tokens of eight channels a lane.
         char* yw = (char*)xbuf[c & 1][wave];
         const uint32_t y0 = (uint32_t)(col * 128 + ((hh ^ (col & 15)) * 8));
+        lq_v4f r4[4][2];
+        if (kHalf) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) r4[ks][j] = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh);
+        }
+        reads_stay();
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            reads_stay();
-            lq_v4f ri;
-            if (kHalf) ri = *(const lq_v4f*)(my + 2 * Q + 16 * ks + 8 * j + 4 * hh);
             sv_v4u y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float v = Y[ks >> 1][8 * (ks & 1) + 4 * j + i], xi = x(ks, 4 * j + i);
-              y[i] = T::from(kHalf ? __builtin_fmaf(v, ri[i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
+              y[i] = T::from(kHalf ? __builtin_fmaf(v, r4[ks][j][i], __builtin_fmaf(Dv, xi, 0.0f)) : __builtin_fmaf(Dv, xi, v));
             }
             *(sv_v4u*)(yw + (y0 ^ (32 * ks + 16 * j))) = y;
           }
