@@ -16,6 +16,7 @@
 // multiplication by a power of two that brings the largest of what is multiplied (a channel's state and weighted x; C B^T of the chunk)
 // below 2^14, so no size of activations overflows a piece, and what is 2^28 times smaller than that largest starts to lose bits.
 #include <algorithm>
+#include <cmath>
 
 #include "serve_common.h"
 
@@ -719,26 +720,52 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 }
 
 // The state in front of each segment, in the place of what the segment adds to one (the last one's is not read).  A workgroup has 1024
-// entries of one head's state and finds the sequence's segments as the other kernels do.
+// entries of one head's state.
 __global__ __launch_bounds__(256) void ssm_join_kernel(PromptParams p) {
   const int64_t per = (int64_t)p.P * p.N;
-  const int h = blockIdx.y, at = (blockIdx.z * 256 + threadIdx.x) * 4;
-  const Segment s0 = segment_of(p, blockIdx.x);
-  if (s0.seq < 0 || !s0.first || s0.last) return;  // a sequence's first segment walks the others
+  const int h = blockIdx.y, at = (blockIdx.z * 256 + threadIdx.x) * 4, seq = blockIdx.x;
+  // the sequence's segments, and how many there are in front of them
+  auto segments = [&](int i) {
+    int b = 0, e = p.seqlen;
+    if (p.starts) {
+      b = p.starts[i], e = p.starts[i + 1];
+      if (b < 0 || e > p.tokens || e < b) b = e = 0;
+    }
+    return ((int)(((uint32_t)(e - b) + (Q - 1)) / Q) + p.seg_chunks - 1) / p.seg_chunks;
+  };
+  const int n = segments(seq);
+  if (n < 2) return;
+  int first = 0;
+  if (p.starts) {
+    for (int i = threadIdx.x & 63; i < seq; i += 64) first += segments(i);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) first += __shfl_xor(first, off, 64);
+  } else {
+    first = seq * n;
+  }
   if (at >= per) return;
-  const int slot = p.state || p.slots ? sv_slot(p.slots, s0.seq, p.num_slots) : kSlotPad;
+  const int slot = p.state || p.slots ? sv_slot(p.slots, seq, p.num_slots) : kSlotPad;
   lq_v4f v = {0.f, 0.f, 0.f, 0.f};
   if (p.state && slot >= 0) v = *(const lq_v4f*)(p.state + slot * p.ss_s + h * per + at);
-  const int nc = (s0.len + Q - 1) / Q, n = (nc + p.seg_chunks - 1) / p.seg_chunks;
-  for (int i = 0; i < n; ++i) {
-    const int64_t sg = blockIdx.x + i;
-    lq_v4f* o = (lq_v4f*)(p.seg_state + (sg * p.H + h) * per + at);
-    const lq_v4f add = *o;
-    *o = v;
-    if (i + 1 < n) {
-      const float d = p.seg_decay[sg * p.H + h];
+  // four segments requested at a time: a chain of one load after the other was most of this kernel
+  constexpr int U = 4;
+  float* base = p.seg_state + ((int64_t)first * p.H + h) * per + at;
+  const float* dec = p.seg_decay + (int64_t)first * p.H + h;
+  const int64_t next = (int64_t)p.H * per;
+  for (int i = 0; i < n; i += U) {
+    lq_v4f add[U];
+    float d[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d, v[e], add[e]);
+    for (int u = 0; u < U; ++u) {
+      const int k = min(i + u, n - 1);
+      add[u] = *(const lq_v4f*)(base + k * next), d[u] = dec[(int64_t)k * p.H];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= n) break;
+      *(lq_v4f*)(base + (i + u) * next) = v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d[u], v[e], add[u][e]);  // (behind the last one: not used)
     }
   }
 }
@@ -766,17 +793,21 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   const int64_t blocks = (int64_t)(a->nheads / a->ngroups) * ((a->headdim + 31) / 32);
   r.per_group = (int)((blocks + W - 1) / W);
   const int64_t parts = (int64_t)a->ngroups * r.per_group;
-  // Chunk steps in a row that the chip takes for segments of n chunks, two workgroups to a compute unit, 512 at a time; cut prompts
-  // need their states first and the join.
-  const int64_t even = std::max<int64_t>(1, r.units / nseq);  // a packed call's prompts are taken to be of one length
-  // in tenths of a microsecond: a step 35, one of the states' 15, and the segments' states written, joined and read at 3 TB/s
-  int64_t best = -1;
+  // Tenths of a microsecond.  A chunk's step takes 50 where a compute unit has one workgroup and 84 where it has two; one of the states' 25
+  // and about 9 for each further; the join moves the segments' states three times at 3 TB/s, and it and two more launches come to 250.  The
+  // lengths of packed prompts are not known here: the longest is taken to be two and a half times the mean.
+  const double mean = (double)r.units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
+  auto step = [](double wgs, double one, double more) {
+    const double n = std::max(1.0, wgs / 256);
+    return n <= 2 ? one + more * (n - 1) : (one + more) * std::ceil(n / 2);
+  };
+  double best = chain * step((double)nseq * parts, 50, 34);
   r.seg_chunks = (int)most, r.cut = 0;
-  for (int64_t k = 1; k <= 64 && (k == 1 || even / k >= 2); ++k) {
-    const int64_t n = (even + k - 1) / k, segs = nseq * ((even + n - 1) / n);
-    const int64_t rounds = (segs * parts + 511) / 512, move = segs * a->nheads * a->headdim * a->dstate * 16 / 300000 + 100;
-    const int64_t cost = k == 1 ? rounds * n * 35 : rounds * n * 35 + ((segs - nseq) * parts + 511) / 512 * n * 15 + move;
-    if (best < 0 || cost < best) best = cost, r.seg_chunks = k == 1 ? (int)most : (int)n, r.cut = k > 1;
+  for (int64_t k = 2; k <= 256; ++k) {  // segments of the longest
+    const int64_t n = std::max<int64_t>(1, (int64_t)std::ceil(chain / k));
+    const double segs = a->seq_starts ? (double)r.units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n));
+    const double cost = n * (step(segs * parts, 50, 34) + step(std::max(0.0, segs - nseq) * parts, 25, 9)) + segs * a->nheads * a->headdim * a->dstate * 12 / 3e5 + 250;
+    if (n < most && cost < best) best = cost, r.seg_chunks = (int)n, r.cut = 1;
   }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
   r.segs = a->seq_starts ? std::min<int64_t>(r.units / r.seg_chunks + nseq, r.units) : nseq * per;
@@ -827,7 +858,7 @@ extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
   const dim3 pre((unsigned)pl.units, (unsigned)(a->ngroups + (a->nheads + kHeads - 1) / kHeads));
   const dim3 grid((unsigned)((pl.segs * a->ngroups * pl.per_group + 7) / 8 * 8)), threads(64 * W);
   const int64_t per = (int64_t)a->headdim * a->dstate;
-  const dim3 join((unsigned)pl.segs, (unsigned)a->nheads, (unsigned)((per + 1023) / 1024));
+  const dim3 join((unsigned)a->nseq, (unsigned)a->nheads, (unsigned)((per + 1023) / 1024));
   if (join.y > 65535 || join.z > 65535) return LQ_ERR_SHAPE;
   auto go = [&](auto t, auto k) {
     using T = decltype(t);
