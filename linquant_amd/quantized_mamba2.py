@@ -13,10 +13,17 @@ Pipeline of ``forward`` (linquant/quantized_mamba2.py:205-378):
 The two projections are not part of this package: ``Int8InputLinear`` stands in for the W4A8 Marlin linear with the
 same ``input_scale`` / ``forward_int8(x_i8, scale)`` surface and an fp16 GEMM from torch behind it, so the mixer runs
 end to end on a ROCm build and the stage names below can be re-bound for per-stage timing exactly like
-bench/mamba2_components.py:56-77 of the reference does.
+bench/mamba2_components.py:56-77 of the reference does.  ``linear=W8A8Linear`` puts this package's INT8 product in their place.
+
+``forward`` is the reference's prefill and keeps nothing.  ``prefill`` and ``step`` serve: they carry each sequence's last
+convolution inputs and its fp32 state from call to call in the slots of a ``Mamba2State``, for prompts of any lengths (whole, in
+parts, packed) and for one token of each sequence, with the convolution and the scan in 16 bits between the same two projections.
+``Mamba2Block`` puts the residual stream and its norm around a mixer.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
@@ -24,9 +31,11 @@ import torch.nn as nn
 from linquant_amd.hadamard_utils import qhad_transform
 from linquant_amd.kernels.hadamard import kronecker_hadamard_fwd  # noqa: F401  (kept re-bindable like the reference's import)
 from linquant_amd.kernels.mamba2.causal_conv1d import causal_conv1d_fn
+from linquant_amd.kernels.mamba2.conv1d_state import conv1d_prompt, conv1d_step
 from linquant_amd.kernels.mamba2.fused_split_rotate_xBC import fused_split_rotate_quant_xBC, prepare_dqk
 from linquant_amd.kernels.mamba2.ssd_combined import _quant_mamba_chunk_scan_combined_fwd
-from linquant_amd.norm import RMSNormGated, rmsnorm_gated_qhad
+from linquant_amd.kernels.mamba2.ssm import ssm_prompt, ssm_step
+from linquant_amd.norm import RMSNormGated, residual_rmsnorm, rmsnorm_gated_qhad
 from linquant_amd.w4a8_linear import _fused_fp16_to_int8
 
 
@@ -61,6 +70,13 @@ class Int8InputLinear(nn.Module):
         return self.forward_int8(q.view(x.shape), self.input_scale)
 
 
+class Mamba2State(NamedTuple):
+    """What sequences leave for their next tokens, a slot for each; zeros are the state of a sequence without tokens."""
+
+    conv: torch.Tensor  # (slots, d_conv - 1, conv_dim) fp16: the last inputs of the convolution, oldest first
+    ssm: torch.Tensor   # (slots, nheads, headdim, d_state) fp32
+
+
 class QuantizedMamba2(nn.Module):
     """Calibrated buffers attached after construction, as in the reference: B_scale/B_inv_scale, C_scale/C_inv_scale
     (G,), A_log_scale, D_scale (scalars), alpha_hp (H, P), bscale_g (G,), static_state_scale (H, P), static_cb_scale
@@ -79,11 +95,14 @@ class QuantizedMamba2(nn.Module):
         self.register_buffer("A_log", A_log)   # INT8, dequantized in the cumsum kernel with A_log_scale
         self.D = D                             # INT8, dequantized in the scan with D_scale
         self.dt_bias = dt_bias
+        self._serving = None
 
     @classmethod
-    def from_fp16(cls, original_mixer, scales, r_signs):
+    def from_fp16(cls, original_mixer, scales, r_signs, linear=Int8InputLinear):
         """Same contract as linquant/quantized_mamba2.py:105-203: ``original_mixer`` is any module with the Mamba2
-        attributes (mamba-ssm or HF names), ``scales`` holds B/C/A_log/D scales and the two projection input scales."""
+        attributes (mamba-ssm or HF names), ``scales`` holds B/C/A_log/D scales and the two projection input scales.
+        ``linear``: what the projections become (``Int8InputLinear`` or ``W8A8Linear``); an ``in_proj_input_scale`` of None
+        lets a ``W8A8Linear`` quantize each row of the mixer's input on a scale of its own."""
 
         def pick(*names):
             for n in names:
@@ -100,8 +119,8 @@ class QuantizedMamba2(nn.Module):
             d_model=pick("d_model", "hidden_size"), d_ssm=nheads * headdim, nheads=nheads, headdim=headdim,
             d_state=pick("d_state", "ssm_state_size"), ngroups=pick("ngroups", "n_groups"),
             d_conv=pick("d_conv", "conv_kernel_size"), chunk_size=original_mixer.chunk_size,
-            in_proj=Int8InputLinear.from_fp16(original_mixer.in_proj, scales["in_proj_input_scale"]),
-            out_proj=Int8InputLinear.from_fp16(original_mixer.out_proj, scales["out_proj_input_scale"]),
+            in_proj=linear.from_fp16(original_mixer.in_proj, scales["in_proj_input_scale"]),
+            out_proj=linear.from_fp16(original_mixer.out_proj, scales["out_proj_input_scale"]),
             conv1d=original_mixer.conv1d, norm=original_mixer.norm, A_log=q_A_log, D=q_D,
             dt_bias=original_mixer.dt_bias, dt_limit=tuple(dt_limit), layer_idx=getattr(original_mixer, "layer_idx", None))
         module.register_buffer("r_signs", r_signs)
@@ -121,17 +140,8 @@ class QuantizedMamba2(nn.Module):
             hidden_states = hidden_states.to(torch.float16)
 
         # 1. in_proj on INT8 activations (rint(x / s) clamped to [-128, 127])
-        if hasattr(self.in_proj, "forward_int8"):
-            s = self.in_proj.input_scale
-            h_i8 = _fused_fp16_to_int8(hidden_states.reshape(-1, hidden_states.shape[-1]), s, clamp_min=-128.0,
-                                       reciprocal=False).view(hidden_states.shape)
-            projected = self.in_proj.forward_int8(h_i8, s)
-        else:
-            h_i8 = None
-            projected = self.in_proj(hidden_states)
-        gn = self.ngroups * self.d_state
-        d_mlp = (projected.shape[-1] - 2 * self.d_ssm - 2 * gn - self.nheads) // 2
-        z0, x0, z, xBC, dt = projected.split([d_mlp, d_mlp, self.d_ssm, self.conv_dim, self.nheads], dim=-1)
+        h_i8, projected = self._in_project(hidden_states)
+        z0, x0, z, xBC, dt = self._split(projected)
 
         # 2. causal conv1d + SiLU
         xBC = _apply_mask(xBC, attention_mask)
@@ -175,30 +185,154 @@ class QuantizedMamba2(nn.Module):
             **dt_limit_kwargs)
         y = y.reshape(y.shape[0], y.shape[1], self.d_ssm)
 
-        # 5 + 6. gated RMSNorm, Hadamard + INT8 of the out_proj input
-        out_scale = self.out_proj.input_scale
-        if d_mlp == 0 and isinstance(self.norm, RMSNormGated):
-            y_i8, scale = rmsnorm_gated_qhad(y, z, self.norm.weight, out_scale, self.norm.eps, self.norm.group_size)
-            normed = None
-        else:
-            normed = self.norm(y, z)
-            if d_mlp > 0:
-                normed = torch.cat([torch.nn.functional.silu(z0) * x0, normed], dim=-1)
-            y_i8, scale = qhad_transform(normed, out_scale)
-        out = self.out_proj.forward_int8(y_i8, scale) if hasattr(self.out_proj, "forward_int8") else self.out_proj(y_i8)
-
-        # 7. output compensation
-        comp_out = getattr(self, "comp_out", None)
-        if comp_out is not None:
-            out = out + comp_out
+        # 5 - 7. gated RMSNorm, Hadamard + INT8 of the out_proj input, out_proj, output compensation
+        out, normed, y_i8 = self._finish(y, z, z0, x0)
         if debug is not None:
             debug.update(h_i8=h_i8, projected=projected, xBC=xBC, x_fp=x_fp, q_B=q_B, q_C=q_C, dt=dt, z=z, y=y,
                          normed=normed, y_i8=y_i8, out=out, b_fp=keyside_kwargs.get("b_fp"))
         return out
 
+    def _in_project(self, hidden_states):
+        """(codes or None, projected)."""
+        s = getattr(self.in_proj, "input_scale", None)
+        if s is None or not hasattr(self.in_proj, "forward_int8"):
+            return None, self.in_proj(hidden_states)
+        h_i8 = _fused_fp16_to_int8(hidden_states.reshape(-1, hidden_states.shape[-1]), s, clamp_min=-128.0,
+                                   reciprocal=False).view(hidden_states.shape)
+        return h_i8, self.in_proj.forward_int8(h_i8, s)
+
+    def _split(self, projected):
+        """z0, x0 (the MLP's halves, mostly of no width), z, xBC, dt."""
+        d_mlp = (projected.shape[-1] - self.d_ssm - self.conv_dim - self.nheads) // 2
+        return projected.split([d_mlp, d_mlp, self.d_ssm, self.conv_dim, self.nheads], dim=-1)
+
+    def _finish(self, y, z, z0, x0, host_scale=None):
+        """``host_scale``: out_proj's input scale as a number, where reading the tensor would wait for the GPU."""
+        out_scale = self.out_proj.input_scale
+        quant_scale = out_scale if host_scale is None else host_scale
+        d_mlp = z0.shape[-1]
+        if d_mlp == 0 and isinstance(self.norm, RMSNormGated):
+            y_i8, _ = rmsnorm_gated_qhad(y, z, self.norm.weight, quant_scale, self.norm.eps, self.norm.group_size)
+            normed = None
+        else:
+            normed = self.norm(y, z)
+            if d_mlp > 0:
+                normed = torch.cat([torch.nn.functional.silu(z0) * x0, normed], dim=-1)
+            y_i8, _ = qhad_transform(normed, quant_scale)
+        out = self.out_proj.forward_int8(y_i8, out_scale) if hasattr(self.out_proj, "forward_int8") else self.out_proj(y_i8)
+        comp_out = getattr(self, "comp_out", None)
+        if comp_out is not None:
+            out = out + comp_out
+        return out, normed, y_i8
+
+    # ---- serving -------------------------------------------------------------------------------------------------------------
+
+    @torch.no_grad()
+    def prepare_serving(self):
+        """Lays out once what ``prefill`` and ``step`` read beside the projections: the convolution's weights in fp16, A, D and dt_bias in
+        fp32 (dequantized as the INT8 kernels do), and out_proj's input scale as a number on the host.  ``allocate_state`` calls it;
+        so does whoever changes those parameters in place.  Moving the module and loading a state dict undo it."""
+        bias = self.conv1d.bias
+        self._serving = dict(
+            weight=self.conv1d.weight.detach().reshape(self.conv_dim, -1).to(torch.float16, copy=True).contiguous(),
+            bias=None if bias is None else bias.detach().to(torch.float16, copy=True),
+            A=-torch.exp(self.A_log.float() * self.A_log_scale.float()), D=self.D.float() * self.D_scale.float(),
+            dt_bias=None if self.dt_bias is None else self.dt_bias.detach().to(torch.float32, copy=True),
+            out_scale=float(self.out_proj.input_scale))
+
+    def _apply(self, fn, *args, **kwargs):
+        self._serving = None
+        return super()._apply(fn, *args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._serving = None
+        return super()._load_from_state_dict(*args, **kwargs)
+
+    def allocate_state(self, num_slots):
+        """Zeroed slots for that many sequences, on the module's device."""
+        if self._serving is None:
+            self.prepare_serving()
+        device = self._serving["A"].device
+        return Mamba2State(torch.zeros(num_slots, self.d_conv - 1, self.conv_dim, dtype=torch.float16, device=device),
+                           torch.zeros(num_slots, self.nheads, self.headdim, self.d_state, dtype=torch.float32, device=device))
+
+    @torch.no_grad()
+    def prefill(self, hidden_states, state, slots=None, seq_starts=None, _debug=None):
+        """The tokens of prompts, or of the next parts of prompts: ``hidden_states`` fp16 or bf16 (B, L, d_model), or (T, d_model) with
+        ``seq_starts`` (n + 1 int32, ascending) for packed prompts of any lengths, or the pair (codes, scale) of its INT8 form.
+        ``slots`` (n,) int32: each prompt's place in ``state`` (None: 0 .. n - 1), all different; a negative one marks a prompt that
+        starts from zero and leaves nothing.  The state goes on from what the slots hold.  Returns fp16 like hidden_states; rows of
+        tokens outside every prompt are undefined."""
+        return self._serve(hidden_states, state, slots, seq_starts, False, _debug)
+
+    @torch.no_grad()
+    def step(self, hidden_states, state, slots=None, _debug=None):
+        """One token of each sequence: ``hidden_states`` (B, d_model), or its (codes, scale) -> (B, d_model).  Entries with a negative
+        slot are padding: they touch no state.  Capturable into a graph."""
+        return self._serve(hidden_states, state, slots, None, True, _debug)
+
+    def _serve(self, hidden_states, state, slots, seq_starts, single, debug):
+        w = self._serving
+        if w is None:
+            raise RuntimeError("QuantizedMamba2 is not prepared for serving: call prepare_serving() after the module was moved or loaded")
+        if isinstance(hidden_states, tuple):
+            projected = self.in_proj.forward_int8(*hidden_states)
+        else:
+            projected = self._in_project(hidden_states.to(torch.float16))[1]
+        assert projected.dim() == (2 if single or seq_starts is not None else 3), \
+            "hidden_states: (B, L, d_model), (T, d_model) with seq_starts, one token each: (B, d_model)"
+        z0, x0, z, xBC, dt = self._split(projected)
+        if single:
+            xBC = conv1d_step(xBC, state.conv, w["weight"], w["bias"], "silu", slots=slots)
+        else:
+            xBC = conv1d_prompt(xBC, w["weight"], w["bias"], "silu", state=state.conv, slots=slots, seq_starts=seq_starts)
+        gn = self.ngroups * self.d_state
+        x, B, C = xBC.split([self.d_ssm, gn, gn], dim=-1)
+        # B and C as they are: the rotation and D_qk rescaling of the INT8 path leave C . B unchanged and prepare for codes only
+        x = x.unflatten(-1, (self.nheads, self.headdim))
+        B, C = (t.unflatten(-1, (self.ngroups, self.d_state)) for t in (B, C))
+        kw = dict(dt_bias=w["dt_bias"], dt_softplus=True, dt_limit=self.dt_limit, slots=slots)
+        if single:
+            y = ssm_step(state.ssm, x, dt, w["A"], B, C, w["D"], **kw)
+        else:
+            y = ssm_prompt(x, dt, w["A"], B, C, w["D"], state=state.ssm, seq_starts=seq_starts, **kw)
+        y = y.flatten(-2)
+        out, _, y_i8 = self._finish(y, z, z0, x0, w["out_scale"])
+        if debug is not None:
+            debug.update(projected=projected, xBC=xBC, dt=dt, z=z, y=y, y_i8=y_i8, out=out)
+        return out
+
+
+class Mamba2Block(nn.Module):
+    """A mixer in a residual stream, for serving: r = residual + x and mixer(rmsnorm(r)), the norm's output going to in_proj as the
+    INT8 codes that the same pass makes of it.  ``x`` and ``residual`` are what the block in front returned (its mixer's output, not
+    yet added, and the stream in fp32); the first block takes the embeddings and None."""
+
+    def __init__(self, mixer: QuantizedMamba2, norm_weight: torch.Tensor, eps=1e-5):
+        super().__init__()
+        self.mixer, self.eps = mixer, eps
+        self.register_buffer("norm_weight", norm_weight.detach().clone())
+
+    def _normed(self, x, residual):
+        s = self.mixer.in_proj.input_scale
+        codes, scale, r = residual_rmsnorm(x, self.norm_weight, residual, self.eps, quantize="rows" if s is None else s,
+                                           residual_dtype=torch.float32 if residual is None else None)
+        return (codes, scale), r
+
+    @torch.no_grad()
+    def prefill(self, x, residual, state, slots=None, seq_starts=None):
+        """-> (the mixer's output, residual); arguments as in ``QuantizedMamba2.prefill``."""
+        codes, r = self._normed(x, residual)
+        return self.mixer.prefill(codes, state, slots, seq_starts), r
+
+    @torch.no_grad()
+    def step(self, x, residual, state, slots=None):
+        codes, r = self._normed(x, residual)
+        return self.mixer.step(codes, state, slots), r
+
 
 def random_calibrated_mixer(*, d_model, nheads, headdim, d_state, ngroups, chunk_size, d_conv=4, batch=2, seqlen=512,
-                            keyside=False, rotate=True, seed=0, device="cuda"):
+                            keyside=False, rotate=True, seed=0, device="cuda", linear=Int8InputLinear):
     """A QuantizedMamba2 with random fp16 weights, calibrated on one synthetic batch (static absmax scales), for tests
     and timing: there are no checkpoints here.  Returns (module, calibration hidden states)."""
     import math
@@ -247,7 +381,7 @@ def random_calibrated_mixer(*, d_model, nheads, headdim, d_state, ngroups, chunk
                                d_conv=d_conv, chunk_size=chunk_size, in_proj=in_proj.to(device), out_proj=out_proj.to(device),
                                conv1d=conv1d.to(device).half(), norm=norm, A_log=params["A_log"].float(), D=params["D"].float(),
                                dt_bias=params["dt_bias"], layer_idx=0)
-    m = QuantizedMamba2.from_fp16(original, scales, params["r_signs"])
+    m = QuantizedMamba2.from_fp16(original, scales, params["r_signs"], linear)
     for name in ("alpha_hp", "bscale_g", "static_state_scale", "static_cb_scale"):
         m.register_buffer(name, sc[name])
     if keyside:

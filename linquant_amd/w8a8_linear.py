@@ -122,8 +122,7 @@ class W8A8Linear(nn.Module):
         a = x_i8.reshape(-1, self.in_features)
         if self.in_features % _K:
             a = nn.functional.pad(a, (0, _padded(self.in_features) - self.in_features))
-        out = torch.empty(a.shape[0], self.out_features, dtype=out_dtype, device=a.device)
-        return _matmul(_lib.rows16(a), self.weight, scale, self.weight_scale, self.bias, out).view(*x_i8.shape[:-1], self.out_features)
+        return int8_matmul(a, self.weight, scale, self.weight_scale, self.bias, out_dtype).view(*x_i8.shape[:-1], self.out_features)
 
     def forward(self, x):
         assert x.shape[-1] == self.in_features and x.dtype in (torch.float16, torch.bfloat16)
@@ -132,5 +131,4 @@ class W8A8Linear(nn.Module):
             return self.forward_int8(q.view(x.shape), self.input_scale, x.dtype)
         assert self.input_scale is None, "a static input scale takes fp16 activations and in_features a multiple of 8"
         q, s = _quantize(x)
-        out = torch.empty(q.shape[0], self.out_features, dtype=x.dtype, device=x.device)
-        return _matmul(q, self.weight, s, self.weight_scale, self.bias, out).view(*x.shape[:-1], self.out_features)
+        return int8_matmul(q, self.weight, s, self.weight_scale, self.bias, x.dtype).view(*x.shape[:-1], self.out_features)

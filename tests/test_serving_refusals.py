@@ -132,3 +132,37 @@ def test_entry_points_refuse_before_a_launch(fn, good, bad):
         assert rc(**{**good, **kw}) == -22, kw
     for name in (n for n in good if n in pointers and n != "workspace"):
         assert rc(**{**good, name: None}) == -14, name
+
+
+def _mixer(**kw):
+    from linquant_amd.norm import RMSNormGated
+    from linquant_amd.quantized_mamba2 import Int8InputLinear, QuantizedMamba2
+
+    lin = lambda n, k: Int8InputLinear(torch.zeros(n, k), 1.0)  # noqa: E731
+    m = QuantizedMamba2(d_model=64, d_ssm=128, nheads=2, headdim=64, d_state=16, ngroups=1, d_conv=4, chunk_size=64,
+                        in_proj=lin(2 * 128 + 32 + 2, 64), out_proj=lin(64, 128), conv1d=torch.nn.Conv1d(160, 160, 4, groups=160),
+                        norm=RMSNormGated(128), A_log=torch.full((2,), 50, dtype=I8), D=torch.full((2,), 100, dtype=I8), dt_bias=torch.zeros(2), **kw)
+    m.register_buffer("A_log_scale", torch.tensor(0.02))
+    m.register_buffer("D_scale", torch.tensor(0.01))
+    return m
+
+
+def test_mixer_serving_refusals():
+    m = _mixer()
+    x = z(1, 64)
+    with pytest.raises(RuntimeError, match="prepare_serving"):
+        m.step(x, None)
+    st = m.allocate_state(3)
+    assert st.conv.shape == (3, 3, 160) and st.conv.dtype == F16 and st.ssm.shape == (3, 2, 64, 16) and st.ssm.dtype == F32
+    assert torch.allclose(m._serving["A"], torch.full((2,), -2.718281828)) and torch.allclose(m._serving["D"], torch.ones(2))
+    for undo in (lambda: m.to("cpu"), lambda: m.load_state_dict(m.state_dict())):       # moved or loaded: what was laid out is gone
+        m.prepare_serving()
+        undo()
+        with pytest.raises(RuntimeError, match="prepare_serving"):
+            m.prefill(x[None], st)
+    with pytest.raises(NotImplementedError, match="prefill-only"):
+        m(x[None], past_key_values=object())
+    m.prepare_serving()
+    refuses(m.step, (z(1, 1, 64, dtype=I8), 1.0), st)                                   # codes of other dimensions
+    refuses(m.prefill, (z(4, 64, dtype=I8), 1.0), st)
+    refuses(m.prefill, (z(1, 4, 64, dtype=I8), 1.0), st, None, z(2, dtype=I32))
