@@ -235,50 +235,71 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
   }
 }
 
-// Few rows of a: 16 MT of them and 16 columns to a workgroup of eight waves, which share the contraction in steps of 64 bytes.
+// Few rows of a: 16 MT of them and 16 NT columns to a workgroup of W waves, which share the contraction in lines of 128 bytes, side by
+// side (a wave that has a range of its own reads 8192 x 8192 a quarter slower).  The weights are read once, a's rows by every workgroup,
+// and those cost as much: 16 x 2560 x 10576 takes 9 us with one row of a, 15 with 16 columns to a workgroup.  So NT is taken such that
+// there is one workgroup to a compute unit (16 x 2560 x 10576, us, NT 1 / 2 / 3: 11.5 / 12.4 / 10.1; 64 rows 24.6 / 22.7 / 16.9; 16 x
+// 5120 x 2560, 160 tiles of 16 columns: 7.5 / 11.8 / 15.6).  Eight waves that request one line at a time are as good as any, but where
+// results are many (MT 4, NT 2 or 3) four that request two: 64 x 2560 x 10576, NT 2: 21.6 and 22.7.
 // v_mfma_i32_16x16x64_i8: lane l has row l & 15 and the 16 bytes of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
-template <int MT, typename O>
-__global__ __launch_bounds__(512) void int8_rows_kernel(MatmulParams p) {
-  __shared__ __align__(16) int sums[8][MT][64][4];
+template <int MT, int NT, int W, int U, typename O>
+__global__ __launch_bounds__(64 * W) void int8_rows_kernel(MatmulParams p) {
+  __shared__ __align__(16) int sums[W][NT][MT][64][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-  const int8_t* b = p.b + min(n0 + (lane & 15), p.cols - 1) * p.b_stride;
-  const int8_t* a[MT];
+  const int n0 = blockIdx.x * 16 * NT;
+  const int8_t *b[NT], *a[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) a[i] = p.a + min(m0 + 16 * i + (lane & 15), p.rows - 1) * p.a_stride;
-  lq_v4i acc[MT];
+  for (int j = 0; j < NT; ++j) b[j] = p.b + min(n0 + 16 * j + (lane & 15), p.cols - 1) * p.b_stride;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = lq_v4i{0, 0, 0, 0};
-  const int steps = (p.inner + 63) / 64;
-  constexpr int U = 4;  // steps requested at a time
-  for (int s0 = wave; s0 < steps; s0 += 8 * U) {
-    lq_v4i fb[U], fa[U][MT];
+  for (int i = 0; i < MT; ++i) a[i] = p.a + min(16 * i + (lane & 15), p.rows - 1) * p.a_stride;
+  lq_v4i acc[NT][MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = (s0 + 8 * u) * 64 + (lane >> 4) * 16, kc = min(k, p.inner - 16);
-      fb[u] = *(const lq_v4i*)(b + kc);
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) fa[u][i] = *(const lq_v4i*)(a[i] + kc);
-    }
+    for (int i = 0; i < MT; ++i) acc[j][i] = lq_v4i{0, 0, 0, 0};
+  const int lines = (p.inner + 127) / 128;
+  for (int s0 = wave; s0 < lines; s0 += W * U) {
+    lq_v4i fb[U][2][NT], fa[U][2][MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = (s0 + 8 * u) * 64 + (lane >> 4) * 16;
-      if (k >= p.inner) fb[u] = lq_v4i{0, 0, 0, 0};  // (a zero of one operand is enough)
+    for (int u = 0; u < U; ++u)
+      if (s0 + W * u < lines) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = lq_mfma_i8(fb[u], fa[u][i], acc[i]);
-    }
+        for (int h = 0; h < 2; ++h) {
+          const int kc = min((s0 + W * u) * 128 + 64 * h + (lane >> 4) * 16, p.inner - 16);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) fb[u][h][j] = *(const lq_v4i*)(b[j] + kc);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) fa[u][h][i] = *(const lq_v4i*)(a[i] + kc);
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + W * u < lines) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool in = (s0 + W * u) * 128 + 64 * h + (lane >> 4) * 16 < p.inner;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            if (!in) fa[u][h][i] = lq_v4i{0, 0, 0, 0};  // (a zero of one operand is enough)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j][i] = lq_mfma_i8(fb[u][h][j], fa[u][h][i], acc[j][i]);
+          }
+        }
+      }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) *(lq_v4i*)sums[wave][i][lane] = acc[i];
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *(lq_v4i*)sums[wave][j][i][lane] = acc[j][i];
   __syncthreads();
   using OT = typename OutOf<O>::type;
   OT* out = (OT*)p.out;
-  for (int t = threadIdx.x; t < MT * 256; t += 512) {  // adjacent threads: adjacent columns
-    const int i = t >> 8, m = (t >> 4) & 15, n = t & 15;
+  for (int t = threadIdx.x; t < NT * MT * 256; t += 64 * W) {  // adjacent threads: adjacent columns
+    const int n = t & 15, j = (t >> 4) % NT, m = (t >> 4) / NT & 15, i = (t >> 4) / NT >> 4;
     int v = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) v += sums[w][i][(n >> 2) * 16 + m][n & 3];
-    const int row = m0 + 16 * i + m, col = n0 + n;
+    for (int w = 0; w < W; ++w) v += sums[w][j][i][(n >> 2) * 16 + m][n & 3];
+    const int row = 16 * i + m, col = n0 + 16 * j + n;
     if (row < p.rows && col < p.cols) {
       const float s = p.a_scale[p.a_scale_rows ? row : 0] * p.b_scale[p.b_scale_cols ? col : 0];
       out[row * p.out_stride + col] = O::from(__builtin_fmaf((float)v, s, p.bias ? sv_load(p.bias, col, p.bias_dtype) : 0.0f));
@@ -288,12 +309,18 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(MatmulParams p) {
 
 template <typename O>
 int launch(const MatmulParams& p, hipStream_t stream) {
+  using std::integral_constant;
   if (p.rows <= 64) {
     const int mt = (p.rows + 15) / 16;
-    const dim3 grid((unsigned)((p.cols + 15) / 16), 1);
-    if (mt == 1) hipLaunchKernelGGL((int8_rows_kernel<1, O>), grid, dim3(512), 0, stream, p);
-    else if (mt == 2) hipLaunchKernelGGL((int8_rows_kernel<2, O>), grid, dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((int8_rows_kernel<4, O>), grid, dim3(512), 0, stream, p);
+    // most tiles of 16 columns that a compute unit gets, n to a workgroup
+    auto most = [&](int n) { return ((p.cols + 16 * n - 1) / (16 * n) + 255) / 256 * n; };
+    const int nt = most(3) <= std::min(most(1), most(2)) ? 3 : (most(2) <= most(1) ? 2 : 1);
+    auto go = [&](auto m, auto n) {
+      constexpr int MT = decltype(m)::value, NT = decltype(n)::value, W = MT == 4 && NT > 1 ? 4 : 8;
+      hipLaunchKernelGGL((int8_rows_kernel<MT, NT, W, 8 / W, O>), dim3((unsigned)((p.cols + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, stream, p);
+    };
+    auto columns = [&](auto m) { nt == 1 ? go(m, integral_constant<int, 1>{}) : (nt == 2 ? go(m, integral_constant<int, 2>{}) : go(m, integral_constant<int, 3>{})); };
+    mt == 1 ? columns(integral_constant<int, 1>{}) : (mt == 2 ? columns(integral_constant<int, 2>{}) : columns(integral_constant<int, 4>{}));
     return lq_check_launch();
   }
   auto tiles = [&](auto tm, auto tn, auto kg) {
@@ -303,7 +330,6 @@ int launch(const MatmulParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, KG, O>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256 * KG), 0, stream, p);
     return lq_check_launch();
   };
-  using std::integral_constant;
   auto count = [&](int tm, int tn) { return (int64_t)((p.rows + tm - 1) / tm) * ((p.cols + tn - 1) / tn); };
   // The larger a tile, the less is fetched; the more tiles, the more compute units fetch, and two or three workgroups must share each.  Where
   // even small tiles are few, groups share their contraction.  us, rows x K x columns, for tiles of 128 x 256 / 128 x 128 / 64 x 128 in two
