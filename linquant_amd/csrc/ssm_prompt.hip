@@ -11,10 +11,12 @@
 //              prompts times heads are too few for 256 compute units)
 //   chunks     walks a segment chunk by chunk, the state in registers
 //
-// Precision.  Activations enter the matrix products as they are.  What is formed in fp32 on the way (weights of C B^T, the state,
-// weighted x) enters as two pieces of the activations' type, with fp32 sums.  bf16: 16 bits, and the range of fp32.  fp16: 22 bits, after a
-// multiplication by a power of two that brings the largest of what is multiplied (a channel's state and weighted x; C B^T of the chunk)
-// below 2^14, so no size of activations overflows a piece, and what is 2^28 times smaller than that largest starts to lose bits.
+// Precision.  Activations enter the matrix products as they are, all sums are fp32, and so is the state.  What is formed in fp32 on the way
+// and reaches only y, which is rounded to the activations' type itself (weighted C B^T, the state that C multiplies), enters rounded to
+// that type, to the nearest: half a step of each term.  What the state gathers over a prompt (weighted x) enters as two pieces of the type,
+// 16 bits (bf16) or 22 (fp16).  bf16 has the range of fp32.  fp16: after a multiplication by a power of two that brings the largest of what
+// is multiplied (a wave's state and weighted x; a row of weighted C B^T) below 2^14, so no size of activations overflows, and what is 2^24
+// times smaller than that largest starts to lose bits.
 #include <algorithm>
 #include <cmath>
 
@@ -66,6 +68,37 @@ LQ_DEV v16f mfma(lq_v4i a, lq_v4i b, v16f c) {
 LQ_DEV uint32_t pack_bf16(float a, float b) {
   const sv_v2bf v = {(__bf16)a, (__bf16)b};
   return __builtin_bit_cast(uint32_t, v);
+}
+// eight numbers, or products, rounded to T
+template <typename T>
+LQ_DEV lq_v4i round8(const float (&a)[8]) {
+  lq_v4i r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, F16>::value) {
+      typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+      typedef float v2f __attribute__((ext_vector_type(2)));
+      const v2f f = {a[2 * i], a[2 * i + 1]};
+      r[i] = __builtin_bit_cast(int, __builtin_convertvector(f, v2h));
+    } else {
+      r[i] = (int)pack_bf16(a[2 * i], a[2 * i + 1]);
+    }
+  }
+  return r;
+}
+template <typename T>
+LQ_DEV lq_v4i round8(const float (&a)[8], const float (&b)[8]) {
+  if constexpr (std::is_same<T, F16>::value) {  // one mixed-precision instruction each
+    lq_v8h h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)__builtin_fmaf(a[i], b[i], 0.0f);
+    return __builtin_bit_cast(lq_v4i, h);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = a[i] * b[i];
+    return round8<T>(v);
+  }
 }
 // eight products a b as two pieces each: fp16, hi = RN(a b), lo = RN(a b - hi), one mixed-precision instruction a piece; bf16 likewise
 // from the rounded product
@@ -498,16 +531,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
         for (int k = 0; k < 2 * NT; ++k) {
           if (k + 2 < 2 * NT) ask(k + 2);
-          reads_stay();
+          __builtin_amdgcn_sched_barrier(0);  // (all of S converted ahead is registers that it lacks)
           float v[8], r[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i], r[i] = rescale;
-          lq_v4i sh, sl;
-          split<T>(v, r, sh, sl);
+          const lq_v4i sh = kHalf ? round8<T>(v, r) : round8<T>(v);
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) Y[tt] = mfma<T>(cc[k % 3][tt], sh, Y[tt]);
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt) Y[tt] = mfma<T>(cc[k % 3][tt], sl, Y[tt]);
         }
       }
       if constexpr (!STATES) {
@@ -582,10 +612,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         // six steps: rows tt, tokens ks (above the diagonal C B^T is stored as zero)
         constexpr int kT[6] = {0, 1, 0, 1, 1, 1}, kS[6] = {0, 0, 1, 1, 2, 3};
         auto add = [&](int n, const float (&f)[8], const float (&a)[8]) {
-          lq_v4i mh, ml;
-          split<T>(f, a, mh, ml);
-          Y[kT[n]] = mfma<T>(mh, xp[kS[n]], Y[kT[n]]);
-          Y[kT[n]] = mfma<T>(ml, xp[kS[n]], Y[kT[n]]);
+          Y[kT[n]] = mfma<T>(round8<T>(f, a), xp[kS[n]], Y[kT[n]]);
         };
         if (apart && !odd) {
           lq_v4f f4[2][2], q4[2][2];  // (the q of a ks serve two steps)

@@ -85,6 +85,13 @@ def ssm_rel(lens, most):
     return 2.0 ** -21 * (max(lens) + 8) + 2.0 ** -22 * most + 2.0 ** -14
 
 
+def ssm_y_rel(lens, most, dtype):
+    """The same for the outputs of a prompt.  What the activations multiply there, an entry of the state and a weight of C B^T, is rounded
+    to their type once more: (1 + e) of each term, |e| half a step, so the sum is off by at most half a step of the sum of magnitudes.
+    (In fp16 that holds for entries above 2^-14 of a unit that the largest of 32 channels fills up to 2^13: down to 2^-27 of it.)"""
+    return ssm_rel(lens, most) + HALF_STEP[dtype]
+
+
 def starts_of(lens, device="cpu", first=0):
     at = [first]
     for n in lens:

@@ -7,7 +7,7 @@ from linquant_amd.kernels.mamba2.conv1d_state import conv1d_prompt, conv1d_step
 from linquant_amd.kernels.mamba2.ssm import ssm_prompt, ssm_step
 from linquant_amd.norm import residual_rmsnorm
 from linquant_amd.w8a8_linear import W8A8Linear, int8_matmul, quantize_rows
-from tests.serving_cases import HALF_STEP, assert_near, conv_ref, ssm_inputs, ssm_ref, ssm_rel, starts_of
+from tests.serving_cases import HALF_STEP, assert_near, conv_ref, ssm_inputs, ssm_ref, ssm_rel, ssm_y_rel, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -294,7 +294,7 @@ def _check_scan(cuda, lens, H, P, G, N, dtype, *, packed=True, softplus=True, li
     first = state[slots.long()] if with_state else torch.zeros(n, H, P, N)
     wy, mag, ws, smag, most = ssm_ref(v["x"], v["dt"], v["A"], v["B"], v["C"], v["D"], v["dt_bias"] if softplus else None, softplus, limit, lens, first)
     rel = ssm_rel(lens, most)
-    assert_near(y, wy, mag, rel, "y")
+    assert_near(y, wy, mag, ssm_y_rel(lens, most, dtype), "y")
     if with_state:
         assert_near(st[slots.long()], ws, smag, rel, "state")
         rest = [i for i in range(n + 2) if i not in slots.tolist()]
@@ -346,7 +346,7 @@ def test_ssm_prompt_views_and_tokens_of_nobody(cuda):
     x, B, C = (t[10:110] for t in cut(xBC))
     wy, mag, ws, smag, most = ssm_ref(x.reshape(-1, H, P), raw[10:110, 9:], A, B.reshape(-1, G, N), C.reshape(-1, G, N), None, None, True, (0.0, float("inf")),
                                       [70, 30], torch.zeros(2, H, P, N))
-    assert_near(y[10:110], wy, mag, ssm_rel([70], most), "y")
+    assert_near(y[10:110], wy, mag, ssm_y_rel([70], most, F16), "y")
     assert_near(st, ws, smag, ssm_rel([70], most), "state")
 
 
@@ -393,7 +393,7 @@ def test_ssm_large_steps_and_values(cuda):
     wy, mag, ws, smag, most = ssm_ref(v["x"], v["dt"], v["A"], v["B"], v["C"], None, None, True, (0.0, float("inf")), [96], torch.ones(1, 2, 64, 64))
     assert_near(st, ws, smag, ssm_rel([96], 200.0), "state")   # (beyond 200 a weight is zero in 32 bits)
     fits = wy.abs() < 60000
-    assert_near(torch.where(fits, y.cpu(), 0.0), torch.where(fits, wy, 0.0), mag, ssm_rel([96], 200.0), "y")
+    assert_near(torch.where(fits, y.cpu(), 0.0), torch.where(fits, wy, 0.0), mag, ssm_y_rel([96], 200.0, F16), "y")
 
 
 def test_ssm_nan_stays_in_its_sequence_and_head(cuda):
