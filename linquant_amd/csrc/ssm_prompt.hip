@@ -6,7 +6,8 @@
 // which are products of matrices.  Three kernels:
 //   operands   per chunk and group: C, B^T and C B^T in the order in which the matrix instruction takes them, shared by the group's
 //              heads; per chunk and head: d, c (in powers of two) and exp(c_63 - c_s) d_s
-//   states     per segment of a prompt: the state at its end if it starts from zero, and what it multiplies an earlier one by;
+//   states     per segment of a prompt, or piece of one: the state at its end if it starts from zero, and what it multiplies an earlier
+//              one by;
 //   join       walks the segments: the state in front of each.  (states and join: only where prompts are cut into segments, because
 //              prompts times heads are too few for 256 compute units)
 //   chunks     walks a segment chunk by chunk, the state in registers
@@ -54,9 +55,9 @@ struct PromptParams {
   char* tables;     // [unit][group] operands
   float* steps;     // [unit][head][d, c, w, most][64]
   float* rows;      // [unit][group][64]: largest |C B^T| of each row
-  float* seg_state;  // [segment][H][P][N], or NULL: prompts are not cut
-  float* seg_decay;  // [segment][H]
-  int units, segs, seg_chunks, per_group;
+  float* seg_state;  // [segment][piece][H][P][N], or NULL: prompts are not cut
+  float* seg_decay;  // [segment][piece][H]
+  int units, segs, seg_chunks, pieces, per_group;  // (seg_chunks a multiple of pieces)
 };
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -364,11 +365,11 @@ constexpr int W = 4;  // waves of a workgroup
 // way, 64 tokens x 32 channels, a chunk ahead into one of two places, and its y leaves through the same place.  Two workgroups share a
 // compute unit, so that one computes while the other's operands are on their way.
 template <typename T, int NT, bool STATES>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : STATES ? 3 : 2, NT == 8 ? 1 : STATES ? 3 : 2))) void ssm_chunks_kernel(PromptParams p) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void ssm_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
   using Tab = Table<NT>;
   constexpr int kSkip = STATES ? kCB + Tab::kC : 0, kLoad = Tab::kBytes - kSkip;  // bytes of a chunk's operands that are needed
-  __shared__ __align__(16) char buf[kLoad];
+  __shared__ __align__(16) char bufs[STATES ? 2 : 1][kLoad];
   __shared__ __align__(256) uint16_t xbuf[2][W][Q * 32];
   __shared__ __align__(16) float tok[W][3 * Q];  // each wave's q (or d), w, exp2(c) (fp16: scaled)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
@@ -376,9 +377,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   place(p, sg, part);
   // (what is the same for the whole wave goes to scalar registers: a division leaves it in vector ones, and every address made of it too)
   sg = uniform(sg), part = uniform(part);
+  int at = 0;  // STATES: which piece of which segment
+  if (STATES) {
+    const int piece = sg % p.pieces;
+    sg /= p.pieces;
+    if (!p.starts) sg += sg / max(p.segs / p.nseq - 1, 1);  // (as many segments to each prompt, the last ones left out)
+    sg = uniform(sg), at = uniform(sg * p.pieces + piece);
+  }
   if (sg >= p.segs) return;
   Segment s = segment_of(p, sg);
   if (s.seq < 0 || (STATES && s.last)) return;
+  if (STATES) {  // (a segment that is not a prompt's last one has all its chunks)
+    s.chunks = p.seg_chunks / p.pieces;
+    const int skip = (at - sg * p.pieces) * s.chunks;
+    s.chunk0 += skip, s.unit0 += skip;
+  }
   s.seq = uniform(s.seq), s.begin = uniform(s.begin), s.len = uniform(s.len), s.chunk0 = uniform(s.chunk0), s.chunks = uniform(s.chunks), s.unit0 = uniform(s.unit0);
   const int g = uniform(part / p.per_group), pblocks = (p.P + 31) >> 5, hpg = uniform(p.H / p.G);
   const int block = (part - g * p.per_group) * W + wave;
@@ -394,7 +407,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   v16f S[NT];
   const int64_t sbase = ((int64_t)h * p.P + chc) * p.N;
   {
-    const float* src = STATES ? nullptr : (p.seg_state && !(s.first && s.last)) ? p.seg_state + (int64_t)sg * p.H * p.P * p.N + sbase : keeps ? p.state + slot * p.ss_s + sbase : nullptr;
+    const float* src = STATES ? nullptr : (p.seg_state && !(s.first && s.last)) ? p.seg_state + (int64_t)sg * p.pieces * p.H * p.P * p.N + sbase : keeps ? p.state + slot * p.ss_s + sbase : nullptr;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -422,7 +435,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
   for (int i = 0; i < 4; ++i) xoff[i] = ((uint32_t)(16 * i + (lane >> 2)) * (uint32_t)p.sx_l + xcol) * 2u;
   float dv = 0.f, cv = 0.f, wv = 0.f, mv = 0.f, rv = 0.f;
-  auto fetch = [&] {  // the next chunk's operands
+  auto fetch = [&](int c) {  // chunk c's operands, one chunk after the other
+    char* buf = bufs[STATES ? c & 1 : 0];
 #pragma unroll
     for (int k = 0; k < kLoad / (1024 * W); ++k) sv_fetch16(tab + (k * W + wave) * 1024, (uint32_t)lane * 16u, buf + (k * W + wave) * 1024);
     tab += (int64_t)p.G * Tab::kBytes;
@@ -449,9 +463,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   // every wave has read all of a chunk's operands: the next chunk's take their place
   auto taken = [&](int c) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (c + 1 < s.chunks) fetch();
+    if (c + 1 < s.chunks) fetch(c + 1);
   };
-  fetch();
+  fetch(0);
   if (live) request(0);
   arrived();
   // What a chunk's products need of the wave's own: x in registers, step sizes in LDS, the state's unit.  Done at the end of the chunk in
@@ -509,7 +523,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   if (live) begin(0);
   for (int c = 0; c < s.chunks; ++c) {
     const bool more = c + 1 < s.chunks;
-    asm volatile("s_barrier" ::: "memory");  // every wave's share of this chunk's operands is there
+    // every wave's share of this chunk's operands is there
+    if (STATES) taken(c);  // (and the chunk's before the last are read: the next one's on their way into that place)
+    else asm volatile("s_barrier" ::: "memory");
+    const char* buf = bufs[STATES ? c & 1 : 0];
     if (live) {
       if (more) request(c + 1);
       const lq_v4i* op = (const lq_v4i*)buf + lane;
@@ -720,16 +737,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         }
       } else {
         arrived();
-        taken(c);
         if (more) begin(c + 1);
-        arrived();
       }
     } else {
-      taken(c);
+      if (!STATES) taken(c);
       arrived();
     }
   }
-  float* dst = STATES ? p.seg_state + (int64_t)sg * p.H * p.P * p.N + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
+  float* dst = STATES ? p.seg_state + (int64_t)at * p.H * p.P * p.N + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
   if (dst && live && ch < p.P) {
     const float ui = kHalf ? 1.0f / unit_S : 1.0f;
 #pragma unroll
@@ -743,11 +758,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         if (n < p.N) *(lq_v4f*)(dst + n) = v;
       }
   }
-  if (STATES && live && lane == 0 && ch0 == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(decay);
+  if (STATES && live && lane == 0 && ch0 == 0) p.seg_decay[(int64_t)at * p.H + h] = exp2_fast(decay);
 }
 
-// The state in front of each segment, in the place of what the segment adds to one (the last one's is not read).  A workgroup has 1024
-// entries of one head's state.
+// The state in front of each segment, in the place of what its first piece adds to one (what the last segment adds is not there).  A
+// workgroup has 1024 entries of one head's state.
 __global__ __launch_bounds__(256) void ssm_join_kernel(PromptParams p) {
   const int64_t per = (int64_t)p.P * p.N;
   const int h = blockIdx.y, at = (blockIdx.z * 256 + threadIdx.x) * 4, seq = blockIdx.x;
@@ -774,23 +789,25 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(PromptParams p) {
   const int slot = p.state || p.slots ? sv_slot(p.slots, seq, p.num_slots) : kSlotPad;
   lq_v4f v = {0.f, 0.f, 0.f, 0.f};
   if (p.state && slot >= 0) v = *(const lq_v4f*)(p.state + slot * p.ss_s + h * per + at);
-  // four segments requested at a time: a chain of one load after the other was most of this kernel
+  // four pieces requested at a time: a chain of one load after the other was most of this kernel
   constexpr int U = 4;
-  float* base = p.seg_state + ((int64_t)first * p.H + h) * per + at;
-  const float* dec = p.seg_decay + (int64_t)first * p.H + h;
+  float* base = p.seg_state + ((int64_t)first * p.pieces * p.H + h) * per + at;
+  const float* dec = p.seg_decay + (int64_t)first * p.pieces * p.H + h;
   const int64_t next = (int64_t)p.H * per;
-  for (int i = 0; i < n; i += U) {
+  const int all = (n - 1) * p.pieces;
+  for (int i = 0, piece = 0; i <= all; i += U) {
     lq_v4f add[U];
     float d[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = min(i + u, n - 1);
+      const int k = min(i + u, all - 1);
       add[u] = *(const lq_v4f*)(base + k * next), d[u] = dec[(int64_t)k * p.H];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i + u >= n) break;
-      *(lq_v4f*)(base + (i + u) * next) = v;
+      if (i + u > all) break;
+      if (piece == 0) *(lq_v4f*)(base + (i + u) * next) = v;
+      piece = piece + 1 == p.pieces ? 0 : piece + 1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d[u], v[e], add[u][e]);  // (behind the last one: not used)
     }
@@ -812,7 +829,7 @@ int table_bytes(const lq_ssm_prompt_args* a) {
 // How a call is cut: the units, the chunks of a segment.
 struct Plan {
   int64_t units, segs, tables, steps, rows, states, decays, bytes;
-  int per_group, seg_chunks, cut;
+  int per_group, seg_chunks, pieces, cut;
 };
 bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   const int64_t nseq = a->nseq, most = ((int64_t)(a->seq_starts ? a->tokens : a->seqlen) + Q - 1) / Q;  // chunks of the longest prompt there can be
@@ -820,22 +837,27 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   const int64_t blocks = (int64_t)(a->nheads / a->ngroups) * ((a->headdim + 31) / 32);
   r.per_group = (int)((blocks + W - 1) / W);
   const int64_t parts = (int64_t)a->ngroups * r.per_group;
-  // Tenths of a microsecond.  A chunk's step takes 50 where a compute unit has one workgroup and 84 where it has two; one of the states' 25
-  // and about 9 for each further; the join moves the segments' states three times at 3 TB/s, and it and two more launches come to 250.  The
-  // lengths of packed prompts are not known here: the longest is taken to be two and a half times the mean.
+  // Tenths of a microsecond.  A chunk's step takes 43 where a compute unit has one workgroup and 72 where it has two; one of the states'
+  // takes 17 and 27 (the younger one's: the older goes first), or 22 where others follow, and a piece of them 40 more; the join moves every piece's state and each segment's twice at 3 TB/s, and it and two
+  // more launches come to 250.  Prompts of one length end with the fullest compute unit; of packed ones only a few are long, and mostly
+  // alone.  Their lengths are not known here: the longest is taken to be two and a half times the mean.  Measured, 80 heads of 64 by 128: 4
+  // prompts of 8192 tokens in 3 segments of one piece 303 us and the states 120, of two pieces 99 (of four 93, but the join takes longer), in 2
+  // segments 397; 7 packed prompts, 3,700 tokens, 1,400 the longest, 140 us uncut, 155 in segments of 12 chunks.
   const double mean = (double)r.units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
-  auto step = [](double wgs, double one, double more) {
-    const double n = std::max(1.0, wgs / 256);
-    return n <= 2 ? one + more * (n - 1) : (one + more) * std::ceil(n / 2);
+  auto step = [&](double wgs, double one, double two) {
+    if (wgs <= 256) return one;
+    return a->seq_starts && wgs <= 512 ? one + (two - one) * (wgs / 256 - 1) : two * std::ceil(wgs / 512);
   };
-  double best = chain * step((double)nseq * parts, 50, 34);
-  r.seg_chunks = (int)most, r.cut = 0;
-  for (int64_t k = 2; k <= 256; ++k) {  // segments of the longest
-    const int64_t n = std::max<int64_t>(1, (int64_t)std::ceil(chain / k));
-    const double segs = a->seq_starts ? (double)r.units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n));
-    const double cost = n * (step(segs * parts, 50, 34) + step(std::max(0.0, segs - nseq) * parts, 25, 9)) + segs * a->nheads * a->headdim * a->dstate * 12 / 3e5 + 250;
-    if (n < most && cost < best) best = cost, r.seg_chunks = (int)n, r.cut = 1;
-  }
+  double best = chain * step((double)nseq * parts, 43, 72);
+  r.seg_chunks = (int)most, r.pieces = 1, r.cut = 0;
+  for (int64_t k = 2; k <= 256; ++k)  // segments of the longest
+    for (int64_t pieces = 1; pieces <= 2; ++pieces) {
+      const int64_t n = (std::max<int64_t>(1, (int64_t)std::ceil(chain / k)) + pieces - 1) / pieces * pieces;
+      const double segs = a->seq_starts ? (double)r.units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n)), ahead = std::max(0.0, segs - nseq) * pieces;
+      const double cost = n * step(segs * parts, 43, 72) + n / pieces * step(ahead * parts, 17, ahead * parts <= 512 ? 27 : 22) + 40 * std::ceil(ahead * parts / 512) +
+                          (ahead + 2 * segs) * a->nheads * a->headdim * a->dstate * 4 / 3e5 + 250;
+      if (n < most && cost < best) best = cost, r.seg_chunks = (int)n, r.pieces = (int)pieces, r.cut = 1;
+    }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
   r.segs = a->seq_starts ? std::min<int64_t>(r.units / r.seg_chunks + nseq, r.units) : nseq * per;
   if (!r.cut) r.segs = nseq;
@@ -844,9 +866,9 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   r.steps = up(r.units * a->ngroups * table_bytes(a));
   r.rows = r.steps + up(r.units * a->nheads * (4 * Q * 4));
   r.states = r.rows + up(r.units * a->ngroups * (Q * 4));
-  r.decays = r.states + (r.cut ? up(r.segs * a->nheads * a->headdim * a->dstate * 4) : 0);
-  r.bytes = r.decays + (r.cut ? up(r.segs * a->nheads * 4) : 0);
-  return r.units <= 0x7fffffff && r.segs * parts <= 0x7ffffff0;
+  r.decays = r.states + (r.cut ? up(r.segs * r.pieces * a->nheads * a->headdim * a->dstate * 4) : 0);
+  r.bytes = r.decays + (r.cut ? up(r.segs * r.pieces * a->nheads * 4) : 0);
+  return r.units <= 0x7fffffff && r.segs * r.pieces * parts <= 0x7ffffff0;
 }
 
 }  // namespace
@@ -881,9 +903,10 @@ extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
                     a->D, a->D_has_hdim, a->dt_bias, a->dt_softplus, a->dt_min, a->dt_max, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots,
                     a->seq_starts, a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->headdim, a->ngroups, a->dstate,
                     ws + pl.tables, (float*)(ws + pl.steps), (float*)(ws + pl.rows), pl.cut ? (float*)(ws + pl.states) : nullptr, pl.cut ? (float*)(ws + pl.decays) : nullptr,
-                    (int)pl.units, (int)pl.segs, pl.seg_chunks, pl.per_group};
+                    (int)pl.units, (int)pl.segs, pl.seg_chunks, pl.pieces, pl.per_group};
   const dim3 pre((unsigned)pl.units, (unsigned)(a->ngroups + (a->nheads + kHeads - 1) / kHeads));
-  const dim3 grid((unsigned)((pl.segs * a->ngroups * pl.per_group + 7) / 8 * 8)), threads(64 * W);
+  auto grid_of = [&](int64_t segs) { return dim3((unsigned)((segs * a->ngroups * pl.per_group + 7) / 8 * 8)); };
+  const dim3 grid = grid_of(pl.segs), pieces = grid_of((a->seq_starts ? pl.segs : pl.segs - a->nseq) * pl.pieces), threads(64 * W);
   const int64_t per = (int64_t)a->headdim * a->dstate;
   const dim3 join((unsigned)a->nseq, (unsigned)a->nheads, (unsigned)((per + 1023) / 1024));
   if (join.y > 65535 || join.z > 65535) return LQ_ERR_SHAPE;
@@ -892,7 +915,7 @@ extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
     constexpr int NT = decltype(k)::value;
     hipLaunchKernelGGL((ssm_operands_kernel<T, NT>), pre, dim3(256), 0, stream, p);
     if (pl.cut) {
-      hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, true>), grid, threads, 0, stream, p);
+      hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, true>), pieces, threads, 0, stream, p);
       hipLaunchKernelGGL(ssm_join_kernel, join, dim3(256), 0, stream, p);
     }
     hipLaunchKernelGGL((ssm_chunks_kernel<T, NT, false>), grid, threads, 0, stream, p);
