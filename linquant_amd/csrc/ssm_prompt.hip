@@ -130,8 +130,10 @@ LQ_DEV float scale_for(float m) {
   return __uint_as_float((uint32_t)(127 + min(max(13 - e, -100), 24)) << 23);
 }
 // the largest of a wave's non-negative values, by lane permutations of the vector unit; the same for the whole wave
-LQ_DEV float wave_top(float v) {
-#define LQ_TOP(CTRL) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)))
+// (whole numbers order like them, and their maximum takes a permuted operand)
+LQ_DEV float wave_top(float f) {
+  uint32_t v = __float_as_uint(f);
+#define LQ_TOP(CTRL) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false))
   LQ_TOP(0xB1);   // lanes 1 0 3 2
   LQ_TOP(0x4E);   // lanes 2 3 0 1
   LQ_TOP(0x141);  // mirrored halves of a row of 16
@@ -139,7 +141,7 @@ LQ_DEV float wave_top(float v) {
   LQ_TOP(0x142);  // the last lane of a row to the next row
   LQ_TOP(0x143);  // the last lane of the first half of the wave to the second
 #undef LQ_TOP
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  return __int_as_float(__builtin_amdgcn_readlane((int)v, 63));
 }
 LQ_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 LQ_DEV float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
@@ -490,11 +492,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     float ui = 1.0f;
     if constexpr (kHalf) {
       // the wave's new unit: its state and what the chunk adds, each below 2^14 of it
-      float m = 0.0f;
+      float m = 0.0f;  // (no number where the channel has one that is none: its scale does not matter then)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(S[nt][e]));
+        for (int e = 0; e < 16; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(S[nt][e]));
       uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
