@@ -827,7 +827,7 @@ int lq_quantize_rows(const lq_quantize_rows_args* args, hipStream_t stream);
 /* no counterpart in the reference (its projections are W4A8, linquant/w4a8_linear.py): INT8 matrix product,
  *   out[m,n] = (sum_k a[m,k] b[n,k]) * a_scale[m] * b_scale[n] + bias[n], the sum exact in 32 bits. */
 typedef struct {
-  const int8_t* a;           /* (rows, inner), unit inner stride, 16-byte aligned rows */
+  const int8_t* a;           /* (rows, inner), unit inner stride, 16-byte aligned rows less than 2^23 apart (b's too) */
   int64_t a_stride;
   const int8_t* b;           /* (cols, inner), unit inner stride, 16-byte aligned rows */
   int64_t b_stride;
@@ -913,7 +913,8 @@ int lq_conv1d_step(const lq_conv1d_step_args* args, hipStream_t stream);
  *   d = clamp(softplus(dt + dt_bias), dt_min, dt_max), or without the softplus;  S = exp(d A[h]) S + d x B^T;  y = S C + D x,
  * S (headdim, dstate) for each head, starting from and ending in its slot of `state`. */
 typedef struct {
-  const void* x;             /* (tokens,H,P) with seq_starts, else (nseq,seqlen,H,P); unit P stride */
+  const void* x;             /* (tokens,H,P) with seq_starts, else (nseq,seqlen,H,P); unit P stride, 16-byte aligned rows (B's and
+                                C's too), tokens less than 2^24 entries apart */
   int64_t x_stride_b, x_stride_l, x_stride_h;
   int32_t dtype;             /* of x, B, C and out: LQ_DT_F16 / LQ_DT_BF16 */
   const void* dt;            /* (tokens,H) or (nseq,seqlen,H) */
@@ -935,7 +936,8 @@ typedef struct {
   const int32_t* slots;      /* (nseq,) or NULL */
   const int32_t* seq_starts; /* (nseq + 1,) or NULL */
   int32_t num_slots, nseq, seqlen, tokens; /* seqlen without seq_starts, tokens with */
-  int32_t nheads, headdim, ngroups, dstate; /* headdim and dstate multiples of 8, dstate up to 256 */
+  int32_t nheads, headdim, ngroups, dstate; /* headdim and dstate multiples of 8, dstate up to 256,
+                                                        nheads * headdim up to 2^23 */
   void* workspace;           /* 256-byte aligned; contents undefined on entry and on return */
   int64_t workspace_bytes;
 } lq_ssm_prompt_args;

@@ -1,8 +1,8 @@
 // lq_int8_matmul: out[m,n] = (sum_k a[m,k] b[n,k]) * a_scale[m] * b_scale[n] + bias[n], INT8 in, the sum exact in 32 bits.
 //
 // Two kernels.  `tiles`: both operands go through LDS in stages of 128 contraction bytes, fetched straight from memory, and each wave has
-// whole 32 x 32 tiles of the result.  `rows`: few rows of a (tokens that answer): a workgroup has 16 columns and its waves parts of the
-// contraction, every operand straight to registers, so that the weights stream from memory once.
+// whole 32 x 32 tiles of the result.  `rows`: few rows of a (tokens that answer): a workgroup has 16 to 48 columns and its waves parts of
+// the contraction, every operand straight to registers, so that the weights stream from memory once: 16 x 2560 x 10576 in 8 us, 3.4 TB/s.
 //
 // The matrix instruction of `tiles` is v_mfma_i32_32x32x32_i8, which reaches 4.9 POPS here where the 16x16x64 form reaches 3.0.  Operands:
 // lane l has row l & 31 and the 16 contraction bytes of half l >> 5; the result: column l & 31, rows 8 (r >> 2) + 4 (l >> 5) + (r & 3).  b is

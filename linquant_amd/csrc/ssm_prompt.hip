@@ -18,6 +18,15 @@
 // 16 bits (bf16) or 22 (fp16).  bf16 has the range of fp32.  fp16: after a multiplication by a power of two that brings the largest of what
 // is multiplied (a wave's state and weighted x; a row of weighted C B^T) below 2^14, so no size of activations overflows, and what is 2^24
 // times smaller than that largest starts to lose bits.
+//
+// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 404 us (operands 32, states 99, join 16, chunks
+// 293; 425 on a slower card), 1.8 TB/s of what has to move and 268 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
+// busy 50 % of the time (scaling, rounding and splitting operands, 690 instructions to 32 channels and 64 tokens), the matrix unit 22 %, and
+// the clock falls from 2.4 to 2.1 GHz; two waves to a SIMD is what the state in registers (64 of 256) and 81 KB of LDS leave.  Few or
+// ragged prompts are a chain of chunks, 4.1 us each: 384 tokens 36 us, 6949 in 10 prompts of up to 2047, 64 heads in 8 groups, bf16, 140.
+// Tried: C B^T formed by each workgroup (its product is the group's, so 80 heads made it 80 times); one piece of a state's additions (a state
+// gathers the rounding of a whole prompt); a higher priority for the younger of two workgroups, which the older one holds up (3 % less here,
+// 3 % more for ragged prompts).
 #include <algorithm>
 #include <cmath>
 
@@ -844,7 +853,7 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   // more launches come to 250.  Prompts of one length end with the fullest compute unit; of packed ones only a few are long, and mostly
   // alone.  Their lengths are not known here: the longest is taken to be two and a half times the mean.  Measured, 80 heads of 64 by 128: 4
   // prompts of 8192 tokens in 3 segments of one piece 303 us and the states 120, of two pieces 99 (of four 93, but the join takes longer), in 2
-  // segments 397; 7 packed prompts, 3,700 tokens, 1,400 the longest, 140 us uncut, 155 in segments of 12 chunks.
+  // segments 397; 10 packed prompts of 6949 tokens, the longest 2047, 64 heads in 8 groups, 140 us uncut, 155 in segments of 12 chunks.
   const double mean = (double)r.units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
   auto step = [&](double wgs, double one, double two) {
     if (wgs <= 256) return one;

@@ -1,6 +1,7 @@
 // lq_ssm_step: one token of each sequence through the selective state space scan, the fp32 state updated in place.
 //   S = exp(d A) S + d x B^T,  y = S C + D x,  d = softplus(dt + bias)
-// HBM-bound: 8 bytes for each entry of the state, five operations.
+// HBM-bound: 8 bytes for each entry of the state, five operations.  80 heads of 64 by 128: 256 sequences 271 us, 5.0 TB/s (a large copy
+// reaches 5.1); 4 sequences 6.7 us, 20 MB behind a launch and two round trips to memory.
 //
 // Eight lanes have one row of the state (a head channel) in pieces of 16 bytes, so that a wave's request covers eight whole 128-byte
 // lines and the sum over the row is three exchanges.
