@@ -311,6 +311,7 @@ template <typename O>
 int launch(const MatmulParams& p, hipStream_t stream) {
   using std::integral_constant;
   if (p.rows <= 64) {
+    if (!sv_fits(((int64_t)p.cols + 15) / 16, 512)) return LQ_ERR_SHAPE;
     const int mt = (p.rows + 15) / 16;
     // most tiles of 16 columns that a compute unit gets, n to a workgroup
     auto most = [&](int n) { return ((p.cols + 16 * n - 1) / (16 * n) + 255) / 256 * n; };
@@ -325,12 +326,12 @@ int launch(const MatmulParams& p, hipStream_t stream) {
   }
   auto tiles = [&](auto tm, auto tn, auto kg) {
     constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, KG = decltype(kg)::value;
-    const int64_t n = (int64_t)((p.rows + TM - 1) / TM) * ((p.cols + TN - 1) / TN);
-    if (n > 0x7ffffff0) return LQ_ERR_SHAPE;
+    const int64_t n = (((int64_t)p.rows + TM - 1) / TM) * (((int64_t)p.cols + TN - 1) / TN);
+    if (!sv_fits(n + 7, 256 * KG)) return LQ_ERR_SHAPE;
     hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, KG, O>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256 * KG), 0, stream, p);
     return lq_check_launch();
   };
-  auto count = [&](int tm, int tn) { return (int64_t)((p.rows + tm - 1) / tm) * ((p.cols + tn - 1) / tn); };
+  auto count = [&](int tm, int tn) { return (((int64_t)p.rows + tm - 1) / tm) * (((int64_t)p.cols + tn - 1) / tn); };
   // The larger a tile, the less is fetched; the more tiles, the more compute units fetch, and two or three workgroups must share each.  Where
   // even small tiles are few, groups share their contraction.  us, rows x K x columns, for tiles of 128 x 256 / 128 x 128 / 64 x 128 in two
   // groups / 64 x 64 in four: 8192 x 2560 x 10576 248 / 249 / 329 / 428, 3001 x 2560 x 10576 92 / 99 / 122 / 162, 1000 x 2560 x 10576 42 / 40 /

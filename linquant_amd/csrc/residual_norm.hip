@@ -245,6 +245,7 @@ int launch_rows(const RowsParams& p, hipStream_t stream) {
   auto go = [&](auto nv, auto th) {
     constexpr int NV = decltype(nv)::value, TH = decltype(th)::value;
     const dim3 grid((unsigned)(((int64_t)p.rows * TH + 255) / 256));
+    if (!sv_fits(grid.x, 256)) return (int)LQ_ERR_SHAPE;
     if constexpr (QUANT) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, TH, VEC>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((residual_norm_kernel<T, RT, NV, TH, VEC>), grid, dim3(256), 0, stream, p);
     return lq_check_launch();

@@ -126,6 +126,8 @@ LQ_DEV void sv_fetch16(const void* base, uint32_t offset, const void* at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
+// whether a grid's first dimension fits a launch (2^32 - 1 threads)
+static inline bool sv_fits(int64_t workgroups, int threads) { return workgroups * threads <= 0xffffffffll; }
 static inline bool sv_al(const void* q, int n) { return ((uintptr_t)q % n) == 0; }
 static inline bool sv_act(int dtype) { return dtype == LQ_DT_F16 || dtype == LQ_DT_BF16; }
 static inline bool sv_float(int dtype) { return sv_act(dtype) || dtype == LQ_DT_F32; }

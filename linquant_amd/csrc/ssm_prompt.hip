@@ -879,7 +879,7 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   r.states = r.rows + up(r.units * a->ngroups * (Q * 4));
   r.decays = r.states + (r.cut ? up(r.segs * r.pieces * a->nheads * a->headdim * a->dstate * 4) : 0);
   r.bytes = r.decays + (r.cut ? up(r.segs * r.pieces * a->nheads * 4) : 0);
-  return r.units <= 0x7fffffff && r.segs * r.pieces * parts <= 0x7ffffff0;
+  return sv_fits(r.units, 256) && sv_fits(nseq, 256) && sv_fits(r.segs * r.pieces * parts + 7, 64 * W);
 }
 
 }  // namespace

@@ -90,7 +90,7 @@ extern "C" int lq_ssm_step(const lq_ssm_step_args* a, hipStream_t stream) {
   if (!sv_act(a->dtype) || !sv_float(a->dt_dtype) || a->batch <= 0 || a->batch > 65535 || a->nheads <= 0 || a->ngroups <= 0 || a->nheads % a->ngroups != 0)
     return LQ_ERR_SHAPE;
   if (a->headdim <= 0 || a->headdim % 8 != 0 || a->dstate <= 0 || a->dstate % 8 != 0 || a->dstate > 256 || a->num_slots <= 0) return LQ_ERR_SHAPE;
-  if ((int64_t)a->nheads * a->headdim > 0x7fffffff) return LQ_ERR_SHAPE;
+  if ((int64_t)a->nheads * a->headdim > 0x7fffffff || !sv_fits(a->nheads, 256)) return LQ_ERR_SHAPE;
   if (a->B_stride_b % 4 != 0 || a->B_stride_g % 4 != 0 || a->C_stride_b % 4 != 0 || a->C_stride_g % 4 != 0 || a->state_stride_s % 4 != 0) return LQ_ERR_SHAPE;
   if (!sv_al(a->B, 8) || !sv_al(a->C, 8) || !sv_al(a->state, 16) || !sv_al(a->x, 2) || !sv_al(a->out, 2) || !sv_al(a->dt, sv_size(a->dt_dtype)) ||
       !sv_al(a->A, 4) || !sv_al(a->D, 4) || !sv_al(a->dt_bias, 4) || !sv_al(a->slots, 4))

@@ -101,21 +101,22 @@ def test_ssm_refusals():
 
 @pytest.mark.parametrize("fn,good,bad", [
     ("lq_quantize_rows", dict(x=1, codes=1, scale=1, rows=2, cols=32, x_stride=32, codes_stride=32),
-     [dict(cols=0), dict(cols=16385), dict(rows=0), dict(dtype=2)]),
+     [dict(cols=0), dict(cols=16385), dict(rows=0), dict(dtype=2), dict(rows=1 << 24, cols=7), dict(rows=1 << 26)]),
     ("lq_int8_matmul", dict(a=1, b=1, a_scale=1, b_scale=1, out=1, rows=2, cols=8, inner=32, a_stride=32, b_stride=32, out_stride=8),
-     [dict(inner=24), dict(inner=131072), dict(a_stride=40), dict(b_stride=8), dict(out_dtype=2), dict(rows=0), dict(cols=-1)]),
+     [dict(inner=24), dict(inner=131072), dict(a_stride=40), dict(b_stride=8), dict(out_dtype=2), dict(rows=0), dict(cols=-1), dict(cols=(1 << 27) + 1),
+      dict(rows=(1 << 31) - 1, cols=(1 << 31) - 1)]),
     ("lq_residual_rmsnorm", dict(x=1, weight=1, out=1, rows=2, dim=32),
      [dict(codes=1, row_scale=1), dict(dtype=1), dict(weight_dtype=2), dict(dim=16385), dict(gate=1, gate_rows=0),
       dict(residual=1, residual_dtype=3)]),
     ("lq_conv1d_prompt", dict(x=1, weight=1, out=1, nseq=1, seqlen=4, dim=16, width=4, x_stride_l=16),
      [dict(dim=12), dict(width=5), dict(width=1), dict(x_stride_l=12), dict(seqlen=0), dict(nseq=0), dict(state=1, num_slots=0), dict(dtype=1),
-      dict(seq_starts=1, tokens=0)]),
+      dict(seq_starts=1, tokens=0), dict(seqlen=1 << 28), dict(nseq=1 << 20, seqlen=1 << 20)]),
     ("lq_conv1d_step", dict(x=1, weight=1, out=1, state=1, num_slots=1, batch=1, dim=16, width=4, x_stride=16),
-     [dict(dim=12), dict(width=5), dict(x_stride=12), dict(batch=0), dict(num_slots=0), dict(state_stride_w=4)]),
+     [dict(dim=12), dict(width=5), dict(x_stride=12), dict(batch=0), dict(num_slots=0), dict(state_stride_w=4), dict(batch=1 << 26)]),
     ("lq_ssm_prompt", dict(x=1, dt=1, A=1, B=1, C=1, out=1, nseq=1, seqlen=4, nheads=2, headdim=8, ngroups=1, dstate=16, workspace=1,
                            workspace_bytes=1 << 40),
      [dict(headdim=12), dict(dstate=264), dict(dstate=12), dict(ngroups=4), dict(seqlen=0), dict(B_stride_l=4), dict(x_stride_l=1 << 24), dict(workspace_bytes=0),
-      dict(state=1, num_slots=0), dict(dtype=1), dict(dt_dtype=2)]),
+      dict(state=1, num_slots=0), dict(dtype=1), dict(dt_dtype=2), dict(seqlen=1 << 30), dict(nseq=1 << 26, seqlen=1)]),
     ("lq_ssm_step", dict(x=1, dt=1, A=1, B=1, C=1, out=1, state=1, num_slots=1, batch=1, nheads=2, headdim=8, ngroups=1, dstate=16),
      [dict(headdim=12), dict(dstate=264), dict(ngroups=4), dict(batch=0), dict(batch=65536), dict(state_stride_s=2), dict(num_slots=0)]),
 ])
