@@ -357,6 +357,7 @@ LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
       return r;
     }
     before += total, ubefore += __builtin_amdgcn_readlane(usum, 63);
+    if (ubefore > p.units) break;
   }
   return r;
 }
@@ -397,7 +398,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   }
   if (sg >= p.segs) return;
   Segment s = segment_of(p, sg);
-  if (s.seq < 0 || (STATES && s.last)) return;
+  // (starts that do not ascend can name the same tokens twice: what is behind the tables' end is left out)
+  if (s.seq < 0 || s.unit0 + s.chunks > p.units || (STATES && s.last)) return;
   if (STATES) {  // (a segment that is not a prompt's last one has all its chunks)
     s.chunks = p.seg_chunks / p.pieces;
     const int skip = (at - sg * p.pieces) * s.chunks;
@@ -796,7 +798,7 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(PromptParams p) {
   } else {
     first = seq * n;
   }
-  if (at >= per) return;
+  if (at >= per || first > p.segs - n) return;
   const int slot = p.state || p.slots ? sv_slot(p.slots, seq, p.num_slots) : kSlotPad;
   lq_v4f v = {0.f, 0.f, 0.f, 0.f};
   if (p.state && slot >= 0) v = *(const lq_v4f*)(p.state + slot * p.ss_s + h * per + at);

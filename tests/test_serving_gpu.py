@@ -396,6 +396,24 @@ def test_ssm_large_steps_and_values(cuda):
     assert_near(torch.where(fits, y.cpu(), 0.0), torch.where(fits, wy, 0.0), mag, ssm_y_rel([96], 200.0, F16), "y")
 
 
+@pytest.mark.parametrize("T", [100, 2500])
+def test_starts_that_do_not_ascend(cuda, T):
+    """Prompts that name the same tokens again and again: more chunks than there is workspace for.  Nothing is touched out of range, and
+    the first one's state is what it is by itself."""
+    v = _dev(ssm_inputs(T, 2, 64, 1, 64, F16, seed=31), cuda)
+    args = [v[k] for k in ("x", "dt", "A", "B", "C")]
+    st, alone = torch.zeros(16, 2, 64, 64, device=cuda), torch.zeros(1, 2, 64, 64, device=cuda)
+    ssm_prompt(*args, state=st, seq_starts=torch.tensor([0, T] * 8 + [0], dtype=torch.int32, device=cuda))
+    ssm_prompt(*args, state=alone, seq_starts=starts_of([T], cuda))
+    torch.cuda.synchronize()
+    scale = alone.abs().max()
+    assert ((st[0] - alone[0]).abs().max() <= 2.0 ** -9 * scale).all()   # (cut into other segments, perhaps)
+    x = v["x"].flatten(1)
+    cst = torch.zeros(16, 3, 128, dtype=F16, device=cuda)
+    conv1d_prompt(x, torch.ones(128, 4, device=cuda).half(), state=cst, seq_starts=torch.tensor([0, T] * 8 + [0], dtype=torch.int32, device=cuda))
+    assert torch.equal(cst[0], x[T - 3:])
+
+
 def test_ssm_nan_stays_in_its_sequence_and_head(cuda):
     v = ssm_inputs(300, 4, 64, 1, 128, BF16, seed=20)
     clean = _dev(v, cuda)
