@@ -62,6 +62,8 @@ class Int8InputLinear(nn.Module):
 
     def forward_int8(self, x_i8: torch.Tensor, scale) -> torch.Tensor:
         s = scale.to(device=x_i8.device, dtype=torch.float32) if isinstance(scale, torch.Tensor) else float(scale)
+        if isinstance(s, torch.Tensor) and s.numel() != 1:  # one for each row
+            s = s.reshape(*x_i8.shape[:-1], 1)
         return torch.nn.functional.linear((x_i8.to(torch.float32) * s).to(torch.float16), self.weight, self.bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -167,3 +167,14 @@ def test_mixer_serving_refusals():
     refuses(m.step, (z(1, 1, 64, dtype=I8), 1.0), st)                                   # codes of other dimensions
     refuses(m.prefill, (z(4, 64, dtype=I8), 1.0), st)
     refuses(m.prefill, (z(1, 4, 64, dtype=I8), 1.0), st, None, z(2, dtype=I32))
+
+
+def test_int8_input_linear_takes_a_scale_for_each_row():
+    from linquant_amd.quantized_mamba2 import Int8InputLinear
+
+    w = torch.arange(12.0).view(3, 4) / 8
+    lin = Int8InputLinear(w, 1.0)
+    codes, scale = torch.arange(-8, 8).to(I8).view(4, 4), torch.tensor([0.5, 1.0, 2.0, 0.25])   # as many rows as columns
+    want = torch.cat([lin.forward_int8(codes[i:i + 1], scale[i]) for i in range(4)])
+    assert torch.equal(lin.forward_int8(codes, scale), want)
+    assert torch.equal(lin.forward_int8(codes.view(2, 2, 4), scale.view(2, 2)), want.view(2, 2, 3))
