@@ -1,7 +1,7 @@
 // lq_ssm_step: one token of each sequence through the selective state space scan, the fp32 state updated in place.
 //   S = exp(d A) S + d x B^T,  y = S C + D x,  d = softplus(dt + bias)
-// HBM-bound: 8 bytes for each entry of the state, five operations.  80 heads of 64 by 128: 256 sequences 271 us, 5.0 TB/s (a large copy
-// reaches 5.1); 4 sequences 6.7 us, 20 MB behind a launch and two round trips to memory.
+// HBM-bound: 8 bytes for each entry of the state, five operations.  80 heads of 64 by 128: 256 sequences 266 us, 5.1 TB/s, the rate
+// of a large copy; 4 sequences 6.5 us, 21 MB behind a launch and two round trips to memory.
 //
 // Eight lanes have one row of the state (a head channel) in pieces of 16 bytes, so that a wave's request covers eight whole 128-byte
 // lines and the sum over the row is three exchanges.
@@ -59,27 +59,38 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(StepParams p) {
   }
   float* S = p.state + slot * p.ss_s + (int64_t)h * p.P * p.N;
   const uint16_t* xp = p.x + b * p.sx_b + h * p.sx_h;
-  for (int r0 = 8 * wave; r0 < p.P; r0 += 32) {
-    const int row = r0 + r8;  // (P is a multiple of 8)
-    float* Sr = S + (int64_t)row * p.N;
-    const float xv = T::to(xp[row]), dx = d * xv;
-    lq_v4f s[KN];
+  // 16 rows of a wave requested together: one round trip to memory where a head has 64 (eight at a time: 271 and 6.8 us)
+  for (int r0 = 8 * wave; r0 < p.P; r0 += 64) {
+    lq_v4f s[2][KN];
+    float xv[2];
 #pragma unroll
-    for (int k = 0; k < KN; ++k) s[k] = *(const lq_v4f*)(Sr + min(32 * k + 4 * sub, p.N - 4));
-    float y = 0.0f;
+    for (int u = 0; u < 2; ++u) {
+      const int row = min(r0 + 32 * u, p.P - 8) + r8;  // (P is a multiple of 8)
+      xv[u] = T::to(xp[row]);
 #pragma unroll
-    for (int k = 0; k < KN; ++k) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[k][e] = __builtin_fmaf(dx, Bv[k][e], decay * s[k][e]);
-        y = __builtin_fmaf(s[k][e], Cv[k][e], y);
-      }
-      if (32 * k + 4 * sub < p.N) *(lq_v4f*)(Sr + 32 * k + 4 * sub) = s[k];
+      for (int k = 0; k < KN; ++k) s[u][k] = *(const lq_v4f*)(S + (int64_t)row * p.N + min(32 * k + 4 * sub, p.N - 4));
     }
 #pragma unroll
-    for (int off = 4; off >= 1; off >>= 1) y += __shfl_xor(y, off, 64);
-    if (p.D) y = __builtin_fmaf(p.D[p.D_has_hdim ? h * p.P + row : h], xv, y);
-    if (sub == 0) op[row] = T::from(y);
+    for (int u = 0; u < 2; ++u) {
+      if (r0 + 32 * u >= p.P) break;
+      const int row = r0 + 32 * u + r8;
+      float* Sr = S + (int64_t)row * p.N;
+      const float dx = d * xv[u];
+      float y = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KN; ++k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[u][k][e] = __builtin_fmaf(dx, Bv[k][e], decay * s[u][k][e]);
+          y = __builtin_fmaf(s[u][k][e], Cv[k][e], y);
+        }
+        if (32 * k + 4 * sub < p.N) *(lq_v4f*)(Sr + 32 * k + 4 * sub) = s[u][k];
+      }
+#pragma unroll
+      for (int off = 4; off >= 1; off >>= 1) y += __shfl_xor(y, off, 64);
+      if (p.D) y = __builtin_fmaf(p.D[p.D_has_hdim ? h * p.P + row : h], xv[u], y);
+      if (sub == 0) op[row] = T::from(y);
+    }
   }
 }
 
