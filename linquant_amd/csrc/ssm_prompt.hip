@@ -110,26 +110,19 @@ LQ_DEV lq_v4i round8(const float (&a)[8], const float (&b)[8]) {
     return round8<T>(v);
   }
 }
-// eight products a b as two pieces each: fp16, hi = RN(a b), lo = RN(a b - hi), one mixed-precision instruction a piece; bf16 likewise
-// from the rounded product
+// two products as two pieces each: fp16, hi = RN(a b), lo = RN(a b - hi), one mixed-precision instruction a piece; bf16 likewise from the
+// rounded product
 template <typename T>
-LQ_DEV void split(const float (&a)[8], const float (&b)[8], lq_v4i& hi, lq_v4i& lo) {
+LQ_DEV void split2(float a0, float b0, float a1, float b1, int& hi, int& lo) {
   if constexpr (std::is_same<T, F16>::value) {
-    lq_v8h h, l;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[i] = (_Float16)__builtin_fmaf(a[i], b[i], 0.0f);
-      l[i] = (_Float16)__builtin_fmaf(a[i], b[i], -(float)h[i]);
-    }
-    hi = __builtin_bit_cast(lq_v4i, h), lo = __builtin_bit_cast(lq_v4i, l);
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const v2h h = {(_Float16)__builtin_fmaf(a0, b0, 0.0f), (_Float16)__builtin_fmaf(a1, b1, 0.0f)};
+    const v2h l = {(_Float16)__builtin_fmaf(a0, b0, -(float)h[0]), (_Float16)__builtin_fmaf(a1, b1, -(float)h[1])};
+    hi = __builtin_bit_cast(int, h), lo = __builtin_bit_cast(int, l);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float u = a[2 * i] * b[2 * i], v = a[2 * i + 1] * b[2 * i + 1];
-      const uint32_t h = pack_bf16(u, v);
-      hi[i] = (int)h;
-      lo[i] = (int)pack_bf16(u - __uint_as_float(h << 16), v - __uint_as_float(h & 0xffff0000u));
-    }
+    const float u = a0 * b0, v = a1 * b1;
+    const uint32_t h = pack_bf16(u, v);
+    hi = (int)h, lo = (int)pack_bf16(u - __uint_as_float(h << 16), v - __uint_as_float(h & 0xffff0000u));
   }
 }
 // The power of two that brings m below 2^14 (and not below 2^13), within 2^-100 and 2^24: the quotient of two is a number, and pieces of
@@ -582,39 +575,71 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       }
       // the state behind the chunk
       {
-        lq_v4i bb[4];
-        lq_v4f w4[4][2];
-        auto ask = [&](int i) {  // operand i = NT ks + nt
-          bb[i & 3] = opB[(4 * (i % NT) + i / NT) * 64];
-          if (i % NT == 0) {
+        // Ahead: what the next products need is formed between these (one issued behind another of the same tile waits for it, and the
+        // vector unit is free): 384 tokens in fp16 36.4 -> 35.3 us.  bf16 lacks the registers from 65 state columns on (ragged prompts 140 ->
+        // 191, ten spilled).
+        constexpr bool kAhead = kHalf || NT < 4;
+        lq_v4i bb[3], wh[2], wl[2];
+        lq_v4f w4[2][2];
+        auto ask = [&](int i) { bb[i % 3] = opB[(4 * (i % NT) + i / NT) * 64]; };  // operand i = NT ks + nt
+        auto ask_w = [&](int ks) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) w4[i / NT][j] = *(const lq_v4f*)(my + Q + 16 * (i / NT) + 8 * j + 4 * hh);
-          }
+          for (int j = 0; j < 2; ++j) w4[ks & 1][j] = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh);
         };
+        auto pair = [&](int ks, int q) {  // a quarter of step ks' weighted x
+          const lq_v4f& w = w4[ks & 1][q >> 1];
+          int h, l;
+          split2<T>(w[2 * (q & 1)], x(ks, 2 * q), w[2 * (q & 1) + 1], x(ks, 2 * q + 1), h, l);
+          wh[kAhead ? ks & 1 : 0][q] = h, wl[kAhead ? ks & 1 : 0][q] = l;
+        };
+        ask_w(0);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) ask(i);
+        for (int i = 0; i < 2; ++i) ask(i);
         reads_stay();
         const float f = kHalf ? all * rescale : all;
+        if (kAhead) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int q = 0; q < 4; ++q) pair(0, q);
+        } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[nt][e] *= f;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) S[nt][e] *= f;
+        }
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          float w[8], xv[8];
-          lq_v4i wh, wl;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const int i = NT * ks + nt;
-            if (i + 3 < 4 * NT) ask(i + 3);
-            reads_stay();
-            if (nt == 0) {
+            if (i + 2 < 4 * NT) ask(i + 2);
+            if (nt == (kAhead ? 0 : NT - 1) && ks < 3) ask_w(ks + 1);
+            if (kAhead && ks == 0) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = w4[ks][e >> 2][e & 3], xv[e] = x(ks, e);
-              split<T>(w, xv, wh, wl);
+              for (int e = 0; e < 16; ++e) S[nt][e] *= f;
             }
-            S[nt] = mfma<T>(bb[i & 3], wh, S[nt]);
-            S[nt] = mfma<T>(bb[i & 3], wl, S[nt]);
+            if (!kAhead) {
+              reads_stay();
+              if (nt == 0) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) pair(ks, q);
+              }
+            }
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+            S[nt] = mfma<T>(bb[i % 3], wh[kAhead ? ks & 1 : 0], S[nt]);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+            if (kAhead && ks < 3 && nt >= NT - 2) {
+              const int q = NT == 1 ? 0 : 2 * (nt - (NT - 2));
+              pair(ks + 1, q);
+              if (NT == 1) pair(ks + 1, q + 1);
+            }
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+            S[nt] = mfma<T>(bb[i % 3], wl[kAhead ? ks & 1 : 0], S[nt]);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+            if (kAhead && ks < 3 && nt >= NT - 2) {
+              const int q = NT == 1 ? 2 : 2 * (nt - (NT - 2)) + 1;
+              pair(ks + 1, q);
+              if (NT == 1) pair(ks + 1, q + 1);
+            }
           }
         }
       }
