@@ -19,11 +19,11 @@
 // is multiplied (a wave's state and weighted x; a row of weighted C B^T) below 2^14, so no size of activations overflows, and what is 2^24
 // times smaller than that largest starts to lose bits.
 //
-// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 404 us (operands 32, states 99, join 16, chunks
-// 293; 425 on a slower card), 1.8 TB/s of what has to move and 268 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
+// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 404 to 425 us by the card (operands 27 to
+// 33, states 94 to 104, join 16, chunks 285 to 312), 1.8 TB/s of what has to move and 268 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
 // busy 50 % of the time (scaling, rounding and splitting operands, 690 instructions to 32 channels and 64 tokens), the matrix unit 22 %, and
 // the clock falls from 2.4 to 2.1 GHz; two waves to a SIMD is what the state in registers (64 of 256) and 81 KB of LDS leave.  Few or
-// ragged prompts are a chain of chunks, 4.1 us each: 384 tokens 36 us, 6949 in 10 prompts of up to 2047, 64 heads in 8 groups, bf16, 140.
+// ragged prompts are a chain of chunks, about 4 us each: 384 tokens 35 us, 6949 in 10 prompts of up to 2047, 64 heads in 8 groups, bf16, 140.
 // Tried: C B^T formed by each workgroup (its product is the group's, so 80 heads made it 80 times); one piece of a state's additions (a state
 // gathers the rounding of a whole prompt); a higher priority for the younger of two workgroups, which the older one holds up (3 % less here,
 // 3 % more for ragged prompts).
