@@ -14,10 +14,12 @@
 //
 // Precision.  Activations enter the matrix products as they are, all sums are fp32, and so is the state.  What is formed in fp32 on the way
 // and reaches only y, which is rounded to the activations' type itself (weighted C B^T, the state that C multiplies), enters rounded to
-// that type, to the nearest: half a step of each term.  What the state gathers over a prompt (weighted x) enters as two pieces of the type,
-// 16 bits (bf16) or 22 (fp16).  bf16 has the range of fp32.  fp16: after a multiplication by a power of two that brings the largest of what
-// is multiplied (a wave's state and weighted x; a row of weighted C B^T) below 2^14, so no size of activations overflows, and what is 2^24
-// times smaller than that largest starts to lose bits.
+// that type, to the nearest: half a step of each term.  What the state gathers over a prompt (weighted x) enters as two pieces of the type:
+// off by 2^-18 of itself (bf16) or 2^-22 (fp16).  bf16 has the range of fp32.  fp16: after a multiplication by a power of two that brings the
+// largest of what is multiplied (a channel's state; its state and weighted x; a row of weighted C B^T) below 2^14, so no size of
+// activations overflows.  Below 2^-14 fp16 is evenly spaced: a state or weight 2^27 below its largest starts to lose bits, weighted x
+// (whose second piece is 2^11 smaller) 2^16 below its channel's.  A unit for 32 channels and 64 tokens together (2 % less time) lost a
+// channel beside one 2^26 above it, and the state that a chunk's first tokens read where a later one was as far above them.
 //
 // What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 404 to 425 us by the card (operands 27 to
 // 33, states 94 to 104, join 16, chunks 285 to 312), 1.8 TB/s of what has to move and 268 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
@@ -125,11 +127,11 @@ LQ_DEV void split2(float a0, float b0, float a1, float b1, int& hi, int& lo) {
     hi = (int)h, lo = (int)pack_bf16(u - __uint_as_float(h << 16), v - __uint_as_float(h & 0xffff0000u));
   }
 }
-// The power of two that brings m below 2^14 (and not below 2^13), within 2^-100 and 2^24: the quotient of two is a number, and pieces of
-// a value times 2^24 are 2^-49 of the activations' unit apart, less than matters to a sum that becomes fp16.
+// The power of two that brings m below 2^(TOP + 1) (and not below 2^TOP), within 2^LO and 2^HI
+template <int TOP, int LO, int HI>
 LQ_DEV float scale_for(float m) {
   const int e = (int)((__float_as_uint(m) >> 23) & 255u) - 127;  // (0: -127)
-  return __uint_as_float((uint32_t)(127 + min(max(13 - e, -100), 24)) << 23);
+  return __uint_as_float((uint32_t)(127 + min(max(TOP - e, LO), HI)) << 23);
 }
 // the largest of a wave's non-negative values, by lane permutations of the vector unit; the same for the whole wave
 // (whole numbers order like them, and their maximum takes a permuted operand)
@@ -147,6 +149,12 @@ LQ_DEV float wave_top(float f) {
 }
 LQ_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 LQ_DEV float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+// the larger of a lane's and the lane's of the other half, which has the same channel (by their bits: non-negative numbers)
+LQ_DEV uint32_t channel_top(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+LQ_DEV float channel_top(float v) { return __uint_as_float(channel_top(__float_as_uint(v))); }
 // a power of two's reciprocal
 LQ_DEV float pow2_inverse(float v) { return __uint_as_float(0x7f000000u - __float_as_uint(v)); }
 // Four rows of 16 entries of 16 bits, given by the 16 lanes of a quarter of the wave as four pieces a row, come back by columns: lane i has
@@ -425,7 +433,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         for (int e = 0; e < 4; ++e) S[nt][4 * j + e] = v[e];
       }
   }
-  float unit_S = 1.0f;  // fp16: S holds the state times this power of two
+  float unit_S = 1.0f;  // fp16: S holds the channel's state times this power of two
   const float Dv = !STATES && p.D ? p.D[p.D_has_hdim ? h * p.P + chc : h] : 0.0f;
   const bool bad = slot == kSlotBad;
 
@@ -480,7 +488,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   float* my = tok[wave];
   lq_v4i xp[4];  // this lane's channel, tokens in the order of an operand
   auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
-  float sum64 = 0.0f, step = 0.0f, all = 0.0f, rescale = 1.0f, row = 1.0f, lrow = 0.0f;
+  float sum64 = 0.0f, step = 0.0f, all = 0.0f, row = 1.0f, lrow = 0.0f;
+  float rescale = 1.0f, read = 1.0f, unread = 1.0f;  // fp16: to the state's new unit; what C multiplies is S times `read`, 1 / unread of the state
+  uint32_t units = 0;                                // fp16: the power of two of x that enters the state, twice
   bool apart = false;
   auto begin = [&](int c) {
     const uint16_t* xl = xbuf[c & 1][wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
@@ -493,10 +503,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     const float last = lane63(cv);
     all = exp2_fast(last);
     decay += last;
-    float ui = 1.0f;
+    float uw = 1.0f;
     if constexpr (kHalf) {
-      // the wave's new unit: its state and what the chunk adds, each below 2^14 of it
-      float m = 0.0f;  // (no number where the channel has one that is none: its scale does not matter then)
+      // Units of the channel, from its largest entry of the state and of x.  What C multiplies has one of its own: what the chunk adds can be
+      // far above the state that its first tokens read.
+      float m = 0.0f;  // (no number where the lane has one that is none: its scale does not matter then)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -509,12 +520,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           typedef uint16_t v2u __attribute__((ext_vector_type(2)));
           top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
         }
-      const float mx = T::to((uint16_t)max(top & 0xffffu, top >> 16));
-      const float u = scale_for(wave_top(fmaxf(finite_size(m) * pow2_inverse(unit_S), finite_size(mx) * wave_top(finite_size(wv)))));
-      rescale = u * pow2_inverse(unit_S);
-      unit_S = u, ui = pow2_inverse(u);
+      const float mx = channel_top(finite_size(T::to((uint16_t)max(top & 0xffffu, top >> 16)))), ms = channel_top(finite_size(m));
+      const float mw = wave_top(finite_size(wv)), iu = pow2_inverse(unit_S);
+      // The state's new unit is uw, which brings the weights below 1, times that of x: within fp16, and such that weighted x is below 2^14 and
+      // the state too, unless it is 2^38 above x (it is kept in 32 bits: nothing overflows)
+      uw = scale_for<-1, -60, 24>(mw);
+      const float k = fminf(fmaxf(scale_for<13, -100, 24>(fmaxf(ms * iu, mx * mw)) * pow2_inverse(uw), 0x1p-24f), 0x1p15f);
+      const uint32_t k16 = F16::from(k);
+      units = k16 | k16 << 16;
+      if (!STATES) read = scale_for<13, -100, 100>(ms), unread = pow2_inverse(read) * iu;
+      unit_S = uw * k, rescale = unit_S * iu;
       if (!STATES) {
-        row = scale_for(rv * mv);  // brings the token's row of weighted C B^T below 2^14
+        row = scale_for<13, -100, 24>(rv * mv);  // brings the token's row of weighted C B^T below 2^14
         lrow = (float)((int)(__float_as_uint(row) >> 23) - 127);
       }
     }
@@ -524,7 +541,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     const float before = __shfl(cv, (lane & 56) - 1, 64), ahead = (lane < 8 ? 0.0f : before) - cv;
     apart = !STATES && __ballot(!(ahead < 60.0f)) == 0;
     my[lane] = apart ? exp2_fast(ahead) * dv : dv;
-    my[Q + lane] = kHalf ? wv * unit_S : wv, my[2 * Q + lane] = kHalf ? exp2_fast(cv) * row * ui : exp2_fast(cv);
+    my[Q + lane] = kHalf ? wv * uw : wv, my[2 * Q + lane] = kHalf ? exp2_fast(cv) * row : exp2_fast(cv);
   };
   if (live) begin(0);
   for (int c = 0; c < s.chunks; ++c) {
@@ -557,7 +574,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           __builtin_amdgcn_sched_barrier(0);  // (all of S converted ahead is registers that it lacks)
           float v[8], r[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i], r[i] = rescale;
+          for (int i = 0; i < 8; ++i) v[i] = S[k >> 1][8 * (k & 1) + i], r[i] = read;
           const lq_v4i sh = kHalf ? round8<T>(v, r) : round8<T>(v);
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) Y[tt] = mfma<T>(cc[k % 3][tt], sh, Y[tt]);
@@ -570,7 +587,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
           for (int j = 0; j < 4; ++j) e4[j] = *(const lq_v4f*)(my + 2 * Q + 32 * tt + 8 * j + 4 * hh);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) Y[tt][e] *= e4[e >> 2][e & 3];
+          for (int e = 0; e < 16; ++e) Y[tt][e] *= kHalf ? e4[e >> 2][e & 3] * unread : e4[e >> 2][e & 3];
         }
       }
       // the state behind the chunk
@@ -588,8 +605,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         };
         auto pair = [&](int ks, int q) {  // a quarter of step ks' weighted x
           const lq_v4f& w = w4[ks & 1][q >> 1];
+          float x0 = x(ks, 2 * q), x1 = x(ks, 2 * q + 1);
+          if constexpr (kHalf) {
+            typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+            const int two = xp[ks][q];  // (an element's bits are not cast in place)
+            const v2h x2 = __builtin_bit_cast(v2h, two) * __builtin_bit_cast(v2h, units);
+            x0 = (float)x2[0], x1 = (float)x2[1];
+          }
           int h, l;
-          split2<T>(w[2 * (q & 1)], x(ks, 2 * q), w[2 * (q & 1) + 1], x(ks, 2 * q + 1), h, l);
+          split2<T>(w[2 * (q & 1)], x0, w[2 * (q & 1) + 1], x1, h, l);
           wh[kAhead ? ks & 1 : 0][q] = h, wl[kAhead ? ks & 1 : 0][q] = l;
         };
         ask_w(0);

@@ -1,0 +1,87 @@
+"""The serving operators at the edges of what they take: one row of a wide tensor, prompts in each way of being cut, steps that let a
+state grow, magnitudes far apart, values that are no numbers."""
+
+import pytest
+import torch
+
+from linquant_amd import _lib
+from linquant_amd.kernels.mamba2.conv1d_state import conv1d_prompt, conv1d_step
+from linquant_amd.kernels.mamba2.ssm import ssm_prompt, ssm_step
+from linquant_amd.norm import residual_rmsnorm, rmsnorm_gated, rmsnorm_gated_qhad
+from linquant_amd.hadamard_utils import qhad_transform
+from linquant_amd.w8a8_linear import W8A8Linear, int8_matmul, quantize_rows
+from tests.serving_cases import HALF_STEP, TINY, assert_near, ssm_inputs, ssm_ref, ssm_rel, ssm_y_rel, starts_of
+from tests.test_serving_mixer_gpu import build, check_call, snapshot, tokens
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+NAN, INF = float("nan"), float("inf")
+
+
+def _gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def _rn(*shape, seed=0):
+    return torch.randn(*shape, generator=_gen(seed))
+
+
+# ------------------------------------------------------------------------------------------------------------- the scan
+def _scan(cuda, v, lens, *, packed=True, state=None, slots=None, **kw):
+    """(y, state behind, the formula's y, its magnitudes, state and magnitudes, the most that |d A| sums to in a chunk); the formula in 64
+    bits on the GPU, where the token loop is quicker."""
+    d = {k: t.to(cuda) for k, t in v.items()}
+    n = len(lens)
+    st = None if state is None else state.to(cuda)
+    call = dict(D=d["D"], dt_bias=d.get("dt_bias"), state=st, slots=None if slots is None else torch.tensor(slots, dtype=torch.int32, device=cuda), **kw)
+    args = [d[k] for k in ("x", "dt", "A", "B", "C")]
+    if packed:
+        y = ssm_prompt(*args, **call, seq_starts=starts_of(lens, cuda))
+    else:
+        y = ssm_prompt(*(a if a is d["A"] else a.unflatten(0, (n, lens[0])) for a in args), **call).flatten(0, 1)
+    H, P, N = v["x"].shape[1], v["x"].shape[2], v["B"].shape[2]
+    use = list(range(n)) if slots is None else slots
+    first = torch.stack([torch.zeros(H, P, N) if state is None or s < 0 else state[s] for s in use]).to(cuda)
+    ref = ssm_ref(*args, d["D"], d.get("dt_bias"), kw.get("dt_softplus", True), kw.get("dt_limit", (0.0, INF)), lens, first)
+    return (y, st, *ref)
+
+
+def _near_where_finite(y, want, mag, rel):
+    """``assert_near`` where even the largest error that it allows, half a step of fp16 and rel * mag, leaves a number of fp16 (or bf16): a result that
+    may be off past 65504 may be an infinity."""
+    fits = want.abs() * (1 + 2.0 ** -8) + 1.01 * rel * mag < torch.finfo(y.dtype).max
+    assert_near(torch.where(fits, y, 0.0), torch.where(fits, want, 0.0), torch.where(fits, mag, 0.0), rel, "y")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("carried", [0, 20, 60])
+@pytest.mark.parametrize("T", [1, 150])
+def test_channels_far_apart(cuda, dtype, carried, T):
+    """One channel of a head far above the others, by its activations (2^26) and by what it carries in: the others are as if it was not there."""
+    H, P, G, N = 2, 64, 1, 128
+    v = ssm_inputs(T, H, P, G, N, dtype, seed=13, a_max=1.3, dt_mean=-4.5)
+    v["x"] = v["x"] * 2.0 ** -12
+    v["x"][:, :, 5] = v["x"][:, :, 5] * 2.0 ** 25
+    state = _rn(1, H, P, N, seed=4) * 2.0 ** -14
+    state[:, :, 37] *= 2.0 ** carried
+    y, st, wy, mag, ws, smag, most = _scan(cuda, v, [T], state=state)
+    assert_near(st[0], ws[0], smag[0], ssm_rel([T], most), "state")
+    _near_where_finite(y, wy, mag, ssm_y_rel([T], most, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("at", [20, 63, 64, 100])
+@pytest.mark.parametrize("T", [110, 600])
+def test_tokens_far_apart(cuda, dtype, at, T):
+    """A token far above those in front of it, which read a small state: they are as if it was not there.  And a prompt that goes on in front of a state far
+    above it."""
+    H, P, G, N = 2, 64, 1, 64
+    v = ssm_inputs(T, H, P, G, N, dtype, seed=14, a_max=1.3, dt_mean=-4.5)
+    v["x"] = v["x"] * 2.0 ** -12
+    v["x"][at] = v["x"][at] * 2.0 ** 25
+    for up in (-14, 30):
+        state = _rn(1, H, P, N, seed=4) * 2.0 ** up
+        y, st, wy, mag, ws, smag, most = _scan(cuda, v, [T], state=state)
+        assert_near(st[0], ws[0], smag[0], ssm_rel([T], most), "state")
+        _near_where_finite(y, wy, mag, ssm_y_rel([T], most, dtype))
