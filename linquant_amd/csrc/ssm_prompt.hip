@@ -537,9 +537,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     }
     // The weight exp(c_t - c_s) d_s of an entry of C B^T.  Where no eight tokens decay by 2^60, it is r q: r = exp(c_t - c) for each row and
     // block of eight tokens, c that in front of the block, and q = exp(c - c_s) d_s, at most 2^60 d_s: twelve exponentials a lane instead of
-    // 48, and what r rounds to zero is below 2^-66.
+    // 48, and what r rounds to zero is below 2^-66.  Nor may c rise (negative steps), for r is cut off at 2^30: half a unit of it to a block
+    // is the rounding of its sums, and what eight blocks add up to then stays below 2^28 with the row's unit, 2^24 at most.
     const float before = __shfl(cv, (lane & 56) - 1, 64), ahead = (lane < 8 ? 0.0f : before) - cv;
-    apart = !STATES && __ballot(!(ahead < 60.0f)) == 0;
+    apart = !STATES && __ballot(!(__builtin_fabsf(ahead - 29.75f) < 30.25f)) == 0;
     my[lane] = apart ? exp2_fast(ahead) * dv : dv;
     my[Q + lane] = kHalf ? wv * uw : wv, my[2 * Q + lane] = kHalf ? exp2_fast(cv) * row : exp2_fast(cv);
   };

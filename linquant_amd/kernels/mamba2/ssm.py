@@ -58,7 +58,8 @@ def ssm_prompt(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_lim
     """S = exp(d A) S + d x B^T,  y = S C + D x  over each prompt, d = clamp(softplus(dt + dt_bias), *dt_limit) (``dt_softplus``
     False: without the softplus).  ``x`` (B, L, H, P) fp16 or bf16, ``dt`` (B, L, H), ``B``, ``C`` (B, L, G, N), or each without
     its first dimension and with T tokens with ``seq_starts`` (n + 1 int32, ascending) for packed prompts of any lengths; tokens
-    outside them keep undefined outputs.  ``A`` (H,) negative, ``D`` (H,) or (H, P).  P and N multiples of 8, N up to 256.
+    outside them keep undefined outputs.  ``A`` (H,) negative, ``D`` (H,) or (H, P).  P and N multiples of 8, N up to 256.  (A ``dt_limit``
+    that lets steps be negative lets the state grow.)
     ``state`` (slots, H, P, N) fp32: what each prompt starts from, replaced by what it ends in (a prompt of no tokens leaves it);
     None: zero, nothing kept.  ``slots`` (n,) int32: each prompt's place in the state, all different; negative: from zero, nothing
     kept; beyond the state: NaN outputs.  Returns y, dense, in the shape and type of x."""

@@ -54,6 +54,35 @@ def _near_where_finite(y, want, mag, rel):
     assert_near(torch.where(fits, y, 0.0), torch.where(fits, want, 0.0), torch.where(fits, mag, 0.0), rel, "y")
 
 
+def _growing(dtype, T, turn, bits):
+    """Steps that are negative for `turn` tokens, so that a state grows by 2^bits over them, and as positive for the next."""
+    H, P, G, N = 3, 40, 1, 64
+    v = ssm_inputs(T, H, P, G, N, dtype, seed=9)
+    v["A"] = torch.full((H,), -1.0)
+    v["dt"] = (torch.full((T, H), bits / turn / 1.4427) * torch.where(torch.arange(T) // turn % 2 == 0, -1.0, 1.0)[:, None]).float()
+    del v["dt_bias"]
+    return v
+
+
+@pytest.mark.parametrize("dtype,turn,bits,scale", [(BF16, 32, 45, 0), (BF16, 64, 60, 0), (BF16, 7, 20, 0), (F16, 32, 26, -14), (F16, 64, 24, -14), (F16, 7, 8, 0)])
+def test_steps_that_let_the_state_grow(cuda, dtype, turn, bits, scale):
+    """Negative steps, where ``dt_limit`` lets them through: the weights of a chunk's tokens grow along it."""
+    v = _growing(dtype, 200, turn, bits)
+    v["B"], v["C"], v["x"] = v["B"] * 2.0 ** scale, v["C"] * 2.0 ** scale, v["x"] * 2.0 ** -(scale // 2)
+    state = _rn(1, 3, 40, 64, seed=3) * 2.0 ** -8
+    y, st, wy, mag, ws, smag, most = _scan(cuda, v, [200], state=state, dt_softplus=False, dt_limit=(-INF, INF))
+    assert (wy.abs() < 60000).all() or dtype == BF16
+    assert_near(y, wy, mag, ssm_y_rel([200], most, dtype), "y")
+    assert_near(st[0], ws[0], smag[0], ssm_rel([200], most), "state")
+    d = {k: t.to(cuda) for k, t in v.items()}
+    one = state.to(cuda)
+    for t in range(70):                                             # token by token
+        ssm_step(one, d["x"][t:t + 1], d["dt"][t:t + 1], d["A"], d["B"][t:t + 1], d["C"][t:t + 1], dt_softplus=False, dt_limit=(-INF, INF))
+    part = {k: x if k in ("A", "D") else x[:70] for k, x in v.items()}
+    y, st, wy, mag, ws, smag, most = _scan(cuda, part, [70], state=state, dt_softplus=False, dt_limit=(-INF, INF))
+    assert_near(one[0], ws[0], smag[0], ssm_rel([70], most), "state of single tokens")
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("carried", [0, 20, 60])
 @pytest.mark.parametrize("T", [1, 150])
