@@ -91,7 +91,7 @@ def residual_rmsnorm(x, weight, residual=None, eps=1e-5, *, gate=None, scale=1.0
     assert x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1
     dim = x.shape[-1]
     assert 1 <= dim <= 16384 and weight.shape == (dim,) and weight.dtype in _CODES
-    assert post_weight is None or post_weight.shape == (dim,)
+    assert post_weight is None or (post_weight.shape == (dim,) and post_weight.dtype in _CODES)
     assert residual is None or (residual.shape == x.shape and residual.dtype in (x.dtype, torch.float32))
     rdt = residual.dtype if residual is not None else (residual_dtype or x.dtype)
     assert rdt in (x.dtype, torch.float32) and residual_dtype in (None, rdt)
@@ -113,8 +113,10 @@ def residual_rmsnorm(x, weight, residual=None, eps=1e-5, *, gate=None, scale=1.0
             assert x.dim() == 3 and gate.shape == (x.shape[0], 1, dim), "gate: (dim,), the shape of x, or (B, 1, dim)"
             gate, gate_rows = _row_view(gate, dim), x.shape[1]
             gate_stride = gate.stride(0)
+    if post_weight is not None and post_weight.dtype != weight.dtype:  # one type for both: neither loses bits or range
+        weight, post_weight = weight.float(), post_weight.float()
     weight = weight.contiguous()
-    post_weight = None if post_weight is None else post_weight.to(weight.dtype).contiguous()
+    post_weight = None if post_weight is None else post_weight.contiguous()
     r_out = torch.empty(x.shape, dtype=rdt, device=x.device)
     out = codes = row_scale = None
     if quantize is None:

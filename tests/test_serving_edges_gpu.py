@@ -27,6 +27,21 @@ def _rn(*shape, seed=0):
     return torch.randn(*shape, generator=_gen(seed))
 
 
+@pytest.mark.parametrize("wt,pt", [(F16, F32), (BF16, F32), (F32, F16), (F16, BF16), (BF16, F16)])
+def test_norm_weights_of_two_types(cuda, wt, pt):
+    """Each weight enters as it is: nothing of the wider type's bits or range is lost to the other's."""
+    x, w = _rn(3, 264).half(), (1 + 0.1 * _rn(264, seed=1)).to(wt)
+    post = (1 + 0.1 * _rn(264, seed=2)).to(pt)
+    post[:8] *= 2.0 ** (30 if pt != F16 else 12)
+    y, r = residual_rmsnorm(x.to(cuda), w.to(cuda), post_weight=post.to(cuda), residual_dtype=F32)
+    u = x.double()
+    want = u * torch.rsqrt(u.square().mean(-1, keepdim=True) + 1e-5) * post.double()
+    # the mean's sum over 264 in four waves, its square root and three products: fewer than 32 roundings
+    assert_near(r, want, want.abs(), 32 * 2.0 ** -24, "r")
+    f = torch.rsqrt(want.square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    assert_near(y, f * want, (f * want).abs(), 64 * 2.0 ** -24, "y")
+
+
 # ------------------------------------------------------------------------------------------------------------- the scan
 def _scan(cuda, v, lens, *, packed=True, state=None, slots=None, **kw):
     """(y, state behind, the formula's y, its magnitudes, state and magnitudes, the most that |d A| sums to in a chunk); the formula in 64
