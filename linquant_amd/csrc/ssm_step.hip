@@ -79,12 +79,14 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(StepParams p) {
       float y = 0.0f;
 #pragma unroll
       for (int k = 0; k < KN; ++k) {
+        if (32 * k + 4 * sub < p.N) {  // (a lane behind the row has another's entries, which are no numbers of its own to add)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[u][k][e] = __builtin_fmaf(dx, Bv[k][e], decay * s[u][k][e]);
-          y = __builtin_fmaf(s[u][k][e], Cv[k][e], y);
+          for (int e = 0; e < 4; ++e) {
+            s[u][k][e] = __builtin_fmaf(dx, Bv[k][e], decay * s[u][k][e]);
+            y = __builtin_fmaf(s[u][k][e], Cv[k][e], y);
+          }
+          *(lq_v4f*)(Sr + 32 * k + 4 * sub) = s[u][k];
         }
-        if (32 * k + 4 * sub < p.N) *(lq_v4f*)(Sr + 32 * k + 4 * sub) = s[u][k];
       }
 #pragma unroll
       for (int off = 4; off >= 1; off >>= 1) y += __shfl_xor(y, off, 64);

@@ -115,6 +115,24 @@ def test_channels_far_apart(cuda, dtype, carried, T):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("N", [8, 24, 40, 96, 128, 200])
+def test_single_tokens_and_infinite_entries(cuda, dtype, N):
+    """An infinite entry of the state gives its row's output its sign; the row's length need be no multiple of what a wave reads."""
+    H, P = 2, 16
+    v = {k: t.to(cuda) for k, t in ssm_inputs(1, H, P, 1, N, dtype, seed=22).items()}
+    for n in sorted({0, N // 2, N - 4, N - 1}):
+        st = torch.ones(1, H, P, N, device=cuda)
+        st[0, 1, 3, n], st[0, 0, 9, n] = INF, NAN
+        y = ssm_step(st, v["x"], v["dt"], v["A"], v["B"], v["C"])
+        assert float(y[0, 1, 3]) == float(v["C"][0, 0, n].sign()) * INF, n
+        assert torch.isnan(y[0, 0, 9])
+        y[0, 1, 3] = y[0, 0, 9] = 0.0
+        assert torch.isfinite(y).all()
+        st[0, 1, 3, n] = st[0, 0, 9, n] = 0.0
+        assert torch.isfinite(st).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("at", [20, 63, 64, 100])
 @pytest.mark.parametrize("T", [110, 600])
 def test_tokens_far_apart(cuda, dtype, at, T):
