@@ -79,6 +79,24 @@ class Mamba2State(NamedTuple):
     ssm: torch.Tensor   # (slots, nheads, headdim, d_state) fp32
 
 
+class _AsLaidOut:
+    """The tensors that something was made of, to tell whether they still are the same: the objects, where their entries lie and how often
+    they were written to.  (A copy or a loaded pickle of it, which has the copied module's tensors, marks them anew.)"""
+
+    def __init__(self, *tensors):
+        self.tensors, self.marks = tensors, [self._mark(t) for t in tensors]
+
+    @staticmethod
+    def _mark(t):
+        return (t.data_ptr(), 0 if t.is_inference() else t._version) if isinstance(t, torch.Tensor) else None
+
+    def __reduce__(self):
+        return _AsLaidOut, self.tensors
+
+    def holds(self, tensors):
+        return all(a is b and self._mark(b) == m for a, b, m in zip(self.tensors, tensors, self.marks))
+
+
 class QuantizedMamba2(nn.Module):
     """Calibrated buffers attached after construction, as in the reference: B_scale/B_inv_scale, C_scale/C_inv_scale
     (G,), A_log_scale, D_scale (scalars), alpha_hp (H, P), bscale_g (G,), static_state_scale (H, P), static_cb_scale
@@ -232,15 +250,23 @@ class QuantizedMamba2(nn.Module):
     @torch.no_grad()
     def prepare_serving(self):
         """Lays out once what ``prefill`` and ``step`` read beside the projections: the convolution's weights in fp16, A, D and dt_bias in
-        fp32 (dequantized as the INT8 kernels do), and out_proj's input scale as a number on the host.  ``allocate_state`` calls it;
-        so does whoever changes those parameters in place.  Moving the module and loading a state dict undo it."""
+        fp32 (dequantized as the INT8 kernels do), and out_proj's input scale as a number on the host.  ``allocate_state`` calls it.
+        Moving the module, loading a state dict, and exchanging, moving, loading or writing to one of those parameters or the modules that hold
+        them undo it."""
         bias = self.conv1d.bias
         self._serving = dict(
+            made_of=_AsLaidOut(*self._laid_out()),
             weight=self.conv1d.weight.detach().reshape(self.conv_dim, -1).to(torch.float16, copy=True).contiguous(),
             bias=None if bias is None else bias.detach().to(torch.float16, copy=True),
             A=-torch.exp(self.A_log.float() * self.A_log_scale.float()), D=self.D.float() * self.D_scale.float(),
             dt_bias=None if self.dt_bias is None else self.dt_bias.detach().to(torch.float32, copy=True),
             out_scale=float(self.out_proj.input_scale))
+
+    def _laid_out(self):
+        return (self.conv1d.weight, self.conv1d.bias, self.A_log, self.A_log_scale, self.D, self.D_scale, self.dt_bias, self.out_proj.input_scale)
+
+    def _prepared(self):
+        return self._serving is not None and self._serving["made_of"].holds(self._laid_out())
 
     def _apply(self, fn, *args, **kwargs):
         self._serving = None
@@ -252,7 +278,7 @@ class QuantizedMamba2(nn.Module):
 
     def allocate_state(self, num_slots):
         """Zeroed slots for that many sequences, on the module's device."""
-        if self._serving is None:
+        if not self._prepared():
             self.prepare_serving()
         device = self._serving["A"].device
         return Mamba2State(torch.zeros(num_slots, self.d_conv - 1, self.conv_dim, dtype=torch.float16, device=device),
@@ -274,9 +300,10 @@ class QuantizedMamba2(nn.Module):
         return self._serve(hidden_states, state, slots, None, True, _debug)
 
     def _serve(self, hidden_states, state, slots, seq_starts, single, debug):
+        if not self._prepared():
+            raise RuntimeError("QuantizedMamba2 is not prepared for serving: call prepare_serving() after the module or a part of it was moved, loaded, "
+                               "exchanged or written to")
         w = self._serving
-        if w is None:
-            raise RuntimeError("QuantizedMamba2 is not prepared for serving: call prepare_serving() after the module was moved or loaded")
         if isinstance(hidden_states, tuple):
             projected = self.in_proj.forward_int8(*hidden_states)
         else:

@@ -1,0 +1,59 @@
+"""The serving operators at the edges of what they take, as far as the host decides it (CPU)."""
+
+import copy
+import io
+
+import pytest
+import torch
+
+from tests.test_serving_refusals import _mixer
+
+F16, BF16, F32, I8, I32 = torch.float16, torch.bfloat16, torch.float32, torch.int8, torch.int32
+
+
+# what makes a prepared mixer's copies stale
+STALE = {
+    "another out_proj": lambda m: setattr(m, "out_proj", copy.deepcopy(m.out_proj)),
+    "another scale": lambda m: setattr(m.out_proj, "input_scale", torch.tensor(0.25)),
+    "a scale written to": lambda m: m.out_proj.input_scale.fill_(0.25),
+    "out_proj loaded": lambda m: m.out_proj.load_state_dict(m.out_proj.state_dict()),
+    "out_proj moved": lambda m: m.out_proj.double(),
+    "another conv1d": lambda m: setattr(m, "conv1d", copy.deepcopy(m.conv1d)),
+    "conv1d moved": lambda m: m.conv1d.half(),
+    "taps written to": lambda m: m.conv1d.weight.detach().add_(1),
+    "another dt_bias": lambda m: setattr(m, "dt_bias", torch.ones(2)),
+    "D written to": lambda m: m.D.zero_(),
+}
+
+
+@pytest.mark.parametrize("how", list(STALE))
+def test_serving_notices_what_changed_after_it_was_prepared(how):
+    m = _mixer()
+    st = m.allocate_state(2)
+    call = lambda: m.step((torch.zeros(1, 64, dtype=I8), 1.0), st)  # noqa: E731
+    with pytest.raises(ValueError, match="GPU"):     # prepared: host tensors get as far as the first kernel
+        call()
+    STALE[how](m)
+    with pytest.raises(RuntimeError, match="prepare_serving"):
+        call()
+    m.allocate_state(1)                              # prepares where it has to
+    with pytest.raises(ValueError, match="GPU"):
+        call()
+
+
+def test_a_prepared_mixer_can_be_copied_and_saved():
+    m = _mixer()
+    st = m.allocate_state(2)
+    m.D.zero_()
+    m.prepare_serving()
+    buf = io.BytesIO()
+    torch.save(m, buf)
+    buf.seek(0)
+    for other in (copy.deepcopy(m), torch.load(buf, weights_only=False)):
+        with pytest.raises(ValueError, match="GPU"):
+            other.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
+        other.out_proj.input_scale.fill_(0.5)
+        with pytest.raises(RuntimeError, match="prepare_serving"):
+            other.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
+    with pytest.raises(ValueError, match="GPU"):
+        m.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
