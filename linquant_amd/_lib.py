@@ -155,6 +155,12 @@ def rows16(t):
     """``t`` itself when it has unit stride along its last axis and every other row of it starts on a 16-byte boundary, else a
     fresh dense copy: kernels that fetch activations as 16-byte pieces take any strides of that kind."""
     n = 16 // t.element_size()
+    if 1 in t.shape[:-1]:  # its stride is no distance between entries, and contiguous() leaves it as it is, but the entry points check it
+        strides = list(t.stride())
+        for i in reversed(range(t.dim() - 1)):
+            if t.shape[i] == 1:
+                strides[i] = t.shape[i + 1] * strides[i + 1]
+        t = t.as_strided(t.shape, strides)
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % n == 0 for s in t.stride()[:-1]):
         return t
     t = t.contiguous()

@@ -28,6 +28,7 @@ from typing import NamedTuple
 import torch
 import torch.nn as nn
 
+from linquant_amd import _lib
 from linquant_amd.hadamard_utils import qhad_transform
 from linquant_amd.kernels.hadamard import kronecker_hadamard_fwd  # noqa: F401  (kept re-bindable like the reference's import)
 from linquant_amd.kernels.mamba2.causal_conv1d import causal_conv1d_fn
@@ -217,7 +218,7 @@ class QuantizedMamba2(nn.Module):
         s = getattr(self.in_proj, "input_scale", None)
         if s is None or not hasattr(self.in_proj, "forward_int8"):
             return None, self.in_proj(hidden_states)
-        h_i8 = _fused_fp16_to_int8(hidden_states.reshape(-1, hidden_states.shape[-1]), s, clamp_min=-128.0,
+        h_i8 = _fused_fp16_to_int8(_lib.rows16(hidden_states.reshape(-1, hidden_states.shape[-1])), s, clamp_min=-128.0,
                                    reciprocal=False).view(hidden_states.shape)
         return h_i8, self.in_proj.forward_int8(h_i8, s)
 

@@ -6,6 +6,7 @@ import io
 import pytest
 import torch
 
+from linquant_amd import _lib
 from tests.test_serving_refusals import _mixer
 
 F16, BF16, F32, I8, I32 = torch.float16, torch.bfloat16, torch.float32, torch.int8, torch.int32
@@ -57,3 +58,19 @@ def test_a_prepared_mixer_can_be_copied_and_saved():
             other.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
     with pytest.raises(ValueError, match="GPU"):
         m.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
+
+
+# ------------------------------------------------------------------------------------------------------- one row of a wide tensor
+@pytest.mark.parametrize("shape,strides", [((1, 32), (77, 1)), ((1, 32), (1 << 24, 1)), ((1, 1, 32), (5, 3, 1)), ((1, 4, 32), (7, 40, 1)), ((4, 1, 32), (40, 9, 1)),
+                                           ((1, 4, 32), (7, 33, 1)), ((1, 1, 4, 32), (3, 3, 33, 1)), ((3, 32), (33, 1)), ((3, 32), (48, 1))])
+@pytest.mark.parametrize("dtype", [F16, I8])
+def test_rows_of_whole_pieces(shape, strides, dtype):
+    """Whatever the strides of dimensions of length one say; a copy only where there are several rows off the grid."""
+    n = 16 // torch.empty(0, dtype=dtype).element_size()
+    base = torch.arange(4096).to(dtype)
+    assert base.data_ptr() % 16 == 0
+    t = base.as_strided(shape, strides)
+    r = _lib.rows16(t)
+    assert torch.equal(r, t) and r.stride(-1) == 1 and r.data_ptr() % 16 == 0 and all(s % n == 0 and s < 1 << 23 for s in r.stride()[:-1])
+    off = any(s % n for m, s in zip(shape[:-1], strides) if m > 1)
+    assert (r.data_ptr() == t.data_ptr()) == (not off)

@@ -27,6 +27,69 @@ def _rn(*shape, seed=0):
     return torch.randn(*shape, generator=_gen(seed))
 
 
+# --------------------------------------------------------------------------------------------- one row of a wide tensor
+def _one(t, pitch, dim=0):
+    """``t``, one entry long along ``dim``, as a view whose stride there is ``pitch``."""
+    strides = list(t.stride())
+    strides[dim] = pitch
+    return t.as_strided(t.shape, strides)
+
+
+@pytest.mark.parametrize("pitch", [77, 1 << 24, (1 << 24) + 1])
+def test_one_row_at_any_distance(cuda, pitch):
+    """The stride along a dimension of length one is no distance between entries: any is taken."""
+    x, w = _rn(1, 64).half().to(cuda), _rn(64, 4, seed=1).half().to(cuda)
+    st = [torch.zeros(1, 3, 64, dtype=F16, device=cuda) for _ in range(2)]
+    assert torch.equal(conv1d_step(_one(x, pitch), st[0], w), conv1d_step(x, st[1], w)) and torch.equal(*st)
+    starts = starts_of([1], cuda)
+    assert torch.equal(conv1d_prompt(_one(x, pitch), w, state=st[0], seq_starts=starts), conv1d_prompt(x, w, state=st[1], seq_starts=starts))
+    assert torch.equal(conv1d_prompt(_one(_one(x[None], pitch), pitch, 1), w), conv1d_prompt(x[None], w))
+    a, b = (torch.randint(-127, 128, (1, 64), generator=_gen(i)).to(torch.int8).to(cuda) for i in (2, 3))
+    assert torch.equal(int8_matmul(_one(a, pitch), _one(b, pitch), 1.0, 1.0), int8_matmul(a, b, 1.0, 1.0))
+    q = W8A8Linear(b, torch.ones(1), input_scale=0.05).to(cuda)
+    assert torch.equal(q(_one(x, pitch)), q(x))
+    assert all(torch.equal(i, j) for i, j in zip(quantize_rows(_one(x, pitch)), quantize_rows(x)))
+    assert all(torch.equal(i, j) for i, j in zip(residual_rmsnorm(_one(x, pitch), x[0], _one(x, pitch)), residual_rmsnorm(x, x[0], x)))
+    v = {k: t.to(cuda) for k, t in ssm_inputs(1, 2, 64, 1, 64, F16).items()}
+    far = {k: t if k == "A" else _one(t, pitch) for k, t in v.items() if k in ("x", "dt", "A", "B", "C")}
+    near = {k: v[k] for k in far}
+    s = [torch.ones(1, 2, 64, 64, device=cuda) for _ in range(2)]
+    assert torch.equal(ssm_step(s[0], **far), ssm_step(s[1], **near)) and torch.equal(*s)
+    assert torch.equal(ssm_prompt(**far, state=s[0], seq_starts=starts), ssm_prompt(**near, state=s[1], seq_starts=starts)) and torch.equal(*s)
+    batch = lambda d, p: {k: t if k == "A" else (_one(t[None], p) if p else t[None]) for k, t in d.items()}  # noqa: E731
+    assert torch.equal(ssm_prompt(**batch(far, pitch), state=s[0]), ssm_prompt(**batch(near, 0), state=s[1])) and torch.equal(*s)
+
+
+def test_norms_of_one_row_of_a_wide_tensor(cuda):
+    x, z, w = _rn(1, 512).half().to(cuda), _rn(1, 1540, seed=1).half().to(cuda)[:, :512], torch.ones(512, device=cuda)
+    assert torch.equal(rmsnorm_gated(x, z, w), rmsnorm_gated(x, z.clone(), w))
+    assert torch.equal(rmsnorm_gated_qhad(x, z, w, 0.05)[0], rmsnorm_gated_qhad(x, z.clone(), w, 0.05)[0])
+    odd = _one(x, 517)
+    assert torch.equal(rmsnorm_gated(odd, z, w), rmsnorm_gated(x, z, w)) and torch.equal(qhad_transform(odd, 0.05)[0], qhad_transform(x, 0.05)[0])
+
+
+@pytest.mark.parametrize("rows", [True, False])
+def test_mixer_with_one_sequence(cuda, rows):
+    """Four heads: a token's projected row is no multiple of 16 bytes, and one sequence has one of them."""
+    m = build(W8A8Linear, 2, 4, 128, rows=rows)
+    st = m.allocate_state(2)
+    slots = torch.tensor([1], dtype=torch.int32, device=cuda)
+    wide = torch.zeros(1, m.d_model + 3, dtype=F16, device=cuda)   # the activations as such a row, too
+    wide[:, :m.d_model] = tokens(1, m, 1).cuda()
+    one = wide[:, :m.d_model]
+
+    def run(call, hidden):
+        before, dbg = snapshot(st), {}
+        call(hidden, dbg)
+        if rows:
+            check_call(m, hidden.cpu(), dbg, [1], before, snapshot(st), [1], slice(None))
+        assert torch.isfinite(dbg["out"]).all()
+
+    run(lambda h, dbg: m.prefill(h, st, slots, starts_of([1], cuda), _debug=dbg), one)
+    run(lambda h, dbg: m.step(h, st, slots, _debug=dbg), one)
+    run(lambda h, dbg: m.prefill(h, st, slots, _debug=dbg), one[None])
+
+
 @pytest.mark.parametrize("wt,pt", [(F16, F32), (BF16, F32), (F32, F16), (F16, BF16), (BF16, F16)])
 def test_norm_weights_of_two_types(cuda, wt, pt):
     """Each weight enters as it is: nothing of the wider type's bits or range is lost to the other's."""
