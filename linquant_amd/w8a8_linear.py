@@ -43,6 +43,8 @@ def quantize_rows(x):
     codes, scale = _quantize(x)
     K = x.shape[-1]
     codes = codes if codes.shape[1] == K else codes[:, :K]
+    if x.dim() == 1:
+        return codes[0], scale[0]
     return (codes, scale) if x.dim() == 2 else (codes.unflatten(0, x.shape[:-1]), scale.view(x.shape[:-1]))
 
 

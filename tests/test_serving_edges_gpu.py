@@ -90,6 +90,17 @@ def test_mixer_with_one_sequence(cuda, rows):
     run(lambda h, dbg: m.prefill(h, st, slots, _debug=dbg), one[None])
 
 
+# ----------------------------------------------------------------------------------------------------- shapes and types
+@pytest.mark.parametrize("K", [32, 21])
+def test_a_single_row_without_a_leading_dimension(cuda, K):
+    x = _rn(K).half().to(cuda)
+    q, s = quantize_rows(x)
+    q2, s2 = quantize_rows(x[None])
+    assert q.shape == (K,) and s.shape == () and torch.equal(q, q2[0]) and torch.equal(s, s2[0])
+    b = torch.randint(-127, 128, (5, K), generator=_gen(1)).to(torch.int8).to(cuda)
+    assert torch.equal(int8_matmul(q, b, s, 1.0), int8_matmul(q2, b, s2, 1.0)[0])
+
+
 @pytest.mark.parametrize("wt,pt", [(F16, F32), (BF16, F32), (F32, F16), (F16, BF16), (BF16, F16)])
 def test_norm_weights_of_two_types(cuda, wt, pt):
     """Each weight enters as it is: nothing of the wider type's bits or range is lost to the other's."""
