@@ -842,7 +842,8 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(PromptParams p) {
   if (n < 2) return;
   int first = 0;
   if (p.starts) {
-    for (int i = threadIdx.x & 63; i < seq; i += 64) first += segments(i);
+    // (starts that do not ascend can name far more than there are, and their sum must not wrap: one too many is enough to know)
+    for (int i = threadIdx.x & 63; i < seq; i += 64) first = min(first + segments(i), p.segs + 1);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) first += __shfl_xor(first, off, 64);
   } else {

@@ -221,3 +221,18 @@ def test_tokens_far_apart(cuda, dtype, at, T):
         y, st, wy, mag, ws, smag, most = _scan(cuda, v, [T], state=state)
         assert_near(st[0], ws[0], smag[0], ssm_rel([T], most), "state")
         _near_where_finite(y, wy, mag, ssm_y_rel([T], most, dtype))
+
+
+def test_starts_that_name_more_segments_than_32_bits_count(cuda):
+    """60,000 prompts of the same 2^24 tokens: the segments in front of the later ones come to 2^33.  Nothing is touched out of range, and the first
+    one's state is what it is by itself."""
+    H, P, G, N, T, n = 1, 8, 1, 8, 1 << 24, 120001
+    v = {k: t.repeat(*([1] if k in ("A", "D", "dt_bias") else [T // 4096] + [1] * (t.dim() - 1))).to(cuda) for k, t in ssm_inputs(4096, H, P, G, N, F16, seed=32).items()}
+    args = [v[k] for k in ("x", "dt", "A", "B", "C")]
+    starts = torch.zeros(n + 1, dtype=torch.int32, device=cuda)
+    starts[1::2] = T
+    st, alone = torch.zeros(n, H, P, N, device=cuda), torch.zeros(1, H, P, N, device=cuda)
+    ssm_prompt(*args, state=st, seq_starts=starts)
+    ssm_prompt(*args, state=alone, seq_starts=starts_of([T], cuda))
+    torch.cuda.synchronize()
+    assert torch.isfinite(alone).all() and ((st[0] - alone[0]).abs().max() <= 2.0 ** -9 * alone.abs().max()).all()   # (cut into other segments)
