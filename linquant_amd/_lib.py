@@ -167,6 +167,13 @@ def rows16(t):
     return aligned(t)
 
 
+def below_2_31(*sizes):
+    """The args structs hold sizes in 32 bits, and a larger one would be cut off without a word."""
+    for n in sizes:
+        if n >= 1 << 31:
+            raise ValueError(f"expected sizes below 2**31, got {n}")
+
+
 def same_device(first, *others):
     """Every tensor (or None) on the device of the first: a kernel must not be handed another device's memory."""
     for t in others:

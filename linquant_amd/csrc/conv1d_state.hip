@@ -167,11 +167,11 @@ extern "C" int lq_conv1d_prompt(const lq_conv1d_prompt_args* a, hipStream_t stre
   if (!sv_al(a->weight, 16) || !sv_al(a->bias, 16) || !sv_al(a->slots, 4) || !sv_al(a->seq_starts, 4)) return LQ_ERR_SHAPE;
   if (a->state && (!sv_al(a->state, 16) || a->state_stride_s % 8 != 0 || a->state_stride_w % 8 != 0 || a->num_slots <= 0)) return LQ_ERR_SHAPE;
   // every sequence is rounded up to whole units, so a packed call has at most so many; the surplus ends at once
-  const int64_t units = a->seq_starts ? (int64_t)a->tokens / kTL + a->nseq : (int64_t)a->nseq * ((a->seqlen + kTL - 1) / kTL);
-  if (!sv_fits(units, 256)) return LQ_ERR_SHAPE;
+  const int64_t units = a->seq_starts ? (int64_t)a->tokens / kTL + a->nseq : (int64_t)a->nseq * (((int64_t)a->seqlen + kTL - 1) / kTL), groups = ((int64_t)a->dim + 2047) / 2048;
+  if (!sv_fits(units, 256) || groups > 65535) return LQ_ERR_SHAPE;
   ConvParams p = {(const uint16_t*)a->x, a->x_stride_b, a->x_stride_l, (const uint16_t*)a->weight, (const uint16_t*)a->bias, (uint16_t*)a->out,
                   (uint16_t*)a->state, a->state_stride_s, a->state_stride_w, a->slots, a->seq_starts, a->num_slots, a->nseq, a->seqlen, a->tokens, a->dim};
-  const dim3 grid((unsigned)units, (unsigned)((a->dim + 2047) / 2048));
+  const dim3 grid((unsigned)units, (unsigned)groups);
   return for_form(a->dtype, a->width, a->silu, [&](auto t, auto w, auto s) {
     hipLaunchKernelGGL((conv1d_prompt_kernel<decltype(t), decltype(w)::value, decltype(s)::value>), grid, dim3(256), 0, stream, p);
     return lq_check_launch();
@@ -183,7 +183,7 @@ extern "C" int lq_conv1d_step(const lq_conv1d_step_args* a, hipStream_t stream) 
   if (!sv_act(a->dtype) || a->dim <= 0 || a->dim % 8 != 0 || a->width < 2 || a->width > 4 || a->batch <= 0 || a->num_slots <= 0) return LQ_ERR_SHAPE;
   if (a->x_stride % 8 != 0 || !sv_al(a->x, 16) || !sv_al(a->out, 16) || !sv_al(a->weight, 16) || !sv_al(a->bias, 16) || !sv_al(a->slots, 4)) return LQ_ERR_SHAPE;
   if (!sv_al(a->state, 16) || a->state_stride_s % 8 != 0 || a->state_stride_w % 8 != 0) return LQ_ERR_SHAPE;
-  const int64_t parts = (a->dim + 511) / 512;
+  const int64_t parts = ((int64_t)a->dim + 511) / 512;
   if (parts > 65535 || !sv_fits(a->batch, 64)) return LQ_ERR_SHAPE;
   ConvParams p = {(const uint16_t*)a->x, a->x_stride, 0, (const uint16_t*)a->weight, (const uint16_t*)a->bias, (uint16_t*)a->out, (uint16_t*)a->state,
                   a->state_stride_s, a->state_stride_w, a->slots, nullptr, a->num_slots, a->batch, 1, 0, a->dim};

@@ -32,6 +32,7 @@ def _taps(x, weight, bias, activation):
     D, W = weight.shape
     assert x.shape[-1] == D and 2 <= W <= 4 and D % 8 == 0, f"{x.shape[-1]} channels, weight {tuple(weight.shape)}"
     assert bias is None or bias.shape == (D,)
+    _lib.below_2_31(*x.shape)
     _lib.same_device(x, weight, bias)
     weight = _lib.aligned(weight.to(x.dtype).contiguous())
     return weight, None if bias is None else _lib.aligned(bias.to(x.dtype).contiguous())

@@ -26,6 +26,7 @@ def _params(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, lead):
     assert B.shape == (*lead, G, N) and C.shape == B.shape, f"B, C: {(*lead, 'G', 'N')}, got {tuple(B.shape)}, {tuple(C.shape)}"
     assert G >= 1 and H % G == 0 and P % 8 == 0 and N % 8 == 0 and 8 <= N <= 256, f"H {H} P {P} G {G} N {N}"
     assert A.shape == (H,) and (dt_bias is None or dt_bias.shape == (H,)) and (D is None or D.shape in ((H,), (H, P)))
+    _lib.below_2_31(*x.shape)
     _lib.same_device(x, dt, A, B, C, D, dt_bias)
     A, D, dt_bias = (None if t is None else _lib.f32(t).contiguous() for t in (A, D, dt_bias))
     fields = dict(dtype=_ACT[x.dtype], dt_dtype=_FLOAT[dt.dtype], A=_lib.ptr(A), D=_lib.ptr(D), D_has_hdim=int(D is not None and D.dim() == 2),

@@ -99,6 +99,7 @@ def residual_rmsnorm(x, weight, residual=None, eps=1e-5, *, gate=None, scale=1.0
     assert quantize is None or quantize == "rows" if not static else quantize.numel() == 1 and quantize.dtype == torch.float32
     _lib.same_device(x, weight, residual, gate, post_weight, quantize if static else None)
     rows = x.numel() // dim
+    _lib.below_2_31(rows)
     x2 = _row_view(x, dim)
     r2 = None if residual is None else _row_view(residual, dim)
     gate_rows, gate_stride = 1, 0

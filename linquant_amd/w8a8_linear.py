@@ -29,6 +29,7 @@ def _quantize(x):
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
     M = x2.shape[0]
+    _lib.below_2_31(M)
     codes = torch.empty(M, _padded(K), dtype=torch.int8, device=x.device)
     scale = torch.empty(M, dtype=torch.float32, device=x.device)
     if M:
@@ -83,6 +84,7 @@ def int8_matmul(a, b, a_scale, b_scale, bias=None, out_dtype=torch.float16, out=
     assert a.dtype == torch.int8 and b.dtype == torch.int8 and b.dim() == 2 and a.dim() >= 1
     K, N = a.shape[-1], b.shape[0]
     assert b.shape[1] == K and 1 <= K <= 131056, f"contraction lengths {K} and {b.shape[1]}"
+    _lib.below_2_31(a.numel() // K, N)
     assert out_dtype in _CODES and (bias is None or (bias.dtype in _CODES and bias.shape == (N,)))
     a2 = a.reshape(-1, K)
     if out is None:

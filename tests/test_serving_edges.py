@@ -1,12 +1,17 @@
 """The serving operators at the edges of what they take, as far as the host decides it (CPU)."""
 
 import copy
+import ctypes
 import io
 
 import pytest
 import torch
 
 from linquant_amd import _lib
+from linquant_amd.kernels.mamba2.conv1d_state import conv1d_prompt, conv1d_step
+from linquant_amd.kernels.mamba2.ssm import ssm_prompt, ssm_step
+from linquant_amd.norm import residual_rmsnorm
+from linquant_amd.w8a8_linear import int8_matmul, quantize_rows
 from tests.test_serving_refusals import _mixer
 
 F16, BF16, F32, I8, I32 = torch.float16, torch.bfloat16, torch.float32, torch.int8, torch.int32
@@ -58,6 +63,45 @@ def test_a_prepared_mixer_can_be_copied_and_saved():
             other.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
     with pytest.raises(ValueError, match="GPU"):
         m.step((torch.zeros(1, 64, dtype=I8), 1.0), st)
+
+
+# ------------------------------------------------------------------------------------------------------- sizes past 32 bits
+def _meta(*shape, dtype=F16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+BIG = (1 << 32) + 5   # 5 in 32 bits
+PAST = {
+    "quantize_rows": lambda: quantize_rows(_meta(BIG, 8)),
+    "int8_matmul rows": lambda: int8_matmul(_meta(BIG, 16, dtype=I8), _meta(8, 16, dtype=I8), 1.0, 1.0),
+    "int8_matmul columns": lambda: int8_matmul(_meta(8, 16, dtype=I8), _meta(BIG, 16, dtype=I8), 1.0, 1.0),
+    "residual_rmsnorm": lambda: residual_rmsnorm(_meta(5, BIG // 5 * 5, 1), _meta(1)),
+    "conv1d_prompt": lambda: conv1d_prompt(_meta(BIG, 8), _meta(8, 4), seq_starts=_meta(3, dtype=I32)),
+    "conv1d_prompt of a batch": lambda: conv1d_prompt(_meta(1, BIG, 8), _meta(8, 4)),
+    "conv1d_step": lambda: conv1d_step(_meta(BIG, 8), _meta(8, 3, 8), _meta(8, 4), slots=_meta(BIG, dtype=I32)),
+    "ssm_prompt": lambda: ssm_prompt(_meta(BIG, 1, 8), _meta(BIG, 1), _meta(1), _meta(BIG, 1, 8), _meta(BIG, 1, 8), seq_starts=_meta(3, dtype=I32)),
+    "ssm_step": lambda: ssm_step(_meta(8, 1, 8, 8, dtype=F32), _meta(BIG, 1, 8), _meta(BIG, 1), _meta(1), _meta(BIG, 1, 8), _meta(BIG, 1, 8),
+                                 slots=_meta(BIG, dtype=I32)),
+}
+
+
+@pytest.mark.parametrize("what", list(PAST))
+def test_sizes_past_32_bits_are_refused(what, monkeypatch):
+    """Not cut off to what their lowest 32 bits say."""
+    monkeypatch.setattr(_lib, "launch", lambda fn, device, st: pytest.fail(f"{fn} with {[(n, getattr(st, n)) for n, _ in st._fields_]}"))
+    with pytest.raises(ValueError, match=r"2\*\*31"):
+        PAST[what]()
+
+
+@pytest.mark.parametrize("fn,sizes", [("lq_conv1d_prompt", dict(seqlen=(1 << 31) - 1)), ("lq_conv1d_prompt", dict(dim=(1 << 31) - 8)), ("lq_conv1d_step", dict(dim=(1 << 31) - 8))])
+def test_sizes_near_the_last_of_32_bits_are_refused(fn, sizes):
+    """Rounding them up to whole units must not wrap: a grid of that would be no refusal but a launch that fails (host memory here)."""
+    buf = ctypes.create_string_buffer(4096)
+    at = (ctypes.addressof(buf) + 255) // 256 * 256
+    args = {n: at for n, t in _lib.STRUCTS[fn + "_args"]._fields_ if t is ctypes.c_void_p and n not in ("seq_starts", "slots", "bias")}
+    args.update(nseq=1, seqlen=4, x_stride_l=16) if fn.endswith("prompt") else args.update(batch=1, x_stride=16)
+    args.update({**dict(dim=16, width=4, num_slots=1), **sizes})
+    assert getattr(_lib.load(), fn)(ctypes.byref(_lib.fill(fn + "_args", **args)), None) == -22
 
 
 # ------------------------------------------------------------------------------------------------------- one row of a wide tensor
