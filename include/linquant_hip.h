@@ -944,6 +944,9 @@ typedef struct {
 int lq_ssm_prompt(const lq_ssm_prompt_args* args, hipStream_t stream);
 /* workspace size for the dims in `args` (pointers are not read but for whether seq_starts is NULL), written to *bytes */
 int lq_ssm_prompt_workspace_bytes(const lq_ssm_prompt_args* args, int64_t* bytes);
+/* How a call of those dims is cut, host work alone: plan[0] segments (with seq_starts the most that there can be), plan[1] chunks
+ * of 64 tokens to a segment, plan[2] pieces in which a segment's own state is formed (0: prompts are not cut). */
+int lq_ssm_prompt_plan(const lq_ssm_prompt_args* args, int64_t* plan);
 
 /* no counterpart in the reference: the same for one token of each sequence; state is updated in place. */
 typedef struct {

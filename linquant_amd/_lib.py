@@ -64,7 +64,7 @@ FUNCTIONS = tuple(_funcs)
 _SHARED_ARGS = {"lq_ssd_combined_static": "lq_ssd_combined_args", "lq_ssd_combined_workspace_bytes": "lq_ssd_combined_args",
                 "lq_zoo_simple_gla_workspace_bytes": "lq_zoo_simple_gla_args",
                 "lq_zoo_chunk_forward_workspace_bytes": "lq_zoo_chunk_forward_args",
-                "lq_ssm_prompt_workspace_bytes": "lq_ssm_prompt_args"}
+                "lq_ssm_prompt_workspace_bytes": "lq_ssm_prompt_args", "lq_ssm_prompt_plan": "lq_ssm_prompt_args"}
 
 _lib = None
 

@@ -947,6 +947,16 @@ extern "C" int lq_ssm_prompt_workspace_bytes(const lq_ssm_prompt_args* a, int64_
   return LQ_OK;
 }
 
+extern "C" int lq_ssm_prompt_plan(const lq_ssm_prompt_args* a, int64_t* out) {
+  if (!a || !out) return LQ_ERR_NULL;
+  const int rc = check_dims(a);
+  Plan pl;
+  if (rc != LQ_OK) return rc;
+  if (!plan(a, pl)) return LQ_ERR_SHAPE;
+  out[0] = pl.segs, out[1] = pl.seg_chunks, out[2] = pl.cut ? pl.pieces : 0;
+  return LQ_OK;
+}
+
 extern "C" int lq_ssm_prompt(const lq_ssm_prompt_args* a, hipStream_t stream) {
   if (!a || !a->x || !a->dt || !a->A || !a->B || !a->C || !a->out || !a->workspace) return LQ_ERR_NULL;
   const int rc = check_dims(a);

@@ -118,3 +118,19 @@ def test_rows_of_whole_pieces(shape, strides, dtype):
     assert torch.equal(r, t) and r.stride(-1) == 1 and r.data_ptr() % 16 == 0 and all(s % n == 0 and s < 1 << 23 for s in r.stride()[:-1])
     off = any(s % n for m, s in zip(shape[:-1], strides) if m > 1)
     assert (r.data_ptr() == t.data_ptr()) == (not off)
+
+
+# ------------------------------------------------------------------------------------------------------- how prompts are cut
+def test_cuts_that_the_gpu_tests_mean():
+    """A change of the plan must not leave the forms that they are there for without a test; the prefill of the benchmark takes 3 segments of two pieces."""
+    from tests.test_serving_edges_gpu import CUT, _plan
+
+    for dtype in (F16, BF16):
+        for dims, lens, packed, cut in CUT:
+            assert _plan(lens, packed, *dims, dtype) == cut
+    assert {(packed, pieces) for _, _, packed, (chunks, pieces) in CUT if chunks > 1} == {(False, 1), (False, 2), (True, 1), (True, 2)}
+    assert _plan([8192] * 4, False, 80, 64, 1, 128, F16) == [44, 2]
+    assert _plan([384], False, 80, 64, 1, 128, F16) == [6, 0]          # one segment, not cut
+    out = (ctypes.c_int64 * 3)()
+    bad = _lib.fill("lq_ssm_prompt_args", nseq=1, seqlen=64, nheads=3, headdim=64, ngroups=2, dstate=16)
+    assert _lib.load().lq_ssm_prompt_plan(ctypes.byref(bad), ctypes.byref(out)) == -22 and _lib.load().lq_ssm_prompt_plan(None, ctypes.byref(out)) == -14

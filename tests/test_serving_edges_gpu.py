@@ -143,6 +143,44 @@ def _near_where_finite(y, want, mag, rel):
     assert_near(torch.where(fits, y, 0.0), torch.where(fits, want, 0.0), torch.where(fits, mag, 0.0), rel, "y")
 
 
+def _plan(lens, packed, H, P, G, N, dtype):
+    import ctypes
+
+    st = _lib.fill("lq_ssm_prompt_args", nseq=len(lens), seqlen=0 if packed else lens[0], tokens=sum(lens) if packed else 0,
+                   seq_starts=16 if packed else None, nheads=H, headdim=P, ngroups=G, dstate=N,
+                   dtype=_lib.LQ_DT_F16 if dtype == F16 else _lib.LQ_DT_BF16)
+    out = (ctypes.c_int64 * 3)()
+    assert _lib.load().lq_ssm_prompt_plan(ctypes.byref(st), ctypes.byref(out)) == 0
+    return list(out)[1:]
+
+
+# H, P, G, N; lengths, packed; a segment's chunks and pieces.  Nearly all leave a last segment that is shorter and a last chunk that is not full.
+CUT = [((80, 64, 1, 128), [2500] * 2, False, [14, 2]), ((16, 64, 2, 128), [2500] * 2, False, [3, 1]), ((40, 64, 2, 64), [2500] * 2, False, [7, 1]),
+       ((64, 64, 8, 128), [3999] * 2, False, [16, 2]), ((128, 8, 1, 8), [2300, 1200, 70, 0, 1900, 1500, 1400, 1230], True, [14, 2]),
+       ((64, 64, 8, 128), [900, 2100, 130], True, [6, 1]), ((32, 32, 4, 16), [4000] * 2, False, [2, 1])]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dims,lens,packed,cut", CUT, ids=lambda c: str(c))
+def test_prompts_cut_into_segments_of_several_chunks(cuda, dims, lens, packed, cut, dtype):
+    """States pass, join and the segments that start inside a prompt, as long prompts of many heads take them: little decay, so that what one
+    segment leaves is most of what the next one has; carried-in states, and a prompt that starts from zero and leaves nothing."""
+    H, P, G, N = dims
+    assert _plan(lens, packed, *dims, dtype) == cut
+    v = ssm_inputs(sum(lens), H, P, G, N, dtype, seed=len(lens), a_max=1.3, dt_mean=-6.0)
+    n = len(lens)
+    state = _rn(n + 1, H, P, N, seed=5)
+    slots = [n - i for i in range(n)]
+    slots[1] = -1
+    y, st, wy, mag, ws, smag, most = _scan(cuda, v, lens, packed=packed, state=state, slots=slots)
+    assert_near(y, wy, mag, ssm_y_rel(lens, most, dtype), "y")
+    for i, s in enumerate(slots):
+        if s >= 0:
+            assert_near(st[s], ws[i], smag[i], ssm_rel(lens, most), f"state {i}")
+    for s in set(range(n + 1)) - set(slots):
+        assert torch.equal(st[s].cpu(), state[s])
+
+
 def _growing(dtype, T, turn, bits):
     """Steps that are negative for `turn` tokens, so that a state grows by 2^bits over them, and as positive for the next."""
     H, P, G, N = 3, 40, 1, 64
