@@ -227,6 +227,31 @@ def test_channels_far_apart(cuda, dtype, carried, T):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("what", ["x", "dt", "B", "C", "state"])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("T,at", [(200, 70), (200, 127), (200, 191), (64, 0), (40, 39)])
+def test_values_that_are_no_numbers(cuda, dtype, what, value, T, at):
+    """They reach what the formula has them reach, and nothing else: no token in front, no other channel, head or sequence."""
+    if what == "dt" and value == -INF:
+        pytest.skip("a step of zero, a number")
+    H, P, G, N = 4, 40, 2, 72
+    lens = [30, T, 9]
+    v = ssm_inputs(sum(lens), H, P, G, N, dtype, seed=21, a_max=2.0, dt_mean=-3.0)
+    state = _rn(3, H, P, N, seed=6)
+    clean = _scan(cuda, v, lens, state=state)
+    t = 30 + at
+    {"x": lambda: v["x"][t, 2].__setitem__(7, value), "dt": lambda: v["dt"][t].__setitem__(1, value), "B": lambda: v["B"][t, 1].__setitem__(66, value),
+     "C": lambda: v["C"][t, 0].__setitem__(3, value), "state": lambda: state[1, 3, 33].__setitem__(70, value)}[what]()
+    y, st, wy, mag, ws, smag, most = _scan(cuda, v, lens, state=state)
+    reach = ~torch.isfinite(wy)
+    assert reach.any() and torch.equal(~torch.isfinite(y), reach)
+    assert_near(torch.where(reach, 0.0, y), torch.where(reach, 0.0, clean[2]), clean[3], ssm_y_rel(lens, clean[-1], dtype), "y elsewhere")
+    gone = ~torch.isfinite(ws)
+    assert torch.equal(~torch.isfinite(st), gone)
+    assert_near(torch.where(gone, 0.0, st), torch.where(gone, 0.0, clean[4]), clean[5], ssm_rel(lens, clean[-1]), "state elsewhere")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("N", [8, 24, 40, 96, 128, 200])
 def test_single_tokens_and_infinite_entries(cuda, dtype, N):
     """An infinite entry of the state gives its row's output its sign; the row's length need be no multiple of what a wave reads."""
