@@ -914,9 +914,12 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   };
   double best = chain * step((double)nseq * parts, 43, 72);
   r.seg_chunks = (int)most, r.pieces = 1, r.cut = 0;
+  int64_t last[3] = {0, 0, 0};        // (many numbers of segments come to the same chunks in each: those cost what the first of them does)
   for (int64_t k = 2; k <= 256; ++k)  // segments of the longest
     for (int64_t pieces = 1; pieces <= 2; ++pieces) {
       const int64_t n = (std::max<int64_t>(1, (int64_t)std::ceil(chain / k)) + pieces - 1) / pieces * pieces;
+      if (n == last[pieces]) continue;
+      last[pieces] = n;
       const double segs = a->seq_starts ? (double)r.units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n)), ahead = std::max(0.0, segs - nseq) * pieces;
       const double cost = n * step(segs * parts, 43, 72) + n / pieces * step(ahead * parts, 17, ahead * parts <= 512 ? 27 : 22) + 40 * std::ceil(ahead * parts / 512) +
                           (ahead + 2 * segs) * a->nheads * a->headdim * a->dstate * 4 / 3e5 + 250;

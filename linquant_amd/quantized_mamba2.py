@@ -85,17 +85,18 @@ class _AsLaidOut:
     they were written to.  (A copy or a loaded pickle of it, which has the copied module's tensors, marks them anew.)"""
 
     def __init__(self, *tensors):
-        self.tensors, self.marks = tensors, [self._mark(t) for t in tensors]
-
-    @staticmethod
-    def _mark(t):
-        return (t.data_ptr(), 0 if t.is_inference() else t._version) if isinstance(t, torch.Tensor) else None
+        self.tensors = tensors
+        # (a tensor of inference mode does not count its writes)
+        self.marks = [(t, t.data_ptr(), not t.is_inference() and t._version) if isinstance(t, torch.Tensor) else (t, None, None) for t in tensors]
 
     def __reduce__(self):
         return _AsLaidOut, self.tensors
 
     def holds(self, tensors):
-        return all(a is b and self._mark(b) == m for a, b, m in zip(self.tensors, tensors, self.marks))
+        for t, (was, at, writes) in zip(tensors, self.marks):
+            if t is not was or (at is not None and (t.data_ptr() != at or (writes is not False and t._version != writes))):
+                return False
+        return True
 
 
 class QuantizedMamba2(nn.Module):
@@ -264,7 +265,8 @@ class QuantizedMamba2(nn.Module):
             out_scale=float(self.out_proj.input_scale))
 
     def _laid_out(self):
-        return (self.conv1d.weight, self.conv1d.bias, self.A_log, self.A_log_scale, self.D, self.D_scale, self.dt_bias, self.out_proj.input_scale)
+        conv = self.conv1d
+        return conv.weight, conv.bias, self.A_log, self.A_log_scale, self.D, self.D_scale, self.dt_bias, self.out_proj.input_scale
 
     def _prepared(self):
         return self._serving is not None and self._serving["made_of"].holds(self._laid_out())
