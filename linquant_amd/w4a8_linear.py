@@ -19,7 +19,8 @@ def _fused_fp16_to_int8(x_2d: torch.Tensor, scale: torch.Tensor, clamp_min: floa
     assert scale.numel() == 1 and scale.dtype in _SCALE_CODES and scale.device == x_2d.device
     M, N = x_2d.shape
     out = torch.empty(M, N, device=x_2d.device, dtype=torch.int8)
-    _lib.call("lq_fp16_to_int8", x_2d.device, x=_lib.ptr(x_2d), x_stride=x_2d.stride(0), out=_lib.ptr(out),
-              scale=_lib.ptr(scale), scale_dtype=_SCALE_CODES[scale.dtype], rows=M, cols=N, clamp_min=float(clamp_min),
-              reciprocal=int(bool(reciprocal)))
+    if M:
+        _lib.call("lq_fp16_to_int8", x_2d.device, x=_lib.ptr(x_2d), x_stride=x_2d.stride(0), out=_lib.ptr(out),
+                  scale=_lib.ptr(scale), scale_dtype=_SCALE_CODES[scale.dtype], rows=M, cols=N, clamp_min=float(clamp_min),
+                  reciprocal=int(bool(reciprocal)))
     return out

@@ -299,3 +299,23 @@ def test_starts_that_name_more_segments_than_32_bits_count(cuda):
     ssm_prompt(*args, state=alone, seq_starts=starts_of([T], cuda))
     torch.cuda.synchronize()
     assert torch.isfinite(alone).all() and ((st[0] - alone[0]).abs().max() <= 2.0 ** -9 * alone.abs().max()).all()   # (cut into other segments)
+
+
+@pytest.mark.parametrize("rows", [True, False])
+def test_mixer_calls_without_tokens(cuda, rows):
+    """No tokens, no sequences: nothing comes out and no state is touched."""
+    from linquant_amd.quantized_mamba2 import Mamba2Block
+
+    m = build(W8A8Linear, rows=rows)
+    b = Mamba2Block(m, torch.ones(m.d_model).half().cuda())
+    st = m.allocate_state(3)
+    for t in st:
+        t.fill_(1.5)
+    none, starts = torch.zeros(0, m.d_model, dtype=F16, device=cuda), torch.zeros(4, dtype=torch.int32, device=cuda)
+    for hidden in (none, (torch.zeros(0, m.d_model, dtype=torch.int8, device=cuda), torch.ones((), device=cuda))):
+        assert m.prefill(hidden, st, None, starts).shape == none.shape and m.step(hidden, st).shape == none.shape
+    assert m.prefill(none.view(3, 0, m.d_model), st).shape == (3, 0, m.d_model)
+    x, r = b.step(none, None, st)
+    assert x.shape == r.shape == none.shape and b.prefill(x, r, st, None, starts)[0].shape == none.shape
+    torch.cuda.synchronize()
+    assert all((t == 1.5).all() for t in st)
