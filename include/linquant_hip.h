@@ -970,7 +970,7 @@ typedef struct {
   float* state;              /* (num_slots,H,P,N), the last three dense */
   int64_t state_stride_s;
   const int32_t* slots;      /* (batch,) or NULL */
-  int32_t num_slots, batch, nheads, headdim, ngroups, dstate;
+  int32_t num_slots, batch, nheads, headdim, ngroups, dstate; /* batch up to 65535 */
 } lq_ssm_step_args;
 int lq_ssm_step(const lq_ssm_step_args* args, hipStream_t stream);
 

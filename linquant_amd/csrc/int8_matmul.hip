@@ -2,7 +2,8 @@
 //
 // Two kernels.  `tiles`: both operands go through LDS in stages of 128 contraction bytes, fetched straight from memory, and each wave has
 // whole 32 x 32 tiles of the result.  `rows`: few rows of a (tokens that answer): a workgroup has 16 to 48 columns and its waves parts of
-// the contraction, every operand straight to registers, so that the weights stream from memory once: 16 x 2560 x 10576 in 8 us, 3.4 TB/s.
+// the contraction, every operand straight to registers, so that the weights stream from memory once: 16 x 2560 x 10576 in 7.6 to
+// 8.2 us by the kernel's own time, 3.4 to 3.6 TB/s.
 //
 // The matrix instruction of `tiles` is v_mfma_i32_32x32x32_i8, which reaches 4.9 POPS here where the 16x16x64 form reaches 3.0.  Operands:
 // lane l has row l & 31 and the 16 contraction bytes of half l >> 5; the result: column l & 31, rows 8 (r >> 2) + 4 (l >> 5) + (r & 3).  b is
@@ -11,7 +12,7 @@
 // What bounds `tiles`: the fetches and the way out.  A compute unit takes in 97 to 115 bytes/ns from its L2 in rows of 128 bytes (in rows of
 // 64 half of that), a wave that waits to issue one issues no product either, and the result, twice the inputs at K = 2560, leaves at the
 // memory's rate.  So a stage has one place in LDS and several workgroups share a compute unit: while one fetches or writes its result out,
-// another multiplies.  32768 x 2560 x 10576: 913 us (1.94 POPS).  Rings of two to four stages with one workgroup of 256 x 256 to a compute
+// another multiplies.  32768 x 2560 x 10576: 913 to 1000 us by the card (1.94 to 1.77 POPS).  Rings of two to four stages with one workgroup of 256 x 256 to a compute
 // unit, the next stages on their way during the products: 1120 to 1380 us; two workgroups of 128 x 256 with three stages of 64: 1080.
 #include <algorithm>
 
@@ -237,10 +238,11 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
 
 // Few rows of a: 16 MT of them and 16 NT columns to a workgroup of W waves, which share the contraction in lines of 128 bytes, side by
 // side (a wave that has a range of its own reads 8192 x 8192 a quarter slower).  The weights are read once, a's rows by every workgroup,
-// and those cost as much: 16 x 2560 x 10576 takes 9 us with one row of a, 15 with 16 columns to a workgroup.  So NT is taken such that
-// there is one workgroup to a compute unit (16 x 2560 x 10576, us, NT 1 / 2 / 3: 11.5 / 12.4 / 10.1; 64 rows 24.6 / 22.7 / 16.9; 16 x
-// 5120 x 2560, 160 tiles of 16 columns: 7.5 / 11.8 / 15.6).  Eight waves that request one line at a time are as good as any, but where
-// results are many (MT 4, NT 2 or 3) four that request two: 64 x 2560 x 10576, NT 2: 21.6 and 22.7.
+// and those cost as much: with 16 columns to a workgroup 16 x 2560 x 10576 takes 11.5 us, with one row of a 7.7.  So NT is taken such that
+// there is one workgroup to a compute unit.  us, launch after launch in a graph (2 us above the kernel's own time), weights from memory, NT 1 / 2 / 3:
+// 16 x 2560 x 10576 11.5 / 12.4 / 10.0, 64 rows 24.6 / 21.7 / 17.0, one row 7.7 / 10.3 / 8.7; 16 x 5120 x 2560, 160 tiles of 16 columns,
+// 7.5 / 11.9 / 15.6.  Eight waves that request one line at a time are as good as any, but where results are many (MT 4, NT 2 or 3) four that
+// request two: 64 x 2560 x 10576, NT 2: 21.7 and 22.7.
 // v_mfma_i32_16x16x64_i8: lane l has row l & 15 and the 16 bytes of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
 template <int MT, int NT, int W, int U, typename O>
 __global__ __launch_bounds__(64 * W) void int8_rows_kernel(MatmulParams p) {

@@ -1,4 +1,4 @@
-// Shared pieces of the serving kernels: 16-bit activations of either type, where a packed sequence lies, reductions.
+// Shared pieces of the serving kernels: 16-bit activations of either type, where a packed sequence lies.
 #pragma once
 
 #include <type_traits>
@@ -10,7 +10,6 @@ namespace {
 
 typedef __bf16 sv_v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 sv_v2bf __attribute__((ext_vector_type(2)));
-typedef float sv_v2f __attribute__((ext_vector_type(2)));
 typedef uint16_t sv_v8u __attribute__((ext_vector_type(8)));
 typedef uint16_t sv_v4u __attribute__((ext_vector_type(4)));
 
@@ -30,17 +29,6 @@ LQ_DEV float sv_load(const void* p, int64_t i, int dtype) {
   if (dtype == LQ_DT_F32) return ((const float*)p)[i];
   const uint16_t u = ((const uint16_t*)p)[i];
   return dtype == LQ_DT_F16 ? F16::to(u) : BF16::to(u);
-}
-
-LQ_DEV float sv_wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = v + __shfl_xor(v, off, 64);
-  return v;
-}
-LQ_DEV float sv_wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
 }
 
 // a * sigmoid(a) on the hardware exp2 / reciprocal units, as the convolution without a state has it

@@ -21,11 +21,12 @@
 // (whose second piece is 2^11 smaller) 2^16 below its channel's.  A unit for 32 channels and 64 tokens together (2 % less time) lost a
 // channel beside one 2^26 above it, and the state that a chunk's first tokens read where a later one was as far above them.
 //
-// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 404 to 425 us by the card (operands 27 to
-// 33, states 94 to 104, join 16, chunks 285 to 312), 1.8 TB/s of what has to move and 268 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
-// busy 50 % of the time (scaling, rounding and splitting operands, 690 instructions to 32 channels and 64 tokens), the matrix unit 22 %, and
+// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 414 to 426 us by the card, call after
+// call (the kernels' own least times: operands 27, states 99, join 16, chunks 287; the profiler's medians are up to 14 % above them), 1.7 TB/s of
+// what has to move and 254 to 261 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
+// busy 53 % of the time (scaling, rounding and splitting operands, 774 instructions to 32 channels and 64 tokens), the matrix unit 22 %, and
 // the clock falls from 2.4 to 2.1 GHz; two waves to a SIMD is what the state in registers (64 of 256) and 81 KB of LDS leave.  Few or
-// ragged prompts are a chain of chunks, about 4 us each: 384 tokens 35 us, 6949 in 10 prompts of up to 2047, 64 heads in 8 groups, bf16, 140.
+// ragged prompts are a chain of chunks, about 4 us each: 384 tokens 36 us, 6949 in 10 prompts of up to 2047, 64 heads in 8 groups, bf16, 140.
 // Tried: C B^T formed by each workgroup (its product is the group's, so 80 heads made it 80 times); one piece of a state's additions (a state
 // gathers the rounding of a whole prompt); a higher priority for the younger of two workgroups, which the older one holds up (3 % less here,
 // 3 % more for ragged prompts).
@@ -594,8 +595,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       // the state behind the chunk
       {
         // Ahead: what the next products need is formed between these (one issued behind another of the same tile waits for it, and the
-        // vector unit is free): 384 tokens in fp16 36.4 -> 35.3 us.  bf16 lacks the registers from 65 state columns on (ragged prompts 140 ->
-        // 191, ten spilled).
+        // vector unit is free): 384 tokens in fp16 36.4 -> 35.3 us (before each channel had a unit).  bf16 lacks the registers from 65
+        // state columns on (ragged prompts 140 -> 191, ten spilled); so does fp16 from 129 on, where it spills ten (4 prompts of 8192 tokens at
+        // 256 columns: 1021 us, bf16 797).
         constexpr bool kAhead = kHalf || NT < 4;
         lq_v4i bb[3], wh[2], wl[2];
         lq_v4f w4[2][2];
@@ -907,6 +909,8 @@ bool plan(const lq_ssm_prompt_args* a, Plan& r) {
   // alone.  Their lengths are not known here: the longest is taken to be two and a half times the mean.  Measured, 80 heads of 64 by 128: 4
   // prompts of 8192 tokens in 3 segments of one piece 303 us and the states 120, of two pieces 99 (of four 93, but the join takes longer), in 2
   // segments 397; 10 packed prompts of 6949 tokens, the longest 2047, 64 heads in 8 groups, 140 us uncut, 155 in segments of 12 chunks.
+  // All of it at 128 state columns; at others the steps are shorter or longer, and above 128 a compute unit has one workgroup.  Where one packed
+  // prompt is most of the tokens the guess is far off: 8000 tokens and 63 single ones are not cut, 661 to 684 us for 125 to 128 of the long one alone.
   const double mean = (double)r.units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
   auto step = [&](double wgs, double one, double two) {
     if (wgs <= 256) return one;

@@ -48,7 +48,7 @@ def _check_state(state, x, W):
 def conv1d_prompt(x, weight, bias=None, activation=None, *, state=None, slots=None, seq_starts=None):
     """y[t] = act(bias + sum_j weight[:, j] x[t - (W-1) + j]) over each prompt.  ``x`` fp16 or bf16: (B, L, D), or (T, D) with
     ``seq_starts`` (n + 1 int32, ascending) for packed prompts of any lengths; tokens outside them keep undefined outputs.
-    ``weight`` (D, W), W 2 to 4, D a multiple of 8.  ``state`` (slots, W-1, D): the inputs in front of each prompt, oldest first,
+    ``weight`` (D, W), W 2 to 4, D a multiple of 8; taps and bias of another type are rounded to x's, as in ``causal_conv1d_fn``.  ``state`` (slots, W-1, D): the inputs in front of each prompt, oldest first,
     read and then replaced by its last W-1 (a prompt of no tokens leaves them); None: zeros in front, nothing kept.  ``slots``
     (n,) int32: each prompt's place in the state, all different; negative: zeros in front, nothing kept; beyond the state: NaN
     outputs.  Returns y, dense, in the shape of x."""

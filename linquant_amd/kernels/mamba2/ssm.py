@@ -63,7 +63,8 @@ def ssm_prompt(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_lim
     that lets steps be negative lets the state grow.)
     ``state`` (slots, H, P, N) fp32: what each prompt starts from, replaced by what it ends in (a prompt of no tokens leaves it);
     None: zero, nothing kept.  ``slots`` (n,) int32: each prompt's place in the state, all different; negative: from zero, nothing
-    kept; beyond the state: NaN outputs.  Returns y, dense, in the shape and type of x."""
+    kept; beyond the state: NaN outputs.  An infinity in x, dt, B, C or the state counts as a NaN: it reaches the outputs and states that the formula
+    has it reach, as one or the other.  Returns y, dense, in the shape and type of x."""
     if state is not None:
         out = _lib.native().ssm_prompt(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots, seq_starts)
         if out is not None:
@@ -105,7 +106,7 @@ def ssm_prompt(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_lim
 
 
 def ssm_step(state, x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=True, dt_limit=(0.0, float("inf")), slots=None):
-    """The same for one token of each sequence: ``x`` (B, H, P), ``dt`` (B, H), ``B``, ``C`` (B, G, N) -> y (B, H, P), ``state``
+    """The same for one token of each of up to 65535 sequences: ``x`` (B, H, P), ``dt`` (B, H), ``B``, ``C`` (B, G, N) -> y (B, H, P), ``state``
     (slots, H, P, N) fp32 moved on by it.  ``slots`` (B,) int32, all different; negative marks a padding entry (zeros out, no
     state touched), beyond the state: NaN outputs."""
     out = _lib.native().ssm_step(x, dt, A, B, C, D, dt_bias, dt_softplus, dt_limit, state, slots)
