@@ -21,9 +21,9 @@
 // (whose second piece is 2^11 smaller) 2^16 below its channel's.  A unit for 32 channels and 64 tokens together (2 % less time) lost a
 // channel beside one 2^26 above it, and the state that a chunk's first tokens read where a later one was as far above them.
 //
-// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 414 to 426 us by the card, call after
+// What bounds it.  4 prompts of 8192 tokens, 80 heads of 64 channels, 128 state columns, fp16: 408 to 426 us by the card, call after
 // call (the kernels' own least times: operands 27, states 99, join 16, chunks 287; the profiler's medians are up to 14 % above them), 1.7 TB/s of
-// what has to move and 254 to 261 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
+// what has to move and 254 to 265 TFLOP/s of the recurrence's operations.  In the last kernel the vector unit is
 // busy 53 % of the time (scaling, rounding and splitting operands, 774 instructions to 32 channels and 64 tokens), the matrix unit 22 %, and
 // the clock falls from 2.4 to 2.1 GHz; two waves to a SIMD is what the state in registers (64 of 256) and 81 KB of LDS leave.  Few or
 // ragged prompts are a chain of chunks, about 4 us each: 384 tokens 36 us, 6949 in 10 prompts of up to 2047, 64 heads in 8 groups, bf16, 140.
