@@ -41,7 +41,7 @@ typedef struct ihipStream_t* hipStream_t;
 #define LQ_DT_BF16 3
 
 /* ABI version; bumped whenever a struct layout, or what a call asks of its caller, changes.  The function gives the library's. */
-#define LQ_ABI_VERSION 22
+#define LQ_ABI_VERSION 23
 int lq_abi_version(void);
 /* sizeof() of the named args struct as compiled into the library (negative if unknown); lets a binding
  * check its own struct layout before the first call. */
@@ -840,6 +840,13 @@ typedef struct {
   int64_t out_stride;
   int32_t out_dtype;         /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
   int32_t rows, cols, inner; /* inner a multiple of 16, at most 131056 (a sum of 128 * 128 each fits 32 bits) */
+  /* the second half of low-rank adapters, added before the one rounding at the output; all NULL / 0: none.
+     out[m,n] += sum_r adapter_h[m,r] adapter_up[j,n,r], j = adapter_ids[m]; a negative id: nothing, beyond adapter_count: NaN */
+  const float* adapter_h;    /* (rows, adapter_rank) dense, 16-byte aligned, as lq_adapter_down leaves it */
+  const int32_t* adapter_ids; /* (rows,) */
+  const void* adapter_up;    /* (adapter_count, cols, adapter_rank) dense, 16-byte aligned */
+  int32_t adapter_dtype;     /* LQ_DT_F16 / LQ_DT_BF16 */
+  int32_t adapter_rank, adapter_count; /* rank a multiple of 16, up to 128 */
 } lq_int8_matmul_args;
 int lq_int8_matmul(const lq_int8_matmul_args* args, hipStream_t stream);
 
@@ -973,6 +980,109 @@ typedef struct {
   int32_t num_slots, batch, nheads, headdim, ngroups, dstate; /* batch up to 65535 */
 } lq_ssm_step_args;
 int lq_ssm_step(const lq_ssm_step_args* args, hipStream_t stream);
+
+/* no counterpart in the reference (its zoo kernels, linquant/kernels/zoo/simple_gla.py:175-212, are INT8, start from zero and take no
+ * single tokens): linear attention with no decay, one for each head, or one for each head and token, on 16-bit activations with an
+ * fp32 state,
+ *   S = exp(min(g, 0)) S + k v^T;  o = scale S^T q,
+ * S (kdim, vdim) for each head, starting from and ending in its slot of `state`. */
+typedef struct {
+  const void* q;             /* (tokens,H,K) with seq_starts, else (nseq,seqlen,H,K); unit K stride, 16-byte aligned rows (k's and v's
+                                too), tokens from 0 to less than 2^24 entries apart */
+  int64_t q_stride_b, q_stride_l, q_stride_h;
+  const void* k;             /* like q */
+  int64_t k_stride_b, k_stride_l, k_stride_h;
+  const void* v;             /* (tokens,H,V) or (nseq,seqlen,H,V) */
+  int64_t v_stride_b, v_stride_l, v_stride_h;
+  int32_t dtype;             /* of q, k, v and out: LQ_DT_F16 / LQ_DT_BF16 */
+  const void* g;             /* log decays, or NULL: none.  One for each head where both other strides are zero */
+  int64_t g_stride_b, g_stride_l, g_stride_h;
+  int32_t g_dtype;           /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  float scale;
+  void* out;                 /* the shape of v, dense */
+  float* state;              /* (num_slots,H,K,V), the last three dense, or NULL: from zero, nothing kept */
+  int64_t state_stride_s;
+  const int32_t* slots;      /* (nseq,) or NULL */
+  const int32_t* seq_starts; /* (nseq + 1,) or NULL */
+  int32_t num_slots, nseq, seqlen, tokens; /* seqlen without seq_starts, tokens with */
+  int32_t nheads, kdim, vdim; /* kdim and vdim multiples of 8, kdim up to 256, nheads * vdim up to 2^23 */
+  void* workspace;           /* 256-byte aligned; contents undefined on entry and on return */
+  int64_t workspace_bytes;
+} lq_linear_attention_prompt_args;
+int lq_linear_attention_prompt(const lq_linear_attention_prompt_args* args, hipStream_t stream);
+/* workspace size for the dims in `args` (pointers are not read but for whether seq_starts is NULL), written to *bytes */
+int lq_linear_attention_prompt_workspace_bytes(const lq_linear_attention_prompt_args* args, int64_t* bytes);
+
+/* no counterpart in the reference: the same for one token of each sequence; state is updated in place. */
+typedef struct {
+  const void* q;             /* (batch,H,K), unit K stride */
+  int64_t q_stride_b, q_stride_h;
+  const void* k;
+  int64_t k_stride_b, k_stride_h;
+  const void* v;             /* (batch,H,V), unit V stride, 8-byte aligned rows */
+  int64_t v_stride_b, v_stride_h;
+  int32_t dtype;
+  const void* g;             /* (batch,H), (H,) with g_stride_b = 0, or NULL */
+  int64_t g_stride_b, g_stride_h;
+  int32_t g_dtype;
+  float scale;
+  void* out;                 /* (batch,H,V) dense */
+  float* state;              /* (num_slots,H,K,V), the last three dense */
+  int64_t state_stride_s;
+  const int32_t* slots;      /* (batch,) or NULL */
+  int32_t num_slots, batch, nheads, kdim, vdim; /* kdim up to 256, vdim a multiple of 4, batch up to 65535 */
+} lq_linear_attention_step_args;
+int lq_linear_attention_step(const lq_linear_attention_step_args* args, hipStream_t stream);
+
+/* no counterpart in the reference (its gated norm, linquant/quantized_mamba2.py:354-358, takes no mean off): group norm of each row,
+ * channels last, statistics over num_groups groups of adjacent channels, in fp32 with one rounding at the output,
+ *   y = (x - mean) * rsqrt(var + eps) * weight + bias;  out = y * act(z), or act(y) where z is NULL. */
+typedef struct {
+  const void* x;             /* (rows, dim), unit dim stride */
+  int64_t x_stride;
+  const void* z;             /* (rows, dim) or NULL */
+  int64_t z_stride;
+  int32_t dtype;             /* of x, z and out: LQ_DT_F16 / LQ_DT_BF16 */
+  const void* weight;        /* (dim,) or NULL: one */
+  const void* bias;          /* (dim,) or NULL: zero */
+  int32_t weight_dtype;      /* of both: LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
+  void* out;                 /* (rows, dim) dense */
+  float eps;
+  int32_t rows, dim, num_groups; /* dim a multiple of num_groups; up to 16384 channels to a group */
+  int32_t act;               /* 0: none, 1: SiLU, 2: sigmoid */
+} lq_groupnorm_gated_args;
+int lq_groupnorm_gated(const lq_groupnorm_gated_args* args, hipStream_t stream);
+
+/* no counterpart in the reference: the first half of low-rank adapters of many requests, h[m] = scaling[j] * (down[j] x[m]), j = ids[m],
+ * for the epilogue of lq_int8_matmul.  x in 16 bits, or INT8 codes with a scale for each row (or one).  A negative id: zeros;
+ * beyond `count`: NaN. */
+typedef struct {
+  const void* x;             /* (rows, inner), unit inner stride, rows on boundaries of 8 entries where inner is a multiple of 8 */
+  int64_t x_stride;
+  int32_t x_dtype;           /* `dtype`, or LQ_DT_I8: codes */
+  const float* x_scale;      /* codes: one, or (rows,) with x_scale_rows = 1 */
+  int32_t x_scale_rows;
+  const void* down;          /* (count, rank, inner_padded) dense, 16-byte aligned, zeros behind `inner` */
+  int32_t dtype;             /* LQ_DT_F16 / LQ_DT_BF16 */
+  const float* scaling;      /* (count,) */
+  const int32_t* ids;        /* (rows,) */
+  float* h;                  /* (rows, rank) dense, 16-byte aligned */
+  int32_t rows, inner, inner_padded, rank, count; /* inner_padded and rank multiples of 16, rank up to 128 */
+} lq_adapter_down_args;
+int lq_adapter_down(const lq_adapter_down_args* args, hipStream_t stream);
+
+/* no counterpart in the reference: slots of state tensors copied, exchanged or cleared, all tensors in one call.
+ *   new[dst[i]] = old[src[i]], or zeros where src[i] < 0, or all bits one (NaN) where it is num_slots or more;
+ * every source is read before anything is written.  Entries with dst outside 0 .. num_slots - 1 do nothing; of several with the same dst the
+ * last one counts.  Other slots are left alone. */
+typedef struct {
+  const int64_t* tensors;    /* HOST array of three numbers a tensor: device address, bytes from slot to slot, bytes of a slot */
+  int32_t num_tensors, num_slots;
+  const int32_t* src;        /* (entries,) on the device */
+  const int32_t* dst;
+  int32_t entries;           /* up to 8192 */
+} lq_copy_slots_args;
+int lq_copy_slots(const lq_copy_slots_args* args, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement aid (no counterpart in the reference): a matrix-core-only launch whose rate is the MFMA issue peak of

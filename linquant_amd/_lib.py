@@ -18,7 +18,7 @@ _NATIVE_ENTRIES = ("lq_zoo_simple_gla", "lq_zoo_simple_gla_workspace_bytes", "lq
                    "lq_zoo_chunk_forward_workspace_bytes", "lq_zoo_rotate_qkv", "lq_split_rotate_quant_xBC", "lq_ssd_combined",
                    "lq_ssd_combined_workspace_bytes", "lq_quantize_rows", "lq_int8_matmul", "lq_residual_rmsnorm", "lq_conv1d_prompt",
                    "lq_conv1d_step", "lq_ssm_prompt", "lq_ssm_prompt_workspace_bytes", "lq_ssm_step", "lq_abi_version", "lq_args_size")
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 LQ_DT_F16, LQ_DT_F32, LQ_DT_I8, LQ_DT_BF16 = 0, 1, 2, 3
 
@@ -64,7 +64,8 @@ FUNCTIONS = tuple(_funcs)
 _SHARED_ARGS = {"lq_ssd_combined_static": "lq_ssd_combined_args", "lq_ssd_combined_workspace_bytes": "lq_ssd_combined_args",
                 "lq_zoo_simple_gla_workspace_bytes": "lq_zoo_simple_gla_args",
                 "lq_zoo_chunk_forward_workspace_bytes": "lq_zoo_chunk_forward_args",
-                "lq_ssm_prompt_workspace_bytes": "lq_ssm_prompt_args", "lq_ssm_prompt_plan": "lq_ssm_prompt_args"}
+                "lq_ssm_prompt_workspace_bytes": "lq_ssm_prompt_args", "lq_ssm_prompt_plan": "lq_ssm_prompt_args",
+                "lq_linear_attention_prompt_workspace_bytes": "lq_linear_attention_prompt_args"}
 
 _lib = None
 

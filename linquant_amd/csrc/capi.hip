@@ -45,6 +45,11 @@ extern "C" int lq_args_size(const char* name) {
   LQ_SIZE_OF(lq_conv1d_step_args);
   LQ_SIZE_OF(lq_ssm_prompt_args);
   LQ_SIZE_OF(lq_ssm_step_args);
+  LQ_SIZE_OF(lq_linear_attention_prompt_args);
+  LQ_SIZE_OF(lq_linear_attention_step_args);
+  LQ_SIZE_OF(lq_groupnorm_gated_args);
+  LQ_SIZE_OF(lq_adapter_down_args);
+  LQ_SIZE_OF(lq_copy_slots_args);
   LQ_SIZE_OF(lq_probe_mfma_args);
   return LQ_ERR_SHAPE;
 }

@@ -1,0 +1,135 @@
+// lq_copy_slots: slots of state tensors copied, exchanged or cleared in place, all tensors of all layers in one launch.
+//   new[dst[i]] = old[src[i]], zeros where src[i] < 0, all bits one where it is beyond the slots
+// HBM-bound: every entry's bytes read once and written once.
+//
+// A workgroup owns a strip of a tensor, some bytes of every slot, for all entries: it requests every entry's part of the strip into
+// registers, waits until all of its waves have theirs, and stores.  So no source is overwritten before it is read, whatever the entries
+// exchange, without a second buffer in memory, and no two workgroups touch the same bytes.  The more entries, the narrower a strip: 1024
+// bytes up to 256 entries, 32 at 8192.
+#include <algorithm>
+
+#include "serve_common.h"
+
+namespace {
+
+constexpr int kWaves = 8, kMaxTensors = 64, kMaxEntries = 8192, kMaxU = 32;
+
+struct Slots {
+  char* base;
+  int64_t stride, bytes;
+  int64_t strips;  // of this tensor and the ones in front of it
+};
+struct CopyParams {
+  Slots t[kMaxTensors];
+  int num_tensors, num_slots;
+  const int32_t* src;
+  const int32_t* dst;
+  int entries, lanes;  // lanes: of one entry's part of a strip, a power of two; a lane has one unit
+};
+
+// of the unit that divides a tensor's address, stride and size: 16, 4, 2 or 1 bytes
+LQ_DEV int unit_of(const Slots& t) {
+  const uint64_t m = (uint64_t)(uintptr_t)t.base | (uint64_t)t.stride | (uint64_t)t.bytes;
+  return m % 16 == 0 ? 16 : (m % 4 == 0 ? 4 : (m % 2 == 0 ? 2 : 1));
+}
+LQ_DEV lq_v4i load_unit(const char* at, int unit) {
+  lq_v4i v = {0, 0, 0, 0};
+  if (unit == 16) v = *(const lq_v4i*)at;
+  else if (unit == 4) v[0] = *(const int*)at;
+  else if (unit == 2) v[0] = *(const uint16_t*)at;
+  else v[0] = *(const uint8_t*)at;
+  return v;
+}
+LQ_DEV void store_unit(char* at, int unit, lq_v4i v) {
+  if (unit == 16) *(lq_v4i*)at = v;
+  else if (unit == 4) *(int*)at = v[0];
+  else if (unit == 2) *(uint16_t*)at = (uint16_t)v[0];
+  else *(uint8_t*)at = (uint8_t)v[0];
+}
+
+enum { kSkip = -2, kClear = -1 };  // what an entry's source says besides a slot; kFill is num_slots
+
+template <int U>
+__global__ __launch_bounds__(64 * kWaves) void copy_slots_kernel(CopyParams p) {
+  extern __shared__ int list[];  // [entries] sources, [entries] destinations
+  int *from = list, *to = list + p.entries;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = p.entries;
+  for (int i = tid; i < n; i += 64 * kWaves) to[i] = p.dst[i];
+  __syncthreads();
+  for (int i = tid; i < n; i += 64 * kWaves) {
+    const int d = to[i];
+    int s = p.src[i];
+    s = s < 0 ? (int)kClear : min(s, p.num_slots);
+    bool drop = d < 0 || d >= p.num_slots || d == s;
+    for (int j = i + 1; j < n; ++j) drop |= to[j] == d;  // the last entry of a destination counts
+    from[i] = drop ? (int)kSkip : s;
+  }
+  __syncthreads();
+  const int part = lane % p.lanes, per = 64 / p.lanes, e0 = wave * per + lane / p.lanes;  // entries e0, e0 + kWaves per, ..
+  const int64_t all = p.t[p.num_tensors - 1].strips;
+  for (int64_t strip = blockIdx.x; strip < all; strip += gridDim.x) {
+    int t = 0;
+    while (strip >= p.t[t].strips) ++t;
+    const Slots& x = p.t[t];
+    const int unit = unit_of(x);
+    const int64_t at = ((strip - (t ? p.t[t - 1].strips : 0)) * p.lanes + part) * unit;
+    const bool in = at < x.bytes;
+    lq_v4i v[U];
+    int f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kWaves * per;
+      f[u] = in && e < n ? from[e] : (int)kSkip;
+      const int fill = f[u] >= p.num_slots ? -1 : 0;
+      v[u] = lq_v4i{fill, fill, fill, fill};
+      if (f[u] >= 0 && f[u] < p.num_slots) v[u] = load_unit(x.base + f[u] * x.stride + at, unit);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every source of the strip is read
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (f[u] != kSkip) store_unit(x.base + to[e0 + u * kWaves * per] * x.stride + at, unit, v[u]);
+  }
+}
+
+}  // namespace
+
+extern "C" int lq_copy_slots(const lq_copy_slots_args* a, hipStream_t stream) {
+  if (!a || !a->tensors || !a->src || !a->dst) return LQ_ERR_NULL;
+  if (a->num_tensors <= 0 || a->num_slots <= 0 || a->entries <= 0 || a->entries > kMaxEntries) return LQ_ERR_SHAPE;
+  if (!sv_al(a->src, 4) || !sv_al(a->dst, 4)) return LQ_ERR_SHAPE;
+  for (int i = 0; i < a->num_tensors; ++i) {
+    if (!a->tensors[3 * i]) return LQ_ERR_NULL;
+    if (a->tensors[3 * i + 2] <= 0 || (a->num_slots > 1 && a->tensors[3 * i + 1] < a->tensors[3 * i + 2])) return LQ_ERR_SHAPE;
+  }
+  // as many lanes to an entry's part as leave every entry a place in the workgroup's registers
+  int lanes = 64;
+  while (lanes > 1 && (int64_t)kWaves * (64 / lanes) * kMaxU < a->entries) lanes /= 2;
+  const int64_t slots = (int64_t)kWaves * (64 / lanes);
+  const int u = (int)((a->entries + slots - 1) / slots);
+  for (int first = 0; first < a->num_tensors; first += kMaxTensors) {
+    CopyParams p = {};
+    p.num_tensors = std::min(kMaxTensors, a->num_tensors - first), p.num_slots = a->num_slots, p.src = a->src, p.dst = a->dst, p.entries = a->entries, p.lanes = lanes;
+    int64_t strips = 0;
+    for (int i = 0; i < p.num_tensors; ++i) {
+      const int64_t* t = a->tensors + 3 * (first + i);
+      const uint64_t m = (uint64_t)t[0] | (uint64_t)t[1] | (uint64_t)t[2];
+      const int64_t width = (int64_t)lanes * (m % 16 == 0 ? 16 : (m % 4 == 0 ? 4 : (m % 2 == 0 ? 2 : 1)));
+      strips += (t[2] + width - 1) / width;
+      p.t[i] = {(char*)t[0], t[1], t[2], strips};
+    }
+    const dim3 grid((unsigned)std::min<int64_t>(strips, 4096)), threads(64 * kWaves);
+    const size_t lds = (size_t)a->entries * 8;
+    auto go = [&](auto k) {
+      auto* kernel = copy_slots_kernel<decltype(k)::value>;
+      hipLaunchKernelGGL(kernel, grid, threads, lds, stream, p);
+      return lq_check_launch();
+    };
+    using std::integral_constant;
+    const int rc = u <= 1 ? go(integral_constant<int, 1>{}) : u <= 2 ? go(integral_constant<int, 2>{}) : u <= 4 ? go(integral_constant<int, 4>{}) :
+                   u <= 8 ? go(integral_constant<int, 8>{}) : u <= 16 ? go(integral_constant<int, 16>{}) : go(integral_constant<int, 32>{});
+    if (rc != LQ_OK) return rc;
+  }
+  return LQ_OK;
+}

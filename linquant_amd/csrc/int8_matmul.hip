@@ -34,6 +34,11 @@ struct MatmulParams {
   int64_t out_stride;
   int rows, cols, inner;
   int vec;  // out's rows can be written 16 bytes at a time
+  // adapters: NULL, or the second half of them
+  const float* h;
+  const int32_t* ids;
+  const uint16_t* up;
+  int rank, count;
 };
 
 struct F32 {
@@ -49,6 +54,47 @@ struct OutOf<F32> {
   using type = float;
 };
 
+// out += h up^T, each row with the adapter that it names.  In `tiles` a row's h enters the matrix instructions as two pieces of the
+// adapters' type, after a multiplication by the power of two that brings the row's largest below 2^14 (fp16's range; bf16 the same way): off
+// by 2^-17 of the row's largest.  The adapters that 32 rows name are taken one after the other, with all 32, and a row keeps what its own
+// gave: nothing is multiplied by zero, and an infinity in one request's adapter stays there.
+typedef float mm_v16f __attribute__((ext_vector_type(16)));
+template <typename T>
+LQ_DEV mm_v16f mfma32(lq_v4i a, lq_v4i b, mm_v16f c) {
+  if constexpr (std::is_same<T, F16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lq_v8h, a), __builtin_bit_cast(lq_v8h, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sv_v8bf, a), __builtin_bit_cast(sv_v8bf, b), c, 0, 0, 0);
+}
+// eight of a row's h times `unit`, as two pieces
+template <typename T>
+LQ_DEV void pieces(const float* h, float unit, lq_v4i& hi, lq_v4i& lo) {
+  const lq_v4f a = *(const lq_v4f*)h, b = *(const lq_v4f*)(h + 4);
+  uint16_t u[8], v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = (e < 4 ? a[e & 3] : b[e & 3]) * unit;
+    u[e] = T::from(f), v[e] = T::from(f - T::to(u[e]));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) hi[i] = (int)(u[2 * i] | (uint32_t)u[2 * i + 1] << 16), lo[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
+}
+// the part of a row that this lane's half has is all that it looks at; its largest over both halves
+LQ_DEV float row_unit(const float* h, int rank, int hh) {
+  float top = 0.0f;
+  for (int r = 8 * hh; r < rank; r += 16)
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const lq_v4f v = *(const lq_v4f*)(h + r + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_fabsf(v[i]);
+        top = fmaxf(top, a < __builtin_inff() ? a : 0.0f);
+      }
+    }
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const int e = (int)(__float_as_uint(top) >> 23) - 127;
+  return __uint_as_float((uint32_t)(127 + min(max(13 - e, -100), 100)) << 23);
+}
+
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void glb_void;
 
@@ -59,7 +105,8 @@ constexpr int KB = 128, PC = KB / 16, FR = 64 / PC;  // contraction bytes of a s
 LQ_DEV int order(int row) { return (row >> 1) & 7; }
 
 // TM x TN of the result to KG groups of four waves, 2 x 2 of a tile; the groups have every KG-th stage each and are summed at the end.
-template <int TM, int TN, int KG, typename O>
+// A: the adapters' type, or void.
+template <int TM, int TN, int KG, typename O, typename A>
 __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) void int8_tiles_kernel(MatmulParams p) {
   constexpr int MI = TM / 64, NI = TN / 64;          // 32-row tiles of a wave
   constexpr int PA = TM / FR / 4, PB = TN / FR / 4;  // fetches of a wave and stage
@@ -201,6 +248,38 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int m = m0 + wm + 32 * i;
+    mm_v16f delta[std::is_void<A>::value ? 1 : NI];
+    if constexpr (!std::is_void<A>::value) {
+      const int mc = min(m + (lane & 31), p.rows - 1), id = p.ids[mc];
+      const float* h = p.h + (int64_t)mc * p.rank;
+      const float unit = row_unit(h, p.rank, hh), none = id < p.count ? 0.0f : __builtin_nanf("");
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) delta[j][e] = none;
+      uint64_t left = __ballot(id >= 0 && id < p.count);
+      while (left) {
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const bool mine = id == a;
+        left &= ~__ballot(mine);
+        const uint16_t* up = p.up + (int64_t)a * p.cols * p.rank + 8 * hh;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const uint16_t* uj = up + (int64_t)min(n0 + wn + 32 * j + (lane & 31), p.cols - 1) * p.rank;
+          mm_v16f d = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < p.rank; r += 16) {
+            lq_v4i hi, lo;
+            pieces<A>(h + r + 8 * hh, unit, hi, lo);
+            const lq_v4i u = *(const lq_v4i*)(uj + r);
+            d = mfma32<A>(u, hi, d);
+            d = mfma32<A>(u, lo, d);
+          }
+          sv_settle(d);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) delta[j][e] = mine ? d[e] * (1.0f / unit) : delta[j][e];
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -210,7 +289,11 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
         typedef OT V4 __attribute__((ext_vector_type(4)));
         V4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = O::from(__builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]));
+        for (int e = 0; e < 4; ++e) {
+          float v = __builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]);
+          if constexpr (!std::is_void<A>::value) v += delta[j][4 * q + e];
+          o[e] = O::from(v);
+        }
         *(V4*)(my + (lane & 31) * kOutRow + n * sizeof(OT)) = o;
       }
     // (a wave's LDS operations are in order)
@@ -244,7 +327,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
 // 7.5 / 11.9 / 15.6.  Eight waves that request one line at a time are as good as any, but where results are many (MT 4, NT 2 or 3) four that
 // request two: 64 x 2560 x 10576, NT 2: 21.7 and 22.7.
 // v_mfma_i32_16x16x64_i8: lane l has row l & 15 and the 16 bytes of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
-template <int MT, int NT, int W, int U, typename O>
+template <int MT, int NT, int W, int U, typename O, typename A>
 __global__ __launch_bounds__(64 * W) void int8_rows_kernel(MatmulParams p) {
   __shared__ __align__(16) int sums[W][NT][MT][64][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -304,12 +387,29 @@ __global__ __launch_bounds__(64 * W) void int8_rows_kernel(MatmulParams p) {
     const int row = 16 * i + m, col = n0 + 16 * j + n;
     if (row < p.rows && col < p.cols) {
       const float s = p.a_scale[p.a_scale_rows ? row : 0] * p.b_scale[p.b_scale_cols ? col : 0];
-      out[row * p.out_stride + col] = O::from(__builtin_fmaf((float)v, s, p.bias ? sv_load(p.bias, col, p.bias_dtype) : 0.0f));
+      float r = __builtin_fmaf((float)v, s, p.bias ? sv_load(p.bias, col, p.bias_dtype) : 0.0f);
+      if constexpr (!std::is_void<A>::value) {
+        const int id = p.ids[row];
+        if (id >= p.count) r = __builtin_nanf("");
+        if (id >= 0 && id < p.count) {
+          const float* h = p.h + (int64_t)row * p.rank;
+          const uint16_t* up = p.up + ((int64_t)id * p.cols + col) * p.rank;
+          float d = 0.0f;
+          for (int k = 0; k < p.rank; k += 8) {
+            const sv_v8u u = *(const sv_v8u*)(up + k);
+            const lq_v4f ha = *(const lq_v4f*)(h + k), hb = *(const lq_v4f*)(h + k + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d = __builtin_fmaf(e < 4 ? ha[e & 3] : hb[e & 3], A::to(u[e]), d);
+          }
+          r += d;
+        }
+      }
+      out[row * p.out_stride + col] = O::from(r);
     }
   }
 }
 
-template <typename O>
+template <typename O, typename A>
 int launch(const MatmulParams& p, hipStream_t stream) {
   using std::integral_constant;
   if (p.rows <= 64) {
@@ -320,7 +420,7 @@ int launch(const MatmulParams& p, hipStream_t stream) {
     const int nt = most(3) <= std::min(most(1), most(2)) ? 3 : (most(2) <= most(1) ? 2 : 1);
     auto go = [&](auto m, auto n) {
       constexpr int MT = decltype(m)::value, NT = decltype(n)::value, W = MT == 4 && NT > 1 ? 4 : 8;
-      hipLaunchKernelGGL((int8_rows_kernel<MT, NT, W, 8 / W, O>), dim3((unsigned)((p.cols + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, stream, p);
+      hipLaunchKernelGGL((int8_rows_kernel<MT, NT, W, 8 / W, O, A>), dim3((unsigned)((p.cols + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, stream, p);
     };
     auto columns = [&](auto m) { nt == 1 ? go(m, integral_constant<int, 1>{}) : (nt == 2 ? go(m, integral_constant<int, 2>{}) : go(m, integral_constant<int, 3>{})); };
     mt == 1 ? columns(integral_constant<int, 1>{}) : (mt == 2 ? columns(integral_constant<int, 2>{}) : columns(integral_constant<int, 4>{}));
@@ -330,7 +430,7 @@ int launch(const MatmulParams& p, hipStream_t stream) {
     constexpr int TM = decltype(tm)::value, TN = decltype(tn)::value, KG = decltype(kg)::value;
     const int64_t n = (((int64_t)p.rows + TM - 1) / TM) * (((int64_t)p.cols + TN - 1) / TN);
     if (!sv_fits(n + 7, 256 * KG)) return LQ_ERR_SHAPE;
-    hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, KG, O>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256 * KG), 0, stream, p);
+    hipLaunchKernelGGL((int8_tiles_kernel<TM, TN, KG, O, A>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(256 * KG), 0, stream, p);
     return lq_check_launch();
   };
   auto count = [&](int tm, int tn) { return (((int64_t)p.rows + tm - 1) / tm) * (((int64_t)p.cols + tn - 1) / tn); };
@@ -355,9 +455,20 @@ extern "C" int lq_int8_matmul(const lq_int8_matmul_args* a, hipStream_t stream) 
   if (a->a_stride < 0 || a->a_stride >= 1 << 23 || a->b_stride < 0 || a->b_stride >= 1 << 23) return LQ_ERR_SHAPE;  // a tile's rows are reached by 32-bit offsets
   if (!sv_al(a->out, sv_size(a->out_dtype)) || (a->bias && !sv_al(a->bias, sv_size(a->bias_dtype))) || !sv_al(a->a_scale, 4) || !sv_al(a->b_scale, 4))
     return LQ_ERR_SHAPE;
+  if (a->adapter_h) {
+    if (!a->adapter_ids || !a->adapter_up) return LQ_ERR_NULL;
+    if (!sv_act(a->adapter_dtype) || a->adapter_rank <= 0 || a->adapter_rank % 16 != 0 || a->adapter_rank > 128 || a->adapter_count <= 0) return LQ_ERR_SHAPE;
+    if (!sv_al(a->adapter_h, 16) || !sv_al(a->adapter_up, 16) || !sv_al(a->adapter_ids, 4)) return LQ_ERR_SHAPE;
+  }
   const int per = 16 / sv_size(a->out_dtype);
   MatmulParams p = {a->a, a->a_stride, a->b, a->b_stride, a->a_scale, a->b_scale, a->a_scale_rows, a->b_scale_cols, a->bias, a->bias_dtype,
-                    a->out, a->out_stride, a->rows, a->cols, a->inner, sv_al(a->out, 16) && a->out_stride % per == 0};
-  if (a->out_dtype == LQ_DT_F32) return launch<F32>(p, stream);
-  return a->out_dtype == LQ_DT_F16 ? launch<F16>(p, stream) : launch<BF16>(p, stream);
+                    a->out, a->out_stride, a->rows, a->cols, a->inner, sv_al(a->out, 16) && a->out_stride % per == 0, nullptr, nullptr, nullptr, 0, 0};
+  auto with = [&](auto t) {
+    using O = decltype(t);
+    if (!a->adapter_h) return launch<O, void>(p, stream);
+    p.h = a->adapter_h, p.ids = a->adapter_ids, p.up = (const uint16_t*)a->adapter_up, p.rank = a->adapter_rank, p.count = a->adapter_count;
+    return a->adapter_dtype == LQ_DT_F16 ? launch<O, F16>(p, stream) : launch<O, BF16>(p, stream);
+  };
+  if (a->out_dtype == LQ_DT_F32) return with(F32{});
+  return a->out_dtype == LQ_DT_F16 ? with(F16{}) : with(BF16{});
 }

@@ -59,6 +59,9 @@ LQ_DEV float sv_step_size(float raw, float bias, int softplus, float lo, float h
   return d != d ? d : fminf(fmaxf(d, lo), hi);
 }
 
+// a log decay: above zero counts as zero; NaN stays NaN
+LQ_DEV float sv_decay(float g) { return g != g ? g : fminf(g, 0.0f); }
+
 // What a sequence's slot asks for.  kSlotPad: no state; kSlotBad: out of range, the outputs are NaN.
 enum { kSlotPad = -1, kSlotBad = -2 };
 LQ_DEV int sv_slot(const int32_t* slots, int seq, int num_slots) {
@@ -113,6 +116,12 @@ LQ_DEV void sv_fetch16(const void* base, uint32_t offset, const void* at) {
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)at;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
+
+// Matrix results that a loop of run-time length leaves are read behind this.  The vector unit may read a result some cycles after its product
+// was issued, which the compiler has to see to; where the last product stands in front of a branch out of the loop it did not (ROCm 7.2: no
+// waits in front of the first reads, and old values there).
+template <typename V>
+LQ_DEV void sv_settle(V& v) { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(v)); }
 
 // whether a grid's first dimension fits a launch (2^32 - 1 threads)
 static inline bool sv_fits(int64_t workgroups, int threads) { return workgroups * threads <= 0xffffffffll; }

@@ -138,6 +138,40 @@ def residual_rmsnorm(x, weight, residual=None, eps=1e-5, *, gate=None, scale=1.0
     return codes, quantize if static else row_scale, r_out
 
 
+_ACTIVATIONS = {None: 0, "silu": 1, "swish": 1, "sigmoid": 2}
+
+
+def groupnorm_gated(x, z=None, weight=None, bias=None, *, num_groups, eps=1e-5, activation="silu"):
+    """Group norm of each row, channels last, such as the heads of a linear attention's output, with a gate; in fp32 with one rounding::
+
+        y = (x - mean) * rsqrt(var + eps) * weight + bias        # over each of num_groups groups of adjacent channels of a row
+        out = y * act(z)                                         # without z: act(y)
+
+    ``x`` (..., dim) fp16 or bf16, ``z`` like x or None; ``weight``, ``bias`` (dim,) or None, fp16, bf16 or fp32; ``activation`` "silu", "sigmoid"
+    or None; dim a multiple of num_groups, up to 16384 channels to a group.  No gradients.  Returns the shape and type of x, dense."""
+    assert x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1
+    dim = x.shape[-1]
+    assert num_groups >= 1 and dim >= 1 and dim % num_groups == 0 and dim // num_groups <= 16384, f"{dim} channels in {num_groups} groups"
+    assert z is None or (z.shape == x.shape and z.dtype == x.dtype), "z: the shape and type of x"
+    assert all(t is None or (t.shape == (dim,) and t.dtype in _CODES) for t in (weight, bias)), "weight, bias: (dim,)"
+    assert activation in _ACTIVATIONS, f"activation {activation!r}"
+    _lib.same_device(x, z, weight, bias)
+    rows = x.numel() // dim
+    _lib.below_2_31(rows, dim)
+    x2 = _row_view(x, dim)
+    z2 = None if z is None else _row_view(z, dim)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:  # one type for both: neither loses bits or range
+        weight, bias = weight.float(), bias.float()
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    wdt = next((_CODES[t.dtype] for t in (weight, bias) if t is not None), 0)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if rows:
+        _lib.call("lq_groupnorm_gated", x.device, x=_lib.ptr(x2), x_stride=x2.stride(0), z=_lib.ptr(z2), z_stride=0 if z2 is None else z2.stride(0),
+                  dtype=_CODES[x.dtype], weight=_lib.ptr(weight), bias=_lib.ptr(bias), weight_dtype=wdt, out=_lib.ptr(out), eps=float(eps), rows=rows,
+                  dim=dim, num_groups=num_groups, act=_ACTIVATIONS[activation])
+    return out
+
+
 class RMSNormGated(nn.Module):
     """Module form with the constructor of the norm the mixer receives (hidden_size, eps, group_size;
     norm_before_gate must be False, the only mode the Mamba-2 mixer uses)."""

@@ -56,19 +56,24 @@ def _scale(s, n, device, what):
     return _lib.f32(s).reshape(-1).contiguous(), int(s.numel() != 1)
 
 
-def _matmul(a, b, a_scale, b_scale, bias, out):
-    """a (M, K), b (N, K) in rows of whole 16-byte pieces; out (M, N) with unit column stride."""
+def _matmul(a, b, a_scale, b_scale, bias, out, adapted=None):
+    """a (M, K), b (N, K) in rows of whole 16-byte pieces; out (M, N) with unit column stride; ``adapted``: what adapters add (h, ids, adapters)."""
     (M, K), N = a.shape, b.shape[0]
     a, b = (t if t.stride(0) < 1 << 23 else t.contiguous() for t in (a, b))
     a_scale, per_row = _scale(a_scale, M, a.device, "a_scale")
     b_scale, per_col = _scale(b_scale, N, a.device, "b_scale")
     bias = None if bias is None else bias.contiguous()
     _lib.same_device(a, b, a_scale, b_scale, bias, out)
+    low = {}
+    if adapted is not None:
+        h, ids, adapters = adapted
+        low = dict(adapter_h=_lib.ptr(h), adapter_ids=_lib.ptr(ids), adapter_up=_lib.ptr(adapters.up), adapter_dtype=_CODES[adapters.up.dtype],
+                   adapter_rank=adapters.up.shape[2], adapter_count=adapters.up.shape[0])
     if M and N:
         _lib.call("lq_int8_matmul", a.device, a=_lib.ptr(a), a_stride=a.stride(0), b=_lib.ptr(b), b_stride=b.stride(0),
                   a_scale=_lib.ptr(a_scale), b_scale=_lib.ptr(b_scale), a_scale_rows=per_row, b_scale_cols=per_col, bias=_lib.ptr(bias),
                   bias_dtype=0 if bias is None else _CODES[bias.dtype], out=_lib.ptr(out), out_stride=out.stride(0),
-                  out_dtype=_CODES[out.dtype], rows=M, cols=N, inner=K)
+                  out_dtype=_CODES[out.dtype], rows=M, cols=N, inner=K, **low)
     return out
 
 
@@ -98,9 +103,53 @@ def int8_matmul(a, b, a_scale, b_scale, bias=None, out_dtype=torch.float16, out=
     return res if out is not None or a.dim() == 2 else res.view(*a.shape[:-1], N)
 
 
+class LowRankAdapters(nn.Module):
+    """Low-rank adapters of many requests beside one projection: ``a`` (n, R, K), ``b`` (n, N, R) fp16 or bf16, R up to 128, and a factor each,
+    ``scaling`` (n,) fp32 (None: one).  A row of activations x that names adapter j gains scaling[j] * (x a[j]^T) b[j]^T.  Laid out once:
+    R and K padded with zeros to multiples of 16.  Adapters of lower rank have zeros behind it."""
+
+    def __init__(self, a, b, scaling=None):
+        super().__init__()
+        assert a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype and a.dtype in (torch.float16, torch.bfloat16), "a (n, R, K), b (n, N, R): one 16-bit type"
+        n, R, K = a.shape
+        assert n >= 1 and 1 <= R <= 128 and b.shape[0] == n and b.shape[2] == R and K >= 1 and b.shape[1] >= 1, f"a {tuple(a.shape)}, b {tuple(b.shape)}"
+        assert scaling is None or scaling.shape == (n,), f"scaling: ({n},)"
+        _lib.below_2_31(K, b.shape[1], n)
+        self.in_features, self.out_features, self.rank = K, b.shape[1], R
+        self.register_buffer("down", nn.functional.pad(a.detach(), (0, _padded(K) - K, 0, _padded(R) - R)).contiguous())
+        self.register_buffer("up", nn.functional.pad(b.detach(), (0, _padded(R) - R)).contiguous())
+        scaling = torch.ones(n, device=a.device) if scaling is None else scaling.detach()
+        self.register_buffer("scaling", scaling.to(torch.float32, copy=True).contiguous())
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        self.scaling = self.scaling.float()  # (a module's .half() or .bfloat16() is for the adapters themselves)
+        return self
+
+    def _down(self, x, x_scale, ids):
+        """x (M, K) of the adapters' type, or codes (M, K or more) with their scale: h (M, padded R) fp32."""
+        M = x.shape[0]
+        assert ids.dtype == torch.int32 and ids.shape == (M,), f"ids: one int32 for each of {M} rows"
+        assert x.dtype in (torch.int8, self.down.dtype), f"x and the adapters: one type, got {x.dtype} and {self.down.dtype}"
+        scale, per_row = (None, 0) if x_scale is None else _scale(x_scale, M, x.device, "scale")
+        _lib.same_device(x, self.down, self.up, self.scaling, ids, scale)
+        x = _lib.rows16(x) if self.in_features % 8 == 0 else x if x.stride(1) == 1 else x.contiguous()
+        n, R, K = self.down.shape
+        h = torch.empty(M, R, dtype=torch.float32, device=x.device)
+        if M:
+            _lib.call("lq_adapter_down", x.device, x=_lib.ptr(x), x_stride=x.stride(0), x_dtype=_lib.LQ_DT_I8 if x.dtype == torch.int8 else _CODES[x.dtype],
+                      x_scale=_lib.ptr(scale), x_scale_rows=per_row, down=_lib.ptr(self.down), dtype=_CODES[self.down.dtype], scaling=_lib.ptr(self.scaling),
+                      ids=_lib.ptr(ids), h=_lib.ptr(h), rows=M, inner=self.in_features, inner_padded=K, rank=R, count=n)
+        return h
+
+
 class W8A8Linear(nn.Module):
     """INT8 weight (N, K) with a scale for each output channel.  ``input_scale`` None: activations are quantized with a scale for
-    each row; a 0-dim tensor: with that scale (clamp(rint(x / s), -128, 127)).  The output has the activations' 16-bit type."""
+    each row; a 0-dim tensor: with that scale (clamp(rint(x / s), -128, 127)).  The output has the activations' 16-bit type.
+
+    ``adapters``, ``ids`` of a call: a ``LowRankAdapters`` beside the projection and the adapter that each row names, int32, the shape of the
+    activations without their last dimension; negative: none, beyond the adapters: NaN.  They take the activations as they are before
+    the quantizer (``forward_int8``: the codes times their scale), in the adapters' type, and their sum with the product is rounded once."""
 
     def __init__(self, weight_i8, weight_scale, input_scale=None, bias=None):
         super().__init__()
@@ -120,19 +169,42 @@ class W8A8Linear(nn.Module):
         codes = torch.round(w / torch.where(s > 0, s, 1.0)[:, None]).to(torch.int8)
         return cls(codes, s, input_scale, linear.bias)
 
-    def forward_int8(self, x_i8, scale, out_dtype=torch.float16):
+    def _ids(self, adapters, ids, lead):
+        assert ids is not None and ids.dtype == torch.int32 and ids.shape == lead, f"ids: int32 {tuple(lead)}"
+        assert (adapters.in_features, adapters.out_features) == (self.in_features, self.out_features), "adapters of another projection"
+        return ids.reshape(-1).contiguous()
+
+    def _adapted(self, a, a_scale, h, ids, adapters, out_dtype):
+        """Codes in rows as the weight's, what the adapters add -> (M, N)."""
+        out = torch.empty(a.shape[0], self.out_features, dtype=out_dtype, device=a.device)
+        return _matmul(_lib.rows16(a), self.weight, a_scale, self.weight_scale, self.bias, out, (h, ids, adapters))
+
+    def forward_int8(self, x_i8, scale, out_dtype=torch.float16, *, adapters=None, ids=None):
         """Codes (..., in_features) on ``scale`` (a number, one entry, or one for each row)."""
         assert x_i8.dtype == torch.int8 and x_i8.shape[-1] == self.in_features
         a = x_i8.reshape(-1, self.in_features)
         if self.in_features % _K:
             a = nn.functional.pad(a, (0, _padded(self.in_features) - self.in_features))
+        if adapters is not None:
+            assert out_dtype in _CODES
+            ids = self._ids(adapters, ids, x_i8.shape[:-1])
+            return self._adapted(a, scale, adapters._down(a, scale, ids), ids, adapters, out_dtype).view(*x_i8.shape[:-1], self.out_features)
         return int8_matmul(a, self.weight, scale, self.weight_scale, self.bias, out_dtype).view(*x_i8.shape[:-1], self.out_features)
 
-    def forward(self, x):
+    def forward(self, x, *, adapters=None, ids=None):
         assert x.shape[-1] == self.in_features and x.dtype in (torch.float16, torch.bfloat16)
-        if self.input_scale is not None and x.dtype == torch.float16 and self.in_features % 8 == 0:
-            q = _fused_fp16_to_int8(_lib.rows16(x.reshape(-1, self.in_features)), self.input_scale, clamp_min=-128.0, reciprocal=False)
-            return self.forward_int8(q.view(x.shape), self.input_scale, x.dtype)
-        assert self.input_scale is None, "a static input scale takes fp16 activations and in_features a multiple of 8"
-        q, s = _quantize(x)
+        static = self.input_scale is not None and x.dtype == torch.float16 and self.in_features % 8 == 0
+        assert static or self.input_scale is None, "a static input scale takes fp16 activations and in_features a multiple of 8"
+        x2 = x.reshape(-1, self.in_features)
+        if static:
+            q, s = _fused_fp16_to_int8(_lib.rows16(x2), self.input_scale, clamp_min=-128.0, reciprocal=False), self.input_scale
+            if adapters is None:
+                return self.forward_int8(q.view(x.shape), s, x.dtype)
+            if self.in_features % _K:
+                q = nn.functional.pad(q, (0, _padded(self.in_features) - self.in_features))
+        else:
+            q, s = _quantize(x)
+        if adapters is not None:
+            ids = self._ids(adapters, ids, x.shape[:-1])
+            return self._adapted(q, s, adapters._down(x2, None, ids), ids, adapters, x.dtype).view(*x.shape[:-1], self.out_features)
         return int8_matmul(q, self.weight, s, self.weight_scale, self.bias, x.dtype).view(*x.shape[:-1], self.out_features)
