@@ -995,9 +995,8 @@ typedef struct {
   const void* v;             /* (tokens,H,V) or (nseq,seqlen,H,V) */
   int64_t v_stride_b, v_stride_l, v_stride_h;
   int32_t dtype;             /* of q, k, v and out: LQ_DT_F16 / LQ_DT_BF16 */
-  const void* g;             /* log decays, or NULL: none.  One for each head where both other strides are zero */
+  const float* g;            /* log decays, tokens as far apart as q's, or NULL: none.  One for each head where both other strides are zero */
   int64_t g_stride_b, g_stride_l, g_stride_h;
-  int32_t g_dtype;           /* LQ_DT_F16 / LQ_DT_BF16 / LQ_DT_F32 */
   float scale;
   void* out;                 /* the shape of v, dense */
   float* state;              /* (num_slots,H,K,V), the last three dense, or NULL: from zero, nothing kept */

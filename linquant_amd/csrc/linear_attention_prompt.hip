@@ -31,10 +31,11 @@ struct PromptParams {
   int64_t sk_b, sk_l, sk_h;
   const uint16_t* v;
   int64_t sv_b, sv_l, sv_h;
-  const void* g;
+  const float* g;
   int64_t sg_b, sg_l, sg_h;
-  int g_dtype, g_same;  // g_same: one decay for all tokens of a head
-  float scale;
+  int g_same;  // g_same: one decay for all tokens of a head
+  float log_scale;  // of its size, a power of two
+  int negative;
   uint16_t* out;
   float* state;
   int64_t ss_s;
@@ -204,20 +205,27 @@ LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
 
 // A wave has 32 channels of v of a head: the state's K x 32 as accumulators (rows channels of k, columns those of v).  STATES: only the
 // segment's state and decay.  A workgroup's waves, up to W, share the chunk's q and k in LDS and the 32 x 32 tiles of weighted q . k that each
-// of them forms one or two of; each wave's v comes the same way, a chunk ahead into one of two places, and its o leaves through the other.
+// of them forms one or two of; each wave's v comes the same way, a chunk ahead.  o is formed with channels as rows, so that a lane has 32
+// bytes of a token's row between two exchanges of its halves and stores them from registers.
+//
+// The state's accumulators are not multiplied by the decay of every chunk: they hold the state over 2^total, which multiplies the rows of q S
+// (with exp(c_t)) and divides the weights of v, until total falls below kFloor.
 template <typename T, int NT, int W, bool STATES>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void linear_attention_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
+  constexpr float kFloor = kHalf ? -6.0f : -30.0f;  // (fp16: weighted v, below 2^8 with its unit, stays within its range; larger v: zero)
   constexpr int RB = 64 * NT, PR = 4 * NT, kTile = Q * RB;  // bytes and pieces of a row of q or k, bytes of a chunk's
   constexpr int kFetch = kTile / (1024 * W), kRows = 1024 / RB;  // fetches of a wave, rows of each
   constexpr int PT = W == 2 ? 2 : 1;                           // tiles of q . k of a wave
-  __shared__ __align__(1024) char kbuf[STATES ? 2 : 1][kTile];
+  __shared__ __align__(1024) char kbuf[2][kTile];
   __shared__ __align__(1024) char qbuf[STATES ? 16 : kTile];
-  __shared__ __align__(256) uint16_t vbuf[2][W][Q * 32];
+  __shared__ __align__(256) uint16_t vbuf[W][Q * 32];
   __shared__ __align__(16) char pbuf[STATES ? 16 : 8 * 1024];  // weighted q . k, operands 4 tt + ks; (0, 2) and (0, 3) are zero
-  __shared__ __align__(16) float punit[kHalf && !STATES ? 4 * 32 : 4];  // fp16: 1 / unit of each tile's rows t, tiles 2 tt + st
+  __shared__ __align__(16) float punit[kHalf && !STATES ? 4 * 32 : 4];  // fp16: 1 / unit of each tile's columns t, tiles 2 tt + st
   __shared__ int podd[4];                                       // fp16: whether a tile has a unit that is not 1
-  __shared__ __align__(16) float tok[W][3 * Q];                 // each wave's c, exp2(c_63 - c), exp2(c) scale
+  __shared__ __align__(16) float tok[W][3 * Q];                 // each wave's c, weights of v, exp2(c + total) |scale|
+  __shared__ __align__(16) float gbuf[W][64];                   // each wave's decays of a chunk
+  __shared__ __align__(16) float vunit[kHalf && !STATES ? W : 1][64];  // fp16: each wave's channels' 1 / unit_S, 1 / read
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   // Workgroups go round the 8 XCDs in launch order; the parts of one head, which read the same q and k, and the heads of one segment, whose
   // rows lie side by side, go to one.
@@ -235,7 +243,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   const bool keeps = p.state && slot >= 0, bad = slot == kSlotBad;
   const int64_t row0 = p.starts ? s.begin : (int64_t)s.seq * p.seqlen;  // of the dense output
   const int64_t ostride = (int64_t)p.H * p.V, first = (int64_t)s.chunk0 * Q;
-  uint16_t* os = p.out + (row0 * p.H + h) * p.V + ch0;
+  uint16_t* os = p.out + ((row0 + first) * p.H + h) * p.V + ch0;
   const int64_t b = p.starts ? 0 : s.seq, l0 = (p.starts ? s.begin : 0) + first;
   const uint16_t* qs = p.q + b * p.sq_b + l0 * p.sq_l + h * p.sq_h;
   const uint16_t* ks_ = p.k + b * p.sk_b + l0 * p.sk_l + h * p.sk_h;
@@ -249,12 +257,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = channel(nt, hh, r);
-        S[nt][r] = src && n < p.K ? src[(int64_t)n * p.V] : 0.0f;
+      for (int r = 0; r < 16; ++r) S[nt][r] = 0.0f;
+    if (src) {  // (all requested together: none behind a condition of its own)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[nt][r] = src[min(channel(nt, hh, r), p.K - 1) * (int64_t)p.V];
+      if (p.K < 32 * NT) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[nt][r] = channel(nt, hh, r) < p.K ? S[nt][r] : 0.0f;
       }
+    }
   }
-  float unit_S = 1.0f;  // fp16: S holds the channel's state times this power of two
 
   if (!STATES) {
     const lq_v4i zero = {0, 0, 0, 0};
@@ -265,96 +281,86 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   if (!whole) {
     const lq_v4i zero = {0, 0, 0, 0};
     for (int i = threadIdx.x; i < kTile / 16; i += 64 * W) {
-      *(lq_v4i*)(kbuf[0] + i * 16) = zero;
-      if (STATES) *(lq_v4i*)(kbuf[STATES ? 1 : 0] + i * 16) = zero;
-      else *(lq_v4i*)(qbuf + i * 16) = zero;
+      *(lq_v4i*)(kbuf[0] + i * 16) = zero, *(lq_v4i*)(kbuf[1] + i * 16) = zero;
+      if (!STATES) *(lq_v4i*)(qbuf + i * 16) = zero;
     }
     __syncthreads();
   }
-  // chunk by chunk: rows behind the prompt are its last one again (at weight zero)
   // (addresses are made of a lane number that the compiler does not know to be the same: kept over the loop they are registers that it lacks)
   auto fresh = [&] {
     int l = lane;
     asm volatile("" : "+v"(l));
     return l;
   };
+  // rows of a chunk; behind the prompt its last one again (at weight zero)
   auto rows_of = [&](const uint16_t* base, int64_t stride, char* to, int left) {
-    const int lane = fresh();
+    const int lane = fresh(), row = wave * kFetch * kRows + lane / PR, c = (lane % PR) ^ order<NT>(row);  // of the first fetch
+    to += wave * kFetch * 1024;
+    if (whole && left >= Q) {  // (the i-th fetch: rows i kRows on, their bits apart from the first one's, and so the order's)
+      const uint32_t off = (uint32_t)row * (uint32_t)stride * 2u;
 #pragma unroll
-    for (int i = 0; i < kFetch; ++i) {
-      const int f = wave * kFetch + i, row = f * kRows + lane / PR, c = (lane % PR) ^ order<NT>(row);
-      const uint32_t off = (uint32_t)min(row, left - 1) * (uint32_t)stride * 2u + (uint32_t)c * 16u;
-      if (whole || c * 8 < p.K) sv_fetch16(base, off, to + f * 1024);
+      for (int i = 0; i < kFetch; ++i) sv_fetch16(base + i * kRows * stride, (uint32_t)((c ^ order<NT>(i * kRows)) << 4) + off, to + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kFetch; ++i) {
+        const int ci = c ^ order<NT>(i * kRows);
+        const uint32_t off = (uint32_t)min(row + i * kRows, left - 1) * (uint32_t)stride * 2u + (uint32_t)ci * 16u;
+        if (ci * 8 < p.K) sv_fetch16(base, off, to + i * 1024);
+      }
     }
   };
-  int kleft = s.len - (int)first, vleft = kleft;
-  auto fetch = [&](int c) {  // a chunk's k and q
-    rows_of(ks_, p.sk_l, kbuf[STATES ? c & 1 : 0], kleft);
-    if (!STATES) rows_of(qs, p.sq_l, qbuf, kleft);
-    ks_ += Q * p.sk_l, qs += Q * p.sq_l, kleft -= Q;
-  };
-  float gv = 0.0f;
-  int64_t gat = g0;
-  auto request = [&](int c) {  // a chunk's v and decays
-    uint16_t* to = vbuf[c & 1][wave];
+  int qleft = s.len - (int)first, kleft = qleft, vleft = qleft;
+  auto fetch_q = [&] { rows_of(qs, p.sq_l, qbuf, qleft), qs += Q * p.sq_l, qleft -= Q; };
+  auto fetch_k = [&](int c) { rows_of(ks_, p.sk_l, kbuf[c & 1], kleft), ks_ += Q * p.sk_l, kleft -= Q; };
+  const float* gs = p.g + g0;
+  auto fetch_v = [&] {  // and the decays
     const int lane = fresh();
     if (live) {
       const uint32_t vcol = (uint32_t)min(8 * (lane & 3), p.V - 8 - ch0);
+      if (vleft >= Q) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sv_fetch16(vs, ((uint32_t)min(16 * i + (lane >> 2), vleft - 1) * (uint32_t)p.sv_l + vcol) * 2u, to + 16 * 32 * i);
+        for (int i = 0; i < 4; ++i) sv_fetch16(vs + 16 * i * p.sv_l, ((uint32_t)(lane >> 2) * (uint32_t)p.sv_l + vcol) * 2u, vbuf[wave] + 16 * 32 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sv_fetch16(vs, ((uint32_t)min(16 * i + (lane >> 2), vleft - 1) * (uint32_t)p.sv_l + vcol) * 2u, vbuf[wave] + 16 * 32 * i);
+      }
     }
-    if (p.g && !p.g_same) gv = sv_load(p.g, gat + min(lane, vleft - 1) * p.sg_l, p.g_dtype);
-    vs += Q * p.sv_l, gat += Q * p.sg_l, vleft -= Q;
+    if (!p.g_same) sv_fetch4(gs, (uint32_t)min(lane, vleft - 1) * (uint32_t)p.sg_l * 4u, gbuf[wave]);
+    vs += Q * p.sv_l, gs += Q * p.sg_l, vleft -= Q;
   };
-  if (p.g && p.g_same) gv = sv_load(p.g, g0, p.g_dtype);
-  auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" : "+v"(gv)::"memory"); };
-  auto all_but_stores = [&] { asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); };
+  const float same = p.g && p.g_same ? lane_of(*gs, 0) : 0.0f;  // (waited for here)
+  auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
   auto meet = [&] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  fetch(0);
-  request(0);
+  fetch_k(0);
+  if (!STATES) fetch_q();
+  fetch_v();
   arrived();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(S[nt]));  // (else the compiler waits for its loads in every chunk, and for all behind them)
 
   // What a chunk's products need of the wave's own: v in registers, decays in LDS, the state's unit.
   float* my = tok[wave];
-  lq_v4i xp[4] = {};  // this lane's channel, tokens in the order of an operand
+  lq_v4i xp[4] = {};  // this lane's channel, tokens in the order of an operand; fp16: times its unit
   auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
-  float total = 0.0f, all = 1.0f;                   // the segment's decay so far; the chunk's
-  float rescale = 1.0f, read = 1.0f, unread = 1.0f;  // fp16: to the state's new unit; what q multiplies is S times `read`, 1 / unread of the state
-  uint32_t units = 0;                                // fp16: the power of two of v that enters the state, twice
+  float total = 0.0f, whole_decay = 0.0f;            // what the accumulators are over, the segment's decay so far (powers of two)
+  float fold = 1.0f;                                 // what the accumulators are multiplied by in this chunk, mostly one
+  float unit_S = 1.0f, read = 1.0f;                  // fp16: powers of two of the channel: of v and the state; what q multiplies is that times `read`
+  bool calm = true, scaled = false;                  // the same for the wave: read is one for all channels; the accumulators are multiplied
   auto begin = [&](int c) {
     const int lane = fresh(), hh = lane >> 5;
     const int rem = s.len - (s.chunk0 + c) * Q;
-    {
-      // one factor of 2^-160 is zero in 32 bits, and sums of larger ones would cost the tokens behind them their last bits
-      const float e = sv_decay(gv) * kLog2e, one = e < -160.0f ? -160.0f : e;
-      float cs, behind;
-      if (p.g_same) {
-        cs = one * (float)min(lane + 1, rem), behind = one * (float)max(min(rem, Q) - 1 - lane, 0);
-      } else {
-        const float a = lane < rem ? one : 0.0f;
-        cs = sums_upto(a), behind = sums_behind(a, lane);
-      }
-      const float last = lane_of(cs, 63);
-      all = exp2_fast(last);
-      total += last;
-      my[lane] = cs, my[Q + lane] = lane < rem ? exp2_fast(behind) : 0.0f;
-      if (!STATES) my[2 * Q + lane] = exp2_fast(cs) * p.scale;
-    }
-    if (!live) return;
-    const uint16_t* xl = vbuf[c & 1][wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
+    bool large = false;
+    float change = 1.0f;
+    if (live) {
+    const uint16_t* xl = vbuf[wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       const lq_v2i lo = read_columns(xl + 16 * ks * 32), hi = read_columns(xl + (16 * ks + 8) * 32);
       xp[ks] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
     }
     if constexpr (kHalf) {
-      // Units of the channel, from its largest entry of the state and of v.  What q multiplies has one of its own: what the chunk adds can be
-      // far above the state that its first tokens read.
-      float m = 0.0f;  // (no number where the lane has one that is none: its scale does not matter then)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(S[nt][e]));
+      // The channel's unit is at least one, so that no entry of v loses bits, and is kept while it brings the largest of v between 2^-1 and 2^4
+      // (weighted v is then evenly spaced by 2^-24 of that or less); but a state that is 2^100 above v would leave 32 bits.
       uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
@@ -363,17 +369,60 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           typedef uint16_t v2u __attribute__((ext_vector_type(2)));
           top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
         }
-      const float mx = channel_top(finite_size(T::to((uint16_t)max(top & 0xffffu, top >> 16)))), ms = channel_top(finite_size(m)), iu = pow2_inverse(unit_S);
-      // Weights are at most 1.  Weighted v is below 2^14 and the state too, unless it is 2^38 above v (it is kept in 32 bits: nothing overflows)
-      const float k = fminf(fmaxf(scale_for<13, -100, 15>(fmaxf(ms * iu, mx)), 0x1p-24f), 0x1p15f);
+      float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (no number where the lane has one that is none: its scale does not matter then)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m4[(e >> 1) & 3] = __builtin_elementwise_maximum(m4[(e >> 1) & 3], __builtin_fabsf(S[nt][e]));
+      const float m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m4[0], m4[1]), __builtin_elementwise_maximum(m4[2], m4[3]));
+      const float mx = channel_top(finite_size(T::to((uint16_t)max(top & 0xffffu, top >> 16)))), ms = channel_top(finite_size(m));
+      const float now = mx * unit_S;
+      const bool keep = mx == 0.0f || (now >= 0.5f && now < 16.0f) || (unit_S == 1.0f && now >= 0.5f);
+      float k = keep ? unit_S : scale_for<2, 0, 15>(mx);
+      if (ms > 0x1p100f) k = fminf(k, unit_S);
+      change = k * pow2_inverse(unit_S);
+      unit_S = k;
+      large = __ballot(mx * k >= 256.0f) != 0;
       const uint32_t k16 = F16::from(k);
-      units = k16 | k16 << 16;
-      if (!STATES) read = scale_for<13, -100, 100>(ms), unread = pow2_inverse(read) * iu;
-      unit_S = k, rescale = k * iu;
+      if (__ballot(k != 1.0f) != 0) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+            const int two = xp[ks][i];  // (an element's bits are not cast in place)
+            xp[ks][i] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, two) * __builtin_bit_cast(v2h, k16 | k16 << 16));
+          }
+      }
+      if (!STATES) {
+        // (the accumulators are read before they are folded; what o is formed from is 1 / `old` of it)
+        const bool plain = change == 1.0f && (ms == 0.0f || (ms >= 0x1p-4f && ms < 0x1p15f));
+        read = plain ? 1.0f : scale_for<13, -100, 100>(ms);
+        calm = __ballot(!plain) == 0;
+        if (lane < 32) vunit[wave][lane] = pow2_inverse(unit_S), vunit[wave][32 + lane] = pow2_inverse(read) * change;
+      }
+    }
+    }
+    {
+      // one factor of 2^-160 is zero in 32 bits, and sums of larger ones would cost the tokens behind them their last bits
+      const float e = sv_decay(p.g_same ? same : gbuf[wave][lane]) * kLog2e, one = e < -160.0f ? -160.0f : e;
+      float cs, behind;
+      if (p.g_same) {
+        cs = one * (float)min(lane + 1, rem), behind = one * (float)max(min(rem, Q) - 1 - lane, 0);
+      } else {
+        const float a = lane < rem ? one : 0.0f;
+        cs = sums_upto(a), behind = sums_behind(a, lane);
+      }
+      const float last = lane_of(cs, 63), after = total + last;
+      whole_decay += last;
+      my[lane] = cs;
+      if (!STATES) my[2 * Q + lane] = exp2_fast(cs + total + p.log_scale);
+      const bool now = after < kFloor || (kHalf && large && after < 0.0f);
+      fold = (now ? exp2_fast(after) : 1.0f) * change, total = now ? 0.0f : after, scaled = now || (kHalf && __ballot(change != 1.0f) != 0);
+      my[Q + lane] = lane < rem ? exp2_fast(behind - total) : 0.0f;
     }
   };
   begin(0);
-  // this lane's place in the rows of q and k as operands: row lane & 31, pieces 2 ks + hh; and in k by columns (see `channel`)
   auto k_columns = [&](const char* buf, int lane, int nt, int ks) {
     const int hh = lane >> 5, r4 = (lane & 15) >> 2, nb = (lane >> 4) & 1, p4 = lane & 3;
     lq_v2i o[2];
@@ -384,17 +433,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     }
     return lq_v4i{o[0][0], o[0][1], o[1][0], o[1][1]};
   };
-  // tiles of q . k: columns t of tile tt, rows s of tile st.  Y[0] has the rows of tile ta, Y[1] of the other
+  // tiles of q . k: columns t of tile tt, rows s of tile st.  Y[0] has the columns of tile ta, Y[1] of the other
   const int ta = wave == 0 && W == 4 ? 0 : 1;
   for (int c = 0; c < s.chunks; ++c) {
-    const int lane = fresh(), hh = lane >> 5, col = lane & 31;
     const bool more = c + 1 < s.chunks;
-    meet();  // every wave's share of this chunk's q and k is there (STATES: and the chunk's in front is read)
-    const char* kb = kbuf[STATES ? c & 1 : 0];
-    if (STATES && more) fetch(c + 1);
-    if (more) request(c + 1);
+    meet();  // every wave's share of this chunk's q and k is there, and the chunk in front is read
+    const char* kb = kbuf[c & 1];
+    if (more) {
+      fetch_k(c + 1);
+      fetch_v();  // (v is in registers since `begin`)
+    }
     v16f Y[2];
     if constexpr (!STATES) {
+      const int lane = fresh(), hh = lane >> 5, col = lane & 31;
       v16f P[PT];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -405,60 +456,75 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       // W = 4: waves 0, 1, 2 have (st, tt) = (0, 0), (0, 1), (1, 1), the last one has none.  W = 2: wave 0 (0, 1) and (0, 0), wave 1 (1, 1)
       const int st = W == 4 ? wave == 2 : wave;
       const char *qa = qbuf + ta * 32 * RB, *qz = qbuf + (1 - ta) * 32 * RB, *kx = kb + st * 32 * RB;
-      const int a0 = col * RB + ((hh ^ order<NT>(col)) << 4);
-      lq_v4i q0[3], q1[3], k0[3];
-      auto ask = [&](int ks) {
-        const int o = a0 ^ (ks << 5);
-        q0[ks % 3] = *(const lq_v4i*)(qa + o), q1[ks % 3] = *(const lq_v4i*)(qz + o), k0[ks % 3] = *(const lq_v4i*)(kx + o);
+      const int a0 = col * RB + ((hh ^ order<NT>(col)) << 4);  // row lane & 31, pieces 2 ks + hh
+      auto products = [&](auto plain) {
+        constexpr int R = 2;
+        lq_v4i q0[R], q1[R], k0[R];
+        auto ask = [&](int ks) {
+          const int o = a0 ^ (ks << 5);
+          q0[ks % R] = *(const lq_v4i*)(qa + o), q1[ks % R] = *(const lq_v4i*)(qz + o), k0[ks % R] = *(const lq_v4i*)(kx + o);
+        };
+#pragma unroll
+        for (int ks = 0; ks + 1 < R; ++ks) ask(ks);
+#pragma unroll
+        for (int ks = 0; ks < 2 * NT; ++ks) {
+          if (ks + R - 1 < 2 * NT) ask(ks + R - 1);
+          __builtin_amdgcn_sched_barrier(0);  // (operands of all steps read ahead are registers that it lacks)
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = S[ks >> 1][8 * (ks & 1) + i];
+          lq_v4i sh;
+          if constexpr (decltype(plain)::value) sh = round8<T>(v);
+          else sh = round8<T>(v, read);
+          P[0] = mfma<T>(k0[ks % R], q0[ks % R], P[0]);
+          if constexpr (PT == 2) P[1] = mfma<T>(k0[ks % R], q1[ks % R], P[1]);
+          Y[0] = mfma<T>(sh, q0[ks % R], Y[0]);
+          Y[1] = mfma<T>(sh, q1[ks % R], Y[1]);
+        }
       };
-      ask(0);
-      ask(1);
-#pragma unroll
-      for (int ks = 0; ks < 2 * NT; ++ks) {
-        if (ks + 2 < 2 * NT) ask(ks + 2);
-        __builtin_amdgcn_sched_barrier(0);  // (operands of all steps read ahead are registers that it lacks)
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = S[ks >> 1][8 * (ks & 1) + i];
-        lq_v4i sh;
-        if constexpr (kHalf) sh = round8<T>(v, read);
-        else sh = round8<T>(v);
-        P[0] = mfma<T>(k0[ks % 3], q0[ks % 3], P[0]);
-        if constexpr (PT == 2) P[1] = mfma<T>(k0[ks % 3], q1[ks % 3], P[1]);
-        Y[0] = mfma<T>(q0[ks % 3], sh, Y[0]);
-        Y[1] = mfma<T>(q1[ks % 3], sh, Y[1]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int tt = y == 0 ? ta : 1 - ta;
+      if (!kHalf || calm) {
+        products(std::true_type{});
+      } else if constexpr (kHalf) {
+        products(std::false_type{});
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const lq_v4f e4 = *(const lq_v4f*)(my + 2 * Q + 32 * tt + 8 * j + 4 * hh);
+          const lq_v4f u4 = *(const lq_v4f*)(vunit[wave] + 32 + 8 * j + 4 * hh);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) Y[y][4 * j + e] *= kHalf ? e4[e] * unread : e4[e];
+          for (int e = 0; e < 4; ++e) Y[0][4 * j + e] *= u4[e], Y[1][4 * j + e] *= u4[e];
         }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      {
+        const float ea = my[2 * Q + 32 * ta + col], ez = my[2 * Q + 32 * (1 - ta) + col];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) Y[0][e] *= ea, Y[1][e] *= ez;
       }
       // weighted q . k, rounded, for all of the workgroup's waves
 #pragma unroll
       for (int i = 0; i < PT; ++i) {
         const int tt = i == 0 ? ta : 1 - ta;
         if ((W == 4 && wave == 3) || (W == 2 && i == 1 && wave == 1)) continue;
-        const float ct = my[32 * tt + col];
+        const float ct = my[32 * tt + col] + p.log_scale;
         float w[16], m = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const lq_v4f c4 = *(const lq_v4f*)(my + 32 * st + 8 * j + 4 * hh);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float f = P[i][4 * j + e] * (exp2_fast(ct - c4[e]) * p.scale);
-            w[4 * j + e] = st == tt && 8 * j + 4 * hh + e > col ? 0.0f : f;
-            if (kHalf) m = fmaxf(m, finite_size(w[4 * j + e]));
+            w[4 * j + e] = P[i][4 * j + e] * exp2_fast(ct - c4[e]);
           }
         }
+        if (st == tt) {  // nothing of tokens behind the column's
+          const int t = col - 4 * hh;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = 8 * (e >> 2) + (e & 3) > t ? 0.0f : w[e];
+        }
         if constexpr (kHalf) {
-          m = channel_top(m);
-          const bool plain = m == 0.0f || (m >= 0x1p-5f && m < 0x1p15f);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(w[e]));
+          // (a column with an infinity or a NaN is none whatever its unit)
+          m = channel_top(finite_size(m));
+          const bool plain = m == 0.0f || (m >= 0x1p-8f && m < 0x1p15f);
           const float u = plain ? 1.0f : scale_for<13, -100, 100>(m);
           const bool odd = __ballot(!plain) != 0;
           if (lane == 0) podd[2 * tt + st] = odd;
@@ -476,80 +542,84 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           *(lq_v4i*)(pbuf + (4 * tt + 2 * st + k2) * 1024 + lane * 16) = round8<T>(v);
         }
       }
+      meet();  // every wave has read the chunk's q, and the weighted q . k is there
+      if (more) fetch_q();
     }
     // the state behind the chunk
-    const int kl = fresh();
-    const float f = kHalf ? all * rescale : all;
+    if (scaled) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) S[nt][e] *= f;
+        for (int e = 0; e < 16; ++e) S[nt][e] *= fold;
+    }
     __builtin_amdgcn_sched_barrier(0);
     {
+      const int kl = fresh(), hh = kl >> 5;
       constexpr int N = kHalf ? 2 : 3;
-      lq_v4i kt[3], w[N];
+      lq_v4i kt[3], w[2][N];
       lq_v4f w4[2][2];
       auto ask = [&](int i) { kt[i % 3] = k_columns(kb, kl, i % NT, i / NT); };  // operand i = NT ks + nt
       auto ask_w = [&](int ks) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) w4[ks & 1][j] = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh);
       };
+      auto pair = [&](int ks, int q) {  // a quarter of step ks' weighted v
+        const lq_v4f& f = w4[ks & 1][q >> 1];
+        int o[3];
+        split2<T>(f[2 * (q & 1)], x(ks, 2 * q), f[2 * (q & 1) + 1], x(ks, 2 * q + 1), o);
+#pragma unroll
+        for (int n = 0; n < N; ++n) w[ks & 1][n][q] = o[n];
+      };
       ask_w(0);
       ask(0);
       ask(1);
+      ask_w(1);
       reads_stay();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) pair(0, q);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int i = NT * ks + nt;
           if (i + 2 < 4 * NT) ask(i + 2);
-          if (nt == NT - 1 && ks < 3) ask_w(ks + 1);
-          reads_stay();
-          if (nt == 0) {
+          if (nt == NT - 1 && ks < 2) ask_w(ks + 2);
+          __builtin_amdgcn_sched_barrier(0);
+          // (the next step's weighted v is formed between these products: one issued behind another of the same tile waits for it)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const lq_v4f& f = w4[ks & 1][q >> 1];
-              float x0 = x(ks, 2 * q), x1 = x(ks, 2 * q + 1);
-              if constexpr (kHalf) {
-                typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-                const int two = xp[ks][q];  // (an element's bits are not cast in place)
-                const v2h x2 = __builtin_bit_cast(v2h, two) * __builtin_bit_cast(v2h, units);
-                x0 = (float)x2[0], x1 = (float)x2[1];
-              }
-              int o[3];
-              split2<T>(f[2 * (q & 1)], x0, f[2 * (q & 1) + 1], x1, o);
+          for (int n = 0; n < N; ++n) {
+            S[nt] = mfma<T>(kt[i % 3], w[ks & 1][n], S[nt]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (ks < 3) {
 #pragma unroll
-              for (int n = 0; n < N; ++n) w[n][q] = o[n];
+              for (int q = 0; q < 4; ++q)
+                if (q * NT * N / 4 == nt * N + n) pair(ks + 1, q);
+              __builtin_amdgcn_sched_barrier(0);
             }
           }
-#pragma unroll
-          for (int n = 0; n < N; ++n) S[nt] = mfma<T>(kt[i % 3], w[n], S[nt]);
         }
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!STATES) {
-      arrived();  // (requested at the chunk's beginning)
-      meet();     // every wave has read the chunk's q and k, and the weighted q . k is there
-      if (more) fetch(c + 1);
       bool four = false;  // whether this wave has stored four times
       if (live) {
         const int lane = fresh(), hh = lane >> 5, col = lane & 31;
         // A v that is no number must not reach the tokens in front of it, which the product below multiplies by zero: the state, which all of
-        // the chunk's tokens reach, tells.  Then such tokens are left out and every output from them on is NaN.
+        // the chunk's tokens reach, tells.  Then such tokens are left out and every output of the channel from them on is NaN.
         const bool odd = bad || __ballot(S[0][0] != S[0][0]) != 0;
-        int from = bad ? -4 : Q;  // counted from token 4 hh, as this lane's entries are
+        int from = bad ? 0 : Q;  // of this lane's channel
         if (odd) {
+          asm volatile("");  // (not to be computed ahead)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               if (!(__builtin_fabsf(x(ks, i)) < __builtin_inff())) {
-                from = min(from, entry(ks, 0, i));
+                from = min(from, entry(ks, hh, i));
                 xp[ks][i >> 1] &= i & 1 ? 0xffff : 0xffff0000;
               }
-          from = min(from, __shfl_xor(from, 32, 64) + (hh ? -4 : 4));
+          from = min(from, __shfl_xor(from, 32, 64));
         }
         bool apart = false;
         if constexpr (kHalf) apart = uniform(podd[0] | podd[2] | podd[3]) != 0;
@@ -558,75 +628,76 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) Y[y] = mfma<T>(weighted(y == 0 ? ta : 1 - ta, ks), xp[ks], Y[y]);
-        } else if constexpr (kHalf) {  // units of their own for the rows of a tile
+            for (int y = 0; y < 2; ++y) Y[y] = mfma<T>(xp[ks], weighted(y == 0 ? ta : 1 - ta, ks), Y[y]);
+        } else if constexpr (kHalf) {  // units of their own for the columns of a tile
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const int tt = y == 0 ? ta : 1 - ta;
             for (int st = 0; st <= tt; ++st) {
               v16f d = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-              d = mfma<T>(weighted(tt, 2 * st), st ? xp[2] : xp[0], d);
-              d = mfma<T>(weighted(tt, 2 * st + 1), st ? xp[3] : xp[1], d);
+              d = mfma<T>(st ? xp[2] : xp[0], weighted(tt, 2 * st), d);
+              d = mfma<T>(st ? xp[3] : xp[1], weighted(tt, 2 * st + 1), d);
               sv_settle(d);
-              const bool own = podd[2 * tt + st] != 0;
+              const float u = podd[2 * tt + st] ? punit[(2 * tt + st) * 32 + col] : 1.0f;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const lq_v4f u4 = *(const lq_v4f*)(punit + (2 * tt + st) * 32 + 8 * j + 4 * hh);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) Y[y][4 * j + e] = __builtin_fmaf(d[4 * j + e], own ? u4[e] : 1.0f, Y[y][4 * j + e]);
-              }
+              for (int e = 0; e < 16; ++e) Y[y][e] = __builtin_fmaf(d[e], u, Y[y][e]);
             }
           }
         }
-        if (odd) {
+        sv_settle(Y[0]), sv_settle(Y[1]);
+        if (odd) {  // (channel of register e: entry(e / 8, hh, e % 8))
+          asm volatile("");
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
+          for (int e = 0; e < 16; ++e) {
+            const int f = __shfl(from, entry(e >> 3, hh, e & 7), 64);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (32 * (y == 0 ? ta : 1 - ta) + entry(e >> 3, 0, e & 7) >= from) Y[y][e] = __builtin_nanf("");
+            for (int y = 0; y < 2; ++y)
+              if (32 * (y == 0 ? ta : 1 - ta) + col >= f) Y[y][e] = __builtin_nanf("");
+          }
         }
-        // Out through the place of v (the wave's own, and in registers since the chunk's beginning): [channel][block of four tokens], block b
-        // at place b ^ channel % 16, and back by columns, 16 tokens of eight channels a lane.
-        char* yw = (char*)vbuf[c & 1][wave];
-        const uint32_t y0 = (uint32_t)(col * 128 + ((hh ^ (col & 15)) * 8));
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint32_t yt = y0 ^ (uint32_t)(64 * (y == 0 ? ta : 1 - ta));
+        if constexpr (kHalf) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sv_v4u o;
+            const lq_v4f u4 = *(const lq_v4f*)(vunit[wave] + 8 * j + 4 * hh);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = T::from(Y[y][4 * j + i]);
-            *(sv_v4u*)(yw + (yt ^ (16 * j))) = o;
+            for (int e = 0; e < 4; ++e) Y[0][4 * j + e] *= u4[e], Y[1][4 * j + e] *= u4[e];
           }
         }
-        lq_v4i yo[4];
-        {
-          const int q8 = 8 * (lane >> 4) + ((lane & 15) >> 2);  // channels q8 and q8 + 4 of this lane's pieces
-          const uint32_t b0 = (uint32_t)(q8 * 128 + (((lane & 3) ^ (q8 & 15)) * 8)), b1 = (uint32_t)((q8 + 4) * 128 + (((lane & 3) ^ ((q8 + 4) & 15)) * 8));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const lq_v2i lo = read_columns(yw + (b0 ^ (32 * i))), hi = read_columns(yw + (b1 ^ (32 * i)));
-            yo[i] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
-          }
-        }
+        // A lane has four channels of eight, the other half of the wave the other four: with every second eight exchanged it has whole eights.
         const int rem = s.len - (s.chunk0 + c) * Q;
-        uint16_t* oc = os + (int64_t)(s.chunk0 + c) * Q * ostride;
-        const uint32_t o0 = (uint32_t)(lane & 15) * (uint32_t)ostride + 8 * (lane >> 4);
         four = rem >= Q && ch0 + 32 <= p.V;
-        if (four) {
+        uint16_t* oc = os + (int64_t)c * Q * ostride;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
-        } else {
+        for (int y = 0; y < 2; ++y) {
+          const int tt = y == 0 ? ta : 1 - ta;
+          float a[8], z[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (16 * i + (lane & 15) < rem && ch0 + 8 * (lane >> 4) < p.V) *(lq_v4i*)(oc + 16 * i * ostride + o0) = yo[i];
+          for (int e = 0; e < 8; ++e) a[e] = Y[y][e], z[e] = Y[y][8 + e];
+          lq_v4i two[2] = {round8<T>(a), round8<T>(z)};
+          if (p.negative) {
+            const int sign = (int)0x80008000u;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) two[0][q] ^= sign, two[1][q] ^= sign;
+          }
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const auto r0 = __builtin_amdgcn_permlane32_swap((uint32_t)two[k2][0], (uint32_t)two[k2][2], false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap((uint32_t)two[k2][1], (uint32_t)two[k2][3], false, false);
+            const lq_v4i o = {(int)r0[0], (int)r1[0], (int)r0[1], (int)r1[1]};
+            const int t = 32 * tt + col, n = 16 * k2 + 8 * hh;
+            uint16_t* to = oc + (uint32_t)t * (uint32_t)ostride + n;
+            if (four) *(lq_v4i*)to = o;
+            else if (t < rem && ch0 + n < p.V) *(lq_v4i*)to = o;
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (more) begin(c + 1);
-      if (four) all_but_stores();
+      // Memory operations end in order: v and the decays, requested at the chunk's beginning, are in front of q and the stores.
+      const bool counted = four && whole;
+      if (counted) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kFetch + 4) : "memory");
       else arrived();
+      if (more) begin(c + 1);
+      if (counted) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     } else {
       arrived();
       if (more) begin(c + 1);
@@ -636,16 +707,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   for (int nt = 0; nt < NT; ++nt) sv_settle(S[nt]);
   float* dst = STATES ? p.seg_state + (int64_t)sg * p.H * p.K * p.V + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
   if (dst && ch < p.V) {
-    const float ui = kHalf ? 1.0f / unit_S : 1.0f;
+    const float ui = exp2_fast(total) * (kHalf ? pow2_inverse(unit_S) : 1.0f);
+    if (whole) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = channel(nt, hh, r);
-        if (n < p.K) dst[(int64_t)n * p.V] = kHalf ? S[nt][r] * ui : S[nt][r];
-      }
+        for (int r = 0; r < 16; ++r) dst[channel(nt, hh, r) * (int64_t)p.V] = S[nt][r] * ui;
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (channel(nt, hh, r) < p.K) dst[channel(nt, hh, r) * (int64_t)p.V] = S[nt][r] * ui;
+    }
   }
-  if (STATES && threadIdx.x == 0 && part == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(total);
+  if (STATES && threadIdx.x == 0 && part == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(whole_decay);
 }
 
 // The state in front of each segment, in the place of what it adds to one.  A workgroup has 1024 entries of one head's state.
@@ -758,21 +834,21 @@ extern "C" int lq_linear_attention_prompt(const lq_linear_attention_prompt_args*
   if (!a || !a->q || !a->k || !a->v || !a->out) return LQ_ERR_NULL;
   const int rc = check_dims(a);
   if (rc != LQ_OK) return rc;
-  if ((a->g && !sv_float(a->g_dtype)) || (a->state && a->num_slots <= 0)) return LQ_ERR_SHAPE;
-  for (const int64_t s : {a->q_stride_l, a->k_stride_l, a->v_stride_l})
+  if (a->state && a->num_slots <= 0) return LQ_ERR_SHAPE;
+  for (const int64_t s : {a->q_stride_l, a->k_stride_l, a->v_stride_l, a->g_stride_l})
     if (s < 0 || s >= 1 << 24) return LQ_ERR_SHAPE;  // a chunk's rows are reached by 32-bit offsets
   for (const int64_t s : {a->q_stride_b, a->q_stride_l, a->q_stride_h, a->k_stride_b, a->k_stride_l, a->k_stride_h, a->v_stride_b, a->v_stride_l, a->v_stride_h})
     if (s % 8 != 0) return LQ_ERR_SHAPE;
   if (!sv_al(a->q, 16) || !sv_al(a->k, 16) || !sv_al(a->v, 16) || !sv_al(a->out, 16) || !sv_al(a->state, 16) || a->state_stride_s % 4 != 0 ||
-      (a->g && !sv_al(a->g, sv_size(a->g_dtype))) || !sv_al(a->slots, 4) || !sv_al(a->seq_starts, 4))
+      !sv_al(a->g, 4) || !sv_al(a->slots, 4) || !sv_al(a->seq_starts, 4))
     return LQ_ERR_SHAPE;
   Plan pl;
   if (!plan(a, pl) || a->workspace_bytes < pl.bytes || !sv_al(a->workspace, 256)) return LQ_ERR_SHAPE;
   if (pl.bytes && !a->workspace) return LQ_ERR_NULL;
   char* ws = (char*)a->workspace;
   PromptParams p = {(const uint16_t*)a->q, a->q_stride_b, a->q_stride_l, a->q_stride_h, (const uint16_t*)a->k, a->k_stride_b, a->k_stride_l, a->k_stride_h,
-                    (const uint16_t*)a->v, a->v_stride_b, a->v_stride_l, a->v_stride_h, a->g, a->g_stride_b, a->g_stride_l, a->g_stride_h, a->g_dtype,
-                    !a->g || (a->g_stride_b == 0 && a->g_stride_l == 0), a->scale, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots, a->seq_starts,
+                    (const uint16_t*)a->v, a->v_stride_b, a->v_stride_l, a->v_stride_h, a->g, a->g_stride_b, a->g_stride_l, a->g_stride_h,
+                    !a->g || (a->g_stride_b == 0 && a->g_stride_l == 0), std::log2(std::fabs(a->scale)), a->scale < 0.0f, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots, a->seq_starts,
                     a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->kdim, a->vdim, pl.cut ? (float*)ws : nullptr,
                     pl.cut ? (float*)(ws + pl.decays) : nullptr, (int)pl.segs, pl.seg_chunks, pl.parts};
   auto grid_of = [&](int64_t segs) { return dim3((unsigned)((segs * a->nheads * pl.parts + 7) / 8 * 8)); };

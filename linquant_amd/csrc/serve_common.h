@@ -117,6 +117,13 @@ LQ_DEV void sv_fetch16(const void* base, uint32_t offset, const void* at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
+// 4 bytes a lane likewise
+LQ_DEV void sv_fetch4(const void* base, uint32_t offset, const void* at) {
+  typedef const __attribute__((address_space(3))) char lds_char;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)at;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+
 // Matrix results that a loop of run-time length leaves are read behind this.  The vector unit may read a result some cycles after its product
 // was issued, which the compiler has to see to; where the last product stands in front of a branch out of the loop it did not (ROCm 7.2: no
 // waits in front of the first reads, and old values there).

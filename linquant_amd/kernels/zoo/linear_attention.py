@@ -26,7 +26,7 @@ def _check(q, k, v, g, scale, lead):
     assert g is None or (g.dtype in _FLOAT and g.shape in ((H,), (*lead, H))), f"g: {(H,)} or {(*lead, H)}, got {None if g is None else tuple(g.shape)}"
     _lib.below_2_31(*q.shape, V)
     _lib.same_device(q, k, v, g)
-    return dict(dtype=_ACT[v.dtype], g=_lib.ptr(g), g_dtype=0 if g is None else _FLOAT[g.dtype], scale=float(K ** -0.5 if scale is None else scale),
+    return dict(dtype=_ACT[v.dtype], scale=float(K ** -0.5 if scale is None else scale),
                 nheads=H, kdim=K, vdim=V)
 
 
@@ -81,12 +81,15 @@ def linear_attention_prompt(q, k, v, g=None, *, scale=None, state=None, slots=No
         return out
     st = lambda t: (0, *t.stride()) if packed else t.stride()  # noqa: E731
     qs, ks, vs = st(q), st(k), st(v)
+    g = _lib.f32(g)
+    if g is not None and g.dim() > 1 and not 0 <= g.stride(-2) < 1 << 24:
+        g = g.contiguous()
     gs = (0, 0, 0) if g is None else (0, 0, g.stride(0)) if g.dim() == 1 else st(g)
     nbytes = prompt_workspace_bytes(n, L, T, packed, H, K, V, fields["dtype"])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=v.device) if nbytes else None
     _lib.call("lq_linear_attention_prompt", v.device, q=_lib.ptr(q), q_stride_b=qs[0], q_stride_l=qs[1], q_stride_h=qs[2], k=_lib.ptr(k),
               k_stride_b=ks[0], k_stride_l=ks[1], k_stride_h=ks[2], v=_lib.ptr(v), v_stride_b=vs[0], v_stride_l=vs[1], v_stride_h=vs[2],
-              g_stride_b=gs[0], g_stride_l=gs[1], g_stride_h=gs[2], out=_lib.ptr(out), state=_lib.ptr(state),
+              g=_lib.ptr(g), g_stride_b=gs[0], g_stride_l=gs[1], g_stride_h=gs[2], out=_lib.ptr(out), state=_lib.ptr(state),
               state_stride_s=0 if state is None else state.stride(0), slots=_lib.ptr(slots if state is not None else None),
               seq_starts=_lib.ptr(seq_starts), num_slots=num_slots, nseq=n, seqlen=L, tokens=T, workspace=_lib.ptr(ws), workspace_bytes=nbytes,
               **fields)
@@ -108,7 +111,8 @@ def linear_attention_step(state, q, k, v, g=None, *, scale=None, slots=None):
     if n and H and V:
         gs = (0, 0) if g is None else (0, g.stride(0)) if g.dim() == 1 else g.stride()
         _lib.call("lq_linear_attention_step", v.device, q=_lib.ptr(q), q_stride_b=q.stride(0), q_stride_h=q.stride(1), k=_lib.ptr(k), k_stride_b=k.stride(0),
-                  k_stride_h=k.stride(1), v=_lib.ptr(v), v_stride_b=v.stride(0), v_stride_h=v.stride(1), g_stride_b=gs[0], g_stride_h=gs[1],
+                  k_stride_h=k.stride(1), v=_lib.ptr(v), v_stride_b=v.stride(0), v_stride_h=v.stride(1), g=_lib.ptr(g),
+                  g_dtype=0 if g is None else _FLOAT[g.dtype], g_stride_b=gs[0], g_stride_h=gs[1],
                   out=_lib.ptr(out), state=_lib.ptr(state), state_stride_s=state.stride(0), slots=_lib.ptr(slots), num_slots=state.shape[0],
                   batch=n, **fields)
     return out

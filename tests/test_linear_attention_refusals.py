@@ -129,7 +129,7 @@ def test_entry_points_refuse():
         assert rc("lq_linear_attention_step", **{**step, **bad}) == -22, bad
     prompt = dict(q=16, k=16, v=16, out=16, dtype=0, nseq=1, seqlen=5, nheads=1, kdim=8, vdim=8)
     for bad in (dict(kdim=264), dict(kdim=12), dict(vdim=12), dict(nheads=70000), dict(nheads=2, vdim=1 << 23), dict(q=8), dict(q_stride_l=1 << 24), dict(v_stride_h=4), dict(seqlen=0),
-                dict(state=16, num_slots=0), dict(g=16, g_dtype=2)):
+                dict(state=16, num_slots=0), dict(g=18), dict(g=16, g_stride_l=-1)):
         assert rc("lq_linear_attention_prompt", **{**prompt, **bad}) == -22, bad
     norm = dict(x=16, out=16, dtype=0, rows=1, dim=8, num_groups=1)
     for bad in (dict(num_groups=3), dict(dim=16385), dict(act=3), dict(dtype=1), dict(weight=16, weight_dtype=2), dict(rows=0)):
