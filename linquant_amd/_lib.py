@@ -17,7 +17,9 @@ BINDING_PATH = ROOT / "_binding.so"
 _NATIVE_ENTRIES = ("lq_zoo_simple_gla", "lq_zoo_simple_gla_workspace_bytes", "lq_zoo_chunk_forward",
                    "lq_zoo_chunk_forward_workspace_bytes", "lq_zoo_rotate_qkv", "lq_split_rotate_quant_xBC", "lq_ssd_combined",
                    "lq_ssd_combined_workspace_bytes", "lq_quantize_rows", "lq_int8_matmul", "lq_residual_rmsnorm", "lq_conv1d_prompt",
-                   "lq_conv1d_step", "lq_ssm_prompt", "lq_ssm_prompt_workspace_bytes", "lq_ssm_step", "lq_abi_version", "lq_args_size")
+                   "lq_conv1d_step", "lq_ssm_prompt", "lq_ssm_prompt_workspace_bytes", "lq_ssm_step", "lq_linear_attention_prompt",
+                   "lq_linear_attention_prompt_workspace_bytes", "lq_linear_attention_step", "lq_groupnorm_gated", "lq_adapter_down", "lq_copy_slots",
+                   "lq_abi_version", "lq_args_size")
 ABI_VERSION = 23
 
 LQ_DT_F16, LQ_DT_F32, LQ_DT_I8, LQ_DT_BF16 = 0, 1, 2, 3

@@ -21,8 +21,11 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
+#include <utility>
+#include <vector>
 
 #include "../../include/linquant_hip.h"
 
@@ -45,6 +48,12 @@ decltype(&lq_conv1d_step) conv_step_entry;
 decltype(&lq_ssm_prompt) ssm_prompt_entry;
 decltype(&lq_ssm_prompt_workspace_bytes) ssm_prompt_bytes;
 decltype(&lq_ssm_step) ssm_step_entry;
+decltype(&lq_linear_attention_prompt) attention_prompt_entry;
+decltype(&lq_linear_attention_prompt_workspace_bytes) attention_prompt_bytes;
+decltype(&lq_linear_attention_step) attention_step_entry;
+decltype(&lq_groupnorm_gated) groupnorm_entry;
+decltype(&lq_adapter_down) adapter_down_entry;
+decltype(&lq_copy_slots) copy_slots_entry;
 PyObject* raise_failed;
 
 using at::ScalarType;
@@ -723,6 +732,261 @@ PyObject* ssm_prompt(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// what both forms of linear attention take: q, k, v with `lead` token dimensions, decays for each head or each token, a state
+struct Attention {
+  Tensor q, k, v, g, state, slots;
+  double scale = 0.0;
+  int64_t H = 0, K = 0, V = 0;
+};
+bool attention_operands(PyObject* const* arg, const c10::Device& dev, int lead, Attention& a) {  // arg = q, k, v, g, scale, state, slots
+  if (!plain(arg[0], dev, a.q) || !plain(arg[1], dev, a.k) || !plain(arg[2], dev, a.v) || !optional(arg[3], dev, a.g) || !(arg[4] == Py_None || number(arg[4], a.scale)) ||
+      !plain(arg[5], dev, a.state) || !optional(arg[6], dev, a.slots))
+    return false;
+  const Tensor &q = a.q, &k = a.k, &v = a.v, &g = a.g, &st = a.state;
+  if (v.dim() != lead + 2 || q.dim() != lead + 2 || !act16(v) || q.scalar_type() != v.scalar_type() || k.scalar_type() != v.scalar_type() || !rows16(q) || !rows16(k) || !rows16(v)) return false;
+  a.H = v.size(lead), a.K = q.size(lead + 1), a.V = v.size(lead + 1);
+  if (k.sizes() != q.sizes() || a.K % 8 != 0 || a.K > 256 || a.V % 8 != 0) return false;
+  for (int i = 0; i <= lead; ++i)
+    if (q.size(i) != v.size(i)) return false;
+  for (const Tensor* t : {&q, &k, &v})
+    if (t->stride(lead - 1) < 0 || t->stride(lead - 1) >= 1 << 24) return false;
+  if (g.defined()) {
+    if (g.scalar_type() != ScalarType::Float || !(g.dim() == 1 || g.dim() == lead + 1) || !fits(g.sizes()) || g.size(-1) != a.H) return false;
+    for (int i = 0; g.dim() > 1 && i < lead; ++i)
+      if (g.size(i) != v.size(i)) return false;
+    if (g.dim() > 1 && (g.stride(-2) < 0 || g.stride(-2) >= 1 << 24)) return false;
+  }
+  if (arg[4] == Py_None) a.scale = std::pow((double)a.K, -0.5);
+  return st.dim() == 4 && st.scalar_type() == ScalarType::Float && fits(st.sizes()) && st.size(1) == a.H && st.size(2) == a.K && st.size(3) == a.V && st.stride(3) == 1 &&
+         st.stride(2) == a.V && st.stride(1) == a.K * a.V && st.stride(0) % 4 == 0 && aligned(st);
+}
+template <typename Args>
+void attention_args(const Attention& s, Args& a) {
+  a.q = s.q.const_data_ptr(), a.k = s.k.const_data_ptr(), a.v = s.v.const_data_ptr(), a.dtype = code(s.v.scalar_type()), a.g = f32(s.g), a.scale = (float)s.scale;
+  a.state = (float*)s.state.data_ptr(), a.state_stride_s = s.state.stride(0), a.slots = i32(s.slots), a.num_slots = (int)s.state.size(0);
+  a.nheads = (int)s.H, a.kdim = (int)s.K, a.vdim = (int)s.V;
+}
+
+// linear_attention_step(q, k, v, g, scale, state, slots)
+PyObject* linear_attention_step(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Attention s;
+  Tensor out;
+  if (!device_of(arg[0], dev) || !attention_operands(arg, dev, 1, s)) Py_RETURN_NONE;
+  const int64_t B = s.v.size(0);
+  if (B > 65535 || !slots_of(s.slots, B, s.state)) Py_RETURN_NONE;
+  lq_linear_attention_step_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(s.v.sizes(), s.v.scalar_type(), dev);
+    attention_args(s, a);
+    a.q_stride_b = s.q.stride(0), a.q_stride_h = s.q.stride(1), a.k_stride_b = s.k.stride(0), a.k_stride_h = s.k.stride(1);
+    a.v_stride_b = s.v.stride(0), a.v_stride_h = s.v.stride(1);
+    a.g_dtype = LQ_DT_F32, a.g_stride_b = s.g.defined() && s.g.dim() == 2 ? s.g.stride(0) : 0, a.g_stride_h = s.g.defined() ? s.g.stride(-1) : 0;
+    a.out = out.data_ptr(), a.batch = (int)B;
+    rc = attention_step_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_linear_attention_step", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_attention_prompt(q, k, v, g, scale, state, slots, seq_starts), with a state
+PyObject* linear_attention_prompt(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Attention s;
+  Tensor starts, out;
+  if (!device_of(arg[0], dev) || !optional(arg[7], dev, starts)) Py_RETURN_NONE;
+  const bool packed = starts.defined();
+  if (!attention_operands(arg, dev, packed ? 1 : 2, s)) Py_RETURN_NONE;
+  if (packed && (starts.dim() != 1 || starts.size(0) < 2 || !list32(starts, starts.size(0)))) Py_RETURN_NONE;
+  const int64_t seqs = packed ? starts.size(0) - 1 : s.v.size(0);
+  if (seqs > INT_MAX || !slots_of(s.slots, seqs, s.state)) Py_RETURN_NONE;
+  lq_linear_attention_prompt_args a = {};
+  attention_args(s, a);
+  const int l = packed ? 0 : 1;
+  auto batch = [&](const Tensor& t) { return packed ? 0 : t.stride(0); };
+  a.q_stride_b = batch(s.q), a.q_stride_l = s.q.stride(l), a.q_stride_h = s.q.stride(l + 1);
+  a.k_stride_b = batch(s.k), a.k_stride_l = s.k.stride(l), a.k_stride_h = s.k.stride(l + 1);
+  a.v_stride_b = batch(s.v), a.v_stride_l = s.v.stride(l), a.v_stride_h = s.v.stride(l + 1);
+  if (s.g.defined()) {
+    if (s.g.dim() > 1) a.g_stride_b = batch(s.g), a.g_stride_l = s.g.stride(l);
+    a.g_stride_h = s.g.stride(-1);
+  }
+  a.seq_starts = i32(starts), a.nseq = (int)seqs, a.seqlen = packed ? 0 : (int)s.v.size(1), a.tokens = packed ? (int)s.v.size(0) : 0;
+  int64_t bytes = 0;
+  if (attention_prompt_bytes(&a, &bytes) != 0) Py_RETURN_NONE;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(s.v.sizes(), s.v.scalar_type(), dev);
+    Tensor ws;
+    if (bytes) ws = empty({bytes}, ScalarType::Byte, dev);
+    a.out = out.data_ptr(), a.workspace = bytes ? ws.data_ptr() : nullptr, a.workspace_bytes = bytes;
+    rc = attention_prompt_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_linear_attention_prompt", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// groupnorm_gated(x, z, weight, bias, num_groups, eps, act): dense rows, weights of one type
+PyObject* groupnorm_gated(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, z, w, b, out;
+  int64_t groups, act;
+  double eps;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !optional(arg[1], dev, z) || !optional(arg[2], dev, w) || !optional(arg[3], dev, b) || !integer(arg[4], groups) ||
+      !number(arg[5], eps) || !integer(arg[6], act))
+    Py_RETURN_NONE;
+  if (!act16(x) || x.dim() < 1 || !fits(x.sizes()) || !x.is_contiguous()) Py_RETURN_NONE;
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  if (rows > INT_MAX || groups < 1 || D % groups != 0 || D / groups > 16384) Py_RETURN_NONE;
+  if (z.defined() && (z.scalar_type() != x.scalar_type() || z.sizes() != x.sizes() || !z.is_contiguous())) Py_RETURN_NONE;
+  for (const Tensor* t : {&w, &b})
+    if (t->defined() && (!floats(*t) || t->dim() != 1 || t->size(0) != D || !t->is_contiguous())) Py_RETURN_NONE;
+  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) Py_RETURN_NONE;
+  lq_groupnorm_gated_args a = {};
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty(x.sizes(), x.scalar_type(), dev);
+    a.x = x.const_data_ptr(), a.x_stride = D, a.z = at(z), a.z_stride = z.defined() ? D : 0, a.dtype = code(x.scalar_type()), a.weight = at(w), a.bias = at(b);
+    a.weight_dtype = w.defined() ? code(w.scalar_type()) : (b.defined() ? code(b.scalar_type()) : 0), a.out = out.data_ptr(), a.eps = (float)eps;
+    a.rows = (int)rows, a.dim = (int)D, a.num_groups = (int)groups, a.act = (int)act;
+    rc = groupnorm_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_groupnorm_gated", rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// adapted(x, scale, weight, weight_scale, bias, out_dtype, down, up, scaling, ids): a W8A8Linear with low-rank adapters.  x (..., K) in the
+// adapters' type and scale None: quantized row by row here; or INT8 codes and their scale, one or one for each row
+PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor x, xs, w, ws, bias, down, up, scaling, ids, codes, h, out;
+  if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !optional(arg[1], dev, xs) || !plain(arg[2], dev, w) || !plain(arg[3], dev, ws) || !optional(arg[4], dev, bias) ||
+      !plain(arg[6], dev, down) || !plain(arg[7], dev, up) || !plain(arg[8], dev, scaling) || !plain(arg[9], dev, ids))
+    Py_RETURN_NONE;
+  if (!THPDtype_Check(arg[5])) Py_RETURN_NONE;
+  const ScalarType ot = ((THPDtype*)arg[5])->scalar_type;
+  if (ot != ScalarType::Half && ot != ScalarType::BFloat16 && ot != ScalarType::Float) Py_RETURN_NONE;
+  const bool coded = xs.defined();
+  if (x.dim() < 1 || !fits(x.sizes()) || !x.is_contiguous() || !aligned(x) || w.dim() != 2 || w.scalar_type() != ScalarType::Char || !fits(w.sizes()) || !w.is_contiguous() || !aligned(w)) Py_RETURN_NONE;
+  const int64_t K = x.size(-1), M = x.numel() / K, N = w.size(0);
+  if (K % 16 != 0 || K > 16384 || w.size(1) != K || M > INT_MAX || K >= 1 << 23) Py_RETURN_NONE;
+  if (!act16(down) || x.scalar_type() != (coded ? ScalarType::Char : down.scalar_type()) || up.scalar_type() != down.scalar_type() || down.dim() != 3 || up.dim() != 3 || !fits(down.sizes()) ||
+      !fits(up.sizes()) || !down.is_contiguous() || !up.is_contiguous() || !aligned(down) || !aligned(up))
+    Py_RETURN_NONE;
+  const int64_t count = down.size(0), R = down.size(1);
+  if (R % 16 != 0 || R > 128 || down.size(2) != K || up.size(0) != count || up.size(1) != N || up.size(2) != R || !table(scaling, count)) Py_RETURN_NONE;
+  if (ids.scalar_type() != ScalarType::Int || !ids.is_contiguous() || ids.numel() != M || ids.sizes() != x.sizes().slice(0, x.dim() - 1)) Py_RETURN_NONE;
+  if (coded && (xs.scalar_type() != ScalarType::Float || !xs.is_contiguous() || (xs.numel() != 1 && xs.numel() != M))) Py_RETURN_NONE;
+  if (ws.scalar_type() != ScalarType::Float || !ws.is_contiguous() || ws.numel() != N) Py_RETURN_NONE;
+  if (bias.defined() && (!floats(bias) || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous())) Py_RETURN_NONE;
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  lq_quantize_rows_args q = {};
+  lq_adapter_down_args d = {};
+  lq_int8_matmul_args a = {};
+  const char* what = "lq_quantize_rows";
+  int rc = 0;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const hipStream_t stream = stream_of(dev);
+    out = empty(sizes, ot, dev), h = empty({M, R}, ScalarType::Float, dev);
+    if (!coded) {
+      codes = empty({M, K}, ScalarType::Char, dev), xs = empty({M}, ScalarType::Float, dev);
+      q.x = x.const_data_ptr(), q.x_stride = K, q.dtype = code(x.scalar_type()), q.codes = (int8_t*)codes.data_ptr(), q.codes_stride = K, q.scale = (float*)xs.data_ptr();
+      q.rows = (int)M, q.cols = (int)K;
+      rc = quantize_entry(&q, stream);
+    }
+    if (rc == 0) {
+      what = "lq_adapter_down";
+      d.x = x.const_data_ptr(), d.x_stride = K, d.x_dtype = coded ? LQ_DT_I8 : code(x.scalar_type()), d.x_scale = coded ? f32(xs) : nullptr, d.x_scale_rows = xs.numel() != 1;
+      d.down = down.const_data_ptr(), d.dtype = code(down.scalar_type()), d.scaling = f32(scaling), d.ids = i32(ids), d.h = (float*)h.data_ptr();
+      d.rows = (int)M, d.inner = (int)K, d.inner_padded = (int)K, d.rank = (int)R, d.count = (int)count;
+      rc = adapter_down_entry(&d, stream);
+    }
+    if (rc == 0) {
+      what = "lq_int8_matmul";
+      a.a = (const int8_t*)(coded ? x : codes).const_data_ptr(), a.a_stride = K, a.b = (const int8_t*)w.const_data_ptr(), a.b_stride = K;
+      a.a_scale = f32(xs), a.b_scale = f32(ws), a.a_scale_rows = xs.numel() != 1 || !coded, a.b_scale_cols = 1;
+      a.bias = at(bias), a.bias_dtype = bias.defined() ? code(bias.scalar_type()) : 0;
+      a.out = out.data_ptr(), a.out_stride = N, a.out_dtype = code(ot), a.rows = (int)M, a.cols = (int)N, a.inner = (int)K;
+      a.adapter_h = f32(h), a.adapter_ids = i32(ids), a.adapter_up = up.const_data_ptr(), a.adapter_dtype = code(up.scalar_type()), a.adapter_rank = (int)R, a.adapter_count = (int)count;
+      rc = matmul_entry(&a, stream);
+    }
+  }
+  if (rc != 0) return failed(what, rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// the tensors of nested lists and tuples: three numbers each
+bool slot_tensors(PyObject* o, const c10::Device& dev, int64_t& slots, std::vector<int64_t>& out) {
+  if (THPVariable_CheckExact(o)) {
+    Tensor t;
+    if (!plain(o, dev, t) || t.dim() < 1 || !fits(t.sizes())) return false;
+    if (slots == 0) slots = t.size(0);
+    int64_t dense = 1;
+    for (int64_t i = t.dim() - 1; i >= 1; --i) {
+      if (t.size(i) != 1 && t.stride(i) != dense) return false;
+      dense *= t.size(i);
+    }
+    if (t.size(0) != slots || (slots > 1 && t.stride(0) < dense)) return false;
+    const int64_t size = t.element_size();
+    out.push_back((int64_t)t.data_ptr()), out.push_back((slots > 1 ? t.stride(0) : dense) * size), out.push_back(dense * size);
+    return true;
+  }
+  const bool list = PyList_CheckExact(o);
+  if (!list && !PyTuple_Check(o)) return false;
+  const Py_ssize_t n = list ? PyList_GET_SIZE(o) : PyTuple_GET_SIZE(o);
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!slot_tensors(list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i), dev, slots, out)) return false;
+  return true;
+}
+
+// copy_slots(states, src, dst) -> True
+PyObject* copy_slots(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3) Py_RETURN_NONE;
+  c10::Device dev(c10::DeviceType::CPU);
+  Tensor src, dst;
+  if (!device_of(arg[1], dev) || !plain(arg[1], dev, src) || !plain(arg[2], dev, dst)) Py_RETURN_NONE;
+  const int64_t entries = src.numel();
+  if (entries < 1 || entries > 8192 || !list32(src, entries) || !list32(dst, entries)) Py_RETURN_NONE;
+  int64_t slots = 0;
+  std::vector<int64_t> t;
+  if (!slot_tensors(arg[0], dev, slots, t) || t.empty()) Py_RETURN_NONE;
+  const size_t count = t.size() / 3;
+  std::vector<std::pair<int64_t, int64_t>> spans(count);
+  for (size_t i = 0; i < count; ++i) spans[i] = {t[3 * i], t[3 * i] + (slots - 1) * t[3 * i + 1] + t[3 * i + 2]};
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < count; ++i)
+    if (spans[i].first < spans[i - 1].second) Py_RETURN_NONE;
+  lq_copy_slots_args a = {};
+  a.tensors = t.data(), a.num_tensors = (int)count, a.num_slots = (int)slots, a.src = i32(src), a.dst = i32(dst), a.entries = (int)entries;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    rc = copy_slots_entry(&a, stream_of(dev));
+  }
+  if (rc != 0) return failed("lq_copy_slots", rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // whether the library was built from the header that this file was: its ABI version and the structs that are filled here
 bool same_abi(decltype(&lq_abi_version) version, decltype(&lq_args_size) size) {
   const int v = version();
@@ -742,6 +1006,11 @@ bool same_abi(decltype(&lq_abi_version) version, decltype(&lq_args_size) size) {
   LQ_SAME_SIZE(lq_conv1d_step_args);
   LQ_SAME_SIZE(lq_ssm_prompt_args);
   LQ_SAME_SIZE(lq_ssm_step_args);
+  LQ_SAME_SIZE(lq_linear_attention_prompt_args);
+  LQ_SAME_SIZE(lq_linear_attention_step_args);
+  LQ_SAME_SIZE(lq_groupnorm_gated_args);
+  LQ_SAME_SIZE(lq_adapter_down_args);
+  LQ_SAME_SIZE(lq_copy_slots_args);
 #undef LQ_SAME_SIZE
   return true;
 }
@@ -776,8 +1045,15 @@ PyObject* init(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   ssm_prompt_entry = (decltype(ssm_prompt_entry))entry("lq_ssm_prompt");
   ssm_prompt_bytes = (decltype(ssm_prompt_bytes))entry("lq_ssm_prompt_workspace_bytes");
   ssm_step_entry = (decltype(ssm_step_entry))entry("lq_ssm_step");
+  attention_prompt_entry = (decltype(attention_prompt_entry))entry("lq_linear_attention_prompt");
+  attention_prompt_bytes = (decltype(attention_prompt_bytes))entry("lq_linear_attention_prompt_workspace_bytes");
+  attention_step_entry = (decltype(attention_step_entry))entry("lq_linear_attention_step");
+  groupnorm_entry = (decltype(groupnorm_entry))entry("lq_groupnorm_gated");
+  adapter_down_entry = (decltype(adapter_down_entry))entry("lq_adapter_down");
+  copy_slots_entry = (decltype(copy_slots_entry))entry("lq_copy_slots");
   if (!quantize_entry || !matmul_entry || !norm_entry || !conv_prompt_entry || !conv_step_entry || !ssm_prompt_entry || !ssm_prompt_bytes || !ssm_step_entry ||
-      !simple_gla_entry || !simple_gla_bytes || !chunk_forward_entry || !chunk_forward_bytes || !rotate_entry || !split_rotate_entry || !ssd_entry || !ssd_bytes) {
+      !simple_gla_entry || !simple_gla_bytes || !chunk_forward_entry || !chunk_forward_bytes || !rotate_entry || !split_rotate_entry || !ssd_entry || !ssd_bytes ||
+      !attention_prompt_entry || !attention_prompt_bytes || !attention_step_entry || !groupnorm_entry || !adapter_down_entry || !copy_slots_entry) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "an entry point is missing");
     return nullptr;
   }
@@ -799,6 +1075,11 @@ PyMethodDef methods[] = {{"init", (PyCFunction)(void*)init, METH_FASTCALL, nullp
                          {"conv1d_prompt", (PyCFunction)(void*)conv1d_prompt, METH_FASTCALL, nullptr},
                          {"ssm_step", (PyCFunction)(void*)ssm_step, METH_FASTCALL, nullptr},
                          {"ssm_prompt", (PyCFunction)(void*)ssm_prompt, METH_FASTCALL, nullptr},
+                         {"linear_attention_step", (PyCFunction)(void*)linear_attention_step, METH_FASTCALL, nullptr},
+                         {"linear_attention_prompt", (PyCFunction)(void*)linear_attention_prompt, METH_FASTCALL, nullptr},
+                         {"groupnorm_gated", (PyCFunction)(void*)groupnorm_gated, METH_FASTCALL, nullptr},
+                         {"adapted", (PyCFunction)(void*)adapted, METH_FASTCALL, nullptr},
+                         {"copy_slots", (PyCFunction)(void*)copy_slots, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods};
 

@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   float total = 0.0f, whole_decay = 0.0f;            // what the accumulators are over, the segment's decay so far (powers of two)
   float fold = 1.0f;                                 // what the accumulators are multiplied by in this chunk, mostly one
   float unit_S = 1.0f, read = 1.0f;                  // fp16: powers of two of the channel: of v and the state; what q multiplies is that times `read`
-  bool calm = true, scaled = false;                  // the same for the wave: read is one for all channels; the accumulators are multiplied
+  bool calm = true, scaled = false, united = false;  // the same for the wave: read is one for all channels; the accumulators are multiplied; a unit is not one
   auto begin = [&](int c) {
     const int lane = fresh(), hh = lane >> 5;
     const int rem = s.len - (s.chunk0 + c) * Q;
@@ -384,7 +384,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       unit_S = k;
       large = __ballot(mx * k >= 256.0f) != 0;
       const uint32_t k16 = F16::from(k);
-      if (__ballot(k != 1.0f) != 0) {
+      united = __ballot(k != 1.0f) != 0;
+      if (united) {
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -655,7 +656,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
               if (32 * (y == 0 ? ta : 1 - ta) + col >= f) Y[y][e] = __builtin_nanf("");
           }
         }
-        if constexpr (kHalf) {
+        if (kHalf && united) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const lq_v4f u4 = *(const lq_v4f*)(vunit[wave] + 8 * j + 4 * hh);
@@ -792,13 +793,17 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
   r.waves = a->vdim <= 64 ? 2 : 4;
   r.parts = (a->vdim + 32 * r.waves - 1) / (32 * r.waves);
   const int64_t parts = (int64_t)a->nheads * r.parts;
-  // Packed prompts' lengths are not known here: the longest is taken to be two and a half times the mean.
+  // Tenths of a microsecond.  A chunk's step takes 40 where a compute unit has one workgroup and 75 where it has two, one of the states' 27 and
+  // 44; the join moves every segment's state three times at 6 TB/s, and it and two more launches come to 100.  Measured, heads of 128 by 128:
+  // 500 tokens of 16 heads uncut 34 us, in segments of 4 chunks 35, of 2 and of one 26; 2 prompts of 8192, 32 heads, in segments of 32 chunks 249, of
+  // 16 205, of 8 229; 10 packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 153, of 12 chunks 119, 8 89, 6 82, 4 94.  Packed
+  // prompts' lengths are not known here: the longest is taken to be two and a half times the mean.
   const double mean = (double)units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
   auto step = [&](double wgs, double one, double two) {
     if (wgs <= 256) return one;
     return a->seq_starts && wgs <= 512 ? one + (two - one) * (wgs / 256 - 1) : two * std::ceil(wgs / 512);
   };
-  double best = chain * step((double)nseq * parts, 30, 50);
+  double best = chain * step((double)nseq * parts, 40, 75);
   r.seg_chunks = (int)most, r.cut = 0;
   int64_t seen = 0;
   for (int64_t k = 2; k <= 256; ++k) {  // segments of the longest
@@ -806,7 +811,7 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
     if (n == seen) continue;
     seen = n;
     const double segs = a->seq_starts ? (double)units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n)), ahead = std::max(0.0, segs - nseq);
-    const double cost = n * step(segs * parts, 30, 50) + n * step(ahead * parts, 15, 25) + (ahead + 2 * segs) * a->nheads * a->kdim * a->vdim * 4 / 3e5 + 150;
+    const double cost = n * step(segs * parts, 40, 75) + n * step(ahead * parts, 27, 44) + (ahead + 2 * segs) * a->nheads * a->kdim * a->vdim * 4 / 6e5 + 100;
     if (n < most && cost < best) best = cost, r.seg_chunks = (int)n, r.cut = 1;
   }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;

@@ -58,6 +58,10 @@ def linear_attention_prompt(q, k, v, g=None, *, scale=None, state=None, slots=No
     None: zero, nothing kept.  ``slots`` (n,) int32: each prompt's place in the state, all different; negative: from zero, nothing
     kept; beyond the state: NaN outputs.  An infinity in q, k, v or the state counts as a NaN: it reaches the outputs and states that the
     formula has it reach, as one or the other.  Returns o, dense, in the shape and type of v."""
+    if state is not None:
+        out = _lib.native().linear_attention_prompt(q, k, v, g, scale, state, slots, seq_starts)
+        if out is not None:
+            return out
     packed = seq_starts is not None
     assert v.dim() == (3 if packed else 4), "v: (B, L, H, V), or (T, H, V) with seq_starts"
     lead = v.shape[:-2]
@@ -100,6 +104,9 @@ def linear_attention_step(state, q, k, v, g=None, *, scale=None, slots=None):
     """The same for one token of each of up to 65535 sequences: ``q``, ``k`` (B, H, K), ``v`` (B, H, V), ``g`` (H,) or (B, H) -> o (B, H, V),
     ``state`` (slots, H, K, V) fp32 moved on by it.  ``slots`` (B,) int32, all different; negative marks a padding entry (zeros out, no
     state touched), beyond the state: NaN outputs."""
+    out = _lib.native().linear_attention_step(q, k, v, g, scale, state, slots)
+    if out is not None:
+        return out
     assert v.dim() == 3, "v: (B, H, V)"
     fields = _check(q, k, v, g, scale, v.shape[:1])
     n, H, V = v.shape

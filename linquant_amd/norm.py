@@ -149,12 +149,16 @@ def groupnorm_gated(x, z=None, weight=None, bias=None, *, num_groups, eps=1e-5, 
 
     ``x`` (..., dim) fp16 or bf16, ``z`` like x or None; ``weight``, ``bias`` (dim,) or None, fp16, bf16 or fp32; ``activation`` "silu", "sigmoid"
     or None; dim a multiple of num_groups, up to 16384 channels to a group.  No gradients.  Returns the shape and type of x, dense."""
+    act = _ACTIVATIONS.get(activation)
+    out = _lib.native().groupnorm_gated(x, z, weight, bias, num_groups, eps, act)
+    if out is not None:
+        return out
     assert x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1
     dim = x.shape[-1]
     assert num_groups >= 1 and dim >= 1 and dim % num_groups == 0 and dim // num_groups <= 16384, f"{dim} channels in {num_groups} groups"
     assert z is None or (z.shape == x.shape and z.dtype == x.dtype), "z: the shape and type of x"
     assert all(t is None or (t.shape == (dim,) and t.dtype in _CODES) for t in (weight, bias)), "weight, bias: (dim,)"
-    assert activation in _ACTIVATIONS, f"activation {activation!r}"
+    assert act is not None, f"activation {activation!r}"
     _lib.same_device(x, z, weight, bias)
     rows = x.numel() // dim
     _lib.below_2_31(rows, dim)
@@ -168,7 +172,7 @@ def groupnorm_gated(x, z=None, weight=None, bias=None, *, num_groups, eps=1e-5, 
     if rows:
         _lib.call("lq_groupnorm_gated", x.device, x=_lib.ptr(x2), x_stride=x2.stride(0), z=_lib.ptr(z2), z_stride=0 if z2 is None else z2.stride(0),
                   dtype=_CODES[x.dtype], weight=_lib.ptr(weight), bias=_lib.ptr(bias), weight_dtype=wdt, out=_lib.ptr(out), eps=float(eps), rows=rows,
-                  dim=dim, num_groups=num_groups, act=_ACTIVATIONS[activation])
+                  dim=dim, num_groups=num_groups, act=act)
     return out
 
 

@@ -169,6 +169,11 @@ class W8A8Linear(nn.Module):
         codes = torch.round(w / torch.where(s > 0, s, 1.0)[:, None]).to(torch.int8)
         return cls(codes, s, input_scale, linear.bias)
 
+    def _native(self, x, scale, out_dtype, adapters, ids):
+        """The ordinary forms of a call with adapters; None for others."""
+        w, a = self._buffers, adapters._buffers
+        return _lib.native().adapted(x, scale, w["weight"], w["weight_scale"], w["bias"], out_dtype, a["down"], a["up"], a["scaling"], ids)
+
     def _ids(self, adapters, ids, lead):
         assert ids is not None and ids.dtype == torch.int32 and ids.shape == lead, f"ids: int32 {tuple(lead)}"
         assert (adapters.in_features, adapters.out_features) == (self.in_features, self.out_features), "adapters of another projection"
@@ -181,6 +186,10 @@ class W8A8Linear(nn.Module):
 
     def forward_int8(self, x_i8, scale, out_dtype=torch.float16, *, adapters=None, ids=None):
         """Codes (..., in_features) on ``scale`` (a number, one entry, or one for each row)."""
+        if adapters is not None and isinstance(scale, torch.Tensor):
+            out = self._native(x_i8, scale, out_dtype, adapters, ids)
+            if out is not None:
+                return out
         assert x_i8.dtype == torch.int8 and x_i8.shape[-1] == self.in_features
         a = x_i8.reshape(-1, self.in_features)
         if self.in_features % _K:
@@ -192,6 +201,10 @@ class W8A8Linear(nn.Module):
         return int8_matmul(a, self.weight, scale, self.weight_scale, self.bias, out_dtype).view(*x_i8.shape[:-1], self.out_features)
 
     def forward(self, x, *, adapters=None, ids=None):
+        if adapters is not None and self._buffers["input_scale"] is None:
+            out = self._native(x, None, x.dtype, adapters, ids)
+            if out is not None:
+                return out
         assert x.shape[-1] == self.in_features and x.dtype in (torch.float16, torch.bfloat16)
         static = self.input_scale is not None and x.dtype == torch.float16 and self.in_features % 8 == 0
         assert static or self.input_scale is None, "a static input scale takes fp16 activations and in_features a multiple of 8"
