@@ -1067,6 +1067,8 @@ typedef struct {
   const int32_t* ids;        /* (rows,) */
   float* h;                  /* (rows, rank) dense, 16-byte aligned */
   int32_t rows, inner, inner_padded, rank, count; /* inner_padded and rank multiples of 16, rank up to 128 */
+  int8_t* codes_out;         /* NULL, or also what lq_quantize_rows makes of x (16 bits, inner a multiple of 8 up to 16384): (rows, inner) dense */
+  float* scale_out;          /* (rows,), with codes_out */
 } lq_adapter_down_args;
 int lq_adapter_down(const lq_adapter_down_args* args, hipStream_t stream);
 

@@ -9,7 +9,7 @@
 // down is the operand of the rows, so that a lane holds four adjacent sums of one row of x.
 //
 // INT8 codes become 16 bits exactly; their scale multiplies the sum.  All sums are fp32.
-#include "serve_common.h"
+#include "row_codes.h"
 
 namespace {
 
@@ -23,6 +23,8 @@ struct DownParams {
   const int32_t* ids;
   float* h;
   int rows, inner, padded, rank, count;
+  int8_t* codes_out;  // NULL, or x's codes and scales as well
+  float* scale_out;
 };
 
 template <typename T>
@@ -31,38 +33,35 @@ LQ_DEV lq_v4f mfma16(lq_v4i a, lq_v4i b, lq_v4f c) {
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sv_v8bf, a), __builtin_bit_cast(sv_v8bf, b), c, 0, 0, 0);
 }
 
-// eight entries of a row from `k` on in T, zero behind the row's end.  (The last eight are read again there: inner is at least 8, or the row
-// is read one by one.)
-template <typename T, bool CODES>
+// Eight entries of a row from `k` on in T, zero behind the row's end.  EIGHTS: rows of whole eights on boundaries of eight entries, of which the
+// last are read again behind the end; else one by one.
+template <typename T, bool CODES, bool EIGHTS>
 LQ_DEV lq_v4i load8(const void* row, int k, int inner) {
-  uint16_t v[8];
-  if (inner % 8 == 0) {
-    const int at = min(k, inner - 8);
-    if constexpr (CODES) {
-      const lq_v2i r = *(const lq_v2i*)((const int8_t*)row + at);
+  if constexpr (EIGHTS && !CODES) {
+    const lq_v4i zero = {0, 0, 0, 0}, r = *(const lq_v4i*)((const uint16_t*)row + min(k, inner - 8));
+    return k < inner ? r : zero;
+  } else {
+    uint16_t v[8];
+    if constexpr (EIGHTS) {
+      lq_v2i r = *(const lq_v2i*)((const int8_t*)row + min(k, inner - 8));
+      if (k >= inner) r = lq_v2i{0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = T::from((float)lq_sbyte((uint32_t)r[e >> 2], e & 3));
     } else {
-      const sv_v8u r = *(const sv_v8u*)((const uint16_t*)row + at);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = r[e];
+      for (int e = 0; e < 8; ++e) {
+        const int at = min(k + e, inner - 1);
+        uint16_t u;
+        if constexpr (CODES) u = T::from((float)((const int8_t*)row)[at]);
+        else u = ((const uint16_t*)row)[at];
+        v[e] = k + e < inner ? u : 0;
+      }
     }
+    lq_v4i o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = k < inner ? v[e] : 0;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = min(k + e, inner - 1);
-      uint16_t u;
-      if constexpr (CODES) u = T::from((float)((const int8_t*)row)[at]);
-      else u = ((const uint16_t*)row)[at];
-      v[e] = k + e < inner ? u : 0;
-    }
+    for (int i = 0; i < 4; ++i) o[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
+    return o;
   }
-  lq_v4i o;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
-  return o;
 }
 
 template <typename T, bool CODES>
@@ -76,9 +75,22 @@ LQ_DEV float factor(const DownParams& p, int m, int id) {
 
 constexpr int kPer = 2;  // sums of a wave in `rows`
 
-template <typename T, bool CODES>
+// QV: 0, or the workgroups in front of the others quantize the rows, each thread 8 QV entries of one
+template <typename T, bool CODES, bool EIGHTS, int QV>
 __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
-  const int m = blockIdx.x, lane = threadIdx.x & 63, r0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kPer;
+  int m = blockIdx.x, lane = threadIdx.x & 63;
+  if constexpr (QV > 0) {
+    if (m < p.rows) {
+      __shared__ float lds[4];
+      float v[8 * QV];
+      Row<T, QV, 256, true>::load(p.x, m * p.x_stride, p.inner, threadIdx.x, v);
+      row_codes<QV, 256, true>(p.scale_out + m, p.codes_out, (int64_t)m * p.inner, p.inner, threadIdx.x, v, lds, 0);
+      return;
+    }
+    m -= p.rows;
+  }
+  const int groups = (p.rank + 4 * kPer - 1) / (4 * kPer), r0 = (m % groups * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kPer;
+  m /= groups;
   if (r0 >= p.rank) return;
   const int id = p.ids[m];
   float* h = p.h + (int64_t)m * p.rank + r0;
@@ -94,7 +106,7 @@ __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int k = k0 + (u * 64 + lane) * 8;
-      xv[u] = load8<T, CODES>(x, k, p.inner);
+      xv[u] = load8<T, CODES, EIGHTS>(x, k, p.inner);
 #pragma unroll
       for (int r = 0; r < kPer; ++r) dv[u][r] = *(const lq_v4i*)(d + (int64_t)r * p.padded + min(k, p.padded - 8));
     }
@@ -119,9 +131,10 @@ __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
   }
 }
 
-// RT tiles of 16 sums; W waves share the contraction in lines of 64 entries, side by side
-template <typename T, bool CODES, int RT, int W>
+// RT tiles of 16 sums; W waves share the contraction in lines of 64 entries, side by side, U of them requested at a time
+template <typename T, bool CODES, bool EIGHTS, int RT, int W>
 __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
+  constexpr int U = RT <= 2 ? 4 : RT <= 4 ? 2 : 1;
   __shared__ __align__(16) lq_v4f sums[W][RT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
   const int m0 = blockIdx.x * 16, m = min(m0 + (lane & 15), p.rows - 1);
@@ -140,22 +153,26 @@ __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
     lq_v4f acc[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[t] = lq_v4f{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave * 64; k0 < p.padded; k0 += 64 * W) {
-      lq_v4i xv[2], dv[2][RT];
+    for (int k0 = wave * 64; k0 < p.padded; k0 += 64 * W * U) {
+      lq_v4i xv[U][2], dv[U][2][RT];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = k0 + 32 * u + 8 * quarter, kc = min(k, p.padded - 8);
-        xv[u] = load8<T, CODES>(x, k, p.inner);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          dv[u][t] = *(const lq_v4i*)(d + (int64_t)16 * t * p.padded + kc);
-          if (k >= p.padded) dv[u][t] = lq_v4i{0, 0, 0, 0};
+        for (int h = 0; h < 2; ++h) {
+          const int k = k0 + 64 * W * u + 32 * h + 8 * quarter;
+          xv[u][h] = load8<T, CODES, EIGHTS>(x, k, p.inner);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) dv[u][h][t] = *(const lq_v4i*)(d + (int64_t)16 * t * p.padded + min(k, p.padded - 8));
         }
-      }
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = mfma16<T>(dv[u][t], xv[u], acc[t]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            if (k0 + 64 * W * u + 32 * h + 8 * quarter >= p.padded) dv[u][h][t] = lq_v4i{0, 0, 0, 0};  // (an infinity of the row's last)
+            acc[t] = mfma16<T>(dv[u][h][t], xv[u][h], acc[t]);
+          }
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -194,21 +211,39 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
   if (a->inner % 8 == 0 ? !sv_al(a->x, codes ? 8 : 16) || a->x_stride % 8 != 0 : !sv_al(a->x, codes ? 1 : 2)) return LQ_ERR_SHAPE;
   if (!sv_al(a->down, 16) || !sv_al(a->h, 16) || !sv_al(a->x_scale, 4) || !sv_al(a->scaling, 4) || !sv_al(a->ids, 4))
     return LQ_ERR_SHAPE;
-  DownParams p = {a->x, a->x_stride, a->x_scale, a->x_scale_rows, (const uint16_t*)a->down, a->scaling, a->ids, a->h, a->rows, a->inner, a->inner_padded, a->rank, a->count};
-  auto go = [&](auto t, auto c) {
+  DownParams p = {a->x, a->x_stride, a->x_scale, a->x_scale_rows, (const uint16_t*)a->down, a->scaling, a->ids, a->h, a->rows, a->inner, a->inner_padded, a->rank, a->count,
+                  a->codes_out, a->scale_out};
+  const bool eights = a->inner % 8 == 0;
+  if (a->codes_out && (!a->scale_out || codes || !eights || a->inner > 16384 || !sv_al(a->codes_out, 8) || !sv_al(a->scale_out, 4))) return LQ_ERR_SHAPE;
+  using std::integral_constant;
+  auto rows = [&](auto t, auto c, auto e, auto qv) {
+    const int64_t wgs = (int64_t)a->rows * ((a->rank + 4 * kPer - 1) / (4 * kPer)) + (decltype(qv)::value ? a->rows : 0);
+    hipLaunchKernelGGL((down_rows_kernel<decltype(t), decltype(c)::value, decltype(e)::value, decltype(qv)::value>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
+    return lq_check_launch();
+  };
+  auto go = [&](auto t, auto c, auto e) {
     using T = decltype(t);
-    constexpr bool C = decltype(c)::value;
-    if (a->rows <= kFewRows) {
-      hipLaunchKernelGGL((down_rows_kernel<T, C>), dim3((unsigned)a->rows, (unsigned)((a->rank + 4 * kPer - 1) / (4 * kPer))), dim3(256), 0, stream, p);
-      return lq_check_launch();
+    constexpr bool C = decltype(c)::value, E = decltype(e)::value;
+    if constexpr (!C && E) {
+      if (a->codes_out && a->rows <= kFewRows) {
+        if (a->inner <= 2048) return rows(t, c, e, integral_constant<int, 1>{});
+        if (a->inner <= 4096) return rows(t, c, e, integral_constant<int, 2>{});
+        if (a->inner <= 8192) return rows(t, c, e, integral_constant<int, 4>{});
+        return rows(t, c, e, integral_constant<int, 8>{});
+      }
+      if (a->codes_out) {
+        lq_quantize_rows_args q = {a->x, a->x_stride, a->x_dtype, a->codes_out, a->inner, a->scale_out, a->rows, a->inner};
+        const int rc = lq_quantize_rows(&q, stream);
+        if (rc != LQ_OK) return rc;
+      }
     }
+    if (a->rows <= kFewRows) return rows(t, c, e, integral_constant<int, 0>{});
     auto tiles = [&](auto rt) {
       constexpr int RT = decltype(rt)::value, W = RT <= 4 ? 8 : 4;
-      hipLaunchKernelGGL((down_tiles_kernel<T, C, RT, W>), dim3((unsigned)(((int64_t)a->rows + 15) / 16)), dim3(64 * W), 0, stream, p);
+      hipLaunchKernelGGL((down_tiles_kernel<T, C, E, RT, W>), dim3((unsigned)(((int64_t)a->rows + 15) / 16)), dim3(64 * W), 0, stream, p);
       return lq_check_launch();
     };
     if (!sv_fits(((int64_t)a->rows + 15) / 16, 512)) return (int)LQ_ERR_SHAPE;
-    using std::integral_constant;
     switch (a->rank / 16) {
       case 1: return tiles(integral_constant<int, 1>{});
       case 2: return tiles(integral_constant<int, 2>{});
@@ -220,6 +255,7 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
       default: return tiles(integral_constant<int, 8>{});
     }
   };
-  auto with = [&](auto t) { return codes ? go(t, std::true_type{}) : go(t, std::false_type{}); };
-  return a->dtype == LQ_DT_F16 ? with(F16{}) : with(BF16{});
+  auto with = [&](auto t, auto c) { return eights ? go(t, c, std::true_type{}) : go(t, c, std::false_type{}); };
+  auto typed = [&](auto t) { return codes ? with(t, std::true_type{}) : with(t, std::false_type{}); };
+  return a->dtype == LQ_DT_F16 ? typed(F16{}) : typed(BF16{});
 }

@@ -896,10 +896,9 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   if (bias.defined() && (!floats(bias) || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous())) Py_RETURN_NONE;
   auto sizes = x.sizes().vec();
   sizes.back() = N;
-  lq_quantize_rows_args q = {};
   lq_adapter_down_args d = {};
   lq_int8_matmul_args a = {};
-  const char* what = "lq_quantize_rows";
+  const char* what = "lq_adapter_down";
   int rc = 0;
   {
     pybind11::gil_scoped_release no_gil;
@@ -907,12 +906,9 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     out = empty(sizes, ot, dev), h = empty({M, R}, ScalarType::Float, dev);
     if (!coded) {
       codes = empty({M, K}, ScalarType::Char, dev), xs = empty({M}, ScalarType::Float, dev);
-      q.x = x.const_data_ptr(), q.x_stride = K, q.dtype = code(x.scalar_type()), q.codes = (int8_t*)codes.data_ptr(), q.codes_stride = K, q.scale = (float*)xs.data_ptr();
-      q.rows = (int)M, q.cols = (int)K;
-      rc = quantize_entry(&q, stream);
+      d.codes_out = (int8_t*)codes.data_ptr(), d.scale_out = (float*)xs.data_ptr();
     }
-    if (rc == 0) {
-      what = "lq_adapter_down";
+    {
       d.x = x.const_data_ptr(), d.x_stride = K, d.x_dtype = coded ? LQ_DT_I8 : code(x.scalar_type()), d.x_scale = coded ? f32(xs) : nullptr, d.x_scale_rows = xs.numel() != 1;
       d.down = down.const_data_ptr(), d.dtype = code(down.scalar_type()), d.scaling = f32(scaling), d.ids = i32(ids), d.h = (float*)h.data_ptr();
       d.rows = (int)M, d.inner = (int)K, d.inner_padded = (int)K, d.rank = (int)R, d.count = (int)count;

@@ -77,10 +77,10 @@ LQ_DEV void pieces(const float* h, float unit, lq_v4i& hi, lq_v4i& lo) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) hi[i] = (int)(u[2 * i] | (uint32_t)u[2 * i + 1] << 16), lo[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
 }
-// the part of a row that this lane's half has is all that it looks at; its largest over both halves
-LQ_DEV float row_unit(const float* h, int rank, int hh) {
+// of a row, whose first entry of this lane's half is at h: the half looks at its own part, and the largest is over both
+LQ_DEV float row_unit(const float* h, int rank) {
   float top = 0.0f;
-  for (int r = 8 * hh; r < rank; r += 16)
+  for (int r = 0; r < rank; r += 16)
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
       const lq_v4f v = *(const lq_v4f*)(h + r + e);
@@ -248,40 +248,54 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int m = m0 + wm + 32 * i;
-    mm_v16f delta[std::is_void<A>::value ? 1 : NI];
+    // adapters: this lane's row, the request that it names, the first adapter of the 32 rows and what it has for the columns, requested together
+    const float* h = nullptr;
+    const uint16_t* up = nullptr;
+    float unit = 1.0f;
+    int id = -1, head = 0;
+    uint64_t named = 0;
+    lq_v4i u0[std::is_void<A>::value ? 1 : NI], hi0 = {0, 0, 0, 0}, lo0 = {0, 0, 0, 0};
     if constexpr (!std::is_void<A>::value) {
-      const int mc = min(m + (lane & 31), p.rows - 1), id = p.ids[mc];
-      const float* h = p.h + (int64_t)mc * p.rank;
-      const float unit = row_unit(h, p.rank, hh), none = id < p.count ? 0.0f : __builtin_nanf("");
+      const int mc = min(m + (lane & 31), p.rows - 1);
+      id = p.ids[mc], h = p.h + (int64_t)mc * p.rank + 8 * hh, up = p.up + 8 * hh;
+      named = __ballot(id >= 0 && id < p.count);
+      if (named) {
+        head = __builtin_amdgcn_readlane(id, __builtin_ctzll(named));
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) delta[j][e] = none;
-      uint64_t left = __ballot(id >= 0 && id < p.count);
-      while (left) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const bool mine = id == a;
-        left &= ~__ballot(mine);
-        const uint16_t* up = p.up + (int64_t)a * p.cols * p.rank + 8 * hh;
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const uint16_t* uj = up + (int64_t)min(n0 + wn + 32 * j + (lane & 31), p.cols - 1) * p.rank;
-          mm_v16f d = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          for (int r = 0; r < p.rank; r += 16) {
-            lq_v4i hi, lo;
-            pieces<A>(h + r + 8 * hh, unit, hi, lo);
-            const lq_v4i u = *(const lq_v4i*)(uj + r);
-            d = mfma32<A>(u, hi, d);
-            d = mfma32<A>(u, lo, d);
-          }
-          sv_settle(d);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) delta[j][e] = mine ? d[e] * (1.0f / unit) : delta[j][e];
-        }
+        for (int j = 0; j < NI; ++j) u0[j] = *(const lq_v4i*)(up + ((int64_t)head * p.cols + min(n0 + wn + 32 * j + (lane & 31), p.cols - 1)) * p.rank);
+        unit = row_unit(h, p.rank);
+        pieces<A>(h, unit, hi0, lo0);
       }
     }
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+    for (int j = 0; j < NI; ++j) {
+    mm_v16f delta;
+    if constexpr (!std::is_void<A>::value) {
+      const float none = id < p.count ? 0.0f : __builtin_nanf(""), back = 1.0f / unit;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) delta[e] = none;
+      for (uint64_t left = named; left;) {
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const bool mine = id == a;
+        left &= ~__ballot(mine);
+        const uint16_t* uj = up + ((int64_t)a * p.cols + min(n0 + wn + 32 * j + (lane & 31), p.cols - 1)) * p.rank;
+        lq_v4i u = u0[j];
+        if (a != head) u = *(const lq_v4i*)uj;
+        mm_v16f d = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        d = mfma32<A>(u, hi0, d);
+        d = mfma32<A>(u, lo0, d);
+        for (int r = 16; r < p.rank; r += 16) {
+          lq_v4i hi, lo;
+          pieces<A>(h + r, unit, hi, lo);
+          u = *(const lq_v4i*)(uj + r);
+          d = mfma32<A>(u, hi, d);
+          d = mfma32<A>(u, lo, d);
+        }
+        sv_settle(d);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) delta[e] = mine ? d[e] * back : delta[e];
+      }
+    }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = 32 * j + 8 * q + 4 * hh;
@@ -291,11 +305,12 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float v = __builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]);
-          if constexpr (!std::is_void<A>::value) v += delta[j][4 * q + e];
+          if constexpr (!std::is_void<A>::value) v += delta[4 * q + e];
           o[e] = O::from(v);
         }
         *(V4*)(my + (lane & 31) * kOutRow + n * sizeof(OT)) = o;
       }
+    }
     // (a wave's LDS operations are in order)
     constexpr int kPieces = TN / 2 * (int)sizeof(OT) / 16, kRows = 64 / kPieces;  // 16-byte pieces of a row, rows written at a time
     constexpr int kPer = 16 / (int)sizeof(OT);
