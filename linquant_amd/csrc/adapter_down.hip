@@ -131,6 +131,27 @@ __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
   }
 }
 
+// the waves' sums together, and out
+template <bool CODES, int RT, int W>
+LQ_DEV void down_finish(const DownParams& p, int m0, const lq_v4f (&keep)[RT], lq_v4f (&sums)[W][RT][64]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) sums[wave][t][lane] = keep[t];
+  __syncthreads();
+  for (int i = threadIdx.x; i < RT * 64; i += 64 * W) {
+    const int t = i >> 6, l = i & 63, row = m0 + (l & 15);
+    lq_v4f v = sums[0][t][l];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += sums[w][t][l];
+    if (row >= p.rows) continue;
+    const int own = p.ids[row];
+    const float f = own >= 0 && own < p.count ? factor<CODES>(p, row, own) : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= f;
+    *(lq_v4f*)(p.h + (int64_t)row * p.rank + 16 * t + 4 * (l >> 4)) = v;
+  }
+}
+
 // RT tiles of 16 sums; W waves share the contraction in lines of 64 entries, side by side, U of them requested at a time
 template <typename T, bool CODES, bool EIGHTS, int RT, int W>
 __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
@@ -180,21 +201,87 @@ __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
       if (mine) keep[t] = acc[t];
     }
   }
+  down_finish<CODES, RT, W>(p, m0, keep, sums);
+}
+
+// The same, x and down through LDS in stages of SE entries, each row's whole 16-byte pieces fetched side by side: as operands they are read
+// from memory 64 bytes of a row at a time, at half the rate.  Piece c of row r lies at place c ^ r % 16, so that the 16 rows that a read serves
+// at once touch each bank once.  Two places, one filled while the other is multiplied.
+template <typename T, bool CODES, int RT, int SE>
+__global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
+  constexpr int W = 8, XB = SE * (CODES ? 1 : 2), DB = SE * 2;              // bytes of a stage's row of x and of down
+  constexpr int XR = 1024 / XB, DR = 1024 / DB;                             // rows of a fetch
+  constexpr int XF = 16 / XR, DF = RT * 16 / DR, kStage = 16 * XB + RT * 16 * DB;  // fetches of a stage
+  constexpr int H = SE / (32 * W);                                          // products of a wave and stage
+  static_assert(2 * kStage >= W * RT * 1024);
+  __shared__ __align__(1024) char lds[2][kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, r16 = lane & 15;
+  const int m0 = blockIdx.x * 16, m = min(m0 + r16, p.rows - 1);
+  const int id = p.ids[m];
+  const char* x = (const char*)p.x + m0 * p.x_stride * (CODES ? 1 : 2);
+  lq_v4f keep[RT];
+  const float none = id < 0 ? 0.0f : __builtin_nanf("");
 #pragma unroll
-  for (int t = 0; t < RT; ++t) sums[wave][t][lane] = keep[t];
-  __syncthreads();
-  for (int i = threadIdx.x; i < RT * 64; i += 64 * W) {
-    const int t = i >> 6, l = i & 63, row = m0 + (l & 15);
-    lq_v4f v = sums[0][t][l];
+  for (int t = 0; t < RT; ++t) keep[t] = lq_v4f{none, none, none, none};
+  const int stages = (p.inner + SE - 1) / SE, xlast = (p.inner - (CODES ? 16 : 8)) * (CODES ? 1 : 2), dlast = (p.padded - 8) * 2;
+  uint64_t left = __ballot(id >= 0 && id < p.count);
+  while (left) {
+    const int j = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    const bool mine = id == j;
+    left &= ~__ballot(mine);
+    const char* d = (const char*)(p.down + (int64_t)j * p.rank * p.padded);
+    auto fetch = [&](int s) {  // (behind a row's end its last piece again: down is zero there as an operand)
+      char* to = lds[s & 1];
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += sums[w][t][l];
-    if (row >= p.rows) continue;
-    const int own = p.ids[row];
-    const float f = own >= 0 && own < p.count ? factor<CODES>(p, row, own) : 1.0f;
+      for (int i = 0; i < (XF + W - 1) / W; ++i) {
+        const int f = i * W + wave, row = f * XR + lane / (64 / XR), c = (lane % (64 / XR)) ^ (row & 15);
+        if (f < XF) sv_fetch16(x, (uint32_t)min(row, p.rows - 1 - m0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u) + (uint32_t)min(s * XB + c * 16, xlast), to + f * 1024);
+      }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= f;
-    *(lq_v4f*)(p.h + (int64_t)row * p.rank + 16 * t + 4 * (l >> 4)) = v;
+      for (int i = 0; i < (DF + W - 1) / W; ++i) {
+        const int f = i * W + wave, row = f * DR + lane / (64 / DR), c = (lane % (64 / DR)) ^ (row & 15);
+        if (f < DF) sv_fetch16(d, (uint32_t)row * (uint32_t)p.padded * 2u + (uint32_t)min(s * DB + c * 16, dlast), to + 16 * XB + f * 1024);
+      }
+    };
+    lq_v4f acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t] = lq_v4f{0.f, 0.f, 0.f, 0.f};
+    fetch(0);
+    for (int s = 0; s < stages; ++s) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is there, and the one in front of it is read
+      if (s + 1 < stages) fetch(s + 1);
+      const char* st = lds[s & 1];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int k = (wave * H + h) * 32 + 8 * quarter;  // of the stage
+        lq_v4i xv;
+        if constexpr (CODES) {
+          const lq_v2i r = *(const lq_v2i*)(st + r16 * XB + (((k >> 4) ^ r16) << 4) + (k & 8));
+          uint16_t v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = T::from((float)lq_sbyte((uint32_t)r[e >> 2], e & 3));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
+        } else {
+          xv = *(const lq_v4i*)(st + r16 * XB + (((k >> 3) ^ r16) << 4));
+        }
+        const bool in = s * SE + k < p.inner;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          lq_v4i dv = *(const lq_v4i*)(st + 16 * XB + (16 * t + r16) * DB + (((k >> 3) ^ r16) << 4));
+          if (!in) dv = lq_v4i{0, 0, 0, 0};
+          acc[t] = mfma16<T>(dv, xv, acc[t]);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      sv_settle(acc[t]);
+      if (mine) keep[t] = acc[t];
+    }
   }
+  down_finish<CODES, RT, W>(p, m0, keep, *(lq_v4f(*)[W][RT][64])lds);  // (nothing of a stage is read any more)
 }
 
 constexpr int kFewRows = 256;
@@ -238,8 +325,14 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
       }
     }
     if (a->rows <= kFewRows) return rows(t, c, e, integral_constant<int, 0>{});
+    // whole 16-byte pieces of both
+    const bool pieces = E && a->inner % (C ? 16 : 8) == 0 && a->x_stride % (C ? 16 : 8) == 0 && sv_al(a->x, 16) && a->x_stride >= 0 && a->x_stride < 1 << 24;
     auto tiles = [&](auto rt) {
       constexpr int RT = decltype(rt)::value, W = RT <= 4 ? 8 : 4;
+      if (pieces) {
+        hipLaunchKernelGGL((down_staged_kernel<T, C, RT, RT <= 2 ? 512 : 256>), dim3((unsigned)(((int64_t)a->rows + 15) / 16)), dim3(512), 0, stream, p);
+        return lq_check_launch();
+      }
       hipLaunchKernelGGL((down_tiles_kernel<T, C, E, RT, W>), dim3((unsigned)(((int64_t)a->rows + 15) / 16)), dim3(64 * W), 0, stream, p);
       return lq_check_launch();
     };
