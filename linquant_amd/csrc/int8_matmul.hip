@@ -55,8 +55,8 @@ struct OutOf<F32> {
 };
 
 // out += h up^T, each row with the adapter that it names.  In `tiles` a row's h enters the matrix instructions as two pieces of the
-// adapters' type, after a multiplication by the power of two that brings the row's largest below 2^14 (fp16's range; bf16 the same way): off
-// by 2^-17 of the row's largest.  The adapters that 32 rows name are taken one after the other, with all 32, and a row keeps what its own
+// adapters' type (fp16: where it needs one, after a multiplication by a power of two that brings the row's largest below 2^14): off by 2^-16 of
+// the row's largest.  The adapters that 32 rows name are taken one after the other, with all 32, and a row keeps what its own
 // gave: nothing is multiplied by zero, and an infinity in one request's adapter stays there.
 typedef float mm_v16f __attribute__((ext_vector_type(16)));
 template <typename T>
@@ -77,8 +77,11 @@ LQ_DEV void pieces(const float* h, float unit, lq_v4i& hi, lq_v4i& lo) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) hi[i] = (int)(u[2 * i] | (uint32_t)u[2 * i + 1] << 16), lo[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
 }
-// of a row, whose first entry of this lane's half is at h: the half looks at its own part, and the largest is over both
+// The unit of a row, whose first entry of this lane's half is at h: the half looks at its own part, and the largest is over both.  One where
+// fp16 holds the row's largest with room to spare on both sides, and always in bf16.
+template <typename T>
 LQ_DEV float row_unit(const float* h, int rank) {
+  if constexpr (std::is_same<T, BF16>::value) return 1.0f;
   float top = 0.0f;
   for (int r = 0; r < rank; r += 16)
 #pragma unroll
@@ -91,9 +94,12 @@ LQ_DEV float row_unit(const float* h, int rank) {
       }
     }
   top = fmaxf(top, __shfl_xor(top, 32, 64));
+  if (top == 0.0f || (top >= 0x1p-9f && top < 0x1p14f)) return 1.0f;
   const int e = (int)(__float_as_uint(top) >> 23) - 127;
   return __uint_as_float((uint32_t)(127 + min(max(13 - e, -100), 100)) << 23);
 }
+
+LQ_DEV float pow2_back(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }  // 1 / unit
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void glb_void;
@@ -249,64 +255,84 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
   for (int i = 0; i < MI; ++i) {
     const int m = m0 + wm + 32 * i;
     // adapters: this lane's row, the request that it names, the first adapter of the 32 rows and what it has for the columns, requested together
+    constexpr bool kAdapters = !std::is_void<A>::value;
     const float* h = nullptr;
-    const uint16_t* up = nullptr;
     float unit = 1.0f;
     int id = -1, head = 0;
     uint64_t named = 0;
-    lq_v4i u0[std::is_void<A>::value ? 1 : NI], hi0 = {0, 0, 0, 0}, lo0 = {0, 0, 0, 0};
-    if constexpr (!std::is_void<A>::value) {
+    bool same = false;  // all 32 rows name one adapter, and no h needs a unit: the product goes on from the projection's
+    lq_v4i u0[kAdapters ? NI : 1], hi0 = {0, 0, 0, 0}, lo0 = {0, 0, 0, 0};
+    auto up_of = [&](int a, int j) { return p.up + 8 * hh + ((int64_t)a * p.cols + min(n0 + wn + 32 * j + (lane & 31), p.cols - 1)) * p.rank; };
+    if constexpr (kAdapters) {
       const int mc = min(m + (lane & 31), p.rows - 1);
-      id = p.ids[mc], h = p.h + (int64_t)mc * p.rank + 8 * hh, up = p.up + 8 * hh;
+      id = p.ids[mc], h = p.h + (int64_t)mc * p.rank + 8 * hh;
       named = __ballot(id >= 0 && id < p.count);
       if (named) {
         head = __builtin_amdgcn_readlane(id, __builtin_ctzll(named));
 #pragma unroll
-        for (int j = 0; j < NI; ++j) u0[j] = *(const lq_v4i*)(up + ((int64_t)head * p.cols + min(n0 + wn + 32 * j + (lane & 31), p.cols - 1)) * p.rank);
-        unit = row_unit(h, p.rank);
+        for (int j = 0; j < NI; ++j) u0[j] = *(const lq_v4i*)up_of(head, j);
+        unit = row_unit<A>(h, p.rank);
         pieces<A>(h, unit, hi0, lo0);
+        same = __ballot(id != head || unit != 1.0f) == 0;
       }
     }
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-    mm_v16f delta;
-    if constexpr (!std::is_void<A>::value) {
-      const float none = id < p.count ? 0.0f : __builtin_nanf(""), back = 1.0f / unit;
+      mm_v16f v;
+      if constexpr (kAdapters) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) delta[e] = none;
-      for (uint64_t left = named; left;) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const bool mine = id == a;
-        left &= ~__ballot(mine);
-        const uint16_t* uj = up + ((int64_t)a * p.cols + min(n0 + wn + 32 * j + (lane & 31), p.cols - 1)) * p.rank;
-        lq_v4i u = u0[j];
-        if (a != head) u = *(const lq_v4i*)uj;
-        mm_v16f d = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        d = mfma32<A>(u, hi0, d);
-        d = mfma32<A>(u, lo0, d);
-        for (int r = 16; r < p.rank; r += 16) {
-          lq_v4i hi, lo;
-          pieces<A>(h + r, unit, hi, lo);
-          u = *(const lq_v4i*)(uj + r);
-          d = mfma32<A>(u, hi, d);
-          d = mfma32<A>(u, lo, d);
+        for (int q = 0; q < 4; ++q) {
+          const int n = 32 * j + 8 * q + 4 * hh;
+          const lq_v4f s4 = *(const lq_v4f*)(sb + wn + n), b4 = *(const lq_v4f*)(sb + TN + wn + n);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * q + e] = __builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]);
         }
-        sv_settle(d);
+        auto products = [&](int a, mm_v16f d) {
+          const uint16_t* uj = up_of(a, j);
+          lq_v4i u = u0[j];
+          if (a != head) u = *(const lq_v4i*)uj;
+          d = mfma32<A>(u, hi0, d);
+          d = mfma32<A>(u, lo0, d);
+          for (int r = 16; r < p.rank; r += 16) {
+            lq_v4i hi, lo;
+            pieces<A>(h + r, unit, hi, lo);
+            u = *(const lq_v4i*)(uj + r);
+            d = mfma32<A>(u, hi, d);
+            d = mfma32<A>(u, lo, d);
+          }
+          sv_settle(d);
+          return d;
+        };
+        if (same) {
+          v = products(head, v);
+        } else {
+          for (uint64_t left = named; left;) {
+            const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+            const bool mine = id == a;
+            left &= ~__ballot(mine);
+            const mm_v16f d = products(a, mm_v16f{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f});
+            const float back = pow2_back(unit);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) delta[e] = mine ? d[e] * back : delta[e];
+            for (int e = 0; e < 16; ++e) v[e] = mine ? __builtin_fmaf(d[e], back, v[e]) : v[e];
+          }
+          if (id >= p.count) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __builtin_nanf("");
+          }
+        }
       }
-    }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = 32 * j + 8 * q + 4 * hh;
-        const lq_v4f s4 = *(const lq_v4f*)(sb + wn + n), b4 = *(const lq_v4f*)(sb + TN + wn + n);
         typedef OT V4 __attribute__((ext_vector_type(4)));
         V4 o;
+        if constexpr (kAdapters) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = __builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]);
-          if constexpr (!std::is_void<A>::value) v += delta[4 * q + e];
-          o[e] = O::from(v);
+          for (int e = 0; e < 4; ++e) o[e] = O::from(v[4 * q + e]);
+        } else {
+          const lq_v4f s4 = *(const lq_v4f*)(sb + wn + n), b4 = *(const lq_v4f*)(sb + TN + wn + n);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = O::from(__builtin_fmaf((float)acc[i][j][4 * q + e], sa[i] * s4[e], b4[e]));
         }
         *(V4*)(my + (lane & 31) * kOutRow + n * sizeof(OT)) = o;
       }
