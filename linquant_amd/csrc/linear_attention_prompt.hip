@@ -667,7 +667,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         // A lane has four channels of eight, the other half of the wave the other four: with every second eight exchanged it has whole eights.
         const int rem = s.len - (s.chunk0 + c) * Q;
         four = rem >= Q && ch0 + 32 <= p.V;
-        uint16_t* oc = os + (int64_t)c * Q * ostride;
+        char* oc = (char*)(os + (int64_t)c * Q * ostride);
+        const uint32_t o0 = ((uint32_t)col * (uint32_t)ostride + 8 * hh) * 2u;  // (a chunk's rows are reached by 32-bit offsets)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int tt = y == 0 ? ta : 1 - ta;
@@ -685,10 +686,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
             const auto r0 = __builtin_amdgcn_permlane32_swap((uint32_t)two[k2][0], (uint32_t)two[k2][2], false, false);
             const auto r1 = __builtin_amdgcn_permlane32_swap((uint32_t)two[k2][1], (uint32_t)two[k2][3], false, false);
             const lq_v4i o = {(int)r0[0], (int)r1[0], (int)r0[1], (int)r1[1]};
-            const int t = 32 * tt + col, n = 16 * k2 + 8 * hh;
-            uint16_t* to = oc + (uint32_t)t * (uint32_t)ostride + n;
-            if (four) *(lq_v4i*)to = o;
-            else if (t < rem && ch0 + n < p.V) *(lq_v4i*)to = o;
+            char* to = oc + 64 * tt * ostride + 32 * k2;
+            if (four) *(lq_v4i*)(to + o0) = o;
+            else if (32 * tt + col < rem && ch0 + 16 * k2 + 8 * hh < p.V) *(lq_v4i*)(to + o0) = o;
           }
         }
       }
@@ -793,17 +793,19 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
   r.waves = a->vdim <= 64 ? 2 : 4;
   r.parts = (a->vdim + 32 * r.waves - 1) / (32 * r.waves);
   const int64_t parts = (int64_t)a->nheads * r.parts;
-  // Tenths of a microsecond.  A chunk's step takes 40 where a compute unit has one workgroup and 75 where it has two, one of the states' 27 and
-  // 44; the join moves every segment's state three times at 6 TB/s, and it and two more launches come to 100.  Measured, heads of 128 by 128:
-  // 500 tokens of 16 heads uncut 34 us, in segments of 4 chunks 35, of 2 and of one 26; 2 prompts of 8192, 32 heads, in segments of 32 chunks 249, of
-  // 16 205, of 8 229; 10 packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 153, of 12 chunks 119, 8 89, 6 82, 4 94.  Packed
-  // prompts' lengths are not known here: the longest is taken to be two and a half times the mean.
+  // Tenths of a microsecond.  A chunk's step takes 42 where a compute unit has one workgroup and 72 where it has two, one of the states' 27 and
+  // 38; the join moves every segment's state three times at 2.6 TB/s (more where there are many), and it and two more launches come to 100.
+  // Measured, heads of 128 by 128, by the chunks of a segment: 500 tokens of 16 heads uncut 34 us, 2 chunks 26, one 26; 2 prompts of 8192, 32
+  // heads, 32 chunks 249 us, 16 203, 8 229; 4 of 4096, 16 heads, 16 chunks 115, 12 120, 8 102; one of 16384, 8 heads, 16 chunks 106, 8 71; 10
+  // packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 153, 12 chunks 119, 8 86, 6 80, 5 87, 4 94.  A segment's own state in two
+  // pieces: 2 prompts of 8192 208, 4 of 4096 115.  Packed prompts' lengths are not known here: the longest is taken to be two and a half times
+  // the mean.
   const double mean = (double)units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
   auto step = [&](double wgs, double one, double two) {
     if (wgs <= 256) return one;
     return a->seq_starts && wgs <= 512 ? one + (two - one) * (wgs / 256 - 1) : two * std::ceil(wgs / 512);
   };
-  double best = chain * step((double)nseq * parts, 40, 75);
+  double best = chain * step((double)nseq * parts, 42, 72);
   r.seg_chunks = (int)most, r.cut = 0;
   int64_t seen = 0;
   for (int64_t k = 2; k <= 256; ++k) {  // segments of the longest
@@ -811,7 +813,7 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
     if (n == seen) continue;
     seen = n;
     const double segs = a->seq_starts ? (double)units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n)), ahead = std::max(0.0, segs - nseq);
-    const double cost = n * step(segs * parts, 40, 75) + n * step(ahead * parts, 27, 44) + (ahead + 2 * segs) * a->nheads * a->kdim * a->vdim * 4 / 6e5 + 100;
+    const double cost = n * step(segs * parts, 42, 72) + n * step(ahead * parts, 27, 38) + (ahead + 2 * segs) * a->nheads * a->kdim * a->vdim * 4 / 2.6e5 + 100;
     if (n < most && cost < best) best = cost, r.seg_chunks = (int)n, r.cut = 1;
   }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
