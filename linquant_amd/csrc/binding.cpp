@@ -929,8 +929,8 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// the tensors of nested lists and tuples: three numbers each
-bool slot_tensors(PyObject* o, const c10::Device& dev, int64_t& slots, std::vector<int64_t>& out) {
+// the tensors of nested lists and tuples (of ones that contain themselves: none): three numbers each
+bool slot_tensors(PyObject* o, const c10::Device& dev, int64_t& slots, std::vector<int64_t>& out, int depth = 0) {
   if (THPVariable_CheckExact(o)) {
     Tensor t;
     if (!plain(o, dev, t) || t.dim() < 1 || !fits(t.sizes())) return false;
@@ -946,10 +946,10 @@ bool slot_tensors(PyObject* o, const c10::Device& dev, int64_t& slots, std::vect
     return true;
   }
   const bool list = PyList_CheckExact(o);
-  if (!list && !PyTuple_Check(o)) return false;
+  if ((!list && !PyTuple_Check(o)) || depth == 16) return false;
   const Py_ssize_t n = list ? PyList_GET_SIZE(o) : PyTuple_GET_SIZE(o);
   for (Py_ssize_t i = 0; i < n; ++i)
-    if (!slot_tensors(list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i), dev, slots, out)) return false;
+    if (!slot_tensors(list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i), dev, slots, out, depth + 1)) return false;
   return true;
 }
 
