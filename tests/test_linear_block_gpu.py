@@ -189,6 +189,23 @@ def test_slots_of_a_mixers_state(cuda):
         copy_slots(loop, src, dst)
 
 
+@pytest.mark.parametrize("n", [3, 64, 65, 700, 5000, 8192])
+@pytest.mark.parametrize("kind", ["all to one", "a few", "far apart", "every one twice"])
+def test_many_entries_with_one_destination(cuda, n, kind):
+    """The last entry of a destination counts, however many there are and however their numbers lie."""
+    gen = torch.Generator().manual_seed(n)
+    slots = 9000
+    t = torch.arange(slots, device=cuda)[:, None].repeat(1, 3)
+    dst = {"all to one": torch.full((n,), 5), "a few": torch.randint(0, 7, (n,), generator=gen) * 1024, "far apart": torch.randperm(9, generator=gen)[torch.arange(n) % 9] * 1000 % slots,
+           "every one twice": torch.randperm(slots, generator=gen)[:(n + 1) // 2].repeat(2)[:n]}[kind]
+    src = torch.randint(0, slots, (n,), generator=gen)
+    want = t.cpu().clone()
+    for s, d in zip(src.tolist(), dst.tolist()):
+        want[d] = s
+    copy_slots(t, src.to(I32).to(cuda), dst.to(I32).to(cuda))
+    assert torch.equal(t.cpu(), want)
+
+
 # ---------------------------------------------------------------------------------------------- native and general calls
 def _both_ways(monkeypatch, name, call, native):
     """The call as it is and without its native form: the same bits; whether the native form served it."""
