@@ -847,6 +847,7 @@ typedef struct {
   const void* adapter_up;    /* (adapter_count, cols, adapter_rank) dense, 16-byte aligned */
   int32_t adapter_dtype;     /* LQ_DT_F16 / LQ_DT_BF16 */
   int32_t adapter_rank, adapter_count; /* rank a multiple of 16, up to 128 */
+  const int32_t* adapter_order; /* NULL, or what lq_adapter_down leaves in `order` */
 } lq_int8_matmul_args;
 int lq_int8_matmul(const lq_int8_matmul_args* args, hipStream_t stream);
 
@@ -1069,6 +1070,8 @@ typedef struct {
   int32_t rows, inner, inner_padded, rank, count; /* inner_padded and rank multiples of 16, rank up to 128 */
   int8_t* codes_out;         /* NULL, or also what lq_quantize_rows makes of x (16 bits, inner a multiple of 8 up to 16384): (rows, inner) dense */
   float* scale_out;          /* (rows,), with codes_out */
+  int32_t* order;            /* NULL, or (rows,): the rows in an order in which those with one id lie together, each within its 512; the product
+                                takes them in it, in fewer passes, and writes them where they belong */
 } lq_adapter_down_args;
 int lq_adapter_down(const lq_adapter_down_args* args, hipStream_t stream);
 

@@ -1,10 +1,16 @@
 // lq_adapter_down: the first half of low-rank adapters of many requests, h[m] = scaling[j] * (down[j] x[m]), j = ids[m], in fp32; the second
 // half is the epilogue of lq_int8_matmul.
 //
-// Two kernels.  `rows`: few rows, each with a request of its own as a rule: a wave has two of a row's sums, so that the adapters stream from
-// memory through many waves.  `tiles`: 16 rows of x to a workgroup, its waves share the contraction, and what meets the rows are the
-// matrix instructions; the adapters that the 16 rows name are taken one after the other, each with all 16 rows, and a row keeps what its own
-// gave (nothing is multiplied by zero: an infinity in one request's row or adapter stays there).  Rows of a prompt name one as a rule.
+// Three kernels.  `rows`, up to 256 rows, each with a request of its own as a rule: a wave has two of a row's sums, so that the adapters stream
+// from memory through many waves; the quantizer of the rows, if the call has one, runs in the same launch.  16 rows of 2560 entries, rank 16,
+// 16 adapters, with the quantizer: 4.0 us, where the launch of an empty kernel takes 2.
+// `staged`, and `tiles` for rows that are no whole 16-byte pieces: 16 rows of x to a workgroup, its waves share the contraction, and what meets
+// the rows are the matrix instructions; the adapters that the 16 rows name are taken one after the other, each with all 16 rows, and a row keeps
+// what its own gave (nothing is multiplied by zero: an infinity in one request's row or adapter stays there).  The bound is memory: 16384 rows of
+// 2560 in 16 bits, 84 MB, rank 16, in 15 us 5.5 TB/s (from the cache behind HBM, where the quantizer left them); 3001 rows of 5120 codes, rank 32, 16 us,
+// where a workgroup's 10 stages one after the other are what it waits for.
+// Rows that name adapters in turn would cost as many passes as there are adapters, so they are taken in an order (below).  us, 310 rows of 5120
+// codes, rank 8, 8 adapters in turn: 44 in their own order, 15 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 37, 14.
 // v_mfma_f32_16x16x32: lane l has row l & 15 and the 8 contraction entries of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
 // down is the operand of the rows, so that a lane holds four adjacent sums of one row of x.
 //
@@ -25,7 +31,79 @@ struct DownParams {
   int rows, inner, padded, rank, count;
   int8_t* codes_out;  // NULL, or x's codes and scales as well
   float* scale_out;
+  int32_t* order;  // NULL, or an order of the rows
 };
+
+// An order of the rows in which those that name one adapter lie together, within windows of 64 W rows; one thread has one row.  What a
+// tile of 16 rows costs here, and one of 32 in the product's epilogue, is one pass for each adapter that it names.  A window with few changes
+// between neighbours stays as it is.  Groups lie in the order of their first rows, a group's rows in their own: the same for the same ids, always.
+constexpr int kWindow = 512, kFewChanges = 16;
+template <int W>
+struct Order {
+  int key[64 * W], first[64 * W], start[W][64 * W], part[W];
+};
+template <int W>
+LQ_DEV int window_place(const int32_t* ids, int n, int count, Order<W>& o) {  // the place of the window's row `threadIdx.x`; n: rows of the window
+  constexpr int N = 64 * W;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const bool in = t < n;
+  const int key = in ? max(-1, min(ids[t], count)) : -2;
+  o.key[t] = key, o.first[t] = N;
+#pragma unroll
+  for (int w = 0; w < W; ++w) o.start[w][t] = 0;
+  __syncthreads();
+  if (__syncthreads_count(in && t > 0 && o.key[t - (t > 0)] != key) <= kFewChanges) return t;
+  uint64_t same = 0;  // the wave's rows with this key
+  for (uint64_t left = __ballot(in); left;) {
+    const int k = __builtin_amdgcn_readlane(key, __builtin_ctzll(left));
+    const uint64_t m = __ballot(key == k);
+    if (key == k) same = m;
+    left &= ~m;
+  }
+  const bool leads = in && __builtin_ctzll(same) == lane;
+  // the key's first row in the window: at a place of the table that the key names; who finds another key's there tries others
+  int first = -1;
+  for (int round = 0;; ++round) {
+    const int at = round == 0 ? key & (N - 1) : (int)(((uint32_t)key * (0x9e3779b1u + 2u * round)) >> 16) & (N - 1);
+    if (leads && first < 0) atomicMin(&o.first[at], t);
+    __syncthreads();
+    if (leads && first < 0 && o.key[o.first[at]] == key) first = o.first[at];
+    const bool open = __syncthreads_or(leads && first < 0);
+    if (!open) break;
+    o.first[t] = N;
+    __syncthreads();
+  }
+  if (leads) o.start[wave][first] = __builtin_popcountll(same);
+  __syncthreads();
+  int rows[W], sum = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) rows[w] = o.start[w][t], sum += rows[w];
+  int upto = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int v = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += v;
+  }
+  if (lane == 63) o.part[wave] = upto;
+  __syncthreads();
+  int at = upto - sum;
+  for (int w = 0; w < wave; ++w) at += o.part[w];
+#pragma unroll
+  for (int w = 0; w < W; ++w) o.start[w][t] = at, at += rows[w];
+  __syncthreads();
+  const int f = __shfl(first, same ? __builtin_ctzll(same) : lane, 64);
+  return in ? o.start[wave][f] + __builtin_popcountll(same & ((1ull << lane) - 1)) : t;
+}
+// The rows of the 16 places from m0 on, to LDS and to the call's order
+template <int W>
+LQ_DEV void ordered_rows(const DownParams& p, int m0, Order<W>& o, int (&rows)[16]) {
+  const int w0 = m0 / (64 * W) * (64 * W), n = min(64 * W, p.rows - w0), i = w0 + window_place<W>(p.ids + w0, n, p.count, o) - m0, row = w0 + (int)threadIdx.x;
+  if ((int)threadIdx.x < n && i >= 0 && i < 16) {
+    rows[i] = row;
+    if (p.order) p.order[m0 + i] = row;
+  }
+  __syncthreads();
+}
 
 template <typename T>
 LQ_DEV lq_v4f mfma16(lq_v4i a, lq_v4i b, lq_v4f c) {
@@ -79,6 +157,12 @@ constexpr int kPer = 2;  // sums of a wave in `rows`
 template <typename T, bool CODES, bool EIGHTS, int QV>
 __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
   int m = blockIdx.x, lane = threadIdx.x & 63;
+  if (p.order && m-- == 0) {  // the first workgroup: the order
+    __shared__ Order<4> o;
+    const int at = window_place<4>(p.ids, p.rows, p.count, o);
+    if ((int)threadIdx.x < p.rows) p.order[at] = threadIdx.x;
+    return;
+  }
   if constexpr (QV > 0) {
     if (m < p.rows) {
       __shared__ float lds[4];
@@ -133,17 +217,18 @@ __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
 
 // the waves' sums together, and out
 template <bool CODES, int RT, int W>
-LQ_DEV void down_finish(const DownParams& p, int m0, const lq_v4f (&keep)[RT], lq_v4f (&sums)[W][RT][64]) {
+LQ_DEV void down_finish(const DownParams& p, int m0, const int (&rows)[16], const lq_v4f (&keep)[RT], lq_v4f (&sums)[W][RT][64]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int t = 0; t < RT; ++t) sums[wave][t][lane] = keep[t];
   __syncthreads();
   for (int i = threadIdx.x; i < RT * 64; i += 64 * W) {
-    const int t = i >> 6, l = i & 63, row = m0 + (l & 15);
+    const int t = i >> 6, l = i & 63;
     lq_v4f v = sums[0][t][l];
 #pragma unroll
     for (int w = 1; w < W; ++w) v += sums[w][t][l];
-    if (row >= p.rows) continue;
+    if (m0 + (l & 15) >= p.rows) continue;
+    const int row = rows[l & 15];
     const int own = p.ids[row];
     const float f = own >= 0 && own < p.count ? factor<CODES>(p, row, own) : 1.0f;
 #pragma unroll
@@ -157,8 +242,12 @@ template <typename T, bool CODES, bool EIGHTS, int RT, int W>
 __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
   constexpr int U = RT <= 2 ? 4 : RT <= 4 ? 2 : 1;
   __shared__ __align__(16) lq_v4f sums[W][RT][64];
+  __shared__ Order<W> order;
+  __shared__ int rows[16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
-  const int m0 = blockIdx.x * 16, m = min(m0 + (lane & 15), p.rows - 1);
+  const int m0 = blockIdx.x * 16;
+  ordered_rows<W>(p, m0, order, rows);
+  const int m = rows[min(lane & 15, p.rows - 1 - m0)];
   const int id = p.ids[m];
   const void* x = row_of<T, CODES>(p, m);
   lq_v4f keep[RT];
@@ -201,7 +290,7 @@ __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
       if (mine) keep[t] = acc[t];
     }
   }
-  down_finish<CODES, RT, W>(p, m0, keep, sums);
+  down_finish<CODES, RT, W>(p, m0, rows, keep, sums);
 }
 
 // The same, x and down through LDS in stages of SE entries, each row's whole 16-byte pieces fetched side by side: as operands they are read
@@ -213,12 +302,19 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
   constexpr int XR = 1024 / XB, DR = 1024 / DB;                             // rows of a fetch
   constexpr int XF = 16 / XR, DF = RT * 16 / DR, kStage = 16 * XB + RT * 16 * DB;  // fetches of a stage
   constexpr int H = SE / (32 * W);                                          // products of a wave and stage
-  static_assert(2 * kStage >= W * RT * 1024);
+  static_assert(2 * kStage >= W * RT * 1024 && 2 * kStage >= sizeof(Order<W>) && kWindow == 64 * W);
   __shared__ __align__(1024) char lds[2][kStage];
+  __shared__ int rows[16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, r16 = lane & 15;
-  const int m0 = blockIdx.x * 16, m = min(m0 + r16, p.rows - 1);
+  const int m0 = blockIdx.x * 16, w0 = m0 / kWindow * kWindow;
+  ordered_rows<W>(p, m0, *(Order<W>*)lds, rows);
+  auto row_at = [&](int i) { return rows[min(i, min(15, p.rows - 1 - m0))]; };
+  const int m = row_at(r16);
   const int id = p.ids[m];
-  const char* x = (const char*)p.x + m0 * p.x_stride * (CODES ? 1 : 2);
+  const char* x = (const char*)p.x + w0 * p.x_stride * (CODES ? 1 : 2);  // (the window's rows by 32-bit offsets)
+  uint32_t xoff[(XF + W - 1) / W];
+#pragma unroll
+  for (int i = 0; i < (XF + W - 1) / W; ++i) xoff[i] = (uint32_t)(row_at((i * W + wave) * XR + lane / (64 / XR)) - w0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u);
   lq_v4f keep[RT];
   const float none = id < 0 ? 0.0f : __builtin_nanf("");
 #pragma unroll
@@ -235,7 +331,7 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
 #pragma unroll
       for (int i = 0; i < (XF + W - 1) / W; ++i) {
         const int f = i * W + wave, row = f * XR + lane / (64 / XR), c = (lane % (64 / XR)) ^ (row & 15);
-        if (f < XF) sv_fetch16(x, (uint32_t)min(row, p.rows - 1 - m0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u) + (uint32_t)min(s * XB + c * 16, xlast), to + f * 1024);
+        if (f < XF) sv_fetch16(x, xoff[i] + (uint32_t)min(s * XB + c * 16, xlast), to + f * 1024);
       }
 #pragma unroll
       for (int i = 0; i < (DF + W - 1) / W; ++i) {
@@ -281,10 +377,10 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
       if (mine) keep[t] = acc[t];
     }
   }
-  down_finish<CODES, RT, W>(p, m0, keep, *(lq_v4f(*)[W][RT][64])lds);  // (nothing of a stage is read any more)
+  down_finish<CODES, RT, W>(p, m0, rows, keep, *(lq_v4f(*)[W][RT][64])lds);  // (nothing of a stage is read any more)
 }
 
-constexpr int kFewRows = 256;
+constexpr int kFewRows = 256;  // (as many as a workgroup of `rows` has threads, which find their order)
 
 }  // namespace
 
@@ -296,15 +392,15 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
   const bool codes = a->x_dtype == LQ_DT_I8;
   // (rows that are not whole eights of entries are read one by one)
   if (a->inner % 8 == 0 ? !sv_al(a->x, codes ? 8 : 16) || a->x_stride % 8 != 0 : !sv_al(a->x, codes ? 1 : 2)) return LQ_ERR_SHAPE;
-  if (!sv_al(a->down, 16) || !sv_al(a->h, 16) || !sv_al(a->x_scale, 4) || !sv_al(a->scaling, 4) || !sv_al(a->ids, 4))
+  if (!sv_al(a->down, 16) || !sv_al(a->h, 16) || !sv_al(a->x_scale, 4) || !sv_al(a->scaling, 4) || !sv_al(a->ids, 4) || !sv_al(a->order, 4))
     return LQ_ERR_SHAPE;
   DownParams p = {a->x, a->x_stride, a->x_scale, a->x_scale_rows, (const uint16_t*)a->down, a->scaling, a->ids, a->h, a->rows, a->inner, a->inner_padded, a->rank, a->count,
-                  a->codes_out, a->scale_out};
+                  a->codes_out, a->scale_out, a->order};
   const bool eights = a->inner % 8 == 0;
   if (a->codes_out && (!a->scale_out || codes || !eights || a->inner > 16384 || !sv_al(a->codes_out, 8) || !sv_al(a->scale_out, 4))) return LQ_ERR_SHAPE;
   using std::integral_constant;
   auto rows = [&](auto t, auto c, auto e, auto qv) {
-    const int64_t wgs = (int64_t)a->rows * ((a->rank + 4 * kPer - 1) / (4 * kPer)) + (decltype(qv)::value ? a->rows : 0);
+    const int64_t wgs = (int64_t)a->rows * ((a->rank + 4 * kPer - 1) / (4 * kPer)) + (decltype(qv)::value ? a->rows : 0) + (a->order ? 1 : 0);
     hipLaunchKernelGGL((down_rows_kernel<decltype(t), decltype(c)::value, decltype(e)::value, decltype(qv)::value>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
     return lq_check_launch();
   };
@@ -326,7 +422,7 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
     }
     if (a->rows <= kFewRows) return rows(t, c, e, integral_constant<int, 0>{});
     // whole 16-byte pieces of both
-    const bool pieces = E && a->inner % (C ? 16 : 8) == 0 && a->x_stride % (C ? 16 : 8) == 0 && sv_al(a->x, 16) && a->x_stride >= 0 && a->x_stride < 1 << 24;
+    const bool pieces = E && a->inner % (C ? 16 : 8) == 0 && a->x_stride % (C ? 16 : 8) == 0 && sv_al(a->x, 16) && a->x_stride >= 0 && a->x_stride < 1 << 22;
     auto tiles = [&](auto rt) {
       constexpr int RT = decltype(rt)::value, W = RT <= 4 ? 8 : 4;
       if (pieces) {

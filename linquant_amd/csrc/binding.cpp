@@ -874,7 +874,7 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 10) Py_RETURN_NONE;
   c10::Device dev(c10::DeviceType::CPU);
-  Tensor x, xs, w, ws, bias, down, up, scaling, ids, codes, h, out;
+  Tensor x, xs, w, ws, bias, down, up, scaling, ids, codes, h, order, out;
   if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !optional(arg[1], dev, xs) || !plain(arg[2], dev, w) || !plain(arg[3], dev, ws) || !optional(arg[4], dev, bias) ||
       !plain(arg[6], dev, down) || !plain(arg[7], dev, up) || !plain(arg[8], dev, scaling) || !plain(arg[9], dev, ids))
     Py_RETURN_NONE;
@@ -908,10 +908,11 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
       codes = empty({M, K}, ScalarType::Char, dev), xs = empty({M}, ScalarType::Float, dev);
       d.codes_out = (int8_t*)codes.data_ptr(), d.scale_out = (float*)xs.data_ptr();
     }
+    if (M > 64) order = empty({M}, ScalarType::Int, dev);
     {
       d.x = x.const_data_ptr(), d.x_stride = K, d.x_dtype = coded ? LQ_DT_I8 : code(x.scalar_type()), d.x_scale = coded ? f32(xs) : nullptr, d.x_scale_rows = xs.numel() != 1;
       d.down = down.const_data_ptr(), d.dtype = code(down.scalar_type()), d.scaling = f32(scaling), d.ids = i32(ids), d.h = (float*)h.data_ptr();
-      d.rows = (int)M, d.inner = (int)K, d.inner_padded = (int)K, d.rank = (int)R, d.count = (int)count;
+      d.rows = (int)M, d.inner = (int)K, d.inner_padded = (int)K, d.rank = (int)R, d.count = (int)count, d.order = order.defined() ? (int32_t*)order.data_ptr() : nullptr;
       rc = adapter_down_entry(&d, stream);
     }
     if (rc == 0) {
@@ -920,7 +921,7 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
       a.a_scale = f32(xs), a.b_scale = f32(ws), a.a_scale_rows = xs.numel() != 1 || !coded, a.b_scale_cols = 1;
       a.bias = at(bias), a.bias_dtype = bias.defined() ? code(bias.scalar_type()) : 0;
       a.out = out.data_ptr(), a.out_stride = N, a.out_dtype = code(ot), a.rows = (int)M, a.cols = (int)N, a.inner = (int)K;
-      a.adapter_h = f32(h), a.adapter_ids = i32(ids), a.adapter_up = up.const_data_ptr(), a.adapter_dtype = code(up.scalar_type()), a.adapter_rank = (int)R, a.adapter_count = (int)count;
+      a.adapter_h = f32(h), a.adapter_ids = i32(ids), a.adapter_up = up.const_data_ptr(), a.adapter_dtype = code(up.scalar_type()), a.adapter_rank = (int)R, a.adapter_count = (int)count, a.adapter_order = i32(order);
       rc = matmul_entry(&a, stream);
     }
   }

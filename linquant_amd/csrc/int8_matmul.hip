@@ -39,7 +39,9 @@ struct MatmulParams {
   const int32_t* ids;
   const uint16_t* up;
   int rank, count;
+  const int32_t* order;  // of the rows, within windows of kWindow; NULL: their own
 };
+constexpr int kWindow = 512;
 
 struct F32 {
   using type = float;
@@ -57,7 +59,11 @@ struct OutOf<F32> {
 // out += h up^T, each row with the adapter that it names.  In `tiles` a row's h enters the matrix instructions as two pieces of the
 // adapters' type (fp16: where it needs one, after a multiplication by a power of two that brings the row's largest below 2^14): off by 2^-16 of
 // the row's largest.  The adapters that 32 rows name are taken one after the other, with all 32, and a row keeps what its own
-// gave: nothing is multiplied by zero, and an infinity in one request's adapter stays there.
+// gave: nothing is multiplied by zero, and an infinity in one request's adapter stays there.  Rows are taken in the order that the first half
+// found, in which few of 32 differ: 128 x 2560 x 10576, rank 16, 16 adapters in turn 24 us, in the rows' own order 32, all of one adapter 20,
+// none 16; 1171 x 4096 x 2048, rank 64: 44, 94, 29, 23.  (The order is one load more in front of the first stage: 2% of 16384 x 2560 x 10576.)
+// Where 32 rows name one adapter and no h needs a unit, its product goes on from the projection's sums.  16384 x 2560 x 10576 with rank 16
+// takes 7% longer than without.  `rows`: a product of a row's h and its adapter's row in fp32 for each result.
 typedef float mm_v16f __attribute__((ext_vector_type(16)));
 template <typename T>
 LQ_DEV mm_v16f mfma32(lq_v4i a, lq_v4i b, mm_v16f c) {
@@ -133,20 +139,31 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
     const int band = i / (8 * nn), first = band * 8, high = min(8, nm - first), j = i - band * 8 * nn;
     m0 = (first + j % high) * TM, n0 = (j / high) * TN;
   }
+  // the row at a place of the order, and the first row that this workgroup may have
+  constexpr bool kAdapters = !std::is_void<A>::value;
+  const int w0 = kAdapters ? m0 / kWindow * kWindow : m0;
+  auto row_at = [&](int m) {
+    m = min(m, p.rows - 1);
+    if constexpr (kAdapters) {
+      static_assert(kWindow % TM == 0);
+      if (p.order) m = min(max(p.order[m], w0), min(w0 + kWindow, p.rows) - 1);
+    }
+    return m;
+  };
   const int fr = lane / PC;
   uint32_t offa[PA], offb[PB];
   auto piece = [&](int row) { return 16 * ((lane & (PC - 1)) ^ order(row)); };
 #pragma unroll
   for (int i = 0; i < PA; ++i) {
     const int row = FR * (wave * PA + i) + fr;
-    offa[i] = (uint32_t)min(row, p.rows - 1 - m0) * (uint32_t)p.a_stride + (uint32_t)piece(row);
+    offa[i] = (uint32_t)(row_at(m0 + row) - w0) * (uint32_t)p.a_stride + (uint32_t)piece(row);
   }
 #pragma unroll
   for (int i = 0; i < PB; ++i) {
     const int row = FR * (wave * PB + i) + fr;
     offb[i] = (uint32_t)min(row, p.cols - 1 - n0) * (uint32_t)p.b_stride + (uint32_t)piece(row);
   }
-  const int8_t* at = p.a + m0 * p.a_stride;
+  const int8_t* at = p.a + w0 * p.a_stride;
   const int8_t* bt = p.b + n0 * p.b_stride;
   const int ns = (p.inner + KB - 1) / KB;
   char* stage = lds + group * kStage;
@@ -178,8 +195,9 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
   };
   if (group < ns) fetch(group);
   float sa[MI];
+  int own[MI];  // this lane's rows
 #pragma unroll
-  for (int i = 0; i < MI; ++i) sa[i] = p.a_scale[p.a_scale_rows ? min(m0 + wm + 32 * i + (lane & 31), p.rows - 1) : 0];
+  for (int i = 0; i < MI; ++i) own[i] = row_at(m0 + wm + 32 * i + (lane & 31)), sa[i] = p.a_scale[p.a_scale_rows ? own[i] : 0];
   for (int i = tid; i < TN; i += 256 * KG) {
     const int n = min(n0 + i, p.cols - 1);
     sb[i] = p.b_scale[p.b_scale_cols ? n : 0];
@@ -255,7 +273,6 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
   for (int i = 0; i < MI; ++i) {
     const int m = m0 + wm + 32 * i;
     // adapters: this lane's row, the request that it names, the first adapter of the 32 rows and what it has for the columns, requested together
-    constexpr bool kAdapters = !std::is_void<A>::value;
     const float* h = nullptr;
     float unit = 1.0f;
     int id = -1, head = 0;
@@ -264,8 +281,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
     lq_v4i u0[kAdapters ? NI : 1], hi0 = {0, 0, 0, 0}, lo0 = {0, 0, 0, 0};
     auto up_of = [&](int a, int j) { return p.up + 8 * hh + ((int64_t)a * p.cols + min(n0 + wn + 32 * j + (lane & 31), p.cols - 1)) * p.rank; };
     if constexpr (kAdapters) {
-      const int mc = min(m + (lane & 31), p.rows - 1);
-      id = p.ids[mc], h = p.h + (int64_t)mc * p.rank + 8 * hh;
+      id = p.ids[own[i]], h = p.h + (int64_t)own[i] * p.rank + 8 * hh;
       named = __ballot(id >= 0 && id < p.count);
       if (named) {
         head = __builtin_amdgcn_readlane(id, __builtin_ctzll(named));
@@ -344,8 +360,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 && TM * TN <= 128 * 128 ? 3 : 2) 
     for (int r = 0; r < 32; r += kRows) {
       const int row = r + lane / kPieces, pc = lane % kPieces, n = n0 + wn + pc * kPer;
       const lq_v4i v = *(const lq_v4i*)(my + row * kOutRow + pc * 16);
+      int64_t to = 0;
+      if constexpr (kAdapters) to = __shfl(own[i], row, 64);
       if (m + row < p.rows) {
-        OT* o = out + (m + row) * p.out_stride + n;
+        OT* o = out + (kAdapters ? to : m + row) * p.out_stride + n;
         if (p.vec && n + kPer <= p.cols) {
           *(lq_v4i*)o = v;
         } else {
@@ -499,15 +517,15 @@ extern "C" int lq_int8_matmul(const lq_int8_matmul_args* a, hipStream_t stream) 
   if (a->adapter_h) {
     if (!a->adapter_ids || !a->adapter_up) return LQ_ERR_NULL;
     if (!sv_act(a->adapter_dtype) || a->adapter_rank <= 0 || a->adapter_rank % 16 != 0 || a->adapter_rank > 128 || a->adapter_count <= 0) return LQ_ERR_SHAPE;
-    if (!sv_al(a->adapter_h, 16) || !sv_al(a->adapter_up, 16) || !sv_al(a->adapter_ids, 4)) return LQ_ERR_SHAPE;
+    if (!sv_al(a->adapter_h, 16) || !sv_al(a->adapter_up, 16) || !sv_al(a->adapter_ids, 4) || !sv_al(a->adapter_order, 4)) return LQ_ERR_SHAPE;
   }
   const int per = 16 / sv_size(a->out_dtype);
   MatmulParams p = {a->a, a->a_stride, a->b, a->b_stride, a->a_scale, a->b_scale, a->a_scale_rows, a->b_scale_cols, a->bias, a->bias_dtype,
-                    a->out, a->out_stride, a->rows, a->cols, a->inner, sv_al(a->out, 16) && a->out_stride % per == 0, nullptr, nullptr, nullptr, 0, 0};
+                    a->out, a->out_stride, a->rows, a->cols, a->inner, sv_al(a->out, 16) && a->out_stride % per == 0, nullptr, nullptr, nullptr, 0, 0, nullptr};
   auto with = [&](auto t) {
     using O = decltype(t);
     if (!a->adapter_h) return launch<O, void>(p, stream);
-    p.h = a->adapter_h, p.ids = a->adapter_ids, p.up = (const uint16_t*)a->adapter_up, p.rank = a->adapter_rank, p.count = a->adapter_count;
+    p.h = a->adapter_h, p.ids = a->adapter_ids, p.up = (const uint16_t*)a->adapter_up, p.rank = a->adapter_rank, p.count = a->adapter_count, p.order = a->adapter_order;
     return a->adapter_dtype == LQ_DT_F16 ? launch<O, F16>(p, stream) : launch<O, BF16>(p, stream);
   };
   if (a->out_dtype == LQ_DT_F32) return with(F32{});

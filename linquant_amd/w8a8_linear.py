@@ -12,6 +12,7 @@ from linquant_amd.w4a8_linear import _fused_fp16_to_int8
 
 _CODES = {torch.float16: _lib.LQ_DT_F16, torch.bfloat16: _lib.LQ_DT_BF16, torch.float32: _lib.LQ_DT_F32}
 _K = 16  # the product's contraction length is a multiple of this
+_ONE_BY_ONE = 64  # up to so many rows the product takes each row's adapter by itself, in any order
 
 
 def _padded(n):
@@ -57,7 +58,7 @@ def _scale(s, n, device, what):
 
 
 def _matmul(a, b, a_scale, b_scale, bias, out, adapted=None):
-    """a (M, K), b (N, K) in rows of whole 16-byte pieces; out (M, N) with unit column stride; ``adapted``: what adapters add (h, ids, adapters)."""
+    """a (M, K), b (N, K) in rows of whole 16-byte pieces; out (M, N) with unit column stride; ``adapted``: what adapters add ((h, order), ids, adapters)."""
     (M, K), N = a.shape, b.shape[0]
     a, b = (t if t.stride(0) < 1 << 23 else t.contiguous() for t in (a, b))
     a_scale, per_row = _scale(a_scale, M, a.device, "a_scale")
@@ -66,8 +67,8 @@ def _matmul(a, b, a_scale, b_scale, bias, out, adapted=None):
     _lib.same_device(a, b, a_scale, b_scale, bias, out)
     low = {}
     if adapted is not None:
-        h, ids, adapters = adapted
-        low = dict(adapter_h=_lib.ptr(h), adapter_ids=_lib.ptr(ids), adapter_up=_lib.ptr(adapters.up), adapter_dtype=_CODES[adapters.up.dtype],
+        (h, order), ids, adapters = adapted
+        low = dict(adapter_order=_lib.ptr(order), adapter_h=_lib.ptr(h), adapter_ids=_lib.ptr(ids), adapter_up=_lib.ptr(adapters.up), adapter_dtype=_CODES[adapters.up.dtype],
                    adapter_rank=adapters.up.shape[2], adapter_count=adapters.up.shape[0])
     if M and N:
         _lib.call("lq_int8_matmul", a.device, a=_lib.ptr(a), a_stride=a.stride(0), b=_lib.ptr(b), b_stride=b.stride(0),
@@ -127,7 +128,7 @@ class LowRankAdapters(nn.Module):
         return self
 
     def _down(self, x, x_scale, ids):
-        """x (M, K) of the adapters' type, or codes (M, K or more) with their scale: h (M, padded R) fp32."""
+        """x (M, K) of the adapters' type, or codes (M, K or more) with their scale: h (M, padded R) fp32, and the rows' order or None."""
         M = x.shape[0]
         assert ids.dtype == torch.int32 and ids.shape == (M,), f"ids: one int32 for each of {M} rows"
         assert x.dtype in (torch.int8, self.down.dtype), f"x and the adapters: one type, got {x.dtype} and {self.down.dtype}"
@@ -136,11 +137,12 @@ class LowRankAdapters(nn.Module):
         x = _lib.rows16(x) if self.in_features % 8 == 0 else x if x.stride(1) == 1 else x.contiguous()
         n, R, K = self.down.shape
         h = torch.empty(M, R, dtype=torch.float32, device=x.device)
+        order = torch.empty(M, dtype=torch.int32, device=x.device) if M > _ONE_BY_ONE else None
         if M:
             _lib.call("lq_adapter_down", x.device, x=_lib.ptr(x), x_stride=x.stride(0), x_dtype=_lib.LQ_DT_I8 if x.dtype == torch.int8 else _CODES[x.dtype],
                       x_scale=_lib.ptr(scale), x_scale_rows=per_row, down=_lib.ptr(self.down), dtype=_CODES[self.down.dtype], scaling=_lib.ptr(self.scaling),
-                      ids=_lib.ptr(ids), h=_lib.ptr(h), rows=M, inner=self.in_features, inner_padded=K, rank=R, count=n)
-        return h
+                      ids=_lib.ptr(ids), h=_lib.ptr(h), order=_lib.ptr(order), rows=M, inner=self.in_features, inner_padded=K, rank=R, count=n)
+        return h, order
 
 
 class W8A8Linear(nn.Module):

@@ -189,6 +189,29 @@ def test_slots_of_a_mixers_state(cuda):
         copy_slots(loop, src, dst)
 
 
+@pytest.mark.parametrize("M,K,n", [(65, 128, 3), (130, 250, 70), (256, 128, 2000), (257, 128, 5), (511, 64, 40), (700, 128, 2000), (1300, 130, 6), (1537, 64, 900)])
+@pytest.mark.parametrize("ids", ["in turn", "random", "far apart", "few changes", "pairs"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_of_many_adapters_in_any_order(cuda, M, K, n, ids, dtype):
+    """Rows are taken in an order by their adapters and come back in their own; twice the same."""
+    gen = torch.Generator().manual_seed(M + n)
+    N, R = 70, 16
+    codes = torch.randint(-127, 128, (N, K), generator=gen).to(torch.int8)
+    ws = torch.rand(N, generator=gen) / 1000
+    a, b, s = (torch.randn(n, R, K, generator=gen) / K ** 0.5).to(dtype), (torch.randn(n, N, R, generator=gen) / 4).to(dtype), 0.25 + torch.rand(n, generator=gen)
+    lin, ad = W8A8Linear(codes, ws).to(cuda), LowRankAdapters(a, b, s).to(cuda)
+    x = torch.randn(M, K, generator=gen).to(dtype)
+    t = torch.arange(M)
+    idx = {"in turn": t % n, "random": torch.randint(-1, n + 1, (M,), generator=gen), "far apart": (t * 512 + t // 3 * 7) % n, "few changes": t * 9 // M % n,
+           "pairs": t // 2 * 5 % n}[ids].to(I32)
+    q, qs = quantize_rows(x.to(cuda))
+    want, mag, low = adapters_ref(q.cpu(), qs.cpu(), codes, ws, None, x, a, b, s, idx)
+    got = lin(x.to(cuda), adapters=ad, ids=idx.to(cuda))
+    # as for a few adapters: sums of K and R terms in 32 bits, h in two pieces
+    assert_near(got, want, mag * 4 * 2.0 ** -24 + low * (2.0 ** -24 * (K / 8 + R + 16) + 2.0 ** -14), 1.0, "adapted")
+    assert torch.equal(torch.nan_to_num(lin(x.to(cuda), adapters=ad, ids=idx.to(cuda))), torch.nan_to_num(got))
+
+
 @pytest.mark.parametrize("n", [3, 64, 65, 700, 5000, 8192])
 @pytest.mark.parametrize("kind", ["all to one", "a few", "far apart", "every one twice"])
 def test_many_entries_with_one_destination(cuda, n, kind):
