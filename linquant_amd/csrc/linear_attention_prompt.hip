@@ -793,29 +793,56 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
   r.waves = a->vdim <= 64 ? 2 : 4;
   r.parts = (a->vdim + 32 * r.waves - 1) / (32 * r.waves);
   const int64_t parts = (int64_t)a->nheads * r.parts;
-  // Tenths of a microsecond.  A chunk's step takes 42 where a compute unit has one workgroup and 72 where it has two, one of the states' 27 and
-  // 38; the join moves every segment's state three times at 2.6 TB/s (more where there are many), and it and two more launches come to 100.
+  // Tenths of a microsecond.  A chunk's step takes `one` where a compute unit has one workgroup and `full` where it has as many as fit
+  // (`fit`), one of the states' 0.64 and 0.53 of it; the join moves every segment's state three times at 2.6 TB/s (more where there are many),
+  // and it and two more launches come to 100.
   // Measured, heads of 128 by 128, by the chunks of a segment: 500 tokens of 16 heads uncut 34 us, 2 chunks 26, one 26; 2 prompts of 8192, 32
   // heads, 32 chunks 249 us, 16 203, 8 229; 4 of 4096, 16 heads, 16 chunks 115, 12 120, 8 102; one of 16384, 8 heads, 16 chunks 106, 8 71; 10
   // packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 153, 12 chunks 119, 8 86, 6 80, 5 87, 4 94.  A segment's own state in two
-  // pieces: 2 prompts of 8192 208, 4 of 4096 115.  Packed prompts' lengths are not known here: the longest is taken to be two and a half times
-  // the mean.
-  const double mean = (double)units / nseq, chain = a->seq_starts ? std::min<double>((double)most, 2.5 * mean) : (double)most;
-  auto step = [&](double wgs, double one, double two) {
-    if (wgs <= 256) return one;
-    return a->seq_starts && wgs <= 512 ? one + (two - one) * (wgs / 256 - 1) : two * std::ceil(wgs / 512);
+  // pieces: 2 prompts of 8192 208, 4 of 4096 115.
+  struct Step { double one, full; int fit; };
+  static constexpr Step steps[4][2] = {{{30, 50, 3}, {32, 42, 2}}, {{37, 59, 3}, {34, 51, 2}}, {{54, 60, 2}, {42, 72, 2}}, {{76, 76, 1}, {76, 76, 1}}};
+  const Step s = steps[a->kdim <= 32 ? 0 : a->kdim <= 64 ? 1 : a->kdim <= 128 ? 2 : 3][r.waves == 4];
+  auto step = [&](double wgs, double one, double full) {
+    double left = std::max(wgs / 256, 1.0), t = 0;
+    if (left > s.fit) t = std::floor(left / s.fit) * full, left -= std::floor(left / s.fit) * s.fit;
+    if (left == 0) return t;
+    if (!a->seq_starts) left = std::ceil(left);  // (prompts of many lengths: what ends early makes room)
+    return t + one + (full - one) * (left <= 1 ? 0 : (left - 1) / (s.fit - 1));
   };
-  double best = chain * step((double)nseq * parts, 42, 72);
+  // `longest`: chunks of the longest prompt, `segs` segments of which `ahead` have one behind them
+  auto cost = [&](double longest, double n, double segs, double ahead) {
+    if (n >= longest) return longest * step(segs * parts, s.one, s.full);
+    return n * step(segs * parts, s.one, s.full) + n * step(ahead * parts, 0.64 * s.one, 0.53 * s.full) + (ahead + 2 * segs) * a->nheads * a->kdim * a->vdim * 4 / 2.6e5 + 100;
+  };
+  // Packed prompts' lengths are not known here.  They may be alike, or the longest two and a half times the mean, or one has nearly all the tokens;
+  // taken is what loses least over the three, the second counted twice, each against what would be best for it.  us, taken, best and uncut:
+  // the 10 prompts above 82, 82, 148; 10 of 695 75, 55, 55; one of 2000 among 60 single tokens 108, 93, 136; one of 4096 among 32, 32 heads, 227,
+  // 174, 264; 64 of 200, 32 heads, 204, 154, 154; 4 of 30 to 700, 8 heads of 64 by 64, 20, 20, 46; 3000 and 200 tokens, 8 heads of 256 by 128, 55, 55, 294.
+  const double mean = (double)units / nseq, rest = (double)nseq - 1;
+  auto costs = [&](int64_t n, double (&c)[3]) {
+    if (!a->seq_starts) {
+      const double segs = (double)(nseq * ((most + n - 1) / n));
+      c[0] = c[1] = c[2] = cost((double)most, (double)n, segs, segs - nseq);
+    } else {
+      const double alike = nseq * std::ceil(mean / n), some = std::max((double)units / n + 0.5 * nseq, (double)nseq), one = std::ceil((double)(units - nseq + 1) / n);
+      c[0] = cost(mean, (double)n, alike, alike - nseq);
+      c[1] = cost(std::min<double>((double)most, 2.5 * mean), (double)n, some, some - nseq);
+      c[2] = cost((double)(units - nseq + 1), (double)n, one + rest, one - 1);
+    }
+  };
+  double best[3] = {}, least = 0, c[3];
   r.seg_chunks = (int)most, r.cut = 0;
-  int64_t seen = 0;
-  for (int64_t k = 2; k <= 256; ++k) {  // segments of the longest
-    const int64_t n = std::max<int64_t>(1, (int64_t)std::ceil(chain / k));
-    if (n == seen) continue;
-    seen = n;
-    const double segs = a->seq_starts ? (double)units / n + 0.5 * nseq : (double)(nseq * ((most + n - 1) / n)), ahead = std::max(0.0, segs - nseq);
-    const double cost = n * step(segs * parts, 42, 72) + n * step(ahead * parts, 27, 38) + (ahead + 2 * segs) * a->nheads * a->kdim * a->vdim * 4 / 2.6e5 + 100;
-    if (n < most && cost < best) best = cost, r.seg_chunks = (int)n, r.cut = 1;
-  }
+  for (int pass = 0; pass < 2; ++pass)
+    for (int64_t n = most; n > 0; n = n > 16 ? n * 7 / 8 : n - 1) {  // (the whole first)
+      costs(n, c);
+      double loss = 0;
+      for (int i = 0; i < 3; ++i) {
+        if (pass == 0) best[i] = n == most ? c[i] : std::min(best[i], c[i]);
+        else loss += (i == 1 ? 2 : 1) * c[i] / best[i];
+      }
+      if (pass == 1 && (n == most || loss < least)) least = loss, r.seg_chunks = (int)n, r.cut = n < most;
+    }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
   r.segs = a->seq_starts ? std::min<int64_t>(units / r.seg_chunks + nseq, units) : nseq * per;
   if (!r.cut) r.segs = nseq;
