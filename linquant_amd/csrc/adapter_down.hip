@@ -7,7 +7,7 @@
 // `staged`, and `tiles` for rows that are no whole 16-byte pieces: 16 rows of x to a workgroup, its waves share the contraction, and what meets
 // the rows are the matrix instructions; the adapters that the 16 rows name are taken one after the other, each with all 16 rows, and a row keeps
 // what its own gave (nothing is multiplied by zero: an infinity in one request's row or adapter stays there).  The bound is memory: 16384 rows of
-// 2560 in 16 bits, 84 MB, rank 16, in 15 us 5.5 TB/s (from the cache behind HBM, where the quantizer left them); 3001 rows of 5120 codes, rank 32, 16 us,
+// 2560 in 16 bits, 84 MB, rank 16, in 18 us 4.7 TB/s (some of it from the cache behind HBM, where the quantizer left it); 3001 rows of 5120 codes, rank 32, 17 us,
 // where a workgroup's 10 stages one after the other are what it waits for.
 // Rows that name adapters in turn would cost as many passes as there are adapters, so they are taken in an order (below).  us, 310 rows of 5120
 // codes, rank 8, 8 adapters in turn: 44 in their own order, 15 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 37, 14.

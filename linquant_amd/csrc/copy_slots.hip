@@ -8,7 +8,7 @@
 // bytes up to 256 entries, 32 at 8192.
 //
 // 1 GiB of slots in another order (a copy of that size reaches 5.2 TB/s): 64 slots 5.1 TB/s, 256 4.9, 1024 4.8, 2048 4.5, 4096 3.9, 8192 2.7.
-// One layer's state of 2 MB to 4 slots: 6 us, most of it the launch and the list.
+// One layer's state of 2 MB to 4 slots: 6.7 us (floor 3.2), most of it the launch and the list.
 #include <algorithm>
 
 #include "serve_common.h"
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * kWaves) void copy_slots_kernel(CopyParams p) {
   int *from = list, *to = list + p.entries, *table = to + p.entries;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = p.entries, places = 1 << p.log_table;
-  if (n <= 64) {  // (the first wave by itself: 4 forks of 2 MB 6.1 us, by the table 8.1)
+  if (n <= 64) {  // (the first wave by itself: 4 forks of 2 MB 6.7 us, by the table 8.1)
     if (tid < n) {
       const int d = p.dst[tid], s = p.src[tid] < 0 ? (int)kClear : min(p.src[tid], p.num_slots);
       bool keep = d >= 0 && d < p.num_slots && d != s;

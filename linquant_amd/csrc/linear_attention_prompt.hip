@@ -8,12 +8,23 @@
 //   join       walks the segments: the state in front of each.  (states and join: only where prompts are cut into segments, because
 //              prompts times heads are too few for 256 compute units)
 //   chunks     walks a segment chunk by chunk, the state in registers
+// A workgroup has 128 columns of a head's state (64 where there are no more), a wave 32 of them over all K: the state and the chunk's products
+// with it never leave the wave.  q, k and v come to LDS by fetches that pass no registers, the next chunk's while one is multiplied.
+//
+// What bounds it.  2 prompts of 8192, 32 heads of 128 by 128, fp16: chunks 125 us for 537 MB (4.3 TB/s; the chunk's step alone, 4.2 us with one
+// workgroup to a compute unit and 7.0 with two, gives 112), states 67 for half of that once more, join 11; a copy's rate for what has to move is
+// 103.  10 packed prompts of 6949 tokens, 16 heads: 50, 25 and 8, by steps one after the other (up to 32 chunks in a prompt, 6 to a segment).  500
+// tokens of 16 heads: 10.6, 7.7 and 4.0, three launches and a chunk's step in each of two.  In a step of 4.2 us (fp16, cycles of 10000): waiting for the
+// chunk 330, its successor's fetches 880, q k 1205, weights and rounding 1150, meeting 600, the state 1840, outputs 2360, operands of v 1800.
+// Tried and no faster: fetches spread between the products, outputs' products between the state's, segments in the other order (so that the
+// caches still have what the states read last), a segment's own state as two pieces of 16 bits.
 //
 // Precision.  Activations enter the matrix products as they are, all sums are fp32, and so is the state.  What is formed in fp32 on the way
 // and reaches only o, which is rounded to the activations' type itself (weighted q . k, the state that q multiplies), enters rounded to
 // that type: half a step of each term.  What the state gathers over a prompt (weighted v) enters as two (fp16) or three (bf16) pieces of the
-// type: off by 2^-22 of itself, or not at all (two of bf16: the state 2.4e-6 off, here and in fp16 below 1e-6).  bf16 has the range of fp32.  fp16: after a multiplication by a power of two that brings the largest of what
-// is multiplied (a channel's state; its state and v; a row of 32 weighted q . k) below 2^14, so no size of activations overflows.
+// type: off by 2^-22 of itself, or not at all (two of bf16: the state 2.4e-6 off, here and in fp16 below 1e-6).  bf16 has the range of fp32.
+// fp16: after a multiplication by a power of two that brings the largest of what is multiplied (a channel's state; its state and v; a row of 32
+// weighted q . k) below 2^14, so no size of activations overflows.
 #include <algorithm>
 #include <cmath>
 

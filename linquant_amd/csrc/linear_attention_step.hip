@@ -5,6 +5,9 @@
 // A group of lanes has one row of the state's columns in pieces of 16 bytes, so that a wave's request covers whole 128-byte lines; each
 // thread keeps its columns' sums over its rows, and the rows' sums meet in LDS at the end.  Where sequences times heads are few, a head's
 // columns are cut into blocks of 32, a workgroup each.
+//
+// 256 sequences of 32 heads of 128 by 128: 211 us, 5.1 TB/s, the rate of a copy.  4 of 16 heads, 8 MB: 4.9 us, 2 of them the launch, then two
+// round trips to memory, one for the slot and one for the rest.
 #include "serve_common.h"
 
 namespace {
