@@ -363,57 +363,57 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     bool large = false;
     float change = 1.0f;
     if (live) {
-    const uint16_t* xl = vbuf[wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
+      const uint16_t* xl = vbuf[wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const lq_v2i lo = read_columns(xl + 16 * ks * 32), hi = read_columns(xl + (16 * ks + 8) * 32);
-      xp[ks] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
-    }
-    if constexpr (kHalf) {
-      // The channel's unit is at least one, so that no entry of v loses bits, and is kept while it brings the largest of v between 2^-1 and 2^4
-      // (weighted v is then evenly spaced by 2^-24 of that or less); but a state that is 2^100 above v would leave 32 bits.
-      uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          typedef uint16_t v2u __attribute__((ext_vector_type(2)));
-          top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
-        }
-      float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (no number where the lane has one that is none: its scale does not matter then)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m4[(e >> 1) & 3] = __builtin_elementwise_maximum(m4[(e >> 1) & 3], __builtin_fabsf(S[nt][e]));
-      const float m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m4[0], m4[1]), __builtin_elementwise_maximum(m4[2], m4[3]));
-      const float mx = channel_top(finite_size(T::to((uint16_t)max(top & 0xffffu, top >> 16)))), ms = channel_top(finite_size(m));
-      const float now = mx * unit_S;
-      const bool keep = mx == 0.0f || (now >= 0.5f && now < 16.0f) || (unit_S == 1.0f && now >= 0.5f);
-      float k = keep ? unit_S : scale_for<2, 0, 15>(mx);
-      if (ms > 0x1p100f) k = fminf(k, unit_S);
-      change = k * pow2_inverse(unit_S);
-      unit_S = k;
-      large = __ballot(mx * k >= 256.0f) != 0;
-      const uint32_t k16 = F16::from(k);
-      united = __ballot(k != 1.0f) != 0;
-      if (united) {
+      for (int ks = 0; ks < 4; ++ks) {
+        const lq_v2i lo = read_columns(xl + 16 * ks * 32), hi = read_columns(xl + (16 * ks + 8) * 32);
+        xp[ks] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
+      }
+      if constexpr (kHalf) {
+        // The channel's unit is at least one, so that no entry of v loses bits, and is kept while it brings the largest of v between 2^-1 and 2^4
+        // (weighted v is then evenly spaced by 2^-24 of that or less); but a state that is 2^100 above v would leave 32 bits.
+        uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-            const int two = xp[ks][i];  // (an element's bits are not cast in place)
-            xp[ks][i] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, two) * __builtin_bit_cast(v2h, k16 | k16 << 16));
+            typedef uint16_t v2u __attribute__((ext_vector_type(2)));
+            top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
           }
+        float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (no number where the lane has one that is none: its scale does not matter then)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m4[(e >> 1) & 3] = __builtin_elementwise_maximum(m4[(e >> 1) & 3], __builtin_fabsf(S[nt][e]));
+        const float m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m4[0], m4[1]), __builtin_elementwise_maximum(m4[2], m4[3]));
+        const float mx = channel_top(finite_size(T::to((uint16_t)max(top & 0xffffu, top >> 16)))), ms = channel_top(finite_size(m));
+        const float now = mx * unit_S;
+        const bool keep = mx == 0.0f || (now >= 0.5f && now < 16.0f) || (unit_S == 1.0f && now >= 0.5f);
+        float k = keep ? unit_S : scale_for<2, 0, 15>(mx);
+        if (ms > 0x1p100f) k = fminf(k, unit_S);
+        change = k * pow2_inverse(unit_S);
+        unit_S = k;
+        large = __ballot(mx * k >= 256.0f) != 0;
+        const uint32_t k16 = F16::from(k);
+        united = __ballot(k != 1.0f) != 0;
+        if (united) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+              const int two = xp[ks][i];  // (an element's bits are not cast in place)
+              xp[ks][i] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, two) * __builtin_bit_cast(v2h, k16 | k16 << 16));
+            }
+        }
+        if (!STATES) {
+          // (the accumulators are read before they are folded; what o is formed from is 1 / `old` of it)
+          const bool plain = change == 1.0f && (ms == 0.0f || (ms >= 0x1p-4f && ms < 0x1p15f));
+          read = plain ? 1.0f : scale_for<13, -100, 100>(ms);
+          calm = __ballot(!plain) == 0;
+          if (lane < 32) vunit[wave][lane] = pow2_inverse(unit_S), vunit[wave][32 + lane] = pow2_inverse(read) * change;
+        }
       }
-      if (!STATES) {
-        // (the accumulators are read before they are folded; what o is formed from is 1 / `old` of it)
-        const bool plain = change == 1.0f && (ms == 0.0f || (ms >= 0x1p-4f && ms < 0x1p15f));
-        read = plain ? 1.0f : scale_for<13, -100, 100>(ms);
-        calm = __ballot(!plain) == 0;
-        if (lane < 32) vunit[wave][lane] = pow2_inverse(unit_S), vunit[wave][32 + lane] = pow2_inverse(read) * change;
-      }
-    }
     }
     {
       // one factor of 2^-160 is zero in 32 bits, and sums of larger ones would cost the tokens behind them their last bits

@@ -123,8 +123,10 @@ class LowRankAdapters(nn.Module):
         self.register_buffer("scaling", scaling.to(torch.float32, copy=True).contiguous())
 
     def _apply(self, fn, *args, **kwargs):
+        scaling = self.scaling
         super()._apply(fn, *args, **kwargs)
-        self.scaling = self.scaling.float()  # (a module's .half() or .bfloat16() is for the adapters themselves)
+        if self.scaling.dtype != torch.float32:  # (a module's .half() or .bfloat16() is for the adapters themselves)
+            self.scaling = scaling.to(self.scaling.device)
         return self
 
     def _down(self, x, x_scale, ids):

@@ -149,3 +149,11 @@ def test_entry_points_refuse():
     assert rc("lq_copy_slots", **slots) == -22
     table[0] = 0
     assert rc("lq_copy_slots", **slots) == -14
+
+
+def test_adapters_keep_their_factors_when_a_module_changes_its_type():
+    f = torch.tensor([0.1, 3.0001])
+    ad = LowRankAdapters(z(2, 4, 32), z(2, 8, 4), f)
+    for other in (ad.bfloat16(), ad.half(), ad.to("cpu", F16)):
+        assert other is ad and torch.equal(ad.scaling, f) and ad.scaling.dtype == F32
+    assert ad.down.dtype == F16 and torch.equal(LowRankAdapters(z(2, 4, 32), z(2, 8, 4), f).double().scaling, f)
