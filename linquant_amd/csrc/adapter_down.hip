@@ -7,10 +7,10 @@
 // `staged`, and `tiles` for rows that are no whole 16-byte pieces: 16 rows of x to a workgroup, its waves share the contraction, and what meets
 // the rows are the matrix instructions; the adapters that the 16 rows name are taken one after the other, each with all 16 rows, and a row keeps
 // what its own gave (nothing is multiplied by zero: an infinity in one request's row or adapter stays there).  The bound is memory: 16384 rows of
-// 2560 in 16 bits, 84 MB, rank 16, in 18 us 4.7 TB/s (some of it from the cache behind HBM, where the quantizer left it); 3001 rows of 5120 codes, rank 32, 17 us,
+// 2560 in 16 bits, 84 MB, rank 16, in 18 us 4.7 TB/s (some of it from the cache behind HBM, where the quantizer left it); 3001 rows of 5120 codes, rank 32, 16 us,
 // where a workgroup's 10 stages one after the other are what it waits for.
 // Rows that name adapters in turn would cost as many passes as there are adapters, so they are taken in an order (below).  us, 310 rows of 5120
-// codes, rank 8, 8 adapters in turn: 44 in their own order, 15 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 37, 14.
+// codes, rank 8, 8 adapters in turn: 44 in their own order, 14 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 31, 12.
 // v_mfma_f32_16x16x32: lane l has row l & 15 and the 8 contraction entries of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
 // down is the operand of the rows, so that a lane holds four adjacent sums of one row of x.
 //
@@ -94,14 +94,11 @@ LQ_DEV int window_place(const int32_t* ids, int n, int count, Order<W>& o) {  //
   const int f = __shfl(first, same ? __builtin_ctzll(same) : lane, 64);
   return in ? o.start[wave][f] + __builtin_popcountll(same & ((1ull << lane) - 1)) : t;
 }
-// The rows of the 16 places from m0 on, to LDS and to the call's order
+// The rows of the 16 places from m0 on, to LDS
 template <int W>
 LQ_DEV void ordered_rows(const DownParams& p, int m0, Order<W>& o, int (&rows)[16]) {
   const int w0 = m0 / (64 * W) * (64 * W), n = min(64 * W, p.rows - w0), i = w0 + window_place<W>(p.ids + w0, n, p.count, o) - m0, row = w0 + (int)threadIdx.x;
-  if ((int)threadIdx.x < n && i >= 0 && i < 16) {
-    rows[i] = row;
-    if (p.order) p.order[m0 + i] = row;
-  }
+  if ((int)threadIdx.x < n && i >= 0 && i < 16) rows[i] = row;
   __syncthreads();
 }
 
@@ -219,6 +216,7 @@ __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
 template <bool CODES, int RT, int W>
 LQ_DEV void down_finish(const DownParams& p, int m0, const int (&rows)[16], const lq_v4f (&keep)[RT], lq_v4f (&sums)[W][RT][64]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (p.order && threadIdx.x < 16 && m0 + (int)threadIdx.x < p.rows) p.order[m0 + threadIdx.x] = rows[threadIdx.x];
 #pragma unroll
   for (int t = 0; t < RT; ++t) sums[wave][t][lane] = keep[t];
   __syncthreads();
@@ -295,15 +293,20 @@ __global__ __launch_bounds__(64 * W) void down_tiles_kernel(DownParams p) {
 
 // The same, x and down through LDS in stages of SE entries, each row's whole 16-byte pieces fetched side by side: as operands they are read
 // from memory 64 bytes of a row at a time, at half the rate.  Piece c of row r lies at place c ^ r % 16, so that the 16 rows that a read serves
-// at once touch each bank once.  Two places, one filled while the other is multiplied.
-template <typename T, bool CODES, int RT, int SE>
+// at once touch each bank once.  ST places, of which all but one are filled while that one is multiplied.
+template <typename T, bool CODES, int RT>
+struct Staged {
+  static constexpr int SE = RT <= 2 ? 512 : 256, bytes = (16 * (CODES ? 1 : 2) + RT * 16 * 2) * SE, deep = std::min(4, 150 * 1024 / bytes);
+};
+template <typename T, bool CODES, int RT, int ST>
 __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
-  constexpr int W = 8, XB = SE * (CODES ? 1 : 2), DB = SE * 2;              // bytes of a stage's row of x and of down
+  constexpr int W = 8, SE = Staged<T, CODES, RT>::SE, XB = SE * (CODES ? 1 : 2), DB = SE * 2;  // bytes of a stage's row of x and of down
   constexpr int XR = 1024 / XB, DR = 1024 / DB;                             // rows of a fetch
   constexpr int XF = 16 / XR, DF = RT * 16 / DR, kStage = 16 * XB + RT * 16 * DB;  // fetches of a stage
+  constexpr int XW = (XF + W - 1) / W, DW = (DF + W - 1) / W;               // of each wave (of those left over the last one again)
   constexpr int H = SE / (32 * W);                                          // products of a wave and stage
-  static_assert(2 * kStage >= W * RT * 1024 && 2 * kStage >= sizeof(Order<W>) && kWindow == 64 * W);
-  __shared__ __align__(1024) char lds[2][kStage];
+  static_assert(2 * kStage >= W * RT * 1024 && 2 * kStage >= sizeof(Order<W>) && kWindow == 64 * W && kStage == Staged<T, CODES, RT>::bytes);
+  __shared__ __align__(1024) char lds[ST][kStage];
   __shared__ int rows[16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, r16 = lane & 15;
   const int m0 = blockIdx.x * 16, w0 = m0 / kWindow * kWindow;
@@ -312,9 +315,9 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
   const int m = row_at(r16);
   const int id = p.ids[m];
   const char* x = (const char*)p.x + w0 * p.x_stride * (CODES ? 1 : 2);  // (the window's rows by 32-bit offsets)
-  uint32_t xoff[(XF + W - 1) / W];
+  uint32_t xoff[XW];
 #pragma unroll
-  for (int i = 0; i < (XF + W - 1) / W; ++i) xoff[i] = (uint32_t)(row_at((i * W + wave) * XR + lane / (64 / XR)) - w0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u);
+  for (int i = 0; i < XW; ++i) xoff[i] = (uint32_t)(row_at(min(i * W + wave, XF - 1) * XR + lane / (64 / XR)) - w0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u);
   lq_v4f keep[RT];
   const float none = id < 0 ? 0.0f : __builtin_nanf("");
 #pragma unroll
@@ -327,26 +330,29 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
     left &= ~__ballot(mine);
     const char* d = (const char*)(p.down + (int64_t)j * p.rank * p.padded);
     auto fetch = [&](int s) {  // (behind a row's end its last piece again: down is zero there as an operand)
-      char* to = lds[s & 1];
+      char* to = lds[s % ST];
 #pragma unroll
-      for (int i = 0; i < (XF + W - 1) / W; ++i) {
-        const int f = i * W + wave, row = f * XR + lane / (64 / XR), c = (lane % (64 / XR)) ^ (row & 15);
-        if (f < XF) sv_fetch16(x, xoff[i] + (uint32_t)min(s * XB + c * 16, xlast), to + f * 1024);
+      for (int i = 0; i < XW; ++i) {
+        const int f = min(i * W + wave, XF - 1), row = f * XR + lane / (64 / XR), c = (lane % (64 / XR)) ^ (row & 15);
+        sv_fetch16(x, xoff[i] + (uint32_t)min(s * XB + c * 16, xlast), to + f * 1024);
       }
 #pragma unroll
-      for (int i = 0; i < (DF + W - 1) / W; ++i) {
-        const int f = i * W + wave, row = f * DR + lane / (64 / DR), c = (lane % (64 / DR)) ^ (row & 15);
-        if (f < DF) sv_fetch16(d, (uint32_t)row * (uint32_t)p.padded * 2u + (uint32_t)min(s * DB + c * 16, dlast), to + 16 * XB + f * 1024);
+      for (int i = 0; i < DW; ++i) {
+        const int f = min(i * W + wave, DF - 1), row = f * DR + lane / (64 / DR), c = (lane % (64 / DR)) ^ (row & 15);
+        sv_fetch16(d, (uint32_t)row * (uint32_t)p.padded * 2u + (uint32_t)min(s * DB + c * 16, dlast), to + 16 * XB + f * 1024);
       }
     };
     lq_v4f acc[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[t] = lq_v4f{0.f, 0.f, 0.f, 0.f};
-    fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (from here on only fetches are counted)
+    for (int s = 0; s < min(ST - 1, stages); ++s) fetch(s);
     for (int s = 0; s < stages; ++s) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is there, and the one in front of it is read
-      if (s + 1 < stages) fetch(s + 1);
-      const char* st = lds[s & 1];
+      // the stage is there, and the one in front of it is read (fetches end in order: all but those of the ST - 2 stages behind it)
+      if (s + ST - 2 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((ST - 2) * (XW + DW)) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + ST - 1 < stages) fetch(s + ST - 1);
+      const char* st = lds[s % ST];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const int k = (wave * H + h) * 32 + 8 * quarter;  // of the stage
@@ -426,7 +432,11 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
     auto tiles = [&](auto rt) {
       constexpr int RT = decltype(rt)::value, W = RT <= 4 ? 8 : 4;
       if (pieces) {
-        hipLaunchKernelGGL((down_staged_kernel<T, C, RT, RT <= 2 ? 512 : 256>), dim3((unsigned)(((int64_t)a->rows + 15) / 16)), dim3(512), 0, stream, p);
+        // Where a compute unit has one workgroup at most, that one has more of its stages on their way: 1171 rows of 4096 codes, rank 64, one
+        // adapter 11.9 us, with two places 13.9, 16 adapters in turn 30.5 and 36.7; 3001 of 5120, rank 32, 16.1 and 16.8.
+        const dim3 grid((unsigned)(((int64_t)a->rows + 15) / 16)), threads(512);
+        if (grid.x <= 256) hipLaunchKernelGGL((down_staged_kernel<T, C, RT, Staged<T, C, RT>::deep>), grid, threads, 0, stream, p);
+        else hipLaunchKernelGGL((down_staged_kernel<T, C, RT, 2>), grid, threads, 0, stream, p);
         return lq_check_launch();
       }
       hipLaunchKernelGGL((down_tiles_kernel<T, C, E, RT, W>), dim3((unsigned)(((int64_t)a->rows + 15) / 16)), dim3(64 * W), 0, stream, p);
