@@ -212,6 +212,26 @@ def test_rows_of_many_adapters_in_any_order(cuda, M, K, n, ids, dtype):
     assert torch.equal(torch.nan_to_num(lin(x.to(cuda), adapters=ad, ids=idx.to(cuda))), torch.nan_to_num(got))
 
 
+@pytest.mark.parametrize("M", [300, 4113])
+@pytest.mark.parametrize("R", [16, 32, 40, 64, 72, 96, 112, 128])
+@pytest.mark.parametrize("dtype,coded", [(F16, False), (BF16, True), (F16, True)])
+def test_every_rank_over_prompts(cuda, M, R, dtype, coded):
+    """Contractions of several stages, the last one cut short; workgroups few and many to a compute unit."""
+    gen = torch.Generator().manual_seed(M + R)
+    K, N, n = 1872, 40, 3
+    codes = torch.randint(-127, 128, (N, K), generator=gen).to(torch.int8)
+    ws = torch.rand(N, generator=gen) / 1000
+    a, b, s = (torch.randn(n, R, K, generator=gen) / K ** 0.5).to(dtype), (torch.randn(n, N, R, generator=gen) / R ** 0.5).to(dtype), 0.25 + torch.rand(n, generator=gen)
+    lin, ad = W8A8Linear(codes, ws).to(cuda), LowRankAdapters(a, b, s).to(cuda)
+    x = torch.randn(M, K, generator=gen).to(dtype)
+    idx = torch.sort(torch.randint(-1, n + 1, (M,), generator=gen)).values.roll(M // 5).to(I32)
+    q, qs = quantize_rows(x.to(cuda))
+    got = lin.forward_int8(q, qs, dtype, adapters=ad, ids=idx.to(cuda)) if coded else lin(x.to(cuda), adapters=ad, ids=idx.to(cuda))
+    want, mag, low = adapters_ref(q.cpu(), qs.cpu(), codes, ws, None, q.cpu().double() * qs.cpu().double()[:, None] if coded else x, a, b, s, idx)
+    # as for few rows: sums of K and R terms in 32 bits, h in two pieces
+    assert_near(got, want, mag * 4 * 2.0 ** -24 + low * (2.0 ** -24 * (K / 8 + R + 16) + 2.0 ** -14), 1.0, "adapted")
+
+
 @pytest.mark.parametrize("n", [3, 64, 65, 700, 5000, 8192])
 @pytest.mark.parametrize("kind", ["all to one", "a few", "far apart", "every one twice"])
 def test_many_entries_with_one_destination(cuda, n, kind):
@@ -227,6 +247,45 @@ def test_many_entries_with_one_destination(cuda, n, kind):
         want[d] = s
     copy_slots(t, src.to(I32).to(cuda), dst.to(I32).to(cuda))
     assert torch.equal(t.cpu(), want)
+
+
+def _prompts(cuda, lens, H, K, V, dtype, g, slots, num_slots, seed):
+    """Packed prompts against the plain form; slots: negative ones start from zero and keep nothing, ones beyond the state give NaN."""
+    T = sum(lens)
+    q, k, v, gd = attention_inputs(T, H, K, V, dtype, g, seed)
+    state = torch.randn(num_slots, H, K, V, generator=torch.Generator().manual_seed(seed + 1))
+    first = torch.stack([state[s] if 0 <= s < num_slots else torch.zeros(H, K, V) for s in slots])
+    o, mag, S, Sm, most = attention_ref(q, k, v, gd, K ** -0.5, lens, first)
+    at = 0
+    for n, s in zip(lens, slots):
+        if s >= num_slots:
+            o[at:at + n] = float("nan")
+        at += n
+    dst = state.to(cuda)
+    got = linear_attention_prompt(*(None if t is None else t.to(cuda) for t in (q, k, v, gd)), state=dst, slots=torch.tensor(slots, dtype=I32, device=cuda),
+                                  seq_starts=starts_of(lens, cuda))
+    assert_near(got, o, mag, out_rel(lens, most, dtype), "o")
+    live = [i for i, s in enumerate(slots) if 0 <= s < num_slots]
+    want, wm = state.double().clone(), state.double().abs()
+    for i in live:
+        want[slots[i]], wm[slots[i]] = S[i], Sm[i]
+    assert_near(dst, want, wm, state_rel(lens, most), "state")
+    rest = [i for i in range(num_slots) if i not in slots]
+    assert torch.equal(dst[rest].cpu(), state[rest])
+
+
+@pytest.mark.parametrize("K", [24, 64, 128, 200])
+@pytest.mark.parametrize("V", [40, 200])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("g", ["token", "none"])
+def test_prompts_in_segments_of_every_width(cuda, K, V, dtype, g):
+    _prompts(cuda, [700, 3, 1, 1000], 2, K, V, dtype, g, [1, 0, 3, 2], 5, 11)
+
+
+@pytest.mark.parametrize("lens", [[600, 800, 700, 64], [1] * 130 + [900] + [2] * 70, [0] * 65 + [1500]])
+def test_segments_of_padding_and_slots_that_do_not_exist(cuda, lens):
+    n = len(lens)
+    _prompts(cuda, lens, 1, 64, 72, F16, "token", ([-1, 99, 0, 1] if n == 4 else [i if i % 9 else -1 - i for i in range(n)]), n, 12)
 
 
 # ---------------------------------------------------------------------------------------------- native and general calls
