@@ -7,10 +7,10 @@
 // `staged`, and `tiles` for rows that are no whole 16-byte pieces: 16 rows of x to a workgroup, its waves share the contraction, and what meets
 // the rows are the matrix instructions; the adapters that the 16 rows name are taken one after the other, each with all 16 rows, and a row keeps
 // what its own gave (nothing is multiplied by zero: an infinity in one request's row or adapter stays there).  The bound is memory: 16384 rows of
-// 2560 in 16 bits, 84 MB, rank 16, in 18 us 4.7 TB/s (some of it from the cache behind HBM, where the quantizer left it); 3001 rows of 5120 codes, rank 32, 16 us,
+// 2560 in 16 bits, 84 MB, rank 16, in 18 us 4.7 TB/s (some of it from the cache behind HBM, where the quantizer left it); 3001 rows of 5120 codes, rank 32, 14 us,
 // where a workgroup's 10 stages one after the other are what it waits for.
 // Rows that name adapters in turn would cost as many passes as there are adapters, so they are taken in an order (below).  us, 310 rows of 5120
-// codes, rank 8, 8 adapters in turn: 44 in their own order, 14 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 31, 12.
+// codes, rank 8, 8 adapters in turn: 44 in their own order, 13 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 29, 11.
 // v_mfma_f32_16x16x32: lane l has row l & 15 and the 8 contraction entries of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
 // down is the operand of the rows, so that a lane holds four adjacent sums of one row of x.
 //
@@ -108,6 +108,20 @@ LQ_DEV lq_v4f mfma16(lq_v4i a, lq_v4i b, lq_v4f c) {
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sv_v8bf, a), __builtin_bit_cast(sv_v8bf, b), c, 0, 0, 0);
 }
 
+// Eight codes in T, exactly: nothing is rounded, so bits may be cut off
+template <typename T>
+LQ_DEV lq_v4i from_codes(lq_v2i r) {
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = (float)lq_sbyte((uint32_t)r[e >> 2], e & 3);
+  lq_v4i o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, F16>::value) o[i] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_pkrtz(f[2 * i], f[2 * i + 1]));
+    else o[i] = (int)__builtin_amdgcn_perm(__float_as_uint(f[2 * i + 1]), __float_as_uint(f[2 * i]), 0x07060302);
+  }
+  return o;
+}
 // Eight entries of a row from `k` on in T, zero behind the row's end.  EIGHTS: rows of whole eights on boundaries of eight entries, of which the
 // last are read again behind the end; else one by one.
 template <typename T, bool CODES, bool EIGHTS>
@@ -116,21 +130,19 @@ LQ_DEV lq_v4i load8(const void* row, int k, int inner) {
     const lq_v4i zero = {0, 0, 0, 0}, r = *(const lq_v4i*)((const uint16_t*)row + min(k, inner - 8));
     return k < inner ? r : zero;
   } else {
-    uint16_t v[8];
     if constexpr (EIGHTS) {
       lq_v2i r = *(const lq_v2i*)((const int8_t*)row + min(k, inner - 8));
       if (k >= inner) r = lq_v2i{0, 0};
+      return from_codes<T>(r);
+    }
+    uint16_t v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = T::from((float)lq_sbyte((uint32_t)r[e >> 2], e & 3));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = min(k + e, inner - 1);
-        uint16_t u;
-        if constexpr (CODES) u = T::from((float)((const int8_t*)row)[at]);
-        else u = ((const uint16_t*)row)[at];
-        v[e] = k + e < inner ? u : 0;
-      }
+    for (int e = 0; e < 8; ++e) {
+      const int at = min(k + e, inner - 1);
+      uint16_t u;
+      if constexpr (CODES) u = T::from((float)((const int8_t*)row)[at]);
+      else u = ((const uint16_t*)row)[at];
+      v[e] = k + e < inner ? u : 0;
     }
     lq_v4i o;
 #pragma unroll
@@ -315,9 +327,15 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
   const int m = row_at(r16);
   const int id = p.ids[m];
   const char* x = (const char*)p.x + w0 * p.x_stride * (CODES ? 1 : 2);  // (the window's rows by 32-bit offsets)
-  uint32_t xoff[XW];
+  // a wave's fetches: the i-th one's number, this lane's row and piece of it
+  struct Piece { int fetch, row, at; };
+  auto of_x = [&](int i) { const int f = min(i * W + wave, XF - 1), row = f * XR + lane / (64 / XR); return Piece{f, row, ((lane % (64 / XR)) ^ (row & 15)) * 16}; };
+  auto of_down = [&](int i) { const int f = min(i * W + wave, DF - 1), row = f * DR + lane / (64 / DR); return Piece{f, row, ((lane % (64 / DR)) ^ (row & 15)) * 16}; };
+  uint32_t xoff[XW], doff[DW];
 #pragma unroll
-  for (int i = 0; i < XW; ++i) xoff[i] = (uint32_t)(row_at(min(i * W + wave, XF - 1) * XR + lane / (64 / XR)) - w0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u);
+  for (int i = 0; i < XW; ++i) xoff[i] = (uint32_t)(row_at(of_x(i).row) - w0) * (uint32_t)p.x_stride * (CODES ? 1u : 2u) + of_x(i).at;
+#pragma unroll
+  for (int i = 0; i < DW; ++i) doff[i] = (uint32_t)of_down(i).row * (uint32_t)p.padded * 2u + of_down(i).at;
   lq_v4f keep[RT];
   const float none = id < 0 ? 0.0f : __builtin_nanf("");
 #pragma unroll
@@ -329,18 +347,15 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
     const bool mine = id == j;
     left &= ~__ballot(mine);
     const char* d = (const char*)(p.down + (int64_t)j * p.rank * p.padded);
-    auto fetch = [&](int s) {  // (behind a row's end its last piece again: down is zero there as an operand)
+    auto fetch = [&](int s) {
       char* to = lds[s % ST];
+      const bool whole = (s + 1) * SE <= p.inner;  // (else behind a row's end its last piece again: down is zero there as an operand)
 #pragma unroll
-      for (int i = 0; i < XW; ++i) {
-        const int f = min(i * W + wave, XF - 1), row = f * XR + lane / (64 / XR), c = (lane % (64 / XR)) ^ (row & 15);
-        sv_fetch16(x, xoff[i] + (uint32_t)min(s * XB + c * 16, xlast), to + f * 1024);
-      }
+      for (int i = 0; i < XW; ++i)
+        sv_fetch16(x + s * XB, xoff[i] - (whole ? 0u : (uint32_t)max(s * XB + of_x(i).at - xlast, 0)), to + of_x(i).fetch * 1024);
 #pragma unroll
-      for (int i = 0; i < DW; ++i) {
-        const int f = min(i * W + wave, DF - 1), row = f * DR + lane / (64 / DR), c = (lane % (64 / DR)) ^ (row & 15);
-        sv_fetch16(d, (uint32_t)row * (uint32_t)p.padded * 2u + (uint32_t)min(s * DB + c * 16, dlast), to + 16 * XB + f * 1024);
-      }
+      for (int i = 0; i < DW; ++i)
+        sv_fetch16(d + s * DB, doff[i] - (whole ? 0u : (uint32_t)max(s * DB + of_down(i).at - dlast, 0)), to + 16 * XB + of_down(i).fetch * 1024);
     };
     lq_v4f acc[RT];
 #pragma unroll
@@ -351,28 +366,30 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
       // the stage is there, and the one in front of it is read (fetches end in order: all but those of the ST - 2 stages behind it)
       if (s + ST - 2 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((ST - 2) * (XW + DW)) : "memory");
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + ST - 1 < stages) fetch(s + ST - 1);
       const char* st = lds[s % ST];
+      // A fetch takes some 100 cycles to go out: behind the operands' reads if they are few.  3001 rows of 5120 codes, rank 32, 14.3 us, in front
+      // 15.0; 1171 of 4096, rank 64, 12.6 and 11.4.
+      auto ahead = [&] { if (s + ST - 1 < stages) fetch(s + ST - 1); };
+      if constexpr (RT > 2) ahead();
+      lq_v2i xc[H];
+      lq_v4i xv[H], dv[H][RT];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const int k = (wave * H + h) * 32 + 8 * quarter;  // of the stage
-        lq_v4i xv;
-        if constexpr (CODES) {
-          const lq_v2i r = *(const lq_v2i*)(st + r16 * XB + (((k >> 4) ^ r16) << 4) + (k & 8));
-          uint16_t v[8];
+        if constexpr (CODES) xc[h] = *(const lq_v2i*)(st + r16 * XB + (((k >> 4) ^ r16) << 4) + (k & 8));
+        else xv[h] = *(const lq_v4i*)(st + r16 * XB + (((k >> 3) ^ r16) << 4));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = T::from((float)lq_sbyte((uint32_t)r[e >> 2], e & 3));
+        for (int t = 0; t < RT; ++t) dv[h][t] = *(const lq_v4i*)(st + 16 * XB + (16 * t + r16) * DB + (((k >> 3) ^ r16) << 4));
+      }
+      if constexpr (RT <= 2) ahead();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) xv[i] = (int)(v[2 * i] | (uint32_t)v[2 * i + 1] << 16);
-        } else {
-          xv = *(const lq_v4i*)(st + r16 * XB + (((k >> 3) ^ r16) << 4));
-        }
-        const bool in = s * SE + k < p.inner;
+      for (int h = 0; h < H; ++h) {
+        const bool in = s * SE + (wave * H + h) * 32 + 8 * quarter < p.inner;
+        if constexpr (CODES) xv[h] = from_codes<T>(xc[h]);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          lq_v4i dv = *(const lq_v4i*)(st + 16 * XB + (16 * t + r16) * DB + (((k >> 3) ^ r16) << 4));
-          if (!in) dv = lq_v4i{0, 0, 0, 0};
-          acc[t] = mfma16<T>(dv, xv, acc[t]);
+          if (!in) dv[h][t] = lq_v4i{0, 0, 0, 0};
+          acc[t] = mfma16<T>(dv[h][t], xv[h], acc[t]);
         }
       }
     }
