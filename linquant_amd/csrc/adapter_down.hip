@@ -1,7 +1,7 @@
 // lq_adapter_down: the first half of low-rank adapters of many requests, h[m] = scaling[j] * (down[j] x[m]), j = ids[m], in fp32; the second
 // half is the epilogue of lq_int8_matmul.
 //
-// Three kernels.  `rows`, up to 256 rows, each with a request of its own as a rule: a wave has two of a row's sums, so that the adapters stream
+// Three kernels.  `rows`, few rows, each with a request of its own as a rule: a wave has two of a row's sums, so that the adapters stream
 // from memory through many waves; the quantizer of the rows, if the call has one, runs in the same launch.  16 rows of 2560 entries, rank 16,
 // 16 adapters, with the quantizer: 4.0 us, where the launch of an empty kernel takes 2.
 // `staged`, and `tiles` for rows that are no whole 16-byte pieces: 16 rows of x to a workgroup, its waves share the contraction, and what meets
@@ -10,11 +10,13 @@
 // 2560 in 16 bits, 84 MB, rank 16, in 18 us 4.7 TB/s (some of it from the cache behind HBM, where the quantizer left it); 3001 rows of 5120 codes, rank 32, 14 us,
 // where a workgroup's 10 stages one after the other are what it waits for.
 // Rows that name adapters in turn would cost as many passes as there are adapters, so they are taken in an order (below).  us, 310 rows of 5120
-// codes, rank 8, 8 adapters in turn: 44 in their own order, 13 ordered, 7 if all name one; 1171 of 4096, rank 64, 16 adapters: 165, 29, 11.
+// codes, rank 8, 8 adapters in turn: 44 in their own order, 13 ordered, 7 if all name one (and by `rows` 7); 1171 of 4096, rank 64, 16 adapters: 165, 29, 12.
 // v_mfma_f32_16x16x32: lane l has row l & 15 and the 8 contraction entries of quarter l >> 4; the result: column l & 15, rows 4 (l >> 4) + r.
 // down is the operand of the rows, so that a lane holds four adjacent sums of one row of x.
 //
 // INT8 codes become 16 bits exactly; their scale multiplies the sum.  All sums are fp32.
+#include <algorithm>
+
 #include "row_codes.h"
 
 namespace {
@@ -166,11 +168,15 @@ constexpr int kPer = 2;  // sums of a wave in `rows`
 template <typename T, bool CODES, bool EIGHTS, int QV>
 __global__ __launch_bounds__(256) void down_rows_kernel(DownParams p) {
   int m = blockIdx.x, lane = threadIdx.x & 63;
-  if (p.order && m-- == 0) {  // the first workgroup: the order
-    __shared__ Order<4> o;
-    const int at = window_place<4>(p.ids, p.rows, p.count, o);
-    if ((int)threadIdx.x < p.rows) p.order[at] = threadIdx.x;
-    return;
+  if (p.order) {  // the first workgroups: the order
+    const int windows = (p.rows + 255) / 256, w0 = m * 256;
+    if (m < windows) {
+      __shared__ Order<4> o;
+      const int n = min(256, p.rows - w0), at = window_place<4>(p.ids + w0, n, p.count, o);
+      if ((int)threadIdx.x < n) p.order[w0 + at] = w0 + (int)threadIdx.x;
+      return;
+    }
+    m -= windows;
   }
   if constexpr (QV > 0) {
     if (m < p.rows) {
@@ -403,7 +409,11 @@ __global__ __launch_bounds__(512) void down_staged_kernel(DownParams p) {
   down_finish<CODES, RT, W>(p, m0, rows, keep, *(lq_v4f(*)[W][RT][64])lds);  // (nothing of a stage is read any more)
 }
 
-constexpr int kFewRows = 256;  // (as many as a workgroup of `rows` has threads, which find their order)
+// How many rows `rows` takes: their adapters are read for each, at the caches' rate.  Whole calls, us, 2560 entries to 1024 columns, one adapter / 16 in
+// turn, `rows` and `staged`: rank 16, 256 rows 16 / 16 and 20 / 22, 1024 21 / 22 and 21 / 24; rank 64, 256 rows 22 / 24 and 25 / 29, 512 28 / 30 and
+// 26 / 29.  From codes, where there is no quantizer to take along: rank 16, 512 rows 15 / 16 and 15 / 17, 1024 18 / 20 and 15 / 18; rank 32, 320 rows
+// 16 / 20 and 16 / 22, 512 18 / 20 and 16 / 19.
+int few_rows(int rank, bool codes) { return std::max(256, (codes ? 8192 : 16384) / rank); }
 
 }  // namespace
 
@@ -423,7 +433,7 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
   if (a->codes_out && (!a->scale_out || codes || !eights || a->inner > 16384 || !sv_al(a->codes_out, 8) || !sv_al(a->scale_out, 4))) return LQ_ERR_SHAPE;
   using std::integral_constant;
   auto rows = [&](auto t, auto c, auto e, auto qv) {
-    const int64_t wgs = (int64_t)a->rows * ((a->rank + 4 * kPer - 1) / (4 * kPer)) + (decltype(qv)::value ? a->rows : 0) + (a->order ? 1 : 0);
+    const int64_t wgs = (int64_t)a->rows * ((a->rank + 4 * kPer - 1) / (4 * kPer)) + (decltype(qv)::value ? a->rows : 0) + (a->order ? (a->rows + 255) / 256 : 0);
     hipLaunchKernelGGL((down_rows_kernel<decltype(t), decltype(c)::value, decltype(e)::value, decltype(qv)::value>), dim3((unsigned)wgs), dim3(256), 0, stream, p);
     return lq_check_launch();
   };
@@ -431,7 +441,7 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
     using T = decltype(t);
     constexpr bool C = decltype(c)::value, E = decltype(e)::value;
     if constexpr (!C && E) {
-      if (a->codes_out && a->rows <= kFewRows) {
+      if (a->codes_out && a->rows <= few_rows(a->rank, codes)) {
         if (a->inner <= 2048) return rows(t, c, e, integral_constant<int, 1>{});
         if (a->inner <= 4096) return rows(t, c, e, integral_constant<int, 2>{});
         if (a->inner <= 8192) return rows(t, c, e, integral_constant<int, 4>{});
@@ -443,7 +453,7 @@ extern "C" int lq_adapter_down(const lq_adapter_down_args* a, hipStream_t stream
         if (rc != LQ_OK) return rc;
       }
     }
-    if (a->rows <= kFewRows) return rows(t, c, e, integral_constant<int, 0>{});
+    if (a->rows <= few_rows(a->rank, codes)) return rows(t, c, e, integral_constant<int, 0>{});
     // whole 16-byte pieces of both
     const bool pieces = E && a->inner % (C ? 16 : 8) == 0 && a->x_stride % (C ? 16 : 8) == 0 && sv_al(a->x, 16) && a->x_stride >= 0 && a->x_stride < 1 << 22;
     auto tiles = [&](auto rt) {

@@ -60,8 +60,8 @@ struct OutOf<F32> {
 // adapters' type (fp16: where it needs one, after a multiplication by a power of two that brings the row's largest below 2^14): off by 2^-16 of
 // the row's largest.  The adapters that 32 rows name are taken one after the other, with all 32, and a row keeps what its own
 // gave: nothing is multiplied by zero, and an infinity in one request's adapter stays there.  Rows are taken in the order that the first half
-// found, in which few of 32 differ: 128 x 2560 x 10576, rank 16, 16 adapters in turn 24 us, in the rows' own order 32, all of one adapter 20,
-// none 16; 1171 x 4096 x 2048, rank 64: 44, 94, 29, 23.  (The order is one load more in front of the first stage: 2% of 16384 x 2560 x 10576.)
+// found, in which few of 32 differ: 128 x 2560 x 10576, rank 16, 16 adapters in turn 24 us, in the rows' own order 32 (tiles of 64 x 64);
+// 1171 x 4096 x 2048, rank 64: 44, 94, all of one adapter 29, none 23.  (The order is one load more in front of the first stage: 2% of 16384 x 2560 x 10576.)
 // Where 32 rows name one adapter and no h needs a unit, its product goes on from the projection's sums.  16384 x 2560 x 10576 with rank 16
 // takes 7% longer than without.  `rows`: a product of a row's h and its adapter's row in fp32 for each result.
 typedef float mm_v16f __attribute__((ext_vector_type(16)));
@@ -500,7 +500,10 @@ int launch(const MatmulParams& p, hipStream_t stream) {
   // 60 / 41 / 26 / 20, 100 x 5120 x 2560 46 / 30 / 19 / 17.
   if (count(128, 256) >= 768) return tiles(integral_constant<int, 128>{}, integral_constant<int, 256>{}, integral_constant<int, 1>{});
   if (count(128, 128) >= 300) return tiles(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 1>{});
-  if (count(64, 64) > 512) return tiles(integral_constant<int, 64>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{});
+  // With adapters the tiles of 64 x 64 have one workgroup to a compute unit, by their registers.  us, one adapter / 8 or 16 in turn, 64 x 128 and 64 x 64:
+  // 449 x 5120 x 2560, rank 12, 33 / 35 and 37 / 38; 128 x 2560 x 10576, rank 16, 19 / 23 and 23 / 27; 500 x 5120 x 2560, rank 64, 43 / 58 and 50 / 66;
+  // 700 x 4096 x 2048, rank 16, 28 / 36 and 32 / 41.  (In half the registers, the rest in memory: 30 / 34, 19 / 26, 40 / 59, 26 / 37.)
+  if (count(64, 64) > (std::is_void<A>::value ? 512 : 256)) return tiles(integral_constant<int, 64>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{});
   return tiles(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 4>{});
 }
 
