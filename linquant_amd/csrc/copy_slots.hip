@@ -8,7 +8,7 @@
 // bytes up to 256 entries, 32 at 8192.
 //
 // 1 GiB of slots in another order (a copy of that size reaches 5.2 TB/s): 64 slots 5.1 TB/s, 256 4.9, 1024 4.8, 2048 4.5, 4096 3.9, 8192 2.7.
-// One layer's state of 2 MB to 4 slots: 6.7 us (floor 3.2), most of it the launch and the list.
+// One layer's state of 2 MB to 4 slots: 5.5 us (floor 3.2), most of it the launch and the list.
 #include <algorithm>
 
 #include "serve_common.h"
@@ -28,6 +28,7 @@ struct CopyParams {
   const int32_t* src;
   const int32_t* dst;
   int entries, lanes;  // lanes: of one entry's part of a strip, a power of two; a lane has one unit
+  int beside;          // parts of a strip side by side, each with waves of its own: more than one where there are fewer entries than waves
   int near;            // strips that share 128 bytes on one die
   int log_table;       // of the places of the table of destinations
 };
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(64 * kWaves) void copy_slots_kernel(CopyParams p) {
   int *from = list, *to = list + p.entries, *table = to + p.entries;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = p.entries, places = 1 << p.log_table;
-  if (n <= 64) {  // (the first wave by itself: 4 forks of 2 MB 6.7 us, by the table 8.1)
+  if (n <= 64) {  // (the first wave by itself: 4 forks of 2 MB 6.7 us, by the table 8.1; with all waves at work 5.5)
     if (tid < n) {
       const int d = p.dst[tid], s = p.src[tid] < 0 ? (int)kClear : min(p.src[tid], p.num_slots);
       bool keep = d >= 0 && d < p.num_slots && d != s;
@@ -98,7 +99,8 @@ __global__ __launch_bounds__(64 * kWaves) void copy_slots_kernel(CopyParams p) {
       if (!__syncthreads_or(open)) break;
     }
   }
-  const int part = lane % p.lanes, per = 64 / p.lanes, e0 = wave * per + lane / p.lanes;  // entries e0, e0 + kWaves per, ..
+  const int per = 64 / p.lanes, waves = kWaves / p.beside, part = wave / waves * p.lanes + lane % p.lanes;
+  const int e0 = wave % waves * per + lane / p.lanes;  // entries e0, e0 + waves per, ..
   const int64_t all = p.t[p.num_tensors - 1].strips;
   const int64_t eighth = (all + 7) / 8;
   for (int64_t i = blockIdx.x; i < (p.near ? 8 * eighth : all); i += gridDim.x) {
@@ -108,13 +110,13 @@ __global__ __launch_bounds__(64 * kWaves) void copy_slots_kernel(CopyParams p) {
     while (strip >= p.t[t].strips) ++t;
     const Slots& x = p.t[t];
     const int unit = unit_of(x);
-    const int64_t at = ((strip - (t ? p.t[t - 1].strips : 0)) * p.lanes + part) * unit;
+    const int64_t at = ((strip - (t ? p.t[t - 1].strips : 0)) * (p.lanes * p.beside) + part) * unit;
     const bool in = at < x.bytes;
     lq_v4i v[U];
     int f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kWaves * per;
+      const int e = e0 + u * waves * per;
       f[u] = in && e < n ? from[e] : (int)kSkip;
       const int fill = f[u] >= p.num_slots ? -1 : 0;
       v[u] = lq_v4i{fill, fill, fill, fill};
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(64 * kWaves) void copy_slots_kernel(CopyParams p) {
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (f[u] != kSkip) store_unit(x.base + to[e0 + u * kWaves * per] * x.stride + at, unit, v[u]);
+      if (f[u] != kSkip) store_unit(x.base + to[e0 + u * waves * per] * x.stride + at, unit, v[u]);
   }
 }
 
@@ -141,7 +143,9 @@ extern "C" int lq_copy_slots(const lq_copy_slots_args* a, hipStream_t stream) {
   // as many lanes to an entry's part as leave every entry a place in the workgroup's registers
   int lanes = 64;
   while (lanes > 1 && (int64_t)kWaves * (64 / lanes) * kMaxU < a->entries) lanes /= 2;
-  const int64_t slots = (int64_t)kWaves * (64 / lanes);
+  int beside = 1;
+  while (2 * beside * a->entries <= kWaves) beside *= 2;
+  const int64_t slots = (int64_t)kWaves / beside * (64 / lanes);
   const int u = (int)((a->entries + slots - 1) / slots);
   // Workgroups go to the 8 dies in turn.  Strips of 128 bytes and less are given out so that those which share a cache line, or are next to
   // each other, meet in one die's cache: 1 GiB of 8192 slots in 0.78 ms, 1.41 without; of 4096 0.55, 0.67.  Wider ones gain nothing by it.
@@ -150,12 +154,12 @@ extern "C" int lq_copy_slots(const lq_copy_slots_args* a, hipStream_t stream) {
   while (1 << log_table < a->entries) ++log_table;
   for (int first = 0; first < a->num_tensors; first += kMaxTensors) {
     CopyParams p = {};
-    p.num_tensors = std::min(kMaxTensors, a->num_tensors - first), p.num_slots = a->num_slots, p.src = a->src, p.dst = a->dst, p.entries = a->entries, p.lanes = lanes, p.log_table = log_table, p.near = near;
+    p.num_tensors = std::min(kMaxTensors, a->num_tensors - first), p.num_slots = a->num_slots, p.src = a->src, p.dst = a->dst, p.entries = a->entries, p.lanes = lanes, p.beside = beside, p.log_table = log_table, p.near = near;
     int64_t strips = 0;
     for (int i = 0; i < p.num_tensors; ++i) {
       const int64_t* t = a->tensors + 3 * (first + i);
       const uint64_t m = (uint64_t)t[0] | (uint64_t)t[1] | (uint64_t)t[2];
-      const int64_t width = (int64_t)lanes * (m % 16 == 0 ? 16 : (m % 4 == 0 ? 4 : (m % 2 == 0 ? 2 : 1)));
+      const int64_t width = (int64_t)lanes * beside * (m % 16 == 0 ? 16 : (m % 4 == 0 ? 4 : (m % 2 == 0 ? 2 : 1)));
       strips += (t[2] + width - 1) / width;
       p.t[i] = {(char*)t[0], t[1], t[2], strips};
     }
