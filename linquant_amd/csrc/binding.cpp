@@ -835,7 +835,22 @@ PyObject* linear_attention_prompt(PyObject*, PyObject* const* arg, Py_ssize_t n)
   END_HANDLE_TH_ERRORS
 }
 
-// groupnorm_gated(x, z, weight, bias, num_groups, eps, act): dense rows, weights of one type
+// entries from row to row of a tensor (..., D) with unit stride along D, if its rows are equally far apart in their order
+bool row_distance(const Tensor& t, int64_t& s) {
+  if (t.size(-1) != 1 && t.stride(-1) != 1) return false;
+  int64_t next = 0;
+  bool first = true;
+  s = t.size(-1);
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (first) s = next = t.stride(i), first = false;
+    else if (t.stride(i) != next) return false;
+    next *= t.size(i);
+  }
+  return s >= 0;
+}
+
+// groupnorm_gated(x, z, weight, bias, num_groups, eps, act): equally distant rows, weights of one type
 PyObject* groupnorm_gated(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 7) Py_RETURN_NONE;
@@ -846,10 +861,11 @@ PyObject* groupnorm_gated(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   if (!device_of(arg[0], dev) || !plain(arg[0], dev, x) || !optional(arg[1], dev, z) || !optional(arg[2], dev, w) || !optional(arg[3], dev, b) || !integer(arg[4], groups) ||
       !number(arg[5], eps) || !integer(arg[6], act))
     Py_RETURN_NONE;
-  if (!act16(x) || x.dim() < 1 || !fits(x.sizes()) || !x.is_contiguous()) Py_RETURN_NONE;
+  int64_t xs = 0, zs = 0;
+  if (!act16(x) || x.dim() < 1 || !fits(x.sizes()) || !row_distance(x, xs)) Py_RETURN_NONE;
   const int64_t D = x.size(-1), rows = x.numel() / D;
   if (rows > INT_MAX || groups < 1 || D % groups != 0 || D / groups > 16384) Py_RETURN_NONE;
-  if (z.defined() && (z.scalar_type() != x.scalar_type() || z.sizes() != x.sizes() || !z.is_contiguous())) Py_RETURN_NONE;
+  if (z.defined() && (z.scalar_type() != x.scalar_type() || z.sizes() != x.sizes() || !row_distance(z, zs))) Py_RETURN_NONE;
   for (const Tensor* t : {&w, &b})
     if (t->defined() && (!floats(*t) || t->dim() != 1 || t->size(0) != D || !t->is_contiguous())) Py_RETURN_NONE;
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) Py_RETURN_NONE;
@@ -858,7 +874,7 @@ PyObject* groupnorm_gated(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     out = empty(x.sizes(), x.scalar_type(), dev);
-    a.x = x.const_data_ptr(), a.x_stride = D, a.z = at(z), a.z_stride = z.defined() ? D : 0, a.dtype = code(x.scalar_type()), a.weight = at(w), a.bias = at(b);
+    a.x = x.const_data_ptr(), a.x_stride = xs, a.z = at(z), a.z_stride = zs, a.dtype = code(x.scalar_type()), a.weight = at(w), a.bias = at(b);
     a.weight_dtype = w.defined() ? code(w.scalar_type()) : (b.defined() ? code(b.scalar_type()) : 0), a.out = out.data_ptr(), a.eps = (float)eps;
     a.rows = (int)rows, a.dim = (int)D, a.num_groups = (int)groups, a.act = (int)act;
     rc = groupnorm_entry(&a, stream_of(dev));

@@ -332,14 +332,27 @@ def test_native_attention(cuda, monkeypatch, form, dtype, L):
     _both_ways(monkeypatch, "linear_attention_step", step, native)
 
 
-@pytest.mark.parametrize("form", ["plain", "bare", "no gate", "x strided", "two types"])
+@pytest.mark.parametrize("form", ["plain", "bare", "no gate", "x strided", "two types", "z slice", "x and z slices", "z reversed", "one row", "z expanded", "z of one row"])
 def test_native_norm(cuda, monkeypatch, form):
     gen = torch.Generator().manual_seed(6)
     x, z, w, b = (torch.randn(*s, generator=gen).to(BF16).to(cuda) for s in ((3, 7, 96), (3, 7, 96), (96,), (96,)))
     x = x.transpose(0, 1) if form == "x strided" else x
     z = None if form in ("bare", "no gate") else z.transpose(0, 1) if form == "x strided" else z
     w, b = (None, None) if form == "bare" else (w, b.float() if form == "two types" else b)
-    _both_ways(monkeypatch, "groupnorm_gated", lambda: [groupnorm_gated(x, z, w, b, num_groups=6)], form not in ("x strided", "two types"))
+    wide = torch.randn(3, 7, 300, generator=gen).to(BF16).to(cuda)
+    if form in ("z slice", "x and z slices"):
+        z = wide[..., 200:296]
+    if form == "x and z slices":
+        x = wide[..., 5:101]                                                                # (not on a 16-byte boundary)
+    if form == "z reversed":
+        z = z.flip(-1).transpose(-1, -2).contiguous().transpose(-1, -2)                     # (channels with a stride)
+    if form == "z expanded":
+        z = wide[:, :1, 100:196].expand(3, 7, 96)                                           # (rows not equally far apart)
+    if form == "z of one row":
+        z = wide[:1, :1, 100:196].expand(3, 7, 96)
+    if form == "one row":
+        x, z = x[1:2, 2:3], wide[:1, ::7, 100:196]
+    _both_ways(monkeypatch, "groupnorm_gated", lambda: [groupnorm_gated(x, z, w, b, num_groups=6)], form not in ("x strided", "two types", "z reversed", "z expanded"))
 
 
 @pytest.mark.parametrize("form", ["plain", "codes", "one scale", "K not padded", "static scale", "x strided", "scale number"])
