@@ -924,7 +924,7 @@ PyObject* adapted(PyObject*, PyObject* const* arg, Py_ssize_t n) {
       codes = empty({M, K}, ScalarType::Char, dev), xs = empty({M}, ScalarType::Float, dev);
       d.codes_out = (int8_t*)codes.data_ptr(), d.scale_out = (float*)xs.data_ptr();
     }
-    if (M > 64) order = empty({M}, ScalarType::Int, dev);
+    if (M > 32) order = empty({M}, ScalarType::Int, dev);
     {
       d.x = x.const_data_ptr(), d.x_stride = K, d.x_dtype = coded ? LQ_DT_I8 : code(x.scalar_type()), d.x_scale = coded ? f32(xs) : nullptr, d.x_scale_rows = xs.numel() != 1;
       d.down = down.const_data_ptr(), d.dtype = code(down.scalar_type()), d.scaling = f32(scaling), d.ids = i32(ids), d.h = (float*)h.data_ptr();

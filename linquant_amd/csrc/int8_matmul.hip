@@ -471,7 +471,12 @@ __global__ __launch_bounds__(64 * W) void int8_rows_kernel(MatmulParams p) {
 template <typename O, typename A>
 int launch(const MatmulParams& p, hipStream_t stream) {
   using std::integral_constant;
-  if (p.rows <= 64) {
+  // With adapters, more than 32 rows and wide results go to `tiles`: `rows` loads what the adapters have for a result once for each.  us, 16 adapters in
+  // turn / one, `rows` and `tiles`: 64 x 2560 x 10576, rank 16, 24 / 23 and 19 / 14, rank 64 41 / 38 and 29 / 17; 64 x 2560 x 5120 18 / 18 and 15 / 13,
+  // 29 / 27 and 27 / 15; 64 x 2560 x 3840 13 / 13 and 15 / 13, 18 / 18 and 25 / 15; 48 x 2048 x 6400 15 / 14 and 15 / 12, 23 / 22 and 27 / 14;
+  // 33 x 2048 x 8512 17 / 16 and 16 / 12, 26 / 24 and 32 / 13; 32 x 2560 x 10576 15 / 14 and 21 / 13, 27 / 21 and 35 / 15.
+  const bool few = p.rows <= 64 && (std::is_void<A>::value || p.rows <= 32 || (int64_t)p.rows * p.cols < 300000);
+  if (few) {
     if (!sv_fits(((int64_t)p.cols + 15) / 16, 512)) return LQ_ERR_SHAPE;
     const int mt = (p.rows + 15) / 16;
     // most tiles of 16 columns that a compute unit gets, n to a workgroup

@@ -12,7 +12,7 @@ from linquant_amd.w4a8_linear import _fused_fp16_to_int8
 
 _CODES = {torch.float16: _lib.LQ_DT_F16, torch.bfloat16: _lib.LQ_DT_BF16, torch.float32: _lib.LQ_DT_F32}
 _K = 16  # the product's contraction length is a multiple of this
-_ONE_BY_ONE = 64  # up to so many rows the product takes each row's adapter by itself, in any order
+_ONE_BY_ONE = 32  # up to so many rows the product takes each row's adapter by itself, in any order
 
 
 def _padded(n):

@@ -232,6 +232,26 @@ def test_every_rank_over_prompts(cuda, M, R, dtype, coded):
     assert_near(got, want, mag * 4 * 2.0 ** -24 + low * (2.0 ** -24 * (K / 8 + R + 16) + 2.0 ** -14), 1.0, "adapted")
 
 
+@pytest.mark.parametrize("M", [32, 33, 48, 64])
+@pytest.mark.parametrize("R", [16, 64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_few_rows_of_wide_results(cuda, M, R, dtype):
+    """Up to 64 rows on either side of what the kernel of few rows takes."""
+    gen = torch.Generator().manual_seed(M + R)
+    K, N, n = 272, 9100, 7
+    codes = torch.randint(-127, 128, (N, K), generator=gen).to(torch.int8)
+    ws = torch.rand(N, generator=gen) / 1000
+    a, b, s = (torch.randn(n, R, K, generator=gen) / K ** 0.5).to(dtype), (torch.randn(n, N, R, generator=gen) / R ** 0.5).to(dtype), 0.25 + torch.rand(n, generator=gen)
+    lin, ad = W8A8Linear(codes, ws).to(cuda), LowRankAdapters(a, b, s).to(cuda)
+    x = torch.randn(M, K, generator=gen).to(dtype)
+    for idx in (torch.arange(M) % (n + 2) - 1, torch.full((M,), 3)):
+        q, qs = quantize_rows(x.to(cuda))
+        want, mag, low = adapters_ref(q.cpu(), qs.cpu(), codes, ws, None, x, a, b, s, idx)
+        got = lin(x.to(cuda), adapters=ad, ids=idx.to(I32).to(cuda))
+        # as for other sizes: sums of K and R terms in 32 bits, h in two pieces
+        assert_near(got, want, mag * 4 * 2.0 ** -24 + low * (2.0 ** -24 * (K / 8 + R + 16) + 2.0 ** -14), 1.0, "adapted")
+
+
 @pytest.mark.parametrize("n", [3, 64, 65, 700, 5000, 8192])
 @pytest.mark.parametrize("kind", ["all to one", "a few", "far apart", "every one twice"])
 def test_many_entries_with_one_destination(cuda, n, kind):
