@@ -174,7 +174,9 @@ class W8A8Linear(nn.Module):
         return cls(codes, s, input_scale, linear.bias)
 
     def _native(self, x, scale, out_dtype, adapters, ids):
-        """The ordinary forms of a call with adapters; None for others."""
+        """The ordinary forms of a call with adapters; None for others.  (The widths are compared here: the padded rows do not tell them.)"""
+        if not (x.dim() and x.shape[-1] == self.in_features == adapters.in_features and self.out_features == adapters.out_features):
+            return None
         w, a = self._buffers, adapters._buffers
         return _lib.native().adapted(x, scale, w["weight"], w["weight_scale"], w["bias"], out_dtype, a["down"], a["up"], a["scaling"], ids)
 
@@ -212,6 +214,8 @@ class W8A8Linear(nn.Module):
         assert x.shape[-1] == self.in_features and x.dtype in (torch.float16, torch.bfloat16)
         static = self.input_scale is not None and x.dtype == torch.float16 and self.in_features % 8 == 0
         assert static or self.input_scale is None, "a static input scale takes fp16 activations and in_features a multiple of 8"
+        if adapters is not None:
+            ids = self._ids(adapters, ids, x.shape[:-1])
         x2 = x.reshape(-1, self.in_features)
         if static:
             q, s = _fused_fp16_to_int8(_lib.rows16(x2), self.input_scale, clamp_min=-128.0, reciprocal=False), self.input_scale
@@ -222,6 +226,5 @@ class W8A8Linear(nn.Module):
         else:
             q, s = _quantize(x)
         if adapters is not None:
-            ids = self._ids(adapters, ids, x.shape[:-1])
             return self._adapted(q, s, adapters._down(x2, None, ids), ids, adapters, x.dtype).view(*x.shape[:-1], self.out_features)
         return int8_matmul(q, self.weight, s, self.weight_scale, self.bias, x.dtype).view(*x.shape[:-1], self.out_features)

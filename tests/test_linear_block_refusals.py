@@ -1,0 +1,50 @@
+"""Further refusals of a linear attention block's operators: widths behind the padding, adapters' ids without adapters, states whose slots overlap (CPU)."""
+
+import pytest
+import torch
+
+from linquant_amd import _lib
+from linquant_amd.w8a8_linear import LowRankAdapters, W8A8Linear
+
+F16, F32, I8, I32 = torch.float16, torch.float32, torch.int8, torch.int32
+
+
+def z(*shape, dtype=F16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+class _Native:
+    """In the place of the native calls: takes every call with adapters, none of the others."""
+
+    def __init__(self):
+        self.taken = 0
+
+    def adapted(self, *args):
+        self.taken += 1
+        return "taken"
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.fixture
+def native(monkeypatch):
+    n = _Native()
+    monkeypatch.setattr(_lib, "native", lambda: n)
+    return n
+
+
+def test_native_calls_with_adapters_keep_the_widths_apart(native):
+    """250 and 256 features lie in rows of the same length, and are not the same."""
+    ids = z(3, dtype=I32)
+    narrow, wide = (W8A8Linear(z(8, k, dtype=I8), torch.ones(8)) for k in (250, 256))
+    a250, a256 = (LowRankAdapters(z(2, 4, k), z(2, 8, 4)) for k in (250, 256))
+    for lin, ad, k in ((narrow, a250, 256), (narrow, a256, 250), (narrow, a256, 256), (wide, a250, 256), (wide, a250, 250), (wide, a256, 250)):
+        with pytest.raises(AssertionError):
+            lin(z(3, k), adapters=ad, ids=ids)
+        with pytest.raises(AssertionError):
+            lin.forward_int8(z(3, k, dtype=I8), torch.ones(3), adapters=ad, ids=ids)
+    with pytest.raises(AssertionError, match="another projection"):
+        wide(z(3, 256), adapters=LowRankAdapters(z(2, 4, 256), z(2, 16, 4)), ids=ids)
+    assert native.taken == 0
+    assert wide(z(3, 256), adapters=a256, ids=ids) == "taken" and wide.forward_int8(z(3, 256, dtype=I8), torch.ones(3), adapters=a256, ids=ids) == "taken"
