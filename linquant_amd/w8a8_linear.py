@@ -197,6 +197,7 @@ class W8A8Linear(nn.Module):
             if out is not None:
                 return out
         assert x_i8.dtype == torch.int8 and x_i8.shape[-1] == self.in_features
+        assert adapters is not None or ids is None, "ids without adapters"
         a = x_i8.reshape(-1, self.in_features)
         if self.in_features % _K:
             a = nn.functional.pad(a, (0, _padded(self.in_features) - self.in_features))
@@ -212,6 +213,7 @@ class W8A8Linear(nn.Module):
             if out is not None:
                 return out
         assert x.shape[-1] == self.in_features and x.dtype in (torch.float16, torch.bfloat16)
+        assert adapters is not None or ids is None, "ids without adapters"
         static = self.input_scale is not None and x.dtype == torch.float16 and self.in_features % 8 == 0
         assert static or self.input_scale is None, "a static input scale takes fp16 activations and in_features a multiple of 8"
         if adapters is not None:

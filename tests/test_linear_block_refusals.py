@@ -48,3 +48,11 @@ def test_native_calls_with_adapters_keep_the_widths_apart(native):
         wide(z(3, 256), adapters=LowRankAdapters(z(2, 4, 256), z(2, 16, 4)), ids=ids)
     assert native.taken == 0
     assert wide(z(3, 256), adapters=a256, ids=ids) == "taken" and wide.forward_int8(z(3, 256, dtype=I8), torch.ones(3), adapters=a256, ids=ids) == "taken"
+
+
+def test_ids_without_adapters_are_refused():
+    lin, ids = W8A8Linear(z(8, 32, dtype=I8), torch.ones(8)), z(3, dtype=I32)
+    static = W8A8Linear(z(8, 32, dtype=I8), torch.ones(8), input_scale=0.5)
+    for call in (lambda: lin(z(3, 32), ids=ids), lambda: static(z(3, 32), ids=ids), lambda: lin.forward_int8(z(3, 32, dtype=I8), 1.0, ids=ids)):
+        with pytest.raises(AssertionError, match="ids without adapters"):
+            call()
