@@ -41,7 +41,7 @@ typedef struct ihipStream_t* hipStream_t;
 #define LQ_DT_BF16 3
 
 /* ABI version; bumped whenever a struct layout, or what a call asks of its caller, changes.  The function gives the library's. */
-#define LQ_ABI_VERSION 23
+#define LQ_ABI_VERSION 24
 int lq_abi_version(void);
 /* sizeof() of the named args struct as compiled into the library (negative if unknown); lets a binding
  * check its own struct layout before the first call. */
@@ -1000,7 +1000,7 @@ typedef struct {
   int64_t g_stride_b, g_stride_l, g_stride_h;
   float scale;
   void* out;                 /* the shape of v, dense */
-  float* state;              /* (num_slots,H,K,V), the last three dense, or NULL: from zero, nothing kept */
+  float* state;              /* (num_slots,H,K,V), the last three dense, slots that do not overlap, or NULL: from zero, nothing kept */
   int64_t state_stride_s;
   const int32_t* slots;      /* (nseq,) or NULL */
   const int32_t* seq_starts; /* (nseq + 1,) or NULL */
@@ -1027,7 +1027,7 @@ typedef struct {
   int32_t g_dtype;
   float scale;
   void* out;                 /* (batch,H,V) dense */
-  float* state;              /* (num_slots,H,K,V), the last three dense */
+  float* state;              /* (num_slots,H,K,V), the last three dense, slots that do not overlap */
   int64_t state_stride_s;
   const int32_t* slots;      /* (batch,) or NULL */
   int32_t num_slots, batch, nheads, kdim, vdim; /* kdim up to 256, vdim a multiple of 4, batch up to 65535 */

@@ -20,7 +20,7 @@ _NATIVE_ENTRIES = ("lq_zoo_simple_gla", "lq_zoo_simple_gla_workspace_bytes", "lq
                    "lq_conv1d_step", "lq_ssm_prompt", "lq_ssm_prompt_workspace_bytes", "lq_ssm_step", "lq_linear_attention_prompt",
                    "lq_linear_attention_prompt_workspace_bytes", "lq_linear_attention_step", "lq_groupnorm_gated", "lq_adapter_down", "lq_copy_slots",
                    "lq_abi_version", "lq_args_size")
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 LQ_DT_F16, LQ_DT_F32, LQ_DT_I8, LQ_DT_BF16 = 0, 1, 2, 3
 

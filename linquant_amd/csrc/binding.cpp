@@ -758,7 +758,7 @@ bool attention_operands(PyObject* const* arg, const c10::Device& dev, int lead, 
   }
   if (arg[4] == Py_None) a.scale = std::pow((double)a.K, -0.5);
   return st.dim() == 4 && st.scalar_type() == ScalarType::Float && fits(st.sizes()) && st.size(1) == a.H && st.size(2) == a.K && st.size(3) == a.V && st.stride(3) == 1 &&
-         st.stride(2) == a.V && st.stride(1) == a.K * a.V && st.stride(0) % 4 == 0 && aligned(st);
+         st.stride(2) == a.V && st.stride(1) == a.K * a.V && st.stride(0) % 4 == 0 && (st.size(0) == 1 || st.stride(0) >= a.H * a.K * a.V) && aligned(st);
 }
 template <typename Args>
 void attention_args(const Attention& s, Args& a) {

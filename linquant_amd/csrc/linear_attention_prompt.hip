@@ -879,7 +879,7 @@ extern "C" int lq_linear_attention_prompt(const lq_linear_attention_prompt_args*
   if (!a || !a->q || !a->k || !a->v || !a->out) return LQ_ERR_NULL;
   const int rc = check_dims(a);
   if (rc != LQ_OK) return rc;
-  if (a->state && a->num_slots <= 0) return LQ_ERR_SHAPE;
+  if (a->state && (a->num_slots <= 0 || (a->num_slots > 1 && a->state_stride_s < (int64_t)a->nheads * a->kdim * a->vdim))) return LQ_ERR_SHAPE;  // (slots that overlap)
   for (const int64_t s : {a->q_stride_l, a->k_stride_l, a->v_stride_l, a->g_stride_l})
     if (s < 0 || s >= 1 << 24) return LQ_ERR_SHAPE;  // a chunk's rows are reached by 32-bit offsets
   for (const int64_t s : {a->q_stride_b, a->q_stride_l, a->q_stride_h, a->k_stride_b, a->k_stride_l, a->k_stride_h, a->v_stride_b, a->v_stride_l, a->v_stride_h})

@@ -103,6 +103,7 @@ extern "C" int lq_linear_attention_step(const lq_linear_attention_step_args* a, 
   if (!sv_act(a->dtype) || (a->g && !sv_float(a->g_dtype)) || a->batch <= 0 || a->batch > 65535 || a->nheads <= 0 || a->num_slots <= 0) return LQ_ERR_SHAPE;
   if (a->kdim <= 0 || a->kdim > kMaxK || a->vdim <= 0 || a->vdim % 4 != 0 || !sv_fits(a->nheads, kThreads)) return LQ_ERR_SHAPE;
   if ((int64_t)a->nheads * a->vdim > 0x7fffffff || a->v_stride_b % 4 != 0 || a->v_stride_h % 4 != 0 || a->state_stride_s % 4 != 0) return LQ_ERR_SHAPE;
+  if (a->num_slots > 1 && a->state_stride_s < (int64_t)a->nheads * a->kdim * a->vdim) return LQ_ERR_SHAPE;  // slots that overlap
   if (!sv_al(a->q, 2) || !sv_al(a->k, 2) || !sv_al(a->v, 8) || !sv_al(a->out, 8) || !sv_al(a->state, 16) || !sv_al(a->slots, 4) ||
       (a->g && !sv_al(a->g, sv_size(a->g_dtype))))
     return LQ_ERR_SHAPE;

@@ -34,7 +34,9 @@ def _check_state(state, q, V):
     H, K = q.shape[-2:]
     assert state.dtype == torch.float32 and state.dim() == 4 and state.shape[1:] == (H, K, V), \
         f"state: (slots, {H}, {K}, {V}) float32, got {tuple(state.shape)} {state.dtype}"
-    assert state.shape[0] == 0 or (state[0].is_contiguous() and state.stride(0) % 4 == 0 and state.data_ptr() % 16 == 0), "state: dense slots"
+    n = state.shape[0]
+    assert n == 0 or (state[0].is_contiguous() and state.stride(0) % 4 == 0 and state.data_ptr() % 16 == 0), "state: dense slots"
+    assert n <= 1 or state.stride(0) >= state[0].numel(), "state: slots that do not overlap"
     _lib.same_device(q, state)
 
 

@@ -1,9 +1,12 @@
 """Further refusals of a linear attention block's operators: widths behind the padding, adapters' ids without adapters, states whose slots overlap (CPU)."""
 
+import ctypes
+
 import pytest
 import torch
 
 from linquant_amd import _lib
+from linquant_amd.kernels.zoo.linear_attention import linear_attention_prompt, linear_attention_step
 from linquant_amd.w8a8_linear import LowRankAdapters, W8A8Linear
 
 F16, F32, I8, I32 = torch.float16, torch.float32, torch.int8, torch.int32
@@ -56,3 +59,18 @@ def test_ids_without_adapters_are_refused():
     for call in (lambda: lin(z(3, 32), ids=ids), lambda: static(z(3, 32), ids=ids), lambda: lin.forward_int8(z(3, 32, dtype=I8), 1.0, ids=ids)):
         with pytest.raises(AssertionError, match="ids without adapters"):
             call()
+
+
+def test_states_whose_slots_overlap_are_refused():
+    """Two sequences would write to one place."""
+    one = z(1, 2, 8, 16, dtype=F32)
+    near = torch.as_strided(z(4 * 256, dtype=F32), (3, 2, 8, 16), (128, 128, 16, 1))
+    for s in (one.expand(3, 2, 8, 16), near):
+        with pytest.raises(AssertionError, match="overlap"):
+            linear_attention_step(s, z(2, 2, 8), z(2, 2, 8), z(2, 2, 16))
+        with pytest.raises(AssertionError, match="overlap"):
+            linear_attention_prompt(z(1, 5, 2, 8), z(1, 5, 2, 8), z(1, 5, 2, 16), state=s)
+    lib = _lib.load()
+    rc = lambda fn, **kw: getattr(lib, fn)(ctypes.byref(_lib.fill(fn + "_args", **kw)), None)  # noqa: E731
+    both = dict(q=16, k=16, v=16, out=16, state=16, dtype=0, nheads=2, num_slots=3, kdim=8, vdim=16, state_stride_s=252)
+    assert rc("lq_linear_attention_step", batch=1, **both) == -22 and rc("lq_linear_attention_prompt", nseq=1, seqlen=5, **both) == -22
