@@ -372,21 +372,22 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       if constexpr (kHalf) {
         // The channel's unit is at least one, so that no entry of v loses bits, and is kept while it brings the largest of v between 2^-1 and 2^4
         // (weighted v is then evenly spaced by 2^-24 of that or less); but a state that is 2^100 above v would leave 32 bits.
-        uint32_t top = 0;  // both halves of a dword at once: magnitudes order like whole numbers
+        // Both halves of a dword at once: magnitudes order like whole numbers, and 2^10 above themselves those that are no numbers, which must not
+        // hide the others', are negative.
+        typedef int16_t v2s __attribute__((ext_vector_type(2)));
+        v2s top2 = {0x400, 0x400};
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            typedef uint16_t v2u __attribute__((ext_vector_type(2)));
-            top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top), __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu)));
-          }
+          for (int i = 0; i < 4; ++i) top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(v2s, ((uint32_t)xp[ks][i] & 0x7fff7fffu) + 0x04000400u));
+        const uint16_t top = (uint16_t)(max((int)top2[0], (int)top2[1]) - 0x400);
         float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (no number where the lane has one that is none: its scale does not matter then)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) m4[(e >> 1) & 3] = __builtin_elementwise_maximum(m4[(e >> 1) & 3], __builtin_fabsf(S[nt][e]));
         const float m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m4[0], m4[1]), __builtin_elementwise_maximum(m4[2], m4[3]));
-        const float mx = channel_top(finite_size(T::to((uint16_t)max(top & 0xffffu, top >> 16)))), ms = channel_top(finite_size(m));
+        const float mx = channel_top(T::to(top)), ms = channel_top(finite_size(m));
         const float now = mx * unit_S;
         const bool keep = mx == 0.0f || (now >= 0.5f && now < 16.0f) || (unit_S == 1.0f && now >= 0.5f);
         float k = keep ? unit_S : scale_for<2, 0, 15>(mx);

@@ -3,7 +3,10 @@
 import pytest
 import torch
 
+from linquant_amd.kernels.zoo.linear_attention import linear_attention_prompt
 from linquant_amd.w8a8_linear import LowRankAdapters, W8A8Linear
+from tests.attention_cases import attention_inputs, attention_ref, out_rel, state_rel
+from tests.serving_cases import assert_near
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +28,21 @@ def test_widths_behind_the_padding_are_told_apart(cuda):
                     else:
                         with pytest.raises(AssertionError):
                             call()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("half", [0, 4])
+def test_large_values_beside_one_that_is_no_number(cuda, half, value):
+    """fp16, a small chunk in front of a large one, whose large values of v stand in one half of the wave's tokens with a value that is no number
+    behind them: the tokens in front of it keep their outputs."""
+    H, K, V, L = 1, 64, 64, 200
+    q, k, v, _ = attention_inputs(L, H, K, V, F16, "none", seed=half)
+    v = (v.float().clamp(-2, 2) * 1e-4).half()
+    v[[t for t in range(64, 128) if t % 8 // 4 * 4 == half]] = 20.0
+    v[64 + 56 + half, 0, 5] = value
+    o, mag, S, Sm, most = attention_ref(q, k, v, None, 0.125, [L], torch.zeros(1, H, K, V))
+    bad = lambda t: torch.where(torch.isfinite(t), t, float("nan"))  # noqa: E731
+    state = torch.zeros(1, H, K, V, device=cuda)
+    got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), scale=0.125, state=state)
+    assert_near(bad(got[0].cpu()), bad(o), bad(mag), out_rel([L], most, F16), "o")
+    assert_near(bad(state.cpu()), bad(S), bad(Sm), state_rel([L], most), "state")
