@@ -24,7 +24,9 @@
 // that type: half a step of each term.  What the state gathers over a prompt (weighted v) enters as two (fp16) or three (bf16) pieces of the
 // type: off by 2^-22 of itself, or not at all (two of bf16: the state 2.4e-6 off, here and in fp16 below 1e-6).  bf16 has the range of fp32.
 // fp16: after a multiplication by a power of two that brings the largest of what is multiplied (a channel's state; its state and v; a row of 32
-// weighted q . k) below 2^14, so no size of activations overflows.
+// weighted q . k) below 2^14, so no size of activations overflows.  Below 2^-14 fp16 is evenly spaced: weighted q . k is off by half a step of itself or
+// by 2^-29 of the largest of its 32 (old tokens of large v still count there: 2^-17, with outputs formed at their own size, cost outputs five
+// times that half step).
 #include <algorithm>
 #include <cmath>
 
@@ -224,6 +226,7 @@ LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
 template <typename T, int NT, int W, bool STATES>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void linear_attention_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
+  constexpr int kLift = kHalf ? 8 : 0;  // outputs are formed 2^kLift times as large: weighted q . k below 2^-14 of that would be evenly spaced
   constexpr float kFloor = kHalf ? -6.0f : -30.0f;  // (fp16: weighted v, below 2^8 with its unit, stays within its range; larger v: zero)
   constexpr int RB = 64 * NT, PR = 4 * NT, kTile = Q * RB;  // bytes and pieces of a row of q or k, bytes of a chunk's
   constexpr int kFetch = kTile / (1024 * W), kRows = 1024 / RB;  // fetches of a wave, rows of each
@@ -351,6 +354,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 
   // What a chunk's products need of the wave's own: v in registers, decays in LDS, the state's unit.
   float* my = tok[wave];
+  const float log_scale = p.log_scale + kLift;
   lq_v4i xp[4] = {};  // this lane's channel, tokens in the order of an operand; fp16: times its unit
   auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
   float total = 0.0f, whole_decay = 0.0f;            // what the accumulators are over, the segment's decay so far (powers of two)
@@ -429,7 +433,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       const float last = lane_of(cs, 63), after = total + last;
       whole_decay += last;
       my[lane] = cs;
-      if (!STATES) my[2 * Q + lane] = exp2_fast(cs + total + p.log_scale);
+      if (!STATES) my[2 * Q + lane] = exp2_fast(cs + total + log_scale);
       const bool now = after < kFloor || (kHalf && large && after < 0.0f);
       fold = (now ? exp2_fast(after) : 1.0f) * change, total = now ? 0.0f : after, scaled = now || (kHalf && __ballot(change != 1.0f) != 0);
       my[Q + lane] = lane < rem ? exp2_fast(behind - total) : 0.0f;
@@ -517,7 +521,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       for (int i = 0; i < PT; ++i) {
         const int tt = i == 0 ? ta : 1 - ta;
         if ((W == 4 && wave == 3) || (W == 2 && i == 1 && wave == 1)) continue;
-        const float ct = my[32 * tt + col] + p.log_scale;
+        const float ct = my[32 * tt + col] + log_scale;
         float w[16], m = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -537,7 +541,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           for (int e = 0; e < 16; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(w[e]));
           // (a column with an infinity or a NaN is none whatever its unit)
           m = channel_top(finite_size(m));
-          const bool plain = m == 0.0f || (m >= 0x1p-8f && m < 0x1p15f);
+          const bool plain = m == 0.0f || (m >= 0x1p4f && m < 0x1p15f);
           const float u = plain ? 1.0f : scale_for<13, -100, 100>(m);
           const bool odd = __ballot(!plain) != 0;
           if (lane == 0) podd[2 * tt + st] = odd;
@@ -687,7 +691,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           float a[8], z[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) a[e] = Y[y][e], z[e] = Y[y][8 + e];
-          lq_v4i two[2] = {round8<T>(a), round8<T>(z)};
+          lq_v4i two[2];
+          if constexpr (kHalf) two[0] = round8<T>(a, 1.0f / (1 << kLift)), two[1] = round8<T>(z, 1.0f / (1 << kLift));
+          else two[0] = round8<T>(a), two[1] = round8<T>(z);
           if (p.negative) {
             const int sign = (int)0x80008000u;
 #pragma unroll

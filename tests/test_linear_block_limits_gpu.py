@@ -46,3 +46,35 @@ def test_large_values_beside_one_that_is_no_number(cuda, half, value):
     got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), scale=0.125, state=state)
     assert_near(bad(got[0].cpu()), bad(o), bad(mag), out_rel([L], most, F16), "o")
     assert_near(bad(state.cpu()), bad(S), bad(Sm), state_rel([L], most), "state")
+
+
+def _weights_off(q, k, v, g, scale, rel):
+    """What outputs lose where weighted q . k is off by ``rel`` of the largest of its token's row within the chunk of 64: (T, H, V)."""
+    T, H = q.shape[:2]
+    g = torch.zeros(T, H).double() if g is None else g.double().expand(T, H)
+    off = torch.zeros(T, H, v.shape[2]).double()
+    for a in range(0, T, 64):
+        c = torch.cumsum(g[a:a + 64], 0)
+        w = abs(scale) * (q[a:a + 64].double()[:, None] * k[a:a + 64].double()[None]).sum(-1).abs() * torch.exp((c[:, None] - c[None]).clamp(max=0.0))
+        w = w * torch.ones(w.shape[:2]).tril().double()[..., None]
+        size = torch.cumsum(v[a:a + 64].double().abs(), 0)                              # of the tokens up to each one
+        off[a:a + 64] = rel * w.amax(1)[..., None] * size
+    return off
+
+
+@pytest.mark.parametrize("L", [64, 128, 200])
+@pytest.mark.parametrize("size", [0.01, 1e-4])
+@pytest.mark.parametrize("near", [2.0 ** -4, 2.0 ** -8, 1.0])
+def test_fp16_old_tokens_of_large_v(cuda, L, size, near):
+    """Weighted q . k of tokens whose v is far above the later ones' keeps its bits while they count; q and k of several sizes."""
+    H, K, V = 2, 64, 64
+    gen = torch.Generator().manual_seed(L)
+    rn = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    q, k = (near * (1 + 0.1 * rn(L, H, K))).half(), (2.0 ** -5 * (1 + 0.1 * rn(L, H, K))).half()
+    v = (size * rn(L, H, V)).half()
+    v[torch.arange(L) % 64 < 24] = 200.0
+    g = torch.full((L, H), -0.6)
+    g[:, 1] = -0.3
+    o, mag, S, Sm, most = attention_ref(q, k, v, g, 2.0 ** -4, [L], torch.zeros(1, H, K, V))
+    got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=2.0 ** -4)
+    assert_near(got[0], o, out_rel([L], most, F16) * mag + _weights_off(q, k, v, g, 2.0 ** -4, 2.0 ** -29), 1.0, "o")
