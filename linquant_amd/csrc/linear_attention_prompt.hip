@@ -23,9 +23,10 @@
 // and reaches only o, which is rounded to the activations' type itself (weighted q . k, the state that q multiplies), enters rounded to
 // that type: half a step of each term.  What the state gathers over a prompt (weighted v) enters as two (fp16) or three (bf16) pieces of the
 // type: off by 2^-22 of itself, or not at all (two of bf16: the state 2.4e-6 off, here and in fp16 below 1e-6).  bf16 has the range of fp32.
-// fp16: after a multiplication by a power of two that brings the largest of what is multiplied (a channel's state; its state and v; a row of 32
-// weighted q . k) below 2^14, so no size of activations overflows.  Below 2^-14 fp16 is evenly spaced: weighted q . k is off by half a step of itself or
-// by 2^-29 of the largest of its 32 (old tokens of large v still count there: 2^-17, with outputs formed at their own size, cost outputs five
+// fp16: after a multiplication by a power of two that brings the largest of what is multiplied (a channel's state; its weighted v; a row of 32 weighted
+// q . k) below 2^15, so no size of activations overflows.  Below 2^-14 fp16 is evenly spaced, which bounds what is far below that largest: weighted v is
+// off by 2^-26 of the channel's largest weighted v of its chunk (by the largest v itself, which may have decayed to nothing, states were 0.3 off), weighted
+// q . k by 2^-29 of the largest of its 32 (old tokens of large v still count there: 2^-17, with outputs formed at their own size, cost outputs five
 // times that half step).
 #include <algorithm>
 #include <cmath>
@@ -119,6 +120,18 @@ LQ_DEV float scale_for(float m) {
 }
 LQ_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 LQ_DEV float lane_of(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
+// the largest of the first 32 lanes' non-negative values (whole numbers order like them)
+LQ_DEV float first_half_top(float f) {
+  uint32_t v = __float_as_uint(f);
+#define LQ_TOP(CTRL) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false))
+  LQ_TOP(0xB1);   // lanes 1 0 3 2
+  LQ_TOP(0x4E);   // lanes 2 3 0 1
+  LQ_TOP(0x141);  // mirrored halves of a row of 16
+  LQ_TOP(0x140);  // mirrored rows
+  LQ_TOP(0x142);  // the last lane of a row to the next row
+#undef LQ_TOP
+  return __int_as_float(__builtin_amdgcn_readlane((int)v, 31));
+}
 // the larger of a lane's and the lane's of the other half, which has the same channel (by their bits: non-negative numbers)
 LQ_DEV float channel_top(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -227,7 +240,8 @@ template <typename T, int NT, int W, bool STATES>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void linear_attention_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
   constexpr int kLift = kHalf ? 8 : 0;  // outputs are formed 2^kLift times as large: weighted q . k below 2^-14 of that would be evenly spaced
-  constexpr float kFloor = kHalf ? -6.0f : -30.0f;  // (fp16: weighted v, below 2^8 with its unit, stays within its range; larger v: zero)
+  constexpr float kFloor = kHalf ? -6.0f : -30.0f;
+  constexpr float kUnit = kHalf ? 16.0f : 1.0f;  // of v and the state where they are of ordinary size
   constexpr int RB = 64 * NT, PR = 4 * NT, kTile = Q * RB;  // bytes and pieces of a row of q or k, bytes of a chunk's
   constexpr int kFetch = kTile / (1024 * W), kRows = 1024 / RB;  // fetches of a wave, rows of each
   constexpr int PT = W == 2 ? 2 : 1;                           // tiles of q . k of a wave
@@ -239,7 +253,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   __shared__ int podd[4];                                       // fp16: whether a tile has a unit that is not 1
   __shared__ __align__(16) float tok[W][3 * Q];                 // each wave's c, weights of v, exp2(c + total) |scale|
   __shared__ __align__(16) float gbuf[W][64];                   // each wave's decays of a chunk
-  __shared__ __align__(16) float vunit[kHalf && !STATES ? W : 1][64];  // fp16: each wave's channels' 1 / unit_S, 1 / read
+  __shared__ __align__(16) float vunit[kHalf && !STATES ? W : 1][32];  // fp16: scale / (unit_S read) of each wave's channels
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hh = lane >> 5, col = lane & 31;
   // Workgroups go round the 8 XCDs in launch order; the parts of one head, which read the same q and k, and the heads of one segment, whose
   // rows lie side by side, go to one.
@@ -355,17 +369,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   // What a chunk's products need of the wave's own: v in registers, decays in LDS, the state's unit.
   float* my = tok[wave];
   const float log_scale = p.log_scale + kLift;
-  lq_v4i xp[4] = {};  // this lane's channel, tokens in the order of an operand; fp16: times its unit
+  lq_v4i xp[4] = {};  // this lane's channel, tokens in the order of an operand
   auto x = [&](int ks, int i) { return T::to((uint16_t)((uint32_t)xp[ks][i >> 1] >> (16 * (i & 1)))); };
   float total = 0.0f, whole_decay = 0.0f;            // what the accumulators are over, the segment's decay so far (powers of two)
   float fold = 1.0f;                                 // what the accumulators are multiplied by in this chunk, mostly one
-  float unit_S = 1.0f, read = 1.0f;                  // fp16: powers of two of the channel: of v and the state; what q multiplies is that times `read`
-  bool calm = true, scaled = false, united = false;  // the same for the wave: read is one for all channels; the accumulators are multiplied; a unit is not one
+  // fp16: powers of two.  The accumulators hold the channel's state, and its weighted v enters them, times unit_S: `common` in all of the wave's
+  // channels but those of other sizes.  What q multiplies is the accumulators times `read`.
+  float unit_S = 1.0f, read = 1.0f, common = 1.0f;
+  bool alike = true, calm = true, scaled = false;  // the same for the wave: unit_S is `common` in all channels; and read is one; the accumulators are multiplied
   auto begin = [&](int c) {
     const int lane = fresh(), hh = lane >> 5;
     const int rem = s.len - (s.chunk0 + c) * Q;
-    bool large = false;
-    float change = 1.0f;
+    float mx = 0.0f, ms = 0.0f;  // the channel's largest v and accumulator
     if (live) {
       const uint16_t* xl = vbuf[wave] + (4 * hh + ((lane & 15) >> 2)) * 32 + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
@@ -374,50 +389,41 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         xp[ks] = lq_v4i{lo[0], lo[1], hi[0], hi[1]};
       }
       if constexpr (kHalf) {
-        // The channel's unit is at least one, so that no entry of v loses bits, and is kept while it brings the largest of v between 2^-1 and 2^4
-        // (weighted v is then evenly spaced by 2^-24 of that or less); but a state that is 2^100 above v would leave 32 bits.
-        // Both halves of a dword at once: magnitudes order like whole numbers, and 2^10 above themselves those that are no numbers, which must not
-        // hide the others', are negative.
-        typedef int16_t v2s __attribute__((ext_vector_type(2)));
-        v2s top2 = {0x400, 0x400};
+        // Both halves of a dword at once: magnitudes order like whole numbers.
+        typedef uint16_t v2u __attribute__((ext_vector_type(2)));
+        v2u top2 = {0, 0};
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(v2s, ((uint32_t)xp[ks][i] & 0x7fff7fffu) + 0x04000400u));
-        const uint16_t top = (uint16_t)(max((int)top2[0], (int)top2[1]) - 0x400);
+          for (int i = 0; i < 4; ++i) top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(v2u, (uint32_t)xp[ks][i] & 0x7fff7fffu));
+        if (__ballot(max(top2[0], top2[1]) >= 0x7c00) != 0) {  // those that are no numbers must not hide the others': 2^10 above themselves they are negative
+          typedef int16_t v2s __attribute__((ext_vector_type(2)));
+          v2s s2 = {0x400, 0x400};
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2 = __builtin_elementwise_max(s2, __builtin_bit_cast(v2s, ((uint32_t)xp[ks][i] & 0x7fff7fffu) + 0x04000400u));
+          top2 = __builtin_bit_cast(v2u, s2) - (uint16_t)0x400;
+        }
         float m4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (no number where the lane has one that is none: its scale does not matter then)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) m4[(e >> 1) & 3] = __builtin_elementwise_maximum(m4[(e >> 1) & 3], __builtin_fabsf(S[nt][e]));
         const float m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m4[0], m4[1]), __builtin_elementwise_maximum(m4[2], m4[3]));
-        const float mx = channel_top(T::to(top)), ms = channel_top(finite_size(m));
-        const float now = mx * unit_S;
-        const bool keep = mx == 0.0f || (now >= 0.5f && now < 16.0f) || (unit_S == 1.0f && now >= 0.5f);
-        float k = keep ? unit_S : scale_for<2, 0, 15>(mx);
-        if (ms > 0x1p100f) k = fminf(k, unit_S);
-        change = k * pow2_inverse(unit_S);
-        unit_S = k;
-        large = __ballot(mx * k >= 256.0f) != 0;
-        const uint32_t k16 = F16::from(k);
-        united = __ballot(k != 1.0f) != 0;
-        if (united) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-              const int two = xp[ks][i];  // (an element's bits are not cast in place)
-              xp[ks][i] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, two) * __builtin_bit_cast(v2h, k16 | k16 << 16));
-            }
-        }
-        if (!STATES) {
-          // (the accumulators are read before they are folded; what o is formed from is 1 / `old` of it)
-          const bool plain = change == 1.0f && (ms == 0.0f || (ms >= 0x1p-4f && ms < 0x1p15f));
-          read = plain ? 1.0f : scale_for<13, -100, 100>(ms);
-          calm = __ballot(!plain) == 0;
-          if (lane < 32) vunit[wave][lane] = pow2_inverse(unit_S), vunit[wave][32 + lane] = pow2_inverse(read) * change;
-        }
+        mx = channel_top(T::to(max(top2[0], top2[1]))), ms = channel_top(finite_size(m));
+      }
+    }
+    float log_read = log_scale;  // what the accumulators' products are multiplied by besides their decays, for all channels
+    if (kHalf && !STATES && live) {
+      const bool plain = ms == 0.0f || (ms >= 0x1p-4f && ms < 0x1p15f);
+      read = plain ? 1.0f : scale_for<13, -114, 100>(ms);
+      calm = alike && __ballot(!plain) == 0;
+      if (calm) {
+        log_read -= (float)((int)(__float_as_uint(common) >> 23) - 127);
+      } else {  // each channel by its own
+        log_read = 0.0f;
+        if (lane < 32) vunit[wave][lane] = exp2_fast(log_scale) * pow2_inverse(read) * pow2_inverse(unit_S);
       }
     }
     {
@@ -433,10 +439,46 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       const float last = lane_of(cs, 63), after = total + last;
       whole_decay += last;
       my[lane] = cs;
-      if (!STATES) my[2 * Q + lane] = exp2_fast(cs + total + log_scale);
-      const bool now = after < kFloor || (kHalf && large && after < 0.0f);
-      fold = (now ? exp2_fast(after) : 1.0f) * change, total = now ? 0.0f : after, scaled = now || (kHalf && __ballot(change != 1.0f) != 0);
-      my[Q + lane] = lane < rem ? exp2_fast(behind - total) : 0.0f;
+      if (!STATES) my[2 * Q + lane] = exp2_fast(cs + total + log_read);
+      const bool now = after < kFloor;
+      fold = now ? exp2_fast(after) : 1.0f, total = now ? 0.0f : after, scaled = now;
+      const float weight = lane < rem ? exp2_fast(behind - total) : 0.0f;
+      my[Q + lane] = weight;
+      if (kHalf && live) {
+        // A unit keeps the largest weighted v of its channel between 2 and 2^15, so that the second piece, evenly spaced by 2^-24, is off by 2^-26 of it at
+        // most.  Weights rise from token to token, and for most chunks those of token 0, 56 and 63 tell that it does.
+        float k = unit_S;
+        if (c == 0) k = common = kUnit;
+        const float least = lane_of(weight, 0) * k, most = exp2_fast(-total) * k;
+        bool search = !alike || __ballot(!(mx == 0.0f || (mx * least >= 2.0f && mx * most < 0x1p15f))) != 0;
+        if (search && alike) {
+          float late = 0.0f;
+#pragma unroll
+          for (int i = 4; i < 8; ++i) late = fmaxf(late, __builtin_fabsf(x(3, i)));
+          late = channel_top(finite_size(late)) * lane_of(weight, 56) * k;
+          search = __ballot(!(mx == 0.0f || ((mx * least >= 2.0f || late >= 2.0f) && mx * most < 0x1p15f))) != 0;
+        }
+        if (search) {
+          float m2[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const lq_v4f f4 = *(const lq_v4f*)(my + Q + 16 * ks + 8 * j + 4 * hh);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) m2[e & 1] = fmaxf(m2[e & 1], __builtin_fabsf(f4[e] * x(ks, 4 * j + e)));
+            }
+          const float mw = channel_top(finite_size(fmaxf(m2[0], m2[1]))), top = first_half_top(mw);
+          if (top > 0.0f && !(top * common >= 2.0f && top * common < 0x1p14f)) common = scale_for<10, -30, 90>(top);
+          k = mw == 0.0f || mw * common >= 2.0f ? common : mw * unit_S >= 2.0f && mw * unit_S < 0x1p14f ? unit_S : scale_for<10, -30, 90>(mw);
+        }
+        if (search || c == 0) {
+          k = fminf(k, unit_S * scale_for<100, 0, 100>(ms));  // (a state far above its v would leave 32 bits)
+          const float change = k * pow2_inverse(unit_S);
+          unit_S = k, fold *= change;
+          alike = __ballot(k != common) == 0, scaled |= __ballot(change != 1.0f) != 0;
+        }
+      }
     }
   };
   begin(0);
@@ -505,7 +547,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
         products(std::false_type{});
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const lq_v4f u4 = *(const lq_v4f*)(vunit[wave] + 32 + 8 * j + 4 * hh);
+          const lq_v4f u4 = *(const lq_v4f*)(vunit[wave] + 8 * j + 4 * hh);
 #pragma unroll
           for (int e = 0; e < 4; ++e) Y[0][4 * j + e] *= u4[e], Y[1][4 * j + e] *= u4[e];
         }
@@ -582,8 +624,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
       };
       auto pair = [&](int ks, int q) {  // a quarter of step ks' weighted v
         const lq_v4f& f = w4[ks & 1][q >> 1];
+        const float u = kHalf ? unit_S : 1.0f;
         int o[3];
-        split2<T>(f[2 * (q & 1)], x(ks, 2 * q), f[2 * (q & 1) + 1], x(ks, 2 * q + 1), o);
+        split2<T>(f[2 * (q & 1)] * u, x(ks, 2 * q), f[2 * (q & 1) + 1] * u, x(ks, 2 * q + 1), o);
 #pragma unroll
         for (int n = 0; n < N; ++n) w[ks & 1][n][q] = o[n];
       };
@@ -670,14 +713,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
             for (int y = 0; y < 2; ++y)
               if (32 * (y == 0 ? ta : 1 - ta) + col >= f) Y[y][e] = __builtin_nanf("");
-          }
-        }
-        if (kHalf && united) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const lq_v4f u4 = *(const lq_v4f*)(vunit[wave] + 8 * j + 4 * hh);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) Y[0][4 * j + e] *= u4[e], Y[1][4 * j + e] *= u4[e];
           }
         }
         // A lane has four channels of eight, the other half of the wave the other four: with every second eight exchanged it has whole eights.

@@ -78,3 +78,62 @@ def test_fp16_old_tokens_of_large_v(cuda, L, size, near):
     o, mag, S, Sm, most = attention_ref(q, k, v, g, 2.0 ** -4, [L], torch.zeros(1, H, K, V))
     got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=2.0 ** -4)
     assert_near(got[0], o, out_rel([L], most, F16) * mag + _weights_off(q, k, v, g, 2.0 ** -4, 2.0 ** -29), 1.0, "o")
+
+
+def _state_off(k, v, g, rel):
+    """What a state loses where a chunk's weighted v is off by ``rel`` of the largest of its channel: (H, K, V)."""
+    T, H = k.shape[:2]
+    g = torch.zeros(T, H).double() if g is None else g.double().expand(T, H)
+    off = torch.zeros(H, k.shape[2], v.shape[2]).double()
+    for a in range(0, T, 64):
+        c = torch.cumsum(g[a:a + 64], 0)
+        top = (torch.exp(c[-1] - c)[..., None] * v[a:a + 64].double().abs()).amax(0)                  # (H, V)
+        off = off * torch.exp(c[-1])[:, None, None] + rel * k[a:a + 64].double().abs().sum(0)[..., None] * top[:, None]
+    return off
+
+
+def _check_sizes(cuda, q, k, v, g, state, scale=0.125):
+    L, H = v.shape[:2]
+    o, mag, S, Sm, most = attention_ref(q, k, v, g, scale, [L], state)
+    got_state = state.to(cuda)
+    got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), None if g is None else g[None].to(cuda), scale=scale, state=got_state)
+    off = _state_off(k, v, g, 2.0 ** -26) if state.abs().max() == 0 else 0.0
+    bad = lambda t: torch.where(torch.isfinite(t), t, float("nan"))  # noqa: E731  (an infinity counts as a NaN)
+    assert_near(bad(got_state[0].cpu()), bad(S[0]), bad(state_rel([L], most) * Sm[0] + off), 1.0, "state")
+    got = got[0].cpu()
+    near = (o.abs() > 65000) & (o.abs() < 66000)                                       # (fp16 ends at 65504: beyond it, infinities)
+    got, o = torch.where(near, 0.0, got), torch.where(near, 0.0, torch.where(o.abs() > 65504, float("inf"), o))
+    assert_near(bad(got), bad(o), bad(out_rel([L], most, F16) * mag + _weights_off(q, k, v, g, scale, 2.0 ** -29)), 1.0, "o")
+
+
+@pytest.mark.parametrize("L", [64, 200, 1500])
+@pytest.mark.parametrize("size", [2.0 ** -11, 2.0 ** -14, 2.0 ** -18, 2.0 ** 8])
+@pytest.mark.parametrize("K,V", [(64, 64), (128, 72)])
+def test_fp16_small_values_behind_a_large_one_that_decays(cuda, L, size, K, V):
+    """The first token of each chunk is large and decays to nothing inside it: the later ones' part of the state keeps its bits."""
+    H = 2
+    q, k, v, _ = attention_inputs(L, H, K, V, F16, "none", seed=L)
+    v = (v.float() * size).half()
+    v[::64] = 1.0
+    g = torch.full((L, H), -0.6931)
+    g[:, 1] = -0.2
+    _check_sizes(cuda, q, k, v, g, torch.zeros(1, H, K, V))
+
+
+@pytest.mark.parametrize("decay", [0.0, -0.02, -0.4, -3.0])
+@pytest.mark.parametrize("first", [0.0, 1.0, 1e-30, 2.0 ** 60])
+@pytest.mark.parametrize("up", [1, -1])
+def test_fp16_sizes_that_change_from_chunk_to_chunk(cuda, decay, first, up):
+    """Chunks and channels of v of many sizes (upwards some are infinite), from states of many sizes."""
+    H, K, V, L = 2, 64, 96, 640
+    q, k, v, _ = attention_inputs(L, H, K, V, F16, "none", seed=3)
+    sizes = 2.0 ** torch.tensor([0.0, -12, -12, 8, -18, 0, 12, 12, -6, -14])
+    v = v.float().clamp(-3, 3) * sizes.repeat_interleave(64)[:, None, None] * 2.0 ** (up * (-torch.arange(V) % 5 * (torch.arange(V) // 32)))
+    state = first * torch.randn(1, H, K, V, generator=torch.Generator().manual_seed(4))
+    _check_sizes(cuda, q, k, v.half(), torch.full((L, H), decay), state)
+
+
+def test_fp16_states_next_to_the_largest_numbers(cuda):
+    H, K, V, L = 1, 64, 64, 70
+    q, k, v, _ = attention_inputs(L, H, K, V, F16, "none", seed=5)
+    _check_sizes(cuda, (q.float() * 2.0 ** -5).half(), k, v, torch.full((L, H), -0.5), torch.full((1, H, K, V), 3e38), scale=2.0 ** -126)
