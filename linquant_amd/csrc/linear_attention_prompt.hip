@@ -27,7 +27,7 @@
 // q . k) below 2^15, so no size of activations overflows.  Below 2^-14 fp16 is evenly spaced, which bounds what is far below that largest: weighted v is
 // off by 2^-26 of the channel's largest weighted v of its chunk (by the largest v itself, which may have decayed to nothing, states were 0.3 off), weighted
 // q . k by 2^-29 of the largest of its 32 (old tokens of large v still count there: 2^-17, with outputs formed at their own size, cost outputs five
-// times that half step).
+// times that half step), the state that q multiplies by 2^-25 of its channel's largest.
 #include <algorithm>
 #include <cmath>
 
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
     }
     float log_read = log_scale;  // what the accumulators' products are multiplied by besides their decays, for all channels
     if (kHalf && !STATES && live) {
-      const bool plain = ms == 0.0f || (ms >= 0x1p-4f && ms < 0x1p15f);
+      const bool plain = ms == 0.0f || (ms >= 1.0f && ms < 0x1p15f);
       read = plain ? 1.0f : scale_for<13, -114, 100>(ms);
       calm = alike && __ballot(!plain) == 0;
       if (calm) {

@@ -137,3 +137,19 @@ def test_fp16_states_next_to_the_largest_numbers(cuda):
     H, K, V, L = 1, 64, 64, 70
     q, k, v, _ = attention_inputs(L, H, K, V, F16, "none", seed=5)
     _check_sizes(cuda, (q.float() * 2.0 ** -5).half(), k, v, torch.full((L, H), -0.5), torch.full((1, H, K, V), 3e38), scale=2.0 ** -126)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -4, 2.0 ** -2, 1.0, 40.0, 2.0 ** -30])
+@pytest.mark.parametrize("below", [2.0 ** -10, 2.0 ** -13, 2.0 ** -16])
+def test_fp16_small_rows_of_a_state(cuda, size, below):
+    """q that reads only the rows of the state that are far below its others: off by half a step, or 2^-25 of the channel's largest entry."""
+    H, K, V, L = 2, 64, 64, 130
+    q, k, v, g = attention_inputs(L, H, K, V, F16, seed=7, g_mean=5.0)
+    q[:, :, :32], v[:] = 0.0, 0.0
+    state = size * (1 + torch.rand(1, H, K, V, generator=torch.Generator().manual_seed(8)))
+    state[:, :, 32:] *= below
+    o, mag, S, Sm, most = attention_ref(q, k, v, g, 0.125 / below, [L], state)
+    got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=0.125 / below, state=state.to(cuda))
+    decay = torch.exp(torch.cumsum(g.double(), 0))[..., None]
+    off = 2.0 ** -25 * 0.125 / below * decay * state[0].double().amax(1) * q.double().abs().sum(-1, keepdim=True)
+    assert_near(got[0], o, out_rel([L], most, F16) * mag + off, 1.0, "o")
