@@ -48,7 +48,8 @@ struct PromptParams {
   const float* g;
   int64_t sg_b, sg_l, sg_h;
   int g_same;  // g_same: one decay for all tokens of a head
-  float log_scale;  // of its size, a power of two
+  float log_scale;  // of its size over post, a power of two
+  float post;       // outputs are multiplied by it at the end: a power of two, one where the scale is of ordinary size
   int negative;
   uint16_t* out;
   float* state;
@@ -727,8 +728,17 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
 #pragma unroll
           for (int e = 0; e < 8; ++e) a[e] = Y[y][e], z[e] = Y[y][8 + e];
           lq_v4i two[2];
-          if constexpr (kHalf) two[0] = round8<T>(a, 1.0f / (1 << kLift)), two[1] = round8<T>(z, 1.0f / (1 << kLift));
-          else two[0] = round8<T>(a), two[1] = round8<T>(z);
+          if constexpr (kHalf) {
+            const float post = p.post * (1.0f / (1 << kLift));
+            two[0] = round8<T>(a, post), two[1] = round8<T>(z, post);
+          } else {
+            if (p.post != 1.0f) {
+              asm volatile("");  // (a branch)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) a[e] *= p.post, z[e] *= p.post;
+            }
+            two[0] = round8<T>(a), two[1] = round8<T>(z);
+          }
           if (p.negative) {
             const int sign = (int)0x80008000u;
 #pragma unroll
@@ -933,9 +943,13 @@ extern "C" int lq_linear_attention_prompt(const lq_linear_attention_prompt_args*
   if (!plan(a, pl) || a->workspace_bytes < pl.bytes || !sv_al(a->workspace, 256)) return LQ_ERR_SHAPE;
   if (pl.bytes && !a->workspace) return LQ_ERR_NULL;
   char* ws = (char*)a->workspace;
+  // Weights and decays are exponentials of sums that the scale's logarithm is part of, and zero below 2^-126: a scale far from one is left out of them.
+  const float size = std::fabs(a->scale);
+  const int exponent = size > 0.0f && std::isfinite(size) ? std::ilogb(size) : 0;
+  const float post = exponent < -40 || exponent > 40 ? std::ldexp(1.0f, std::max(exponent, -110)) : 1.0f;
   PromptParams p = {(const uint16_t*)a->q, a->q_stride_b, a->q_stride_l, a->q_stride_h, (const uint16_t*)a->k, a->k_stride_b, a->k_stride_l, a->k_stride_h,
                     (const uint16_t*)a->v, a->v_stride_b, a->v_stride_l, a->v_stride_h, a->g, a->g_stride_b, a->g_stride_l, a->g_stride_h,
-                    !a->g || (a->g_stride_b == 0 && a->g_stride_l == 0), std::log2(std::fabs(a->scale)), a->scale < 0.0f, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots, a->seq_starts,
+                    !a->g || (a->g_stride_b == 0 && a->g_stride_l == 0), std::log2(size / post), post, a->scale < 0.0f, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots, a->seq_starts,
                     a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->kdim, a->vdim, pl.cut ? (float*)ws : nullptr,
                     pl.cut ? (float*)(ws + pl.decays) : nullptr, (int)pl.segs, pl.seg_chunks, pl.parts};
   auto grid_of = [&](int64_t segs) { return dim3((unsigned)((segs * a->nheads * pl.parts + 7) / 8 * 8)); };

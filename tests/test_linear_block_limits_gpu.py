@@ -153,3 +153,20 @@ def test_fp16_small_rows_of_a_state(cuda, size, below):
     decay = torch.exp(torch.cumsum(g.double(), 0))[..., None]
     off = 2.0 ** -25 * 0.125 / below * decay * state[0].double().amax(1) * q.double().abs().sum(-1, keepdim=True)
     assert_near(got[0], o, out_rel([L], most, F16) * mag + off, 1.0, "o")
+
+
+@pytest.mark.parametrize("dtype,log", [(BF16, -116), (BF16, -60), (BF16, 70), (F16, -44), (F16, 90)])
+@pytest.mark.parametrize("decay", [0.0, -0.3, -2.0])
+def test_scales_far_from_one(cuda, dtype, log, decay):
+    """Such a scale takes nothing from the weights of old tokens."""
+    H, K, V, L = 2, 64, 64, 200
+    q, k, v, _ = attention_inputs(L, H, K, V, dtype, "none", seed=-log)
+    up = -log - 26 if dtype == BF16 else 0
+    v = (v.float() * 2.0 ** up).to(dtype)
+    state = torch.randn(1, H, K, V, generator=torch.Generator().manual_seed(9)) * 2.0 ** (up if dtype == BF16 else -log)
+    g, scale = torch.full((L, H), decay), -1.3 * 2.0 ** log
+    if dtype == F16:
+        v = v * 0.0 if log > 0 else v
+    o, mag, S, Sm, most = attention_ref(q, k, v, g, scale, [L], state)
+    got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=scale, state=state.to(cuda))
+    assert_near(got[0], o, mag, out_rel([L], most, dtype), "o")
