@@ -241,7 +241,7 @@ template <typename T, int NT, int W, bool STATES>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 ? 1 : 2, NT == 8 ? 1 : 2))) void linear_attention_chunks_kernel(PromptParams p) {
   constexpr bool kHalf = std::is_same<T, F16>::value;
   constexpr int kLift = kHalf ? 8 : 0;  // outputs are formed 2^kLift times as large: weighted q . k below 2^-14 of that would be evenly spaced
-  constexpr float kFloor = kHalf ? -6.0f : -30.0f;
+  constexpr float kFloor = kHalf ? -6.0f : 0.0f;  // (bf16: no room above the formula's range, which weights above one would need)
   constexpr float kUnit = kHalf ? 16.0f : 1.0f;  // of v and the state where they are of ordinary size
   constexpr int RB = 64 * NT, PR = 4 * NT, kTile = Q * RB;  // bytes and pieces of a row of q or k, bytes of a chunk's
   constexpr int kFetch = kTile / (1024 * W), kRows = 1024 / RB;  // fetches of a wave, rows of each

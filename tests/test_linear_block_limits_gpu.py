@@ -170,3 +170,22 @@ def test_scales_far_from_one(cuda, dtype, log, decay):
     o, mag, S, Sm, most = attention_ref(q, k, v, g, scale, [L], state)
     got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=scale, state=state.to(cuda))
     assert_near(got[0], o, mag, out_rel([L], most, dtype), "o")
+
+
+@pytest.mark.parametrize("L", [64, 200, 1500])
+@pytest.mark.parametrize("decay", [0.0, -0.05, -0.3, -2.0])
+@pytest.mark.parametrize("size", [100, 116])
+def test_bf16_has_the_range_of_fp32(cuda, L, decay, size):
+    """Nothing overflows that the formula leaves below 2^128: v, and k v with large k, next to that."""
+    H, K, V = 2, 64, 64
+    q, k, v, _ = attention_inputs(L, H, K, V, BF16, "none", seed=L)
+    v = v.float()
+    v[:, 0] *= 2.0 ** size
+    k[:, 1] = (k[:, 1].float() * 2.0 ** (size - 20)).to(BF16)
+    v[:, 1] *= 2.0 ** 20
+    v, g = v.to(BF16), torch.full((L, H), decay)
+    o, mag, S, Sm, most = attention_ref(q, k, v, g, 2.0 ** -size, [L], torch.zeros(1, H, K, V))
+    state = torch.zeros(1, H, K, V, device=cuda)
+    got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=2.0 ** -size, state=state)
+    assert_near(got[0], o, mag, out_rel([L], most, BF16), "o")
+    assert_near(state, S, Sm, state_rel([L], most), "state")
