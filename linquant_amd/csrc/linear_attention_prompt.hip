@@ -57,9 +57,10 @@ struct PromptParams {
   const int32_t* slots;
   const int32_t* starts;
   int num_slots, nseq, seqlen, tokens, H, K, V;
-  float* seg_state;  // [segment][H][K][V], or NULL: prompts are not cut
-  float* seg_decay;  // [segment][H]
+  float* seg_state;  // [place][H][K][V], or NULL: prompts are not cut
+  float* seg_decay;  // [place][H]
   int segs, seg_chunks, parts;
+  int blocks, places;  // packed prompts: STATES' units, and places of the workspace
 };
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -186,46 +187,71 @@ LQ_DEV int order(int row) {
   else return (row << 2 & 12) | (row >> 2 & 3);
 }
 
+// Segments have places in the workspace if their prompt has more than one.  Packed prompts, w tokens to a segment: prompt r of those that have more
+// than w, from token b on, has its places from b / w + r on, a segment each.  Ascending prompts so have places of their own, and however many short prompts
+// there are, places are no more than tokens / w and the prompts that can be longer than w.  (Starts that do not ascend could lead beyond them: `fit` tells.)
 struct Segment {
   int seq, begin, len;  // tokens of the sequence
   int chunk0, chunks;   // its first chunk in the sequence, how many
-  bool first, last;
+  int place;            // of the segment
+  bool first, last, fit;
 };
+LQ_DEV int tokens_of(const PromptParams& p, int s, int& begin) {  // 0 for what is no prompt
+  int b = 0, e = 0;
+  if (s < p.nseq) b = p.starts[s], e = p.starts[s + 1];
+  if (b < 0 || e > p.tokens || e < b) b = e = 0;
+  begin = b;
+  return e - b;
+}
+LQ_DEV int segments_of(const PromptParams& p, int len) { return ((int)(((uint32_t)len + (Q - 1)) / Q) + p.seg_chunks - 1) / p.seg_chunks; }
+// STATES: the segment, not a prompt's last one, that starts at a token of sg w .. sg w + w - 1.  There is one at most, and its prompt has token sg w + w too.
+template <bool STATES>
 LQ_DEV Segment segment_of(const PromptParams& p, int sg) {
   Segment r;
+  int index = 0, base = 0;  // of the prompt's segments; the first one's place
   if (p.starts) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
+    const uint32_t w = (uint32_t)p.seg_chunks * Q;
+    const int64_t behind = (int64_t)(sg + 1) * w;
+    int before = 0, cut = 0;
     r.seq = -1;
     for (int s0 = 0; s0 < p.nseq; s0 += 64) {
-      const int s = s0 + lane;
-      int b = 0, e = 0;
-      if (s < p.nseq) b = p.starts[s], e = p.starts[s + 1];
-      if (b < 0 || e > p.tokens || e < b) b = e = 0;
-      const int chunks = (int)(((uint32_t)(e - b) + (Q - 1)) / Q), n = (chunks + p.seg_chunks - 1) / p.seg_chunks;
-      int sum = n;
+      int b;
+      const int len = tokens_of(p, s0 + lane, b);
+      uint64_t found;
+      int n = 0, sum = 0, total = 0;
+      if (STATES) {
+        found = __ballot(b < behind && behind < (int64_t)b + len);
+      } else {
+        sum = n = segments_of(p, len);
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(sum, off, 64);
-        sum += lane >= off ? o : 0;
+        for (int off = 1; off < 64; off <<= 1) {
+          const int o = __shfl_up(sum, off, 64);
+          sum += lane >= off ? o : 0;
+        }
+        total = __builtin_amdgcn_readlane(sum, 63);
+        found = sg < before + total ? __ballot(sg < before + sum) : 0;
       }
-      const int total = __builtin_amdgcn_readlane(sum, 63);
-      if (sg < before + total) {
-        const int l = __builtin_ctzll(__ballot(sg < before + sum));
-        r.seq = s0 + l, r.begin = __builtin_amdgcn_readlane(b, l), r.len = __builtin_amdgcn_readlane(e, l) - r.begin;
-        r.chunk0 = (sg - before - __builtin_amdgcn_readlane(sum - n, l)) * p.seg_chunks;
+      const uint64_t longer = __ballot((uint32_t)len > w);
+      if (found) {
+        const int l = __builtin_ctzll(found);
+        r.seq = s0 + l, r.begin = __builtin_amdgcn_readlane(b, l), r.len = __builtin_amdgcn_readlane(len, l);
+        const int at = (int)((uint32_t)r.begin / w);
+        index = STATES ? sg - at : sg - before - __builtin_amdgcn_readlane(sum - n, l), base = at + cut + __builtin_popcountll(longer & ((1ull << l) - 1));
         break;
       }
-      before += total;
+      before += total, cut += __builtin_popcountll(longer);
       if (before >= p.segs) break;  // (starts that do not ascend can name far more than there are, and their sum must not wrap)
     }
   } else {
-    const int per = ((p.seqlen + Q - 1) / Q + p.seg_chunks - 1) / p.seg_chunks;
-    r.seq = sg / per, r.begin = 0, r.len = p.seqlen, r.chunk0 = (sg - r.seq * per) * p.seg_chunks;
+    const int per = segments_of(p, p.seqlen);
+    r.seq = sg / per, r.begin = 0, r.len = p.seqlen, base = r.seq * per, index = sg - base;
   }
   if (r.seq >= 0) {
     const int nc = (r.len + Q - 1) / Q;
-    r.chunks = min(p.seg_chunks, nc - r.chunk0), r.first = r.chunk0 == 0, r.last = r.chunk0 + r.chunks == nc;
+    r.chunk0 = index * p.seg_chunks, r.place = base + index;
+    r.chunks = min(p.seg_chunks, nc - r.chunk0), r.first = r.chunk0 == 0, r.last = r.chunk0 + r.chunks >= nc;
+    r.fit = !p.starts || (r.first && r.last) || base <= p.places - segments_of(p, r.len);
   }
   return r;
 }
@@ -262,10 +288,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   int sg = uniform(at / per);
   const int h = uniform((at - sg * per) / p.parts), part = uniform(at - sg * per - h * p.parts);
   if (STATES && !p.starts) sg = uniform(sg + sg / max(p.segs / p.nseq - 1, 1));  // (as many segments to each prompt, the last ones left out)
-  if (sg >= p.segs) return;
-  Segment s = segment_of(p, sg);
-  if (s.seq < 0 || (STATES && s.last)) return;
+  if (sg >= (STATES && p.starts ? p.blocks : p.segs)) return;
+  Segment s = segment_of<STATES>(p, sg);
+  if (s.seq < 0 || (STATES && s.last) || !s.fit) return;
   s.seq = uniform(s.seq), s.begin = uniform(s.begin), s.len = uniform(s.len), s.chunk0 = uniform(s.chunk0), s.chunks = uniform(s.chunks);
+  const int64_t place = uniform(s.place);
   const int ch0 = (part * W + wave) * 32, ch = ch0 + col, chc = min(ch, p.V - 1);
   const bool live = ch0 < p.V;  // a wave without channels only helps
   const int slot = p.state || p.slots ? uniform(sv_slot(p.slots, s.seq, p.num_slots)) : kSlotPad;
@@ -282,7 +309,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   v16f S[NT];
   const int64_t sbase = (int64_t)h * p.K * p.V + chc;
   {
-    const float* src = STATES ? nullptr : (p.seg_state && !(s.first && s.last)) ? p.seg_state + (int64_t)sg * p.H * p.K * p.V + sbase : keeps ? p.state + slot * p.ss_s + sbase : nullptr;
+    const float* src = STATES ? nullptr : (p.seg_state && !(s.first && s.last)) ? p.seg_state + place * p.H * p.K * p.V + sbase : keeps ? p.state + slot * p.ss_s + sbase : nullptr;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -769,7 +796,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) sv_settle(S[nt]);
-  float* dst = STATES ? p.seg_state + (int64_t)sg * p.H * p.K * p.V + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
+  float* dst = STATES ? p.seg_state + place * p.H * p.K * p.V + sbase : s.last && keeps ? p.state + slot * p.ss_s + sbase : nullptr;
   if (dst && ch < p.V) {
     const float ui = exp2_fast(total) * (kHalf ? pow2_inverse(unit_S) : 1.0f);
     if (whole) {
@@ -785,34 +812,33 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(NT == 8 
           if (channel(nt, hh, r) < p.K) dst[channel(nt, hh, r) * (int64_t)p.V] = S[nt][r] * ui;
     }
   }
-  if (STATES && threadIdx.x == 0 && part == 0) p.seg_decay[(int64_t)sg * p.H + h] = exp2_fast(whole_decay);
+  if (STATES && threadIdx.x == 0 && part == 0) p.seg_decay[place * p.H + h] = exp2_fast(whole_decay);
 }
 
 // The state in front of each segment, in the place of what it adds to one.  A workgroup has 1024 entries of one head's state.
 __global__ __launch_bounds__(256) void linear_attention_join_kernel(PromptParams p) {
   const int64_t per = (int64_t)p.K * p.V;
-  const int h = blockIdx.y, at = (blockIdx.z * 256 + threadIdx.x) * 4, seq = blockIdx.x;
-  // the sequence's segments, and how many there are in front of them
-  auto segments = [&](int i) {
-    int b = 0, e = p.seqlen;
-    if (p.starts) {
-      b = p.starts[i], e = p.starts[i + 1];
-      if (b < 0 || e > p.tokens || e < b) b = e = 0;
+  const int h = blockIdx.y, at = (blockIdx.z * 256 + threadIdx.x) * 4;
+  int seq = blockIdx.x, n, first;
+  if (p.starts) {  // of the prompts that are cut the one with this number
+    const uint32_t w = (uint32_t)p.seg_chunks * Q;
+    int left = seq, s0 = 0, b = 0, len = 0;
+    uint64_t longer = 0;
+    for (; s0 < p.nseq; s0 += 64) {
+      len = tokens_of(p, s0 + (threadIdx.x & 63), b);
+      longer = __ballot((uint32_t)len > w);
+      if (left < __builtin_popcountll(longer)) break;
+      left -= __builtin_popcountll(longer);
     }
-    return ((int)(((uint32_t)(e - b) + (Q - 1)) / Q) + p.seg_chunks - 1) / p.seg_chunks;
-  };
-  const int n = segments(seq);
-  if (n < 2) return;
-  int first = 0;
-  if (p.starts) {
-    // (starts that do not ascend can name far more than there are, and their sum must not wrap: one too many is enough to know)
-    for (int i = threadIdx.x & 63; i < seq; i += 64) first = min(first + segments(i), p.segs + 1);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) first = min(first + __shfl_xor(first, off, 64), p.segs + 1);
+    if (s0 >= p.nseq) return;
+    for (; left > 0; --left) longer &= longer - 1;
+    const int l = __builtin_ctzll(longer);
+    first = (int)((uint32_t)__builtin_amdgcn_readlane(b, l) / w) + seq, seq = s0 + l, n = segments_of(p, __builtin_amdgcn_readlane(len, l));
+    if (first > p.places - n) return;
   } else {
-    first = seq * n;
+    n = segments_of(p, p.seqlen), first = seq * n;
   }
-  if (at >= per || first > p.segs - n) return;
+  if (at >= per) return;
   const int slot = p.state || p.slots ? sv_slot(p.slots, seq, p.num_slots) : kSlotPad;
   lq_v4f v = {0.f, 0.f, 0.f, 0.f};
   if (p.state && slot >= 0) v = *(const lq_v4f*)(p.state + slot * p.ss_s + h * per + at);
@@ -847,7 +873,7 @@ int check_dims(const lq_linear_attention_prompt_args* a) {
 
 // How a call is cut: the chunks of a segment.
 struct Plan {
-  int64_t segs, decays, bytes;
+  int64_t segs, blocks, longer, places, decays, bytes;  // packed prompts: blocks of a segment's tokens, prompts that can be longer than one
   int waves, parts, seg_chunks, cut;
 };
 bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
@@ -857,8 +883,8 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
   r.parts = (a->vdim + 32 * r.waves - 1) / (32 * r.waves);
   const int64_t parts = (int64_t)a->nheads * r.parts;
   // Tenths of a microsecond.  A chunk's step takes `one` where a compute unit has one workgroup and `full` where it has as many as fit
-  // (`fit`), one of the states' 0.64 and 0.53 of it; the join moves every segment's state three times at 2.6 TB/s (more where there are many),
-  // and it and two more launches come to 100.
+  // (`fit`), one of the states' 0.64 and 0.53 of it; every segment's state is taken to move three times at 2.6 TB/s (more where there are many;
+  // those of prompts that are not cut do not), and the join and two more launches to come to 100.
   // Measured, heads of 128 by 128, by the chunks of a segment: 500 tokens of 16 heads uncut 34 us, 2 chunks 26, one 26; 2 prompts of 8192, 32
   // heads, 32 chunks 249 us, 16 203, 8 229; 4 of 4096, 16 heads, 16 chunks 115, 12 120, 8 102; one of 16384, 8 heads, 16 chunks 106, 8 71; 10
   // packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 153, 12 chunks 119, 8 86, 6 80, 5 87, 4 94.  A segment's own state in two
@@ -908,10 +934,14 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
     }
   const int64_t per = (most + r.seg_chunks - 1) / r.seg_chunks;
   r.segs = a->seq_starts ? std::min<int64_t>(units / r.seg_chunks + nseq, units) : nseq * per;
+  const int64_t w = (int64_t)Q * r.seg_chunks;
+  r.blocks = a->seq_starts ? (a->tokens - 1) / w : nseq * (per - 1), r.longer = a->seq_starts ? std::min<int64_t>(nseq, a->tokens / (w + 1)) : nseq;
+  r.places = a->seq_starts ? r.blocks + r.longer : r.segs;
+  if (r.blocks == 0) r.cut = 0;
   if (!r.cut) r.segs = nseq;
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  r.decays = r.cut ? up(r.segs * a->nheads * a->kdim * a->vdim * 4) : 0;
-  r.bytes = r.decays + (r.cut ? up(r.segs * a->nheads * 4) : 0);
+  r.decays = r.cut ? up(r.places * a->nheads * a->kdim * a->vdim * 4) : 0;
+  r.bytes = r.decays + (r.cut ? up(r.places * a->nheads * 4) : 0);
   return sv_fits(nseq, 256) && sv_fits(r.segs * parts + 7, 256) && r.segs * parts < 0x7fffffff;
 }
 
@@ -951,10 +981,10 @@ extern "C" int lq_linear_attention_prompt(const lq_linear_attention_prompt_args*
                     (const uint16_t*)a->v, a->v_stride_b, a->v_stride_l, a->v_stride_h, a->g, a->g_stride_b, a->g_stride_l, a->g_stride_h,
                     !a->g || (a->g_stride_b == 0 && a->g_stride_l == 0), std::log2(size / post), post, a->scale < 0.0f, (uint16_t*)a->out, a->state, a->state_stride_s, a->slots, a->seq_starts,
                     a->num_slots, a->nseq, a->seqlen, a->tokens, a->nheads, a->kdim, a->vdim, pl.cut ? (float*)ws : nullptr,
-                    pl.cut ? (float*)(ws + pl.decays) : nullptr, (int)pl.segs, pl.seg_chunks, pl.parts};
+                    pl.cut ? (float*)(ws + pl.decays) : nullptr, (int)pl.segs, pl.seg_chunks, pl.parts, (int)pl.blocks, (int)pl.places};
   auto grid_of = [&](int64_t segs) { return dim3((unsigned)((segs * a->nheads * pl.parts + 7) / 8 * 8)); };
-  const dim3 grid = grid_of(pl.segs), ahead = grid_of(a->seq_starts ? pl.segs : pl.segs - a->nseq), threads(64 * pl.waves);
-  const dim3 join((unsigned)a->nseq, (unsigned)a->nheads, (unsigned)(((int64_t)a->kdim * a->vdim + 1023) / 1024));
+  const dim3 grid = grid_of(pl.segs), ahead = grid_of(pl.blocks), threads(64 * pl.waves);
+  const dim3 join((unsigned)pl.longer, (unsigned)a->nheads, (unsigned)(((int64_t)a->kdim * a->vdim + 1023) / 1024));
   auto go = [&](auto t, auto k, auto w) {
     using T = decltype(t);
     constexpr int NT = decltype(k)::value, W = decltype(w)::value;

@@ -6,7 +6,7 @@ import torch
 from linquant_amd.kernels.zoo.linear_attention import linear_attention_prompt
 from linquant_amd.w8a8_linear import LowRankAdapters, W8A8Linear
 from tests.attention_cases import attention_inputs, attention_ref, out_rel, state_rel
-from tests.serving_cases import assert_near
+from tests.serving_cases import assert_near, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +189,23 @@ def test_bf16_has_the_range_of_fp32(cuda, L, decay, size):
     got = linear_attention_prompt(q[None].to(cuda), k[None].to(cuda), v[None].to(cuda), g[None].to(cuda), scale=2.0 ** -size, state=state)
     assert_near(got[0], o, mag, out_rel([L], most, BF16), "o")
     assert_near(state, S, Sm, state_rel([L], most), "state")
+
+
+@pytest.mark.parametrize("seed", range(8))
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_packed_prompts_cut_at_every_place(cuda, seed, dtype):
+    """Prompts around whole segments among empty and single ones, more than 64 of them; each segment's state lies where its neighbours expect it."""
+    gen = torch.Generator().manual_seed(seed)
+    pick = lambda n: int(torch.randint(0, n, (1,), generator=gen))  # noqa: E731
+    choices = [0, 0, 1, 1, 2, 63, 64, 65, 127, 128, 129, 192, 193, 256, 257, 384, 385, 512, 513, 1025]
+    lens = [choices[pick(len(choices) if i % 3 == 0 else 6)] for i in range([5, 9, 30, 70, 130, 3, 200, 12][seed])] + [600 + pick(400)]
+    first, H, K, V = [0, 64, 5, 0, 63, 200, 0, 1][seed], 1 + seed % 2, 64, 64
+    T, n = sum(lens), len(lens)
+    q, k, v, g = attention_inputs(T, H, K, V, dtype, seed=seed, g_mean=5.0)
+    state = torch.randn(n, H, K, V, generator=gen)
+    o, mag, S, Sm, most = attention_ref(q, k, v, g, 0.125, lens, state)
+    room = lambda t: torch.cat([torch.full((first, *t.shape[1:]), float("nan")).to(t.dtype), t]).to(cuda)  # noqa: E731
+    got_state = state.to(cuda)
+    got = linear_attention_prompt(*(room(t) for t in (q, k, v, g)), scale=0.125, state=got_state, seq_starts=starts_of(lens, cuda, first=first))
+    assert_near(got[first:], o, mag, out_rel(lens, most, dtype), "o")
+    assert_near(got_state, S, Sm, state_rel(lens, most), "state")

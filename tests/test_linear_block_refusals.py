@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from linquant_amd import _lib
-from linquant_amd.kernels.zoo.linear_attention import linear_attention_prompt, linear_attention_step
+from linquant_amd.kernels.zoo.linear_attention import linear_attention_prompt, linear_attention_step, prompt_workspace_bytes
 from linquant_amd.w8a8_linear import LowRankAdapters, W8A8Linear
 
 F16, F32, I8, I32 = torch.float16, torch.float32, torch.int8, torch.int32
@@ -74,3 +74,11 @@ def test_states_whose_slots_overlap_are_refused():
     rc = lambda fn, **kw: getattr(lib, fn)(ctypes.byref(_lib.fill(fn + "_args", **kw)), None)  # noqa: E731
     both = dict(q=16, k=16, v=16, out=16, state=16, dtype=0, nheads=2, num_slots=3, kdim=8, vdim=16, state_stride_s=252)
     assert rc("lq_linear_attention_step", batch=1, **both) == -22 and rc("lq_linear_attention_prompt", nseq=1, seqlen=5, **both) == -22
+
+
+@pytest.mark.parametrize("nseq,tokens", [(256, 256), (1024, 4096), (4096, 16384), (10, 6949), (61, 2060), (1, 500), (1, 40000), (65535, 65535)])
+@pytest.mark.parametrize("H,K,V", [(32, 128, 128), (1, 64, 64), (8, 256, 72)])
+def test_workspace_of_packed_prompts_goes_by_their_tokens(nseq, tokens, H, K, V):
+    """However many prompts there are: a place for each 64 tokens, and one for each prompt that can be longer."""
+    most = (tokens - 1) // 64 + min(nseq, tokens // 65)
+    assert prompt_workspace_bytes(nseq, 0, tokens, True, H, K, V, 0) <= most * H * (K * V + 1) * 4 + 512
