@@ -4,18 +4,19 @@
 //   o_t = scale (exp(c_t) S^T q_t + sum_{s <= t} exp(c_t - c_s) (q_t . k_s) v_s)
 //   S'  = exp(c_63) S + sum_s exp(c_63 - c_s) k_s v_s^T
 // which are products of matrices.  Three kernels:
-//   states     per segment of a prompt: the state at its end if it starts from zero, and what it multiplies an earlier one by;
+//   states     per segment of a prompt but the last: the state at its end if it starts from zero, and what it multiplies an earlier one by;
 //   join       walks the segments: the state in front of each.  (states and join: only where prompts are cut into segments, because
 //              prompts times heads are too few for 256 compute units)
 //   chunks     walks a segment chunk by chunk, the state in registers
 // A workgroup has 128 columns of a head's state (64 where there are no more), a wave 32 of them over all K: the state and the chunk's products
 // with it never leave the wave.  q, k and v come to LDS by fetches that pass no registers, the next chunk's while one is multiplied.
 //
-// What bounds it.  2 prompts of 8192, 32 heads of 128 by 128, fp16: chunks 125 us for 537 MB (4.3 TB/s; the chunk's step alone, 4.2 us with one
-// workgroup to a compute unit and 7.0 with two, gives 112), states 67 for half of that once more, join 11; a copy's rate for what has to move is
-// 103.  10 packed prompts of 6949 tokens, 16 heads: 50, 25 and 8, by steps one after the other (up to 32 chunks in a prompt, 6 to a segment).  500
-// tokens of 16 heads: 10.6, 7.7 and 4.0, three launches and a chunk's step in each of two.  In a step of 4.2 us (fp16, cycles of 10000): waiting for the
-// chunk 330, its successor's fetches 880, q k 1205, weights and rounding 1150, meeting 600, the state 1840, outputs 2360, operands of v 1800.
+// What bounds it.  2 prompts of 8192, 32 heads of 128 by 128, fp16: chunks 129 us for 537 MB (4.2 TB/s), states 66 for half of that once more,
+// join 13; a copy's rate for what has to move is 103.  10 packed prompts of 6949 tokens, 16 heads: 52, 26 and 8, by steps one after the other (up to
+// 32 chunks in a prompt, 6 to a segment).  500 tokens of 16 heads, bf16: 9.7, 7.6 and 3.9, three launches and a chunk's step in each of two.  In a step of
+// the long prompts (fp16, two workgroups to a compute unit, 11300 cycles): waiting for the chunk 450, its successor's fetches 1200, q k 1190, weights and
+// rounding 1130, meeting 850, the state 1950, outputs 3100, operands of v 1490.  Units that go by weighted v and outputs formed 2^8 times as large (fp16,
+// below) are 110 and 130 of these; with v's own sizes the calls took 1 to 4 % less.
 // Tried and no faster: fetches spread between the products, outputs' products between the state's, segments in the other order (so that the
 // caches still have what the states read last), a segment's own state as two pieces of 16 bits.
 //
@@ -28,6 +29,8 @@
 // off by 2^-26 of the channel's largest weighted v of its chunk (by the largest v itself, which may have decayed to nothing, states were 0.3 off), weighted
 // q . k by 2^-29 of the largest of its 32 (old tokens of large v still count there: 2^-17, with outputs formed at their own size, cost outputs five
 // times that half step), the state that q multiplies by 2^-25 of its channel's largest.
+// Decays are summed over a chunk in 32 bits, each a factor of 2^-160 at least: behind 32 tokens that decay to nothing a weight is off by up to 2e-4 of itself,
+// less than half a step of fp16.
 #include <algorithm>
 #include <cmath>
 
@@ -885,10 +888,9 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
   // Tenths of a microsecond.  A chunk's step takes `one` where a compute unit has one workgroup and `full` where it has as many as fit
   // (`fit`), one of the states' 0.64 and 0.53 of it; every segment's state is taken to move three times at 2.6 TB/s (more where there are many;
   // those of prompts that are not cut do not), and the join and two more launches to come to 100.
-  // Measured, heads of 128 by 128, by the chunks of a segment: 500 tokens of 16 heads uncut 34 us, 2 chunks 26, one 26; 2 prompts of 8192, 32
-  // heads, 32 chunks 249 us, 16 203, 8 229; 4 of 4096, 16 heads, 16 chunks 115, 12 120, 8 102; one of 16384, 8 heads, 16 chunks 106, 8 71; 10
-  // packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 153, 12 chunks 119, 8 86, 6 80, 5 87, 4 94.  A segment's own state in two
-  // pieces: 2 prompts of 8192 208, 4 of 4096 115.
+  // Measured, heads of 128 by 128, by the chunks of a segment: 500 tokens of 16 heads, bf16, uncut 36 us, 2 chunks 27, one 26; 2 prompts of 8192, 32
+  // heads, 32 chunks 233 us, 16 208, 8 226; 4 of 4096, 16 heads, 16 chunks 118, 12 125, 8 106; one of 16384, 8 heads, 16 chunks 108, 8 73; 10
+  // packed prompts of 6949 tokens, the longest 2047, 16 heads, uncut 160, 12 chunks 116, 8 93, 6 85, 4 91, 3 94.
   struct Step { double one, full; int fit; };
   static constexpr Step steps[4][2] = {{{30, 50, 3}, {32, 42, 2}}, {{37, 59, 3}, {34, 51, 2}}, {{54, 60, 2}, {42, 72, 2}}, {{76, 76, 1}, {76, 76, 1}}};
   const Step s = steps[a->kdim <= 32 ? 0 : a->kdim <= 64 ? 1 : a->kdim <= 128 ? 2 : 3][r.waves == 4];
@@ -906,8 +908,8 @@ bool plan(const lq_linear_attention_prompt_args* a, Plan& r) {
   };
   // Packed prompts' lengths are not known here.  They may be alike, or the longest two and a half times the mean, or one has nearly all the tokens;
   // taken is what loses least over the three, the second counted twice, each against what would be best for it.  us, taken, best and uncut:
-  // the 10 prompts above 82, 82, 148; 10 of 695 75, 55, 55; one of 2000 among 60 single tokens 108, 93, 136; one of 4096 among 32, 32 heads, 227,
-  // 174, 264; 64 of 200, 32 heads, 204, 154, 154; 4 of 30 to 700, 8 heads of 64 by 64, 20, 20, 46; 3000 and 200 tokens, 8 heads of 256 by 128, 55, 55, 294.
+  // the 10 prompts above 86, 85, 160; 10 of 695 72, 56, 56; one of 2000 among 60 single tokens 97, 87, 140; one of 4096 among 32, 32 heads, 200,
+  // 150, 274; 64 of 200, 32 heads, 195, 157, 157; 4 of 30 to 700, 8 heads of 64 by 64, 20, 20, 47; 3000 and 200 tokens, 8 heads of 256 by 128, 56, 55, 300.
   const double mean = (double)units / nseq, rest = (double)nseq - 1;
   auto costs = [&](int64_t n, double (&c)[3]) {
     if (!a->seq_starts) {

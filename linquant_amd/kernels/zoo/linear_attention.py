@@ -56,7 +56,7 @@ def linear_attention_prompt(q, k, v, g=None, *, scale=None, state=None, slots=No
     without its first dimension and with T tokens with ``seq_starts`` (n + 1 int32, ascending) for packed prompts of any lengths;
     tokens outside them keep undefined outputs.  ``g``: log decays, (H,) or one for each token like q without K, fp16, bf16 or fp32;
     one above zero counts as zero; None: no decay.  K and V multiples of 8, K up to 256; ``scale`` K ** -0.5 by default.
-    ``state`` (slots, H, K, V) fp32: what each prompt starts from, replaced by what it ends in (a prompt of no tokens leaves it);
+    ``state`` (slots, H, K, V) fp32, dense slots that do not overlap: what each prompt starts from, replaced by what it ends in (a prompt of no tokens leaves it);
     None: zero, nothing kept.  ``slots`` (n,) int32: each prompt's place in the state, all different; negative: from zero, nothing
     kept; beyond the state: NaN outputs.  An infinity in q, k, v or the state counts as a NaN: it reaches the outputs and states that the
     formula has it reach, as one or the other.  Returns o, dense, in the shape and type of v."""
