@@ -29,8 +29,9 @@
 // off by 2^-26 of the channel's largest weighted v of its chunk (by the largest v itself, which may have decayed to nothing, states were 0.3 off), weighted
 // q . k by 2^-29 of the largest of its 32 (old tokens of large v still count there: 2^-17, with outputs formed at their own size, cost outputs five
 // times that half step), the state that q multiplies by 2^-25 of its channel's largest.
-// Decays are summed over a chunk in 32 bits, each a factor of 2^-160 at least: behind 32 tokens that decay to nothing a weight is off by up to 2e-4 of itself,
-// less than half a step of fp16.
+// Decays are summed over a chunk in 32 bits, each a factor of 2^-160 at least: behind 32 tokens that decay to nothing the weights of the chunk's others are
+// off by up to 3.4e-4 of themselves, behind 52 of them by 9e-4 (half a step of fp16 is 4.9e-4); the state's weights, summed from the end, are not.  Sums of
+// whole parts and of fractions by themselves, where a chunk's decays are that large, would make every call 1 % longer.
 #include <algorithm>
 #include <cmath>
 
